@@ -32,6 +32,10 @@ EXPORTED = [
     # include/chimera_workload.h
     "chimera_synth_tokens_device", "chimera_gather_rows_device", "chimera_exact_maxsim_device",
     "chimera_maxsim_rescore_device", "chimera_matrix_core_rate",
+    # include/chimera_operators.h (chimera_amd.operators)
+    "chimera_linear_workspace", "chimera_linear_forward_device", "chimera_linear_backward_device",
+    "chimera_cache_row", "chimera_cache_write_device", "chimera_cache_read_device",
+    "chimera_cache_maxsim_workspace", "chimera_cache_maxsim_device",
 ]
 
 # chimera_matrix_core_rate kinds: instruction and operands
@@ -243,9 +247,13 @@ class Context:
     def free(self, ptr: int) -> None:
         check(lib().chimera_device_free(self._ctx, P(ptr)))
 
-    def to_device(self, arr: np.ndarray) -> "DeviceArray":
+    def to_device(self, arr: np.ndarray, bf16: bool = False) -> "DeviceArray":
+        """A copy on the device; bf16: arr holds the bits (uint16) of brain
+        floats."""
         a = np.ascontiguousarray(arr)
-        d = DeviceArray(self, a.shape, a.dtype)
+        if bf16 and a.dtype != np.uint16:
+            raise ValueError("the bits of brain floats are uint16")
+        d = DeviceArray(self, a.shape, "bf16" if bf16 else a.dtype)
         check(lib().chimera_copy_to_device(self._ctx, P(d.ptr), _ptr(a), C.c_size_t(a.nbytes)))
         return d
 
@@ -432,12 +440,14 @@ class Context:
 
 class DeviceArray:
     """A device allocation made through the C ABI (no other HIP runtime is
-    loaded into the process)."""
+    loaded into the process). dtype is numpy's, or "bf16" for 16-bit brain
+    floats, whose bits numpy() returns as uint16."""
 
     def __init__(self, ctx: Context, shape, dtype):
         self.ctx = ctx
         self.shape = tuple(shape) if isinstance(shape, (tuple, list)) else (int(shape),)
-        self.dtype = np.dtype(dtype)
+        self.bf16 = isinstance(dtype, str) and dtype == "bf16"
+        self.dtype = np.dtype(np.uint16 if self.bf16 else dtype)
         self.nbytes = int(np.prod(self.shape)) * self.dtype.itemsize
         self.ptr = ctx.alloc(self.nbytes)
 

@@ -1,0 +1,547 @@
+// The quantised token cache (include/chimera_operators.h): rows written as
+// codes with one scale per group of values, read back, and late interaction
+//   score(q, d) = sum over tokens i of q of max over tokens t of d of <q_i, x_t>
+// on the codes as they lie in the cache's pages.
+#include "operators.hpp"
+
+#include <algorithm>
+
+namespace chimera {
+
+namespace {
+
+int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
+
+// A group whose largest magnitude is below this is stored as zeros: top / max
+// and max / top stay within the normal 32-bit range (448 * 2^117 < 2^126).
+constexpr float kLeastGroup = 0x1p-117f;
+
+template <int kFormat>
+constexpr float top_code() {
+    return kFormat == CHIMERA_CACHE_INT8 ? 127.0f : kFormat == CHIMERA_CACHE_INT4 ? 7.0f : 448.0f;
+}
+
+struct CacheView {
+    uint8_t* codes;
+    float* scales;
+    int64_t slots, num_pages;
+    int dim, row_bytes, row_scales;
+    int group_log2;  // of values per scale
+    int page_log2;   // of tokens per page
+};
+
+CacheView view_of(const chimera_cache& c) {
+    CacheView v;
+    v.codes = c.codes;
+    v.scales = c.scales;
+    v.slots = c.num_pages * c.page_tokens;
+    v.num_pages = c.num_pages;
+    v.dim = c.dim;
+    v.row_bytes = cache_row_bytes(c);
+    v.row_scales = cache_row_scales(c);
+    v.group_log2 = c.group == 32 ? 5 : c.group == 64 ? 6 : 7;
+    v.page_log2 = __builtin_ctz(static_cast<unsigned>(c.page_tokens));
+    return v;
+}
+
+// ---- writing -------------------------------------------------------------------
+
+// 16 lanes a row, eight neighbouring values a lane: a group is 4, 8 or 16
+// neighbouring lanes.
+template <typename T, int kFormat>
+__global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, const T* __restrict__ rows, int64_t stride,
+                                                          const int64_t* __restrict__ slots, int64_t n, bool vec) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
+    const int col = static_cast<int>(threadIdx.x) % 16 * 8;
+    const int64_t slot = i < n ? slots[i] : -1;
+    const bool in = slot >= 0 && slot < c.slots;
+    float x[8] = {};
+    if (in) {
+        const T* src = rows + i * stride + col;
+        if (vec && col + 8 <= c.dim) {
+            T t[8];
+#pragma unroll
+            for (int j = 0; j < 8 * static_cast<int>(sizeof(T)) / 16; ++j)
+                reinterpret_cast<u32x4_t*>(t)[j] = reinterpret_cast<const u32x4_t*>(src)[j];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = to_float(t[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (col + j < c.dim) x[j] = to_float(src[j]);
+        }
+    }
+    float most = 0.0f;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        most = fmaxf(most, fabsf(x[j]));
+        bad |= !(fabsf(x[j]) <= 3.402823466e38f);
+    }
+    if (bad) most = INFINITY;
+    const int lanes = 1 << (c.group_log2 - 3);
+    for (int o = 1; o < lanes; o <<= 1) most = fmaxf(most, __shfl_xor(most, o, kWave));
+    constexpr float kTop = top_code<kFormat>();
+    const bool finite = most <= 3.402823466e38f;
+    const bool zero = most < kLeastGroup || !finite;
+    const float inv = zero ? 0.0f : kTop * (1.0f / most);
+    const float scale = !finite ? NAN : zero ? 0.0f : most * (1.0f / kTop);
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        v[j] = zero ? 0.0f : x[j] * inv;
+        if (kFormat != CHIMERA_CACHE_FP8) v[j] = rintf(v[j]);
+        v[j] = fminf(fmaxf(v[j], -kTop), kTop);
+    }
+    if (!in) return;
+    if (col < (c.dim + 31) / 32 * 32) {
+        uint8_t* dst = c.codes + slot * c.row_bytes;
+        if constexpr (kFormat == CHIMERA_CACHE_INT4) {
+            uint32_t u = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) u |= static_cast<uint32_t>(static_cast<int>(v[j]) + 8) << (4 * j);
+            *reinterpret_cast<uint32_t*>(dst + col / 2) = u;
+        } else {
+            u32x2_t u = {0, 0};
+            if constexpr (kFormat == CHIMERA_CACHE_INT8) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j / 4] |= (static_cast<uint32_t>(static_cast<int>(v[j])) & 0xFFu) << (8 * (j % 4));
+            } else {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    int p = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j], v[4 * j + 1], 0, false);
+                    p = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * j + 2], v[4 * j + 3], p, true);
+                    u[j] = static_cast<uint32_t>(p);
+                }
+            }
+            *reinterpret_cast<u32x2_t*>(dst + col) = u;
+        }
+    }
+    if (col < c.dim && (col & ((1 << c.group_log2) - 1)) == 0)
+        c.scales[slot * c.row_scales + (col >> c.group_log2)] = scale;
+}
+
+// ---- reading -------------------------------------------------------------------
+
+template <typename T, int kFormat>
+__global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, const int64_t* __restrict__ slots, int64_t n,
+                                                         T* __restrict__ out, int64_t stride, bool vec) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
+    const int col = static_cast<int>(threadIdx.x) % 16 * 8;
+    if (i >= n || col >= c.dim) return;
+    const int64_t slot = slots[i];
+    float v[8] = {};
+    if (slot >= 0 && slot < c.slots) {
+        const uint8_t* src = c.codes + slot * c.row_bytes;
+        const float scale = c.scales[slot * c.row_scales + (col >> c.group_log2)];
+        if constexpr (kFormat == CHIMERA_CACHE_INT4) {
+            const uint32_t u = *reinterpret_cast<const uint32_t*>(src + col / 2);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = static_cast<float>(static_cast<int>((u >> (4 * j)) & 15u) - 8);
+        } else {
+            const u32x2_t u = *reinterpret_cast<const u32x2_t*>(src + col);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (kFormat == CHIMERA_CACHE_INT8)
+                    v[j] = static_cast<float>(static_cast<int8_t>(u[j / 4] >> (8 * (j % 4))));
+                else
+                    v[j] = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(u[j / 4] >> (8 * (j % 4))), 0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= scale;
+    }
+    T t[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
+    T* dst = out + i * stride + col;
+    if (vec && col + 8 <= c.dim) {
+#pragma unroll
+        for (int j = 0; j < 8 * static_cast<int>(sizeof(T)) / 16; ++j)
+            reinterpret_cast<u32x4_t*>(dst)[j] = reinterpret_cast<const u32x4_t*>(t)[j];
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (col + j < c.dim) dst[j] = t[j];
+    }
+}
+
+// ---- late interaction ----------------------------------------------------------
+
+// Eight codes as fp16 values, exactly, in the order code_order() gives.
+__device__ __forceinline__ f16x8_t int8_values(u32x2_t u) {
+    // a byte plus 128 below the exponent of 1024 is 1152 + code
+    const f16x2_t bias = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    f16x8_t v;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const uint32_t x = u[j] ^ 0x80808080u;
+        const f16x2_t lo = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04010400u)) - bias;
+        const f16x2_t hi = __builtin_bit_cast(f16x2_t, __builtin_amdgcn_perm(0x64646464u, x, 0x04030402u)) - bias;
+        v[4 * j] = lo[0];
+        v[4 * j + 1] = lo[1];
+        v[4 * j + 2] = hi[0];
+        v[4 * j + 3] = hi[1];
+    }
+    return v;
+}
+__device__ __forceinline__ f16x8_t int4_values(uint32_t u) {
+    const f16x2_t bias = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
+    f16x8_t v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const f16x2_t p = __builtin_bit_cast(f16x2_t, ((u >> (4 * j)) & 0x000F000Fu) | 0x64006400u) - bias;
+        v[2 * j] = p[0];
+        v[2 * j + 1] = p[1];
+    }
+    return v;
+}
+__device__ __forceinline__ f16x8_t fp8_values(u32x2_t u) {
+    // e4m3 bits under fp16's exponent are the value times 2^-8, also below
+    // the least normal one; 2^8 brings it back exactly
+    const f16x2_t up = {static_cast<_Float16>(256.0f), static_cast<_Float16>(256.0f)};
+    f16x8_t v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint32_t x = u[j / 2] >> (16 * (j % 2));
+        const uint32_t pair = ((x & 0x7Fu) << 7) | ((x & 0x80u) << 8) | ((x & 0x7F00u) << 15) | ((x & 0x8000u) << 16);
+        const f16x2_t p = __builtin_bit_cast(f16x2_t, pair) * up;
+        v[2 * j] = p[0];
+        v[2 * j + 1] = p[1];
+    }
+    return v;
+}
+// Which of eight neighbouring values the j-th one is.
+template <int kFormat>
+__device__ __forceinline__ constexpr int code_order(int j) {
+    return kFormat == CHIMERA_CACHE_INT4 ? (j & 1) * 4 + j / 2 : j;
+}
+
+struct MaxsimArgs {
+    CacheView c;
+    const void* queries;
+    const int32_t* query_lens;
+    const int64_t* page_start;
+    const int32_t* doc_lens;
+    const int32_t* pages;
+    const int32_t* cand_ids;
+    const int32_t* cand_counts;
+    float* scores;
+    float* parts;  // [nq * cap][splits][query rows] maxima where documents are split
+    int64_t num_docs, num_page_entries;
+    int nq, query_len, cap;
+    int split_tokens, splits, max_tokens;
+};
+
+// One query tile of 32 tokens as matrix operand (rows: query tokens), in fp16
+// parts after a power of two per token that brings its largest value to
+// [0.5, 1); kParts 2 keeps 22 bits of 32-bit queries. A token past the end is
+// zeros.
+template <typename T, int kFormat, int kParts>
+struct QueryTile {
+    f16x8_t part[kParts][4][2];
+    float back;  // 2^e of the row that maxima_to_rows leaves in this lane
+
+    __device__ __forceinline__ void load(const T* q, int rows, int dim, int l) {
+        const int row = l & 31, half = l >> 5;
+        float x[4][16];
+        float most = 0.0f;
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const int at = 32 * g + 16 * half + j;
+                x[g][j] = row < rows && at < dim ? to_float(q[static_cast<int64_t>(row) * dim + at]) : 0.0f;
+                most = fmaxf(most, fabsf(x[g][j]));
+            }
+        most = fmaxf(most, __shfl_xor(most, 32, kWave));
+        int e = 0;
+        frexpf(most > 0.0f ? most : 1.0f, &e);
+        e = min(max(e, -126), 126);  // both powers of two are normal numbers
+        const float to = ldexpf(1.0f, -e);
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float v = x[g][8 * h + code_order<kFormat>(j)] * to;
+                    const _Float16 hi = static_cast<_Float16>(v);
+                    part[0][g][h][j] = hi;
+                    if constexpr (kParts == 2) part[1][g][h][j] = static_cast<_Float16>(v - static_cast<float>(hi));
+                }
+        back = __shfl(ldexpf(1.0f, e), row_of(l), kWave);
+    }
+    // The query row whose maximum lane l ends up with.
+    static __device__ __forceinline__ int row_of(int l) {
+        const int r = ((l >> 4) & 1) * 8 + ((l >> 3) & 1) * 4 + ((l >> 2) & 1) * 2 + ((l >> 1) & 1);
+        return 8 * (r >> 2) + 4 * (l >> 5) + (r & 3);
+    }
+};
+
+template <typename T, int kFormat>
+__global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
+    constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+    const int l = lane_id();
+    const int q = static_cast<int>(blockIdx.y);
+    const int item = static_cast<int>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(wave_id());
+    const int j = item / a.splits, split = item - j * a.splits;
+    if (j >= a.cap) return;
+    const int64_t at = static_cast<int64_t>(q) * a.cap + j;
+    const int count = a.cand_counts ? a.cand_counts[q] : a.cap;
+    const int doc = j < count ? a.cand_ids[at] : -1;
+    int len = 0;
+    int64_t first = 0;
+    if (doc >= 0 && doc < a.num_docs) {
+        len = min(a.doc_lens[doc], a.max_tokens);
+        first = a.page_start[doc];
+    }
+    const int t_begin = split * a.split_tokens, t_end = min(len, t_begin + a.split_tokens);
+    const int q_len = a.query_lens ? min(max(a.query_lens[q], 0), a.query_len) : a.query_len;
+    const int groups = (a.c.dim + 31) / 32;
+    const int half = l >> 5;
+    const int rows_padded = (a.query_len + 31) / 32 * 32;
+    float total = 0.0f;
+    for (int q0 = 0; q0 < rows_padded; q0 += 32) {
+        if (q0 >= q_len && q0 > 0) break;
+        QueryTile<T, kFormat, kParts> qt;
+        qt.load(static_cast<const T*>(a.queries) + (static_cast<int64_t>(q) * a.query_len + q0) * a.c.dim, q_len - q0,
+                a.c.dim, l);
+        float best[16];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) best[r] = -INFINITY;
+        for (int t0 = t_begin; t0 < t_end; t0 += 32) {
+            const int t = t0 + (l & 31);
+            const int64_t entry = first + (t >> a.c.page_log2);
+            int64_t slot = -1;
+            if (t < t_end && entry >= 0 && entry < a.num_page_entries) {
+                const int page = a.pages[entry];
+                if (page >= 0 && page < a.c.num_pages)
+                    slot = (static_cast<int64_t>(page) << a.c.page_log2) + (t & ((1 << a.c.page_log2) - 1));
+            }
+            const bool in = slot >= 0;
+            const int64_t from = in ? slot : 0;
+            const uint8_t* codes = a.c.codes + from * a.c.row_bytes;
+            const float* scales = a.c.scales + from * a.c.row_scales;
+            f32x16_t sum = {}, acc = {};
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                if (g >= groups) break;
+                f16x8_t v0, v1;
+                if constexpr (kFormat == CHIMERA_CACHE_INT4) {
+                    const u32x2_t u = *reinterpret_cast<const u32x2_t*>(codes + 16 * g + 8 * half);
+                    v0 = int4_values(u[0]);
+                    v1 = int4_values(u[1]);
+                } else {
+                    const u32x4_t u = *reinterpret_cast<const u32x4_t*>(codes + 32 * g + 16 * half);
+                    v0 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[0], u[1]}) : fp8_values(u32x2_t{u[0], u[1]});
+                    v1 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[2], u[3]}) : fp8_values(u32x2_t{u[2], u[3]});
+                }
+#pragma unroll
+                for (int s = 0; s < kParts; ++s) {
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qt.part[s][g][0], v0, acc, 0, 0, 0);
+                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qt.part[s][g][1], v1, acc, 0, 0, 0);
+                }
+                // the end of a scale's group
+                if (((g + 1) & ((1 << (a.c.group_log2 - 5)) - 1)) == 0 || g + 1 == groups) {
+                    const float scale = scales[g >> (a.c.group_log2 - 5)];
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        sum[r] = fmaf(acc[r], scale, sum[r]);
+                        acc[r] = 0.0f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) best[r] = fmaxf(best[r], in ? sum[r] : -INFINITY);
+        }
+        // the maxima over the 32 tokens of the lanes, each step leaving a lane
+        // half of the rows
+#pragma unroll
+        for (int o = 16, keep = 8; o >= 2; o >>= 1, keep >>= 1) {
+            const bool upper = (l & o) != 0;
+#pragma unroll
+            for (int r = 0; r < keep; ++r) {
+                const float mine = upper ? best[r + keep] : best[r], theirs = upper ? best[r] : best[r + keep];
+                best[r] = fmaxf(mine, __shfl_xor(theirs, o, kWave));
+            }
+        }
+        best[0] = fmaxf(best[0], __shfl_xor(best[0], 1, kWave)) * qt.back;
+        const int row = QueryTile<T, kFormat, kParts>::row_of(l);
+        if (a.splits > 1) {
+            if ((l & 1) == 0) a.parts[(at * a.splits + split) * rows_padded + q0 + row] = best[0];
+            continue;
+        }
+        float s = (l & 1) == 0 && q0 + row < q_len ? best[0] : 0.0f;
+#pragma unroll
+        for (int o = 2; o < kWave; o <<= 1) s += __shfl_xor(s, o, kWave);
+        total += s;
+    }
+    if (a.splits > 1) return;
+    if (l == 0) a.scores[at] = len > 0 ? total : -INFINITY;
+}
+
+// The parts of split documents: a wave a candidate, a lane a query token.
+__global__ __launch_bounds__(256) void cache_maxsim_join_kernel(MaxsimArgs a) {
+    const int l = lane_id();
+    const int q = static_cast<int>(blockIdx.y);
+    const int j = static_cast<int>(blockIdx.x) * 4 + wave_id();
+    if (j >= a.cap) return;
+    const int64_t at = static_cast<int64_t>(q) * a.cap + j;
+    const int count = a.cand_counts ? a.cand_counts[q] : a.cap;
+    const int doc = j < count ? a.cand_ids[at] : -1;
+    const int len = doc >= 0 && doc < a.num_docs ? min(a.doc_lens[doc], a.max_tokens) : 0;
+    const int q_len = a.query_lens ? min(max(a.query_lens[q], 0), a.query_len) : a.query_len;
+    const int rows_padded = (a.query_len + 31) / 32 * 32;
+    const int parts = (len + a.split_tokens - 1) / a.split_tokens;
+    float s = 0.0f;
+    for (int i = l; i < q_len; i += kWave) {
+        float best = -INFINITY;
+        for (int p = 0; p < parts; ++p) best = fmaxf(best, a.parts[(at * a.splits + p) * rows_padded + i]);
+        s += best;
+    }
+#pragma unroll
+    for (int o = 1; o < kWave; o <<= 1) s += __shfl_xor(s, o, kWave);
+    if (l == 0) a.scores[at] = parts > 0 ? s : -INFINITY;
+}
+
+// The best k candidates of a query by score, ties to the larger id: one block
+// of 1,024 threads sorts them all.
+__global__ __launch_bounds__(1024) void cache_topk_kernel(const float* __restrict__ scores,
+                                                          const int32_t* __restrict__ ids,
+                                                          const int32_t* __restrict__ counts, int cap, int sort_cap, int k,
+                                                          int64_t* __restrict__ top_ids, float* __restrict__ top_scores,
+                                                          int32_t* __restrict__ top_counts) {
+    extern __shared__ uint64_t keys[];
+    const int64_t q = blockIdx.x;
+    const int n = counts ? min(max(counts[q], 0), cap) : cap;
+    for (int t = threadIdx.x; t < sort_cap; t += 1024) {
+        uint64_t key = ~0ull;
+        if (t < n) {
+            // descending (score, id) as an ascending key; the sign bit makes
+            // absent candidates' negative ids the smallest
+            const uint32_t id = static_cast<uint32_t>(ids[q * cap + t]) ^ 0x80000000u;
+            key = ~((static_cast<uint64_t>(float_to_ordered(scores[q * cap + t])) << 32) | id);
+        }
+        keys[t] = key;
+    }
+    __syncthreads();
+    block_sort_u64(keys, sort_cap);
+    for (int64_t t = threadIdx.x; t < k; t += 1024) {
+        const uint64_t v = t < n ? ~keys[t] : 0ull;
+        top_ids[q * k + t] = t < n ? static_cast<int32_t>(static_cast<uint32_t>(v) ^ 0x80000000u) : -1;
+        if (top_scores) top_scores[q * k + t] = t < n ? ordered_to_float(static_cast<uint32_t>(v >> 32)) : 0.0f;
+    }
+    if (threadIdx.x == 0) top_counts[q] = min(k, n);
+}
+
+// How documents are split: enough waves for the GPU where there are few
+// candidates, 128 tokens a part at least.
+struct Split {
+    int tokens, count;
+};
+Split split_of(const chimera_cache_maxsim& m) {
+    constexpr int64_t kWaves = 8192;
+    const int64_t docs = static_cast<int64_t>(m.nq) * m.cand_cap;
+    const int64_t longest = std::max(m.max_doc_tokens, 1);
+    const int64_t count = std::max<int64_t>(1, std::min(ceil_div(kWaves, std::max<int64_t>(docs, 1)), longest / 128));
+    Split s;
+    s.tokens = static_cast<int>(ceil_div(ceil_div(longest, count), 32) * 32);
+    s.count = static_cast<int>(ceil_div(longest, s.tokens));
+    return s;
+}
+
+template <typename Call>
+hipError_t by_format(int format, int type, Call&& call) {
+    auto by_type = [&](auto f) {
+        switch (type) {
+            case CHIMERA_F32: call(f, float{}); break;
+            case CHIMERA_F16: call(f, _Float16{}); break;
+            default: call(f, __bf16{}); break;
+        }
+    };
+    switch (format) {
+        case CHIMERA_CACHE_INT8: by_type(std::integral_constant<int, CHIMERA_CACHE_INT8>{}); break;
+        case CHIMERA_CACHE_INT4: by_type(std::integral_constant<int, CHIMERA_CACHE_INT4>{}); break;
+        default: by_type(std::integral_constant<int, CHIMERA_CACHE_FP8>{}); break;
+    }
+    return hipGetLastError();
+}
+
+bool aligned16(const void* p, int64_t stride, size_t elem) {
+    return (reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(stride) * elem) % 16 == 0;
+}
+
+}  // namespace
+
+hipError_t launch_cache_write(hipStream_t st, const chimera_cache& c, const void* rows, int type, int64_t stride,
+                              const int64_t* slots, int64_t n) {
+    const CacheView v = view_of(c);
+    const unsigned blocks = static_cast<unsigned>(ceil_div(n, 16));
+    const bool vec = aligned16(rows, stride, type_bytes(type));
+    return by_format(c.format, type, [&](auto f, auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((cache_write_kernel<T, decltype(f)::value>), dim3(blocks), dim3(256), 0, st, v,
+                           static_cast<const T*>(rows), stride, slots, n, vec);
+    });
+}
+
+hipError_t launch_cache_read(hipStream_t st, const chimera_cache& c, const int64_t* slots, int64_t n, void* out,
+                             int type, int64_t stride) {
+    const CacheView v = view_of(c);
+    const unsigned blocks = static_cast<unsigned>(ceil_div(n, 16));
+    const bool vec = aligned16(out, stride, type_bytes(type));
+    return by_format(c.format, type, [&](auto f, auto t) {
+        using T = decltype(t);
+        hipLaunchKernelGGL((cache_read_kernel<T, decltype(f)::value>), dim3(blocks), dim3(256), 0, st, v, slots, n,
+                           static_cast<T*>(out), stride, vec);
+    });
+}
+
+size_t cache_maxsim_workspace(const chimera_cache_maxsim& m) {
+    const Split s = split_of(m);
+    if (s.count <= 1) return 0;
+    return static_cast<size_t>(m.nq) * m.cand_cap * s.count * (ceil_div(m.query_len, 32) * 32) * sizeof(float);
+}
+
+hipError_t launch_cache_maxsim(hipStream_t st, const chimera_cache& c, const chimera_cache_maxsim& m) {
+    const Split s = split_of(m);
+    MaxsimArgs a = {};
+    a.c = view_of(c);
+    a.queries = m.queries;
+    a.query_lens = m.query_lens;
+    a.page_start = m.page_start;
+    a.doc_lens = m.doc_lens;
+    a.pages = m.pages;
+    a.cand_ids = m.cand_ids;
+    a.cand_counts = m.cand_counts;
+    a.scores = m.scores;
+    a.parts = static_cast<float*>(m.workspace);
+    a.num_docs = m.num_docs;
+    a.num_page_entries = m.num_page_entries;
+    a.nq = m.nq;
+    a.query_len = m.query_len;
+    a.cap = m.cand_cap;
+    a.split_tokens = s.tokens;
+    a.splits = s.count;
+    a.max_tokens = m.max_doc_tokens;
+    const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(m.cand_cap) * s.count, 4)),
+                    static_cast<unsigned>(m.nq));
+    hipError_t e = by_format(c.format, m.type, [&](auto f, auto t) {
+        hipLaunchKernelGGL((cache_maxsim_kernel<decltype(t), decltype(f)::value>), grid, dim3(256), 0, st, a);
+    });
+    if (e != hipSuccess) return e;
+    if (s.count > 1) hipLaunchKernelGGL(cache_maxsim_join_kernel, dim3(static_cast<unsigned>(ceil_div(m.cand_cap, 4)), static_cast<unsigned>(m.nq)),
+                       dim3(256), 0, st, a);
+    if (m.k > 0) {
+        // at least one key per thread of the block's merge sort
+        int sort_cap = 1024;
+        while (sort_cap < m.cand_cap) sort_cap *= 2;
+        hipLaunchKernelGGL(cache_topk_kernel, dim3(static_cast<unsigned>(m.nq)), dim3(1024), static_cast<size_t>(sort_cap) * 8,
+                           st, m.scores, m.cand_ids, m.cand_counts, m.cand_cap, sort_cap, m.k, m.top_ids, m.top_scores,
+                           m.top_counts);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace chimera

@@ -1,0 +1,861 @@
+// Dense layers that turn hidden states into token embeddings, forward and
+// backward (include/chimera_operators.h):
+//   Z = X W^T + b,  H = act(Z) + R,  Y = H or H / max(|H|, 1e-12)
+//   dH = dY or (dY - Y <Y, dY>) / norm,  dZ = dH act'(Z),
+//   dX = dZ W,  dW = dZ^T X,  db = sum of dZ's rows,  dR = dH
+// All three products are C = A B^T with both operands' rows along the summed
+// axis; the backward pass lays W, X and dZ out that way (transposed) first.
+#include "operators.hpp"
+
+#include <algorithm>
+
+namespace chimera {
+
+namespace {
+
+constexpr float kLeastNorm = 1e-12f;
+
+// ---- activations ---------------------------------------------------------------
+
+__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
+
+constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
+constexpr float kGeluTanhA = 0.044715f;
+
+__device__ __forceinline__ float activation(float z, int act) {
+    switch (act) {
+        case CHIMERA_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
+        case CHIMERA_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+        case CHIMERA_ACT_GELU_TANH:
+            return 0.5f * z * (1.0f + tanhf(kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z)));
+        case CHIMERA_ACT_SILU: return z * sigmoid(z);
+        default: return z;
+    }
+}
+
+__device__ __forceinline__ float activation_slope(float z, int act) {
+    switch (act) {
+        case CHIMERA_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
+        case CHIMERA_ACT_GELU:
+            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.3989422804014327f;
+        case CHIMERA_ACT_GELU_TANH: {
+            const float t = tanhf(kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
+            return 0.5f * (1.0f + t) +
+                   0.5f * z * (1.0f - t * t) * kGeluTanhC * fmaf(3.0f * kGeluTanhA * z, z, 1.0f);
+        }
+        case CHIMERA_ACT_SILU: {
+            const float s = sigmoid(z);
+            return s * fmaf(z, 1.0f - s, 1.0f);
+        }
+        default: return 1.0f;
+    }
+}
+
+// ---- eight neighbouring values of a row ----------------------------------------
+
+// `vec`: the eight lie within the row and at a multiple of 16 bytes (of 8
+// values of T); otherwise the first `count` of them one by one.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, int count, float (&v)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = a[j];
+                v[4 + j] = b[j];
+            }
+        } else {
+            T t[8];
+            *reinterpret_cast<u32x4_t*>(t) = *reinterpret_cast<const u32x4_t*>(p);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, bool vec, int count, const float (&v)[8]) {
+    if (vec) {
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
+        } else {
+            T t[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
+            *reinterpret_cast<u32x4_t*>(p) = *reinterpret_cast<const u32x4_t*>(t);
+        }
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+        if (j < count) p[j] = from_float<T>(v[j]);
+}
+
+// Whether rows of `stride` elements from p all start at multiples of 16 bytes.
+bool rows_aligned(const void* p, int64_t stride, size_t elem) {
+    return (reinterpret_cast<uintptr_t>(p) | (static_cast<uint64_t>(stride) * elem)) % 16 == 0;
+}
+
+// ---- what happens to a product's sums ------------------------------------------
+
+struct Epilogue {
+    const void* bias;
+    const void* residual;
+    void* y;
+    void* saved;
+    float* norms;
+    float* partial;  // [split][m][n] sums of a split product instead of all that follows
+    int64_t residual_stride, y_stride, saved_stride;
+    int64_t m;
+    int n;
+    int act;
+    bool out_f32, normalize;
+    bool residual_vec, y_vec, saved_vec;
+};
+
+// The layer's epilogue on eight neighbouring sums of one row; with
+// normalize the row lies in kLanes neighbouring lanes, which all call it.
+template <typename T, int kLanes>
+__device__ __forceinline__ void finish8(const Epilogue& e, int split, int64_t m, int n0, float (&v)[8]) {
+    const int count = m < e.m ? e.n - n0 : 0;  // may be <= 0
+    const bool whole = count >= 8;
+    if (e.partial) {
+        if (count > 0) store8(e.partial + (split * e.m + m) * e.n + n0, whole && e.y_vec, count, v);
+        return;
+    }
+    if (count > 0) {
+        if (e.bias) {
+            const T* b = static_cast<const T*>(e.bias) + n0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += j < count ? to_float(b[j]) : 0.0f;
+        }
+        if (e.saved) store8(static_cast<T*>(e.saved) + m * e.saved_stride + n0, whole && e.saved_vec, count, v);
+        if (e.act != CHIMERA_ACT_NONE) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = activation(v[j], e.act);
+        }
+        if (e.residual) {
+            float r[8];
+            load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n0, whole && e.residual_vec, count, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += r[j];
+        }
+    }
+    if (e.normalize) {
+        float s = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s = j < count ? fmaf(v[j], v[j], s) : s;
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) s += __shfl_xor(s, o, kWave);
+        const float norm = sqrtf(s);
+        const float held = norm < kLeastNorm ? kLeastNorm : norm;  // NaN stays
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] / held;
+        if (e.norms && n0 == 0 && count > 0) e.norms[m] = held;
+    }
+    if (count <= 0) return;
+    const int64_t at = m * e.y_stride + n0;
+    if (e.out_f32)
+        store8(static_cast<float*>(e.y) + at, whole && e.y_vec, count, v);
+    else
+        store8(static_cast<T*>(e.y) + at, whole && e.y_vec, count, v);
+}
+
+// ---- matrix-core steps ---------------------------------------------------------
+
+// One 16-byte chunk of a row of A and of B per lane: a 32 x 32 tile's product
+// over 32 bytes of the summed axis (lanes 0..31 hold the rows' first chunk,
+// lanes 32..63 the second). For 32-bit operands the four values of a chunk go
+// into four instructions; which index of the axis a lane's value has does not
+// matter as long as A and B agree.
+template <typename T>
+__device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, _Float16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+}
+// The same for a 16 x 16 tile over 64 bytes (lane / 16 is the chunk).
+template <typename T>
+__device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, _Float16)) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
+                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+    }
+}
+
+__device__ __forceinline__ __attribute__((address_space(3))) void* lds_at(void* p) {
+    return (__attribute__((address_space(3))) void*)(p);
+}
+
+// What lanes past the end of the summed axis load.
+__device__ __align__(256) unsigned char g_zero_chunk[256];
+
+struct Product {
+    const void* a;  // [m, k]
+    const void* b;  // [n, k]
+    int64_t a_stride, b_stride;  // bytes; rows at multiples of 16 bytes
+    int64_t m;
+    int n;
+    int64_t k_bytes;  // of a row, a multiple of 16
+    int tiles_m, tiles_n;
+    int steps, steps_per_split;  // of 128 bytes
+};
+
+// ---- tiled product -------------------------------------------------------------
+
+constexpr int kStepBytes = 128;  // of the summed axis per step: 64 or 32 values
+
+// C tile of BM x BN by WM x WN waves. Each step's rows of A and B (128 bytes
+// each) go straight from memory to one of two LDS buffers while the matrix
+// cores work on the other. Chunk c of row r lies at chunk place c ^ (r % 8),
+// so that the 8 lanes that an LDS read serves at a time hit different banks.
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, Epilogue e) {
+    constexpr int W = WM * WN;
+    constexpr int TM = BM / WM, TN = BN / WN;
+    constexpr int IM = TM / 32, IN = TN / 32;
+    constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // loads of 8 rows per wave and step
+    static_assert(LA * 8 * W == BM && LB * 8 * W == BN, "every wave loads the same number of rows");
+    constexpr int kBuffer = (BM + BN) * kStepBytes;
+    constexpr int kPitch = TN + 4;
+    constexpr int kStage = W * 32 * kPitch * 4;
+    __shared__ __align__(1024) unsigned char lds[2 * kBuffer > kStage ? 2 * kBuffer : kStage];
+
+    const int l = lane_id();
+    const int w = __builtin_amdgcn_readfirstlane(wave_id());
+    const int wm = w / WN, wn = w % WN;
+
+    // blocks go round the 8 XCDs; each XCD takes a run of tiles, in bands of
+    // 8 tiles of rows, so that its L2 serves a band's rows and columns
+    const int tiles = p.tiles_m * p.tiles_n;
+    const int id = static_cast<int>(blockIdx.x);
+    const int per = tiles / 8, rest = tiles % 8, xcd = id % 8;
+    const int t = xcd * per + (xcd < rest ? xcd : rest) + id / 8;
+    constexpr int kBand = 8;
+    const int band = t / (kBand * p.tiles_n);
+    const int height = min(kBand, p.tiles_m - band * kBand);
+    const int in_band = t - band * kBand * p.tiles_n;
+    const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % height) * BM;
+    const int n0 = in_band / height * BN;
+    const int split = static_cast<int>(blockIdx.y);
+    const int step0 = split * p.steps_per_split;
+    const int steps = min(p.steps_per_split, p.steps - step0);
+
+    // lane l loads chunk (l % 8) ^ (l / 8) of row l / 8 of its eight rows;
+    // rows past the end load the last row
+    const int chunk = (l & 7) ^ (l >> 3);
+    const char* base_a = static_cast<const char*>(p.a) + m0 * p.a_stride + static_cast<int64_t>(step0) * kStepBytes;
+    const char* base_b = static_cast<const char*>(p.b) + n0 * p.b_stride + static_cast<int64_t>(step0) * kStepBytes;
+    uint32_t off_a[LA], off_b[LB];
+    const int last_a = static_cast<int>(min(p.m - m0, static_cast<int64_t>(BM))) - 1, last_b = min(p.n - n0, BN) - 1;
+#pragma unroll
+    for (int i = 0; i < LA; ++i)
+        off_a[i] = static_cast<uint32_t>(min((i * W + w) * 8 + (l >> 3), last_a)) * static_cast<uint32_t>(p.a_stride) +
+                   16u * chunk;
+#pragma unroll
+    for (int i = 0; i < LB; ++i)
+        off_b[i] = static_cast<uint32_t>(min((i * W + w) * 8 + (l >> 3), last_b)) * static_cast<uint32_t>(p.b_stride) +
+                   16u * chunk;
+    auto fetch = [&](int s, unsigned char* to) {
+        const char* a = base_a + static_cast<int64_t>(s) * kStepBytes;
+        const char* b = base_b + static_cast<int64_t>(s) * kStepBytes;
+        const int64_t left = p.k_bytes - static_cast<int64_t>(step0 + s) * kStepBytes;
+        const bool zero = 16 * chunk >= left;
+#pragma unroll
+        for (int i = 0; i < LA; ++i) {
+            const void* src = a + off_a[i];
+            if (left < kStepBytes) src = zero ? static_cast<const void*>(g_zero_chunk) : src;
+            __builtin_amdgcn_global_load_lds(src, lds_at(to + (i * W + w) * 1024), 16, 0, 0);
+        }
+#pragma unroll
+        for (int i = 0; i < LB; ++i) {
+            const void* src = b + off_b[i];
+            if (left < kStepBytes) src = zero ? static_cast<const void*>(g_zero_chunk) : src;
+            __builtin_amdgcn_global_load_lds(src, lds_at(to + BM * kStepBytes + (i * W + w) * 1024), 16, 0, 0);
+        }
+    };
+
+    f32x16_t acc[IM][IN];
+#pragma unroll
+    for (int i = 0; i < IM; ++i)
+#pragma unroll
+        for (int j = 0; j < IN; ++j) acc[i][j] = f32x16_t{};
+
+    const uint32_t row_a = (wm * TM + (l & 31)) * kStepBytes, row_b = BM * kStepBytes + (wn * TN + (l & 31)) * kStepBytes;
+    auto compute = [&](const unsigned char* from) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            const uint32_t place = (((2 * s) ^ (l >> 5) ^ (l & 7)) << 4);
+            u32x4_t fa[IM], fb[IN];
+#pragma unroll
+            for (int i = 0; i < IM; ++i) fa[i] = *reinterpret_cast<const u32x4_t*>(from + row_a + i * 32 * kStepBytes + place);
+#pragma unroll
+            for (int j = 0; j < IN; ++j) fb[j] = *reinterpret_cast<const u32x4_t*>(from + row_b + j * 32 * kStepBytes + place);
+#pragma unroll
+            for (int i = 0; i < IM; ++i)
+#pragma unroll
+                for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(fa[i], fb[j], acc[i][j]);
+        }
+    };
+
+    fetch(0, lds);
+    for (int s = 0; s < steps; ++s) {
+        __syncthreads();  // this step's rows are in LDS, the other buffer is read
+        if (s + 1 < steps) fetch(s + 1, lds + ((s + 1) & 1) * kBuffer);
+        compute(lds + (s & 1) * kBuffer);
+    }
+    __syncthreads();
+
+    // D lane l holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4: through
+    // LDS into eight neighbouring columns a lane
+    float* stage = reinterpret_cast<float*>(lds) + w * 32 * kPitch;
+    constexpr int kLanes = TN / 8, kRows = kWave / kLanes;
+#pragma unroll
+    for (int i = 0; i < IM; ++i) {
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                stage[(8 * (r >> 2) + 4 * (l >> 5) + (r & 3)) * kPitch + 32 * j + (l & 31)] = acc[i][j][r];
+        wave_lds_sync();
+#pragma unroll
+        for (int q = 0; q < 32 / kRows; ++q) {
+            const int row = q * kRows + l / kLanes, col = l % kLanes * 8;
+            float v[8];
+            const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(stage + row * kPitch + col);
+            const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(stage + row * kPitch + col + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = lo[j];
+                v[4 + j] = hi[j];
+            }
+            finish8<T, kLanes>(e, split, m0 + wm * TM + 32 * i + row, n0 + wn * TN + col, v);
+        }
+        wave_lds_sync();
+    }
+}
+
+// ---- few rows ------------------------------------------------------------------
+
+// 16 rows of X against NT tiles of 16 rows of W; KW waves share the summed
+// axis of each tile and join in LDS. Every row of W is read by one wave
+// straight into registers, with no barrier before the join.
+template <typename T, int NT, int KW>
+__global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, Epilogue e, int k, bool aligned) {
+    constexpr int kCols = NT * 16;
+    constexpr int kPitch = kCols + 4;
+    __shared__ __align__(16) float part[KW][16][kPitch];
+    const int l = lane_id();
+    const int w = __builtin_amdgcn_readfirstlane(wave_id());
+    const int nt = w % NT, kw = w / NT;
+    const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16;
+    const int n0 = static_cast<int>(blockIdx.x) * kCols;
+    const int64_t row_x = min(m0 + (l & 15), p.m - 1);
+    const int row_w = min(n0 + nt * 16 + (l & 15), p.n - 1);
+    const char* x = static_cast<const char*>(p.a) + row_x * p.a_stride;
+    const char* wt = static_cast<const char*>(p.b) + row_w * p.b_stride;
+    constexpr int kPer = 16 / sizeof(T);  // values of a chunk
+    const int steps = (k + 4 * kPer - 1) / (4 * kPer);
+    const int share = (steps + KW - 1) / KW;
+    const int s_end = min(steps, (kw + 1) * share);
+    auto chunk = [&](const char* row, int s) {
+        const int at = (4 * s + (l >> 4)) * kPer;  // first value
+        u32x4_t v = {0, 0, 0, 0};
+        if (aligned) {
+            if (at < k) v = *reinterpret_cast<const u32x4_t*>(row + static_cast<int64_t>(at) * sizeof(T));
+        } else {
+            T t[kPer];
+#pragma unroll
+            for (int j = 0; j < kPer; ++j)
+                t[j] = at + j < k ? reinterpret_cast<const T*>(row)[at + j] : from_float<T>(0.0f);
+            v = *reinterpret_cast<const u32x4_t*>(t);
+        }
+        return v;
+    };
+    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s = kw * share; s < s_end; s += 4) {
+        u32x4_t a[4], b[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const bool in = s + u < s_end;
+            a[u] = in ? chunk(wt, s + u) : u32x4_t{0, 0, 0, 0};
+            b[u] = in ? chunk(x, s + u) : u32x4_t{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) acc = mma16<T>(a[u], b[u], acc);
+    }
+    // D lane l holds row l % 16 of X, columns 4 (l / 16) .. + 3 of the tile
+    *reinterpret_cast<f32x4_t*>(&part[kw][l & 15][nt * 16 + 4 * (l >> 4)]) = acc;
+    __syncthreads();
+    constexpr int kLanes = kCols / 8;
+    const int tid = static_cast<int>(threadIdx.x);
+    if (tid >= 16 * kLanes) return;
+    const int row = tid / kLanes, col = tid % kLanes * 8;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = part[0][row][col + j];
+#pragma unroll
+    for (int o = 1; o < KW; ++o)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += part[o][row][col + j];
+    finish8<T, kLanes>(e, 0, m0 + row, n0 + col, v);
+}
+
+// ---- layouts -------------------------------------------------------------------
+
+// dst [rows][dst_stride] = src, zeros from column `cols` on: rows of any
+// alignment laid out at multiples of 16 bytes.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_align_kernel(const T* __restrict__ src, int64_t src_stride, int64_t rows,
+                                                           int cols, T* __restrict__ dst, int dst_cols) {
+    constexpr int kPer = 16 / sizeof(T);
+    const int chunks = dst_cols / kPer;
+    const int64_t total = rows * chunks;
+    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+        const int64_t r = i / chunks;
+        const int c = static_cast<int>(i - r * chunks) * kPer;
+        T t[kPer];
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) t[j] = c + j < cols ? src[r * src_stride + c + j] : from_float<T>(0.0f);
+        *reinterpret_cast<u32x4_t*>(dst + r * dst_cols + c) = *reinterpret_cast<const u32x4_t*>(t);
+    }
+}
+
+// dst [cols][dst_cols] = src^T, zeros from column `rows` on; dst_cols a
+// multiple of 64. A block takes 64 x 64 values.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_transpose_kernel(const T* __restrict__ src, int64_t src_stride,
+                                                               int64_t rows, int cols, T* __restrict__ dst,
+                                                               int64_t dst_cols) {
+    __shared__ T tile[64][65];
+    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
+    const int c0 = static_cast<int>(blockIdx.y) * 64;
+    const int x = static_cast<int>(threadIdx.x) & 63, y = static_cast<int>(threadIdx.x) >> 6;
+#pragma unroll 4
+    for (int i = y; i < 64; i += 4)
+        tile[i][x] = r0 + i < rows && c0 + x < cols ? src[(r0 + i) * src_stride + c0 + x] : from_float<T>(0.0f);
+    __syncthreads();
+#pragma unroll 4
+    for (int i = y; i < 64; i += 4)
+        if (c0 + i < cols) dst[static_cast<int64_t>(c0 + i) * dst_cols + r0 + x] = tile[x][i];
+}
+
+// ---- the gradient before the products ------------------------------------------
+
+struct GradArgs {
+    const void* dy;
+    const void* y;
+    const void* saved;
+    const float* norms;
+    void* dresidual;
+    void* g;    // dZ [m][g_cols], zeros from column n on, or NULL
+    void* gt;   // dZ^T [n][gt_cols], zeros from column m on, or NULL
+    float* sums;  // column sums of dZ by blocks of 64 rows [blocks][n], or NULL
+    int64_t dy_stride, y_stride, saved_stride, dresidual_stride, gt_cols;
+    int64_t m;
+    int n, g_cols, act;
+    bool out_f32, normalize, dy_vec, y_vec, saved_vec, dresidual_vec;
+};
+
+// 64 rows x 128 columns a block, eight neighbouring columns of four rows a
+// thread: with normalize (n <= 128) a row is 16 neighbouring lanes.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
+    __shared__ T tile[64][129];
+    __shared__ float sums[16][129];
+    const int tid = static_cast<int>(threadIdx.x);
+    const int col = tid % 16 * 8, n0 = static_cast<int>(blockIdx.y) * 128 + col;
+    const int64_t m0 = static_cast<int64_t>(blockIdx.x) * 64;
+    float sum[8] = {};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = tid / 16 + 16 * i;
+        const int64_t m = m0 + row;
+        const int count = m < a.m ? a.n - n0 : 0;
+        const bool whole = count >= 8;
+        float g[8] = {};
+        auto load = [&](const void* p, int64_t stride, bool vec, float(&v)[8]) {
+            if (a.out_f32)
+                load8(static_cast<const float*>(p) + m * stride + n0, whole && vec, count, v);
+            else
+                load8(static_cast<const T*>(p) + m * stride + n0, whole && vec, count, v);
+        };
+        if (count > 0) load(a.dy, a.dy_stride, a.dy_vec, g);
+        if (a.normalize) {
+            float y[8] = {};
+            if (count > 0) load(a.y, a.y_stride, a.y_vec, y);
+            float dot = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) dot = fmaf(y[j], g[j], dot);
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) dot += __shfl_xor(dot, o, kWave);
+            const float norm = count > 0 ? a.norms[m] : 1.0f;
+            // at its least value the norm is a constant
+            dot = norm > kLeastNorm ? dot : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] = fmaf(-y[j], dot, g[j]) / norm;
+        }
+        if (a.dresidual && count > 0)
+            store8(static_cast<T*>(a.dresidual) + m * a.dresidual_stride + n0, whole && a.dresidual_vec, count, g);
+        if (a.act != CHIMERA_ACT_NONE && count > 0) {
+            float z[8];
+            load8(static_cast<const T*>(a.saved) + m * a.saved_stride + n0, whole && a.saved_vec, count, z);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) g[j] = j < count ? g[j] * activation_slope(z[j], a.act) : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sum[j] += g[j];
+        if (a.g && m < a.m && n0 < a.g_cols) store8(static_cast<T*>(a.g) + m * a.g_cols + n0, true, 8, g);
+        if (a.gt) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) tile[row][col + j] = from_float<T>(g[j]);
+        }
+    }
+    if (a.sums) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[tid / 16][col + j] = sum[j];
+    }
+    __syncthreads();
+    const int nb = static_cast<int>(blockIdx.y) * 128;
+    if (a.sums && tid < 128 && nb + tid < a.n) {
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += sums[i][tid];
+        a.sums[static_cast<int64_t>(blockIdx.x) * a.n + nb + tid] = s;
+    }
+    if (a.gt) {
+        for (int i = tid; i < 128 * 64; i += 256) {
+            const int c = i / 64, r = i % 64;
+            if (nb + c < a.n) static_cast<T*>(a.gt)[static_cast<int64_t>(nb + c) * a.gt_cols + m0 + r] = tile[r][c];
+        }
+    }
+}
+
+// dst[i] = sum over s of src[s][i], in order, for i < count: the parts of a
+// split product (rows of `cols` values to rows of dst_stride) or the blocks'
+// column sums. Four waves share the parts of 64 values.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ src, int64_t parts, int64_t count,
+                                                          int cols, T* __restrict__ dst, int64_t dst_stride) {
+    __shared__ float sums[4][kWave];
+    const int l = lane_id(), w = wave_id();
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kWave + l;
+    const int64_t share = (parts + 3) / 4;
+    float s = 0.0f;
+    if (i < count) {
+        const int64_t end = min(parts, (w + 1) * share);
+        for (int64_t k = w * share; k < end; ++k) s += src[k * count + i];
+    }
+    sums[w][l] = s;
+    __syncthreads();
+    if (w != 0 || i >= count) return;
+    s = ((sums[0][l] + sums[1][l]) + sums[2][l]) + sums[3][l];
+    dst[i / cols * dst_stride + i % cols] = from_float<T>(s);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void linear_zero_kernel(T* dst, int64_t rows, int cols, int64_t stride) {
+    const int64_t i = blockIdx.x * 256ll + threadIdx.x;
+    if (i < rows * cols) dst[i / cols * stride + i % cols] = from_float<T>(0.0f);
+}
+
+// ---- plans ---------------------------------------------------------------------
+
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
+
+// Arrays one after the other at multiples of 256 bytes.
+struct Carve {
+    char* base;
+    size_t off = 0;
+    void* take(size_t bytes) {
+        off = (off + 255) / 256 * 256;
+        void* p = base ? base + off : nullptr;
+        off += bytes;
+        return p;
+    }
+};
+
+constexpr int kNormalizeCols = 128;
+// Rows up to which a product without a split goes by 16 rows a block.
+constexpr int64_t kFewRows = 64;
+
+template <typename T>
+void launch_tiles(hipStream_t st, Product p, Epilogue e, int splits) {
+    p.steps = static_cast<int>(ceil_div(p.k_bytes, kStepBytes));
+    p.steps_per_split = static_cast<int>(ceil_div(p.steps, splits));
+    splits = static_cast<int>(ceil_div(p.steps, p.steps_per_split));
+    auto plan = [&](int bm, int bn) {
+        p.tiles_m = static_cast<int>(ceil_div(p.m, bm));
+        p.tiles_n = static_cast<int>(ceil_div(p.n, bn));
+        return dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n), static_cast<unsigned>(splits));
+    };
+    if (e.normalize) {
+        const dim3 grid = plan(128, 128);
+        hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, 1>), grid, dim3(256), 0, st, p, e);
+        return;
+    }
+    if (ceil_div(p.m, 256) * ceil_div(p.n, 256) * splits >= 256) {
+        const dim3 grid = plan(256, 256);
+        hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, p, e);
+        return;
+    }
+    const dim3 grid = plan(128, 128);
+    hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, p, e);
+}
+
+// A matrix as a product reads it: as it lies where its rows start at
+// multiples of 16 bytes and end at one, else laid out again in `copy`
+// (rows x round_up(cols, 64)).
+template <typename T>
+void aligned_rows(hipStream_t st, const void* src, int64_t stride, int64_t rows, int cols, void* copy, const void** p,
+                  int64_t* stride_bytes, int64_t* k_bytes) {
+    constexpr int64_t kMostStride = int64_t{1} << 22;  // a tile's rows within 32-bit offsets
+    if (rows_aligned(src, stride, sizeof(T)) && cols * sizeof(T) % 16 == 0 && stride * static_cast<int64_t>(sizeof(T)) <= kMostStride) {
+        *p = src;
+        *stride_bytes = stride * static_cast<int64_t>(sizeof(T));
+        *k_bytes = cols * static_cast<int64_t>(sizeof(T));
+        return;
+    }
+    const int wide = static_cast<int>(round_up(cols, 64));
+    const int64_t chunks = rows * (wide * static_cast<int64_t>(sizeof(T)) / 16);
+    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(chunks, 256), 65536));
+    hipLaunchKernelGGL((linear_align_kernel<T>), dim3(blocks), dim3(256), 0, st, static_cast<const T*>(src), stride, rows,
+                       cols, static_cast<T*>(copy), wide);
+    *p = copy;
+    *stride_bytes = wide * static_cast<int64_t>(sizeof(T));
+    *k_bytes = *stride_bytes;
+}
+
+struct ForwardPlan {
+    void* x;
+    void* weight;
+};
+size_t carve_forward(const chimera_linear_shape& s, void* base, ForwardPlan* plan) {
+    Carve c{static_cast<char*>(base)};
+    const size_t wide = round_up(s.in_features, 64) * type_bytes(s.type);
+    plan->x = c.take(static_cast<size_t>(s.rows) * wide);
+    plan->weight = c.take(static_cast<size_t>(s.out_features) * wide);
+    return c.off;
+}
+
+template <typename T>
+hipError_t forward(hipStream_t st, const LinearForward& f) {
+    const auto& s = f.s;
+    const auto& a = f.a;
+    const size_t out = s.out_type == CHIMERA_F32 ? 4 : sizeof(T);
+    Epilogue e = {};
+    e.bias = a.bias;
+    e.residual = a.residual;
+    e.y = a.y;
+    e.saved = a.saved;
+    e.norms = a.norms;
+    e.residual_stride = a.residual_stride;
+    e.y_stride = a.y_stride;
+    e.saved_stride = a.saved_stride;
+    e.m = s.rows;
+    e.n = s.out_features;
+    e.act = s.activation;
+    e.out_f32 = out == 4;
+    e.normalize = s.normalize != 0;
+    e.residual_vec = rows_aligned(a.residual, a.residual_stride, sizeof(T));
+    e.y_vec = rows_aligned(a.y, a.y_stride, out);
+    e.saved_vec = rows_aligned(a.saved, a.saved_stride, sizeof(T));
+    Product p = {};
+    p.m = s.rows;
+    p.n = s.out_features;
+    if (s.rows <= kFewRows) {
+        p.a = a.x;
+        p.b = a.weight;
+        p.a_stride = a.x_stride * static_cast<int64_t>(sizeof(T));
+        p.b_stride = a.weight_stride * static_cast<int64_t>(sizeof(T));
+        const bool aligned = rows_aligned(a.x, a.x_stride, sizeof(T)) && rows_aligned(a.weight, a.weight_stride, sizeof(T)) &&
+                             s.in_features * sizeof(T) % 16 == 0;
+        const unsigned by = static_cast<unsigned>(ceil_div(s.rows, 16));
+        if (e.normalize)
+            hipLaunchKernelGGL((linear_rows_kernel<T, 8, 2>), dim3(1, by), dim3(1024), 0, st, p, e, s.in_features, aligned);
+        else
+            hipLaunchKernelGGL((linear_rows_kernel<T, 1, 8>), dim3(static_cast<unsigned>(ceil_div(s.out_features, 16)), by),
+                               dim3(512), 0, st, p, e, s.in_features, aligned);
+        return hipGetLastError();
+    }
+    ForwardPlan plan;
+    (void)carve_forward(s, a.workspace, &plan);
+    int64_t k_x = 0, k_w = 0;
+    aligned_rows<T>(st, a.x, a.x_stride, s.rows, s.in_features, plan.x, &p.a, &p.a_stride, &k_x);
+    aligned_rows<T>(st, a.weight, a.weight_stride, s.out_features, s.in_features, plan.weight, &p.b, &p.b_stride, &k_w);
+    p.k_bytes = std::min(k_x, k_w);
+    launch_tiles<T>(st, p, e, 1);
+    return hipGetLastError();
+}
+
+struct BackwardPlan {
+    int64_t m_pad;
+    int n_pad;
+    int splits;
+    void *g, *gt, *xt, *wt;
+    float *sums, *parts;
+};
+
+// Parts of dW's sum over the rows: enough blocks of 128 x 128 for the GPU,
+// eight steps of 64 rows a part at least.
+int dweight_splits(const chimera_linear_shape& s) {
+    const int64_t tiles = ceil_div(s.out_features, 128) * ceil_div(s.in_features, 128);
+    const int64_t steps = ceil_div(round_up(s.rows, 64) * type_bytes(s.type), kStepBytes);
+    return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(512, tiles), steps / 8)));
+}
+
+size_t carve_backward(const chimera_linear_shape& s, void* base, BackwardPlan* plan) {
+    Carve c{static_cast<char*>(base)};
+    const size_t e = type_bytes(s.type);
+    plan->m_pad = round_up(s.rows, 64);
+    plan->n_pad = static_cast<int>(round_up(s.out_features, 64));
+    plan->splits = dweight_splits(s);
+    const size_t k = static_cast<size_t>(s.in_features), n = static_cast<size_t>(s.out_features);
+    plan->g = c.take(static_cast<size_t>(s.rows) * plan->n_pad * e);
+    plan->gt = c.take(n * plan->m_pad * e);
+    plan->xt = c.take(k * plan->m_pad * e);
+    plan->wt = c.take(k * plan->n_pad * e);
+    plan->sums = static_cast<float*>(c.take(static_cast<size_t>(plan->m_pad / 64) * n * 4));
+    plan->parts = static_cast<float*>(c.take(plan->splits > 1 ? plan->splits * n * k * 4 : 0));
+    return c.off;
+}
+
+template <typename T>
+hipError_t backward(hipStream_t st, const LinearBackward& b) {
+    const auto& s = b.s;
+    const auto& a = b.a;
+    const int n = s.out_features, k = s.in_features;
+    auto zero = [&](void* dst, int64_t rows, int cols, int64_t stride) {
+        hipLaunchKernelGGL((linear_zero_kernel<T>), dim3(static_cast<unsigned>(ceil_div(rows * cols, 256))), dim3(256), 0,
+                           st, static_cast<T*>(dst), rows, cols, stride);
+    };
+    if (s.rows == 0) {
+        if (a.dweight) zero(a.dweight, n, k, a.dweight_stride);
+        if (a.dbias) zero(a.dbias, 1, n, n);
+        return hipGetLastError();
+    }
+    BackwardPlan plan;
+    (void)carve_backward(s, a.workspace, &plan);
+    const size_t out = s.out_type == CHIMERA_F32 ? 4 : sizeof(T);
+    const unsigned row_blocks = static_cast<unsigned>(plan.m_pad / 64);
+    GradArgs g = {};
+    g.dy = a.dy;
+    g.y = a.y;
+    g.saved = a.saved;
+    g.norms = a.norms;
+    g.dresidual = a.dresidual;
+    g.g = a.dx ? plan.g : nullptr;
+    g.gt = a.dweight ? plan.gt : nullptr;
+    g.sums = a.dbias ? plan.sums : nullptr;
+    g.dy_stride = a.dy_stride;
+    g.y_stride = a.y_stride;
+    g.saved_stride = a.saved_stride;
+    g.dresidual_stride = a.dresidual_stride;
+    g.gt_cols = plan.m_pad;
+    g.m = s.rows;
+    g.n = n;
+    g.g_cols = plan.n_pad;
+    g.act = s.activation;
+    g.out_f32 = out == 4;
+    g.normalize = s.normalize != 0;
+    g.dy_vec = rows_aligned(a.dy, a.dy_stride, out);
+    g.y_vec = rows_aligned(a.y, a.y_stride, out);
+    g.saved_vec = rows_aligned(a.saved, a.saved_stride, sizeof(T));
+    g.dresidual_vec = rows_aligned(a.dresidual, a.dresidual_stride, sizeof(T));
+    hipLaunchKernelGGL((linear_grad_kernel<T>), dim3(row_blocks, static_cast<unsigned>(ceil_div(n, 128))), dim3(256), 0, st, g);
+    auto join = [&](const float* src, int64_t parts, int64_t count, int cols, void* dst, int64_t stride) {
+        hipLaunchKernelGGL((linear_join_kernel<T>), dim3(static_cast<unsigned>(ceil_div(count, kWave))), dim3(256), 0, st,
+                           src, parts, count, cols, static_cast<T*>(dst), stride);
+    };
+    if (a.dbias) join(plan.sums, row_blocks, n, n, a.dbias, n);
+    auto product = [&](const void* pa, int64_t m, int64_t sum, const void* pb, int cols, void* dst, int64_t stride,
+                       int splits) {
+        Product p = {};
+        p.a = pa;
+        p.b = pb;
+        p.a_stride = p.b_stride = p.k_bytes = sum * static_cast<int64_t>(sizeof(T));
+        p.m = m;
+        p.n = cols;
+        Epilogue e = {};
+        e.y = dst;
+        e.y_stride = stride;
+        e.m = m;
+        e.n = cols;
+        e.out_f32 = sizeof(T) == 4;
+        e.y_vec = rows_aligned(dst, stride, sizeof(T));
+        if (splits > 1) {
+            e.partial = plan.parts;
+            e.y_vec = cols % 4 == 0;
+        }
+        launch_tiles<T>(st, p, e, splits);
+        if (splits > 1) {
+            const int64_t steps = ceil_div(p.k_bytes, kStepBytes);
+            join(plan.parts, ceil_div(steps, ceil_div(steps, splits)), m * cols, cols, dst, stride);
+        }
+    };
+    if (a.dx) {
+        hipLaunchKernelGGL((linear_transpose_kernel<T>),
+                           dim3(static_cast<unsigned>(plan.n_pad / 64), static_cast<unsigned>(ceil_div(k, 64))), dim3(256),
+                           0, st, static_cast<const T*>(a.weight), a.weight_stride, static_cast<int64_t>(n), k,
+                           static_cast<T*>(plan.wt), static_cast<int64_t>(plan.n_pad));
+        product(plan.g, s.rows, plan.n_pad, plan.wt, k, a.dx, a.dx_stride, 1);
+    }
+    if (a.dweight) {
+        hipLaunchKernelGGL((linear_transpose_kernel<T>), dim3(row_blocks, static_cast<unsigned>(ceil_div(k, 64))), dim3(256),
+                           0, st, static_cast<const T*>(a.x), a.x_stride, s.rows, k, static_cast<T*>(plan.xt), plan.m_pad);
+        product(plan.gt, n, plan.m_pad, plan.xt, k, a.dweight, a.dweight_stride, plan.splits);
+    }
+    return hipGetLastError();
+}
+
+template <typename Call>
+hipError_t by_type(int type, Call&& call) {
+    switch (type) {
+        case CHIMERA_F32: return call(float{});
+        case CHIMERA_F16: return call(_Float16{});
+        default: return call(__bf16{});
+    }
+}
+
+}  // namespace
+
+size_t linear_forward_workspace(const chimera_linear_shape& s) {
+    ForwardPlan plan;
+    return carve_forward(s, nullptr, &plan);
+}
+size_t linear_backward_workspace(const chimera_linear_shape& s) {
+    BackwardPlan plan;
+    return carve_backward(s, nullptr, &plan);
+}
+
+hipError_t launch_linear_forward(hipStream_t st, const LinearForward& f) {
+    return by_type(f.s.type, [&](auto t) { return forward<decltype(t)>(st, f); });
+}
+hipError_t launch_linear_backward(hipStream_t st, const LinearBackward& b) {
+    return by_type(b.s.type, [&](auto t) { return backward<decltype(t)>(st, b); });
+}
+
+}  // namespace chimera

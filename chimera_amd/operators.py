@@ -1,0 +1,286 @@
+"""The operators beside the index (include/chimera_operators.h): dense layers
+that turn hidden states into token embeddings, a quantised cache of token
+embeddings and late interaction on it, and a store of documents that come and
+go on top of the cache.
+
+Arrays are device arrays: capi.DeviceArray, or any object with `ptr`, `shape`
+and `dtype` ("f32", "f16", "bf16", a numpy dtype or its name) and, for a
+matrix whose rows lie apart, `stride` in elements. Calls are asynchronous on
+the context's stream.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+from . import capi
+from .capi import P, check
+
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+FORMATS = {"int8": 0, "int4": 1, "fp8": 2}
+_NAMES = {"f32": "f32", "f16": "f16", "bf16": "bf16", "float32": "f32", "float16": "f16", "bfloat16": "bf16"}
+
+
+class LinearShape(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("in_features", C.c_int32), ("out_features", C.c_int32), ("type", C.c_int32),
+                ("out_type", C.c_int32), ("activation", C.c_int32), ("normalize", C.c_int32)]
+
+
+class LinearForward(C.Structure):
+    _fields_ = [("x", P), ("weight", P), ("bias", P), ("residual", P), ("y", P), ("saved", P), ("norms", P),
+                ("x_stride", C.c_int64), ("weight_stride", C.c_int64), ("residual_stride", C.c_int64),
+                ("y_stride", C.c_int64), ("saved_stride", C.c_int64), ("workspace", P), ("workspace_bytes", C.c_size_t)]
+
+
+class LinearBackward(C.Structure):
+    _fields_ = [("x", P), ("weight", P), ("dy", P), ("saved", P), ("y", P), ("norms", P), ("dx", P), ("dweight", P),
+                ("dbias", P), ("dresidual", P), ("x_stride", C.c_int64), ("weight_stride", C.c_int64),
+                ("dy_stride", C.c_int64), ("saved_stride", C.c_int64), ("y_stride", C.c_int64),
+                ("dx_stride", C.c_int64), ("dweight_stride", C.c_int64), ("dresidual_stride", C.c_int64),
+                ("workspace", P), ("workspace_bytes", C.c_size_t)]
+
+
+class CacheDesc(C.Structure):
+    _fields_ = [("format", C.c_int32), ("dim", C.c_int32), ("group", C.c_int32), ("page_tokens", C.c_int32),
+                ("num_pages", C.c_int64), ("codes", P), ("scales", P)]
+
+
+class CacheMaxsim(C.Structure):
+    _fields_ = [("queries", P), ("type", C.c_int32), ("nq", C.c_int32), ("query_len", C.c_int32), ("query_lens", P),
+                ("page_start", P), ("doc_lens", P), ("pages", P), ("num_docs", C.c_int64),
+                ("num_page_entries", C.c_int64), ("max_doc_tokens", C.c_int32), ("cand_ids", P), ("cand_counts", P),
+                ("cand_cap", C.c_int32), ("scores", P), ("k", C.c_int32), ("top_ids", P), ("top_scores", P),
+                ("top_counts", P), ("workspace", P), ("workspace_bytes", C.c_size_t)]
+
+
+def _type_name(a) -> str:
+    if getattr(a, "bf16", False):
+        return "bf16"
+    name = a.dtype if isinstance(a.dtype, str) else np.dtype(a.dtype).name
+    return _NAMES.get(name, name)
+
+
+def _type(a, what: str) -> int:
+    t = TYPES.get(_type_name(a))
+    if t is None:
+        raise ValueError(f"{what} must be f32, f16 or bf16, not {_type_name(a)}")
+    return t
+
+
+def _expect(a, what: str, shape: tuple, type_name: str) -> None:
+    if tuple(a.shape) != shape:
+        raise ValueError(f"{what} must have shape {shape}, not {tuple(a.shape)}")
+    if _type_name(a) != type_name:
+        raise ValueError(f"{what} must be {type_name}, not {_type_name(a)}")
+
+
+def _stride(a) -> int:
+    s = getattr(a, "stride", None)
+    return a.shape[-1] if s is None else s
+
+
+def _ptr(a):
+    return None if a is None else a.ptr
+
+
+class Linear:
+    """One dense layer, Y = act(X W^T + b) + R, divided row by row by its
+    length with `normalize` (at most 128 outputs). weight [out, in] and bias
+    [out] stay the caller's arrays and may change between calls. The object
+    holds the workspace for calls of up to max_rows rows, and with `training`
+    for the backward pass."""
+
+    def __init__(self, ctx: capi.Context, weight, bias=None, activation: str = "none", normalize: bool = False,
+                 max_rows: int = 1, training: bool = False):
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}")
+        if len(weight.shape) != 2:
+            raise ValueError("weight must be [out_features, in_features]")
+        self.ctx = ctx
+        self.weight, self.bias = weight, bias
+        self.out_features, self.in_features = weight.shape
+        self.type = _type_name(weight)
+        t = _type(weight, "weight")
+        if bias is not None:
+            _expect(bias, "bias", (self.out_features,), self.type)
+        self.training = training
+        self._shape = LinearShape(0, self.in_features, self.out_features, t, t, ACTIVATIONS[activation], int(normalize))
+        self._forward = LinearForward(weight=weight.ptr, bias=_ptr(bias), weight_stride=_stride(weight))
+        self._backward = LinearBackward(weight=weight.ptr, weight_stride=_stride(weight))
+        self._workspace = None
+        need = C.c_size_t()
+        self._shape.rows = max_rows
+        check(capi.lib().chimera_linear_workspace(C.byref(self._shape), int(training), C.byref(need)))
+        if need.value:
+            self._workspace = ctx.empty(need.value, np.uint8)
+            for args in (self._forward, self._backward):
+                args.workspace, args.workspace_bytes = self._workspace.ptr, need.value
+
+    def close(self) -> None:
+        if getattr(self, "_workspace", None) is not None:
+            self.ctx.synchronize()
+            self._workspace.free()
+            self._workspace = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _rows(self, x, y, what: str) -> int:
+        rows = x.shape[0]
+        if tuple(y.shape) != (rows, self.out_features):
+            raise ValueError(f"{what} must have shape {(rows, self.out_features)}, not {tuple(y.shape)}")
+        self._shape.rows, self._shape.out_type = rows, _type(y, what)
+        return rows
+
+    def forward(self, x, y, residual=None, saved=None, norms=None) -> None:
+        """y [rows, out] (the layer's type or f32) from x [rows, in]. For the
+        backward pass, `saved` [rows, out] gets the sums before the activation
+        and `norms` [rows] f32 the lengths."""
+        rows = self._rows(x, y, "y")
+        _expect(x, "x", (rows, self.in_features), self.type)
+        a = self._forward
+        a.x, a.x_stride, a.y, a.y_stride = x.ptr, _stride(x), y.ptr, _stride(y)
+        a.residual = a.saved = a.norms = None
+        if residual is not None:
+            _expect(residual, "residual", (rows, self.out_features), self.type)
+            a.residual, a.residual_stride = residual.ptr, _stride(residual)
+        if saved is not None:
+            _expect(saved, "saved", (rows, self.out_features), self.type)
+            a.saved, a.saved_stride = saved.ptr, _stride(saved)
+        if norms is not None:
+            _expect(norms, "norms", (rows,), "f32")
+            a.norms = norms.ptr
+        check(capi.lib().chimera_linear_forward_device(self.ctx.handle, C.byref(self._shape), C.byref(a)))
+
+    def backward(self, x, dy, saved=None, y=None, norms=None, dx=None, dweight=None, dbias=None,
+                 dresidual=None) -> None:
+        """Gradients from dy [rows, out]; those left out are not computed.
+        `saved` is read with an activation, `y` and `norms` with normalize, as
+        forward() left them."""
+        if not self.training:
+            raise ValueError("the layer was made without training")
+        rows = self._rows(x, dy, "dy")
+        n, k, t = self.out_features, self.in_features, self.type
+        _expect(x, "x", (rows, k), t)
+        a = self._backward
+        a.x, a.x_stride, a.dy, a.dy_stride = x.ptr, _stride(x), dy.ptr, _stride(dy)
+        for name, v, shape, kind in (("saved", saved, (rows, n), t), ("y", y, (rows, n), _type_name(dy)),
+                                     ("norms", norms, (rows,), "f32"), ("dx", dx, (rows, k), t),
+                                     ("dweight", dweight, (n, k), t), ("dbias", dbias, (n,), t),
+                                     ("dresidual", dresidual, (rows, n), t)):
+            if v is not None:
+                _expect(v, name, shape, kind)
+                if len(shape) == 2:
+                    setattr(a, name + "_stride", _stride(v))
+            setattr(a, name, _ptr(v))
+        check(capi.lib().chimera_linear_backward_device(self.ctx.handle, C.byref(self._shape), C.byref(a)))
+
+
+def cache_row(format: str, dim: int, group: int) -> tuple[int, int]:
+    """(bytes of codes, number of scales) of one slot of a cache."""
+    if format not in FORMATS:
+        raise ValueError(f"unknown cache format {format!r}")
+    row, scales = C.c_int32(), C.c_int32()
+    check(capi.lib().chimera_cache_row(C.byref(CacheDesc(FORMATS[format], dim, group, 1, 0, None, None)),
+                                       C.byref(row), C.byref(scales)))
+    return row.value, scales.value
+
+
+class TokenCache:
+    """Quantised token embeddings in pages of page_tokens slots: codes [slots,
+    row bytes] uint8 and scales [slots, scales] f32, the caller's arrays. A
+    call's workspace is kept for the next one and grows as needed (a call that
+    needs a larger one waits for the work before it)."""
+
+    def __init__(self, ctx: capi.Context, codes, scales, format: str = "int8", dim: int = 128, group: int = 128,
+                 page_tokens: int = 16):
+        row, groups = cache_row(format, dim, group)
+        slots = codes.shape[0]
+        if tuple(codes.shape) != (slots, row) or tuple(scales.shape) != (slots, groups):
+            raise ValueError(f"the cache needs codes [slots, {row}] and scales [slots, {groups}]")
+        if _type_name(codes) != "uint8" or _type_name(scales) != "f32":
+            raise ValueError("codes must be uint8 and scales f32")
+        if page_tokens < 1 or slots % page_tokens:
+            raise ValueError("the slots must fill whole pages")
+        self.ctx, self.codes, self.scales = ctx, codes, scales
+        self.format, self.dim, self.group, self.page_tokens = format, dim, group, page_tokens
+        self.slots = slots
+        self._desc = CacheDesc(FORMATS[format], dim, group, page_tokens, slots // page_tokens, codes.ptr, scales.ptr)
+        self._workspace = None
+        self._sizes = None
+        self._args = CacheMaxsim()
+
+    def close(self) -> None:
+        if getattr(self, "_workspace", None) is not None:
+            self.ctx.synchronize()
+            self._workspace.free()
+            self._workspace = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def write(self, rows, slots) -> None:
+        """Quantises rows [n, dim] into slots [n] (int64; entries outside the
+        cache are skipped, the others must differ)."""
+        n = rows.shape[0]
+        if tuple(rows.shape) != (n, self.dim):
+            raise ValueError(f"rows must be [n, {self.dim}]")
+        _expect(slots, "slots", (n,), "int64")
+        check(capi.lib().chimera_cache_write_device(self.ctx.handle, C.byref(self._desc), P(rows.ptr),
+                                                    _type(rows, "rows"), C.c_int64(_stride(rows)), P(slots.ptr),
+                                                    C.c_int64(n)))
+
+    def read(self, slots, out) -> None:
+        """out [n, dim] = the values in slots [n], zeros for a slot outside
+        the cache."""
+        n = out.shape[0]
+        if tuple(out.shape) != (n, self.dim):
+            raise ValueError(f"out must be [n, {self.dim}]")
+        _expect(slots, "slots", (n,), "int64")
+        check(capi.lib().chimera_cache_read_device(self.ctx.handle, C.byref(self._desc), P(slots.ptr), C.c_int64(n),
+                                                   P(out.ptr), _type(out, "out"), C.c_int64(_stride(out))))
+
+    def maxsim(self, queries, page_start, doc_lens, pages, max_doc_tokens: int, cand_ids, scores, query_lens=None,
+               cand_counts=None, k: int = 0, top_ids=None, top_scores=None, top_counts=None) -> None:
+        """scores [nq, cap] f32 of the documents cand_ids [nq, cap] int32 for
+        queries [nq, query_len, dim]; token t of document d is in slot t %
+        page_tokens of page pages[page_start[d] + t / page_tokens] (int32,
+        int64), t < doc_lens[d] (int32). With k the best k of each query
+        too."""
+        nq, query_len, dim = queries.shape
+        if dim != self.dim:
+            raise ValueError(f"queries must have {self.dim} dimensions")
+        docs, cap = doc_lens.shape[0], cand_ids.shape[1]
+        a = self._args
+        t = _type(queries, "queries")
+        for name, v, shape, kind in (("page_start", page_start, (docs,), "int64"), ("doc_lens", doc_lens, (docs,), "int32"),
+                                     ("pages", pages, (pages.shape[0],), "int32"),
+                                     ("cand_ids", cand_ids, (nq, cap), "int32"), ("scores", scores, (nq, cap), "f32"),
+                                     ("query_lens", query_lens, (nq,), "int32"),
+                                     ("cand_counts", cand_counts, (nq,), "int32"), ("top_ids", top_ids, (nq, k), "int64"),
+                                     ("top_scores", top_scores, (nq, k), "f32"),
+                                     ("top_counts", top_counts, (nq,), "int32")):
+            if v is not None:
+                _expect(v, name, shape, kind)
+            setattr(a, name, _ptr(v))
+        a.queries, a.type, a.nq, a.query_len = queries.ptr, t, nq, query_len
+        a.num_docs, a.num_page_entries, a.max_doc_tokens = docs, pages.shape[0], max_doc_tokens
+        a.cand_cap, a.k = cap, k
+        sizes = (nq, query_len, cap, max_doc_tokens)
+        if sizes != self._sizes:
+            need = C.c_size_t()
+            check(capi.lib().chimera_cache_maxsim_workspace(C.byref(a), C.byref(need)))
+            if need.value > (0 if self._workspace is None else self._workspace.nbytes):
+                self.close()
+                self._workspace = self.ctx.empty(need.value, np.uint8)
+                a.workspace, a.workspace_bytes = self._workspace.ptr, need.value
+            self._sizes = sizes
+        check(capi.lib().chimera_cache_maxsim_device(self.ctx.handle, C.byref(self._desc), C.byref(a)))
