@@ -17,17 +17,40 @@ constexpr float kLeastNorm = 1e-12f;
 
 // ---- activations ---------------------------------------------------------------
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.0f / (1.0f + expf(-z)); }
-
+constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kGeluTanhC = 0.7978845608028654f;  // sqrt(2 / pi)
 constexpr float kGeluTanhA = 0.044715f;
+
+__device__ __forceinline__ float sigmoid(float z) {
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
+}
+
+// Phi(z) = (1 + erf(z / sqrt 2)) / 2 and exp(-z^2 / 2). The error function is
+// Abramowitz and Stegun's rational approximation 7.1.26, within 1.5e-7; below
+// zero its complement is Phi itself, so small values keep their digits. A
+// tenth of the instructions of the library's erff: the epilogue of a layer of
+// 65,536 x 4096 outputs is not hidden by its products.
+__device__ __forceinline__ float normal_cdf(float z, float* gauss) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+    float p = fmaf(1.061405429f, t, -1.453152027f);
+    p = fmaf(p, t, 1.421413741f);
+    p = fmaf(p, t, -0.284496736f);
+    p = fmaf(p, t, 0.254829592f);
+    *gauss = __builtin_amdgcn_exp2f(-kLog2e * x * x);
+    const float tail = 0.5f * p * t * *gauss;
+    return z < 0.0f ? tail : 1.0f - tail;
+}
 
 __device__ __forceinline__ float activation(float z, int act) {
     switch (act) {
         case CHIMERA_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
-        case CHIMERA_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case CHIMERA_ACT_GELU_TANH:
-            return 0.5f * z * (1.0f + tanhf(kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z)));
+        case CHIMERA_ACT_GELU: {
+            float gauss;
+            return z * normal_cdf(z, &gauss);
+        }
+        case CHIMERA_ACT_GELU_TANH:  // (1 + tanh u) / 2 is the sigmoid of 2 u
+            return z * sigmoid(2.0f * kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
         case CHIMERA_ACT_SILU: return z * sigmoid(z);
         default: return z;
     }
@@ -36,16 +59,18 @@ __device__ __forceinline__ float activation(float z, int act) {
 __device__ __forceinline__ float activation_slope(float z, int act) {
     switch (act) {
         case CHIMERA_ACT_RELU: return z > 0.0f ? 1.0f : (z != z ? z : 0.0f);
-        case CHIMERA_ACT_GELU:
-            return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.3989422804014327f;
+        case CHIMERA_ACT_GELU: {
+            float gauss;
+            const float cdf = normal_cdf(z, &gauss);
+            return fmaf(z * 0.3989422804014327f, gauss, cdf);
+        }
         case CHIMERA_ACT_GELU_TANH: {
-            const float t = tanhf(kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
-            return 0.5f * (1.0f + t) +
-                   0.5f * z * (1.0f - t * t) * kGeluTanhC * fmaf(3.0f * kGeluTanhA * z, z, 1.0f);
+            const float g = sigmoid(2.0f * kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
+            return fmaf(2.0f * kGeluTanhC * z * g * (1.0f - g), fmaf(3.0f * kGeluTanhA * z, z, 1.0f), g);
         }
         case CHIMERA_ACT_SILU: {
-            const float s = sigmoid(z);
-            return s * fmaf(z, 1.0f - s, 1.0f);
+            const float g = sigmoid(z);
+            return g * fmaf(z, 1.0f - g, 1.0f);
         }
         default: return 1.0f;
     }
@@ -115,33 +140,64 @@ struct Epilogue {
     int n;
     int act;
     bool out_f32, normalize;
-    bool residual_vec, y_vec, saved_vec;
+    bool bias_vec, residual_vec, y_vec, saved_vec;
+    bool vec;  // all of them
 };
+
+// act(v) for eight values, one branch for all.
+__device__ __forceinline__ void activate8(float (&v)[8], int act) {
+    switch (act) {
+#define CHIMERA_ACTIVATE(A)                                       \
+    case A:                                                       \
+        _Pragma("unroll") for (int j = 0; j < 8; ++j) v[j] = activation(v[j], A); \
+        break;
+        CHIMERA_ACTIVATE(CHIMERA_ACT_RELU)
+        CHIMERA_ACTIVATE(CHIMERA_ACT_GELU)
+        CHIMERA_ACTIVATE(CHIMERA_ACT_GELU_TANH)
+        CHIMERA_ACTIVATE(CHIMERA_ACT_SILU)
+#undef CHIMERA_ACTIVATE
+        default: break;
+    }
+}
+// act'(z) for eight values.
+__device__ __forceinline__ void slope8(const float (&z)[8], float (&v)[8], int act) {
+    switch (act) {
+#define CHIMERA_SLOPE(A)                                          \
+    case A:                                                       \
+        _Pragma("unroll") for (int j = 0; j < 8; ++j) v[j] = activation_slope(z[j], A); \
+        break;
+        CHIMERA_SLOPE(CHIMERA_ACT_RELU)
+        CHIMERA_SLOPE(CHIMERA_ACT_GELU)
+        CHIMERA_SLOPE(CHIMERA_ACT_GELU_TANH)
+        CHIMERA_SLOPE(CHIMERA_ACT_SILU)
+#undef CHIMERA_SLOPE
+        default: break;
+    }
+}
 
 // The layer's epilogue on eight neighbouring sums of one row; with
 // normalize the row lies in kLanes neighbouring lanes, which all call it.
-template <typename T, int kLanes>
+// kInside: the eight exist and every matrix takes 16-byte accesses.
+template <typename T, int kLanes, bool kInside>
 __device__ __forceinline__ void finish8(const Epilogue& e, int split, int64_t m, int n0, float (&v)[8]) {
-    const int count = m < e.m ? e.n - n0 : 0;  // may be <= 0
+    const int count = kInside ? 8 : m < e.m ? e.n - n0 : 0;  // may be <= 0
     const bool whole = count >= 8;
     if (e.partial) {
-        if (count > 0) store8(e.partial + (split * e.m + m) * e.n + n0, whole && e.y_vec, count, v);
+        if (count > 0) store8(e.partial + (split * e.m + m) * e.n + n0, kInside || (whole && e.y_vec), count, v);
         return;
     }
     if (count > 0) {
         if (e.bias) {
-            const T* b = static_cast<const T*>(e.bias) + n0;
+            float b[8];
+            load8(static_cast<const T*>(e.bias) + n0, kInside || (whole && e.bias_vec), count, b);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += j < count ? to_float(b[j]) : 0.0f;
+            for (int j = 0; j < 8; ++j) v[j] += b[j];
         }
-        if (e.saved) store8(static_cast<T*>(e.saved) + m * e.saved_stride + n0, whole && e.saved_vec, count, v);
-        if (e.act != CHIMERA_ACT_NONE) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = activation(v[j], e.act);
-        }
+        if (e.saved) store8(static_cast<T*>(e.saved) + m * e.saved_stride + n0, kInside || (whole && e.saved_vec), count, v);
+        activate8(v, e.act);
         if (e.residual) {
             float r[8];
-            load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n0, whole && e.residual_vec, count, r);
+            load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n0, kInside || (whole && e.residual_vec), count, r);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += r[j];
         }
@@ -161,9 +217,9 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int split, int64_t m,
     if (count <= 0) return;
     const int64_t at = m * e.y_stride + n0;
     if (e.out_f32)
-        store8(static_cast<float*>(e.y) + at, whole && e.y_vec, count, v);
+        store8(static_cast<float*>(e.y) + at, kInside || (whole && e.y_vec), count, v);
     else
-        store8(static_cast<T*>(e.y) + at, whole && e.y_vec, count, v);
+        store8(static_cast<T*>(e.y) + at, kInside || (whole && e.y_vec), count, v);
 }
 
 // ---- matrix-core steps ---------------------------------------------------------
@@ -220,28 +276,43 @@ struct Product {
     int n;
     int64_t k_bytes;  // of a row, a multiple of 16
     int tiles_m, tiles_n;
-    int steps, steps_per_split;  // of 128 bytes
+    int steps, steps_per_split;  // of kStepBytes
 };
 
 // ---- tiled product -------------------------------------------------------------
 
-constexpr int kStepBytes = 128;  // of the summed axis per step: 64 or 32 values
+constexpr int kStepBytes = 64;  // of the summed axis per step: 32 or 16 values
+constexpr int kSlots = 4;       // steps in LDS: one at work, three on their way
 
-// C tile of BM x BN by WM x WN waves. Each step's rows of A and B (128 bytes
-// each) go straight from memory to one of two LDS buffers while the matrix
-// cores work on the other. Chunk c of row r lies at chunk place c ^ (r % 8),
-// so that the 8 lanes that an LDS read serves at a time hit different banks.
+// Waits until at most kLoads of the wave's loads (and no LDS access) are under
+// way, then for the block.
+template <int kLoads>
+__device__ __forceinline__ void wait_and_meet() {
+    __builtin_amdgcn_s_waitcnt((kLoads & 15) | (kLoads >> 4 << 14) | (7 << 4));
+    asm volatile("" ::: "memory");  // LDS accesses stay on their side
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// C tile of BM x BN by WM x WN waves. The rows of A and B, 64 bytes of the
+// summed axis a step, go straight from memory to a ring of four LDS slots:
+// with three steps on their way the loads' latency is covered at full rate
+// (256 x 256 tiles read 16 KB of LDS-bound data in the 512 cycles that a
+// step's products take a wave). Chunk c of row r lies at place c ^ (r / 4 % 4),
+// so that the 16 lanes that follow each other in an LDS read hit different
+// banks. A wave reads the operands of one half of a step while the matrix
+// cores work on the other half.
 template <typename T, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, Epilogue e) {
     constexpr int W = WM * WN;
     constexpr int TM = BM / WM, TN = BN / WN;
     constexpr int IM = TM / 32, IN = TN / 32;
-    constexpr int LA = BM / 8 / W, LB = BN / 8 / W;  // loads of 8 rows per wave and step
-    static_assert(LA * 8 * W == BM && LB * 8 * W == BN, "every wave loads the same number of rows");
-    constexpr int kBuffer = (BM + BN) * kStepBytes;
+    constexpr int LA = BM / 16 / W, LB = BN / 16 / W;  // loads of 16 rows per wave and step
+    static_assert(LA * 16 * W == BM && LB * 16 * W == BN, "every wave loads the same number of rows");
+    constexpr int kSlot = (BM + BN) * kStepBytes;
     constexpr int kPitch = TN + 4;
     constexpr int kStage = W * 32 * kPitch * 4;
-    __shared__ __align__(1024) unsigned char lds[2 * kBuffer > kStage ? 2 * kBuffer : kStage];
+    __shared__ __align__(1024) unsigned char lds[kSlots * kSlot > kStage ? kSlots * kSlot : kStage];
 
     const int l = lane_id();
     const int w = __builtin_amdgcn_readfirstlane(wave_id());
@@ -263,22 +334,23 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     const int step0 = split * p.steps_per_split;
     const int steps = min(p.steps_per_split, p.steps - step0);
 
-    // lane l loads chunk (l % 8) ^ (l / 8) of row l / 8 of its eight rows;
+    // lane l loads chunk (l % 4) ^ (l / 16) of row l / 4 of its sixteen rows;
     // rows past the end load the last row
-    const int chunk = (l & 7) ^ (l >> 3);
+    const int chunk = (l & 3) ^ (l >> 4);
     const char* base_a = static_cast<const char*>(p.a) + m0 * p.a_stride + static_cast<int64_t>(step0) * kStepBytes;
     const char* base_b = static_cast<const char*>(p.b) + n0 * p.b_stride + static_cast<int64_t>(step0) * kStepBytes;
     uint32_t off_a[LA], off_b[LB];
     const int last_a = static_cast<int>(min(p.m - m0, static_cast<int64_t>(BM))) - 1, last_b = min(p.n - n0, BN) - 1;
 #pragma unroll
     for (int i = 0; i < LA; ++i)
-        off_a[i] = static_cast<uint32_t>(min((i * W + w) * 8 + (l >> 3), last_a)) * static_cast<uint32_t>(p.a_stride) +
+        off_a[i] = static_cast<uint32_t>(min((i * W + w) * 16 + (l >> 2), last_a)) * static_cast<uint32_t>(p.a_stride) +
                    16u * chunk;
 #pragma unroll
     for (int i = 0; i < LB; ++i)
-        off_b[i] = static_cast<uint32_t>(min((i * W + w) * 8 + (l >> 3), last_b)) * static_cast<uint32_t>(p.b_stride) +
+        off_b[i] = static_cast<uint32_t>(min((i * W + w) * 16 + (l >> 2), last_b)) * static_cast<uint32_t>(p.b_stride) +
                    16u * chunk;
-    auto fetch = [&](int s, unsigned char* to) {
+    auto fetch = [&](int s) {
+        unsigned char* to = lds + s % kSlots * kSlot;
         const char* a = base_a + static_cast<int64_t>(s) * kStepBytes;
         const char* b = base_b + static_cast<int64_t>(s) * kStepBytes;
         const int64_t left = p.k_bytes - static_cast<int64_t>(step0 + s) * kStepBytes;
@@ -303,35 +375,65 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
 #pragma unroll
         for (int j = 0; j < IN; ++j) acc[i][j] = f32x16_t{};
 
-    const uint32_t row_a = (wm * TM + (l & 31)) * kStepBytes, row_b = BM * kStepBytes + (wn * TN + (l & 31)) * kStepBytes;
-    auto compute = [&](const unsigned char* from) {
+    // halves of a step: chunks 0, 1 and 2, 3
+    const uint32_t place = (((l >> 5) ^ ((l >> 2) & 3)) << 4);
+    const uint32_t row_a = (wm * TM + (l & 31)) * kStepBytes + place;
+    const uint32_t row_b = BM * kStepBytes + (wn * TN + (l & 31)) * kStepBytes + place;
+    struct Operands {
+        u32x4_t a[IM], b[IN];
+    };
+    auto read = [&](int s, int half, Operands& o) {
+        const unsigned char* from = lds + s % kSlots * kSlot;
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            const uint32_t place = (((2 * s) ^ (l >> 5) ^ (l & 7)) << 4);
-            u32x4_t fa[IM], fb[IN];
+        for (int i = 0; i < IM; ++i)
+            o.a[i] = *reinterpret_cast<const u32x4_t*>(from + i * 32 * kStepBytes + (row_a ^ (half << 5)));
 #pragma unroll
-            for (int i = 0; i < IM; ++i) fa[i] = *reinterpret_cast<const u32x4_t*>(from + row_a + i * 32 * kStepBytes + place);
+        for (int j = 0; j < IN; ++j)
+            o.b[j] = *reinterpret_cast<const u32x4_t*>(from + j * 32 * kStepBytes + (row_b ^ (half << 5)));
+    };
+    auto multiply = [&](const Operands& o) {
 #pragma unroll
-            for (int j = 0; j < IN; ++j) fb[j] = *reinterpret_cast<const u32x4_t*>(from + row_b + j * 32 * kStepBytes + place);
+        for (int i = 0; i < IM; ++i)
 #pragma unroll
-            for (int i = 0; i < IM; ++i)
-#pragma unroll
-                for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(fa[i], fb[j], acc[i][j]);
-        }
+            for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(o.a[i], o.b[j], acc[i][j]);
     };
 
-    fetch(0, lds);
+    constexpr int kLoads = LA + LB;
+    Operands first, second;
+#pragma unroll
+    for (int i = 0; i < IM; ++i) second.a[i] = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int j = 0; j < IN; ++j) second.b[j] = u32x4_t{0, 0, 0, 0};
+#pragma unroll
+    for (int s = 0; s < kSlots - 1; ++s)
+        if (s < steps) fetch(s);
+    if (steps >= kSlots - 1)
+        wait_and_meet<2 * kLoads>();
+    else
+        wait_and_meet<0>();
     for (int s = 0; s < steps; ++s) {
-        __syncthreads();  // this step's rows are in LDS, the other buffer is read
-        if (s + 1 < steps) fetch(s + 1, lds + ((s + 1) & 1) * kBuffer);
-        compute(lds + (s & 1) * kBuffer);
+        if (s + 3 < steps) fetch(s + 3);
+        read(s, 0, first);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(second);  // the step before's; zeros at first
+        __builtin_amdgcn_sched_barrier(0);
+        read(s, 1, second);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(first);
+        __builtin_amdgcn_sched_barrier(0);
+        if (s + 3 < steps)
+            wait_and_meet<2 * kLoads>();
+        else
+            wait_and_meet<0>();
+        __builtin_amdgcn_sched_barrier(0);
     }
-    __syncthreads();
+    multiply(second);
 
     // D lane l holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4: through
     // LDS into eight neighbouring columns a lane
     float* stage = reinterpret_cast<float*>(lds) + w * 32 * kPitch;
     constexpr int kLanes = TN / 8, kRows = kWave / kLanes;
+    const bool inside = m0 + BM <= p.m && n0 + BN <= p.n && e.vec;
 #pragma unroll
     for (int i = 0; i < IM; ++i) {
 #pragma unroll
@@ -340,7 +442,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
             for (int r = 0; r < 16; ++r)
                 stage[(8 * (r >> 2) + 4 * (l >> 5) + (r & 3)) * kPitch + 32 * j + (l & 31)] = acc[i][j][r];
         wave_lds_sync();
-#pragma unroll
+#pragma unroll 1
         for (int q = 0; q < 32 / kRows; ++q) {
             const int row = q * kRows + l / kLanes, col = l % kLanes * 8;
             float v[8];
@@ -351,7 +453,10 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
                 v[j] = lo[j];
                 v[4 + j] = hi[j];
             }
-            finish8<T, kLanes>(e, split, m0 + wm * TM + 32 * i + row, n0 + wn * TN + col, v);
+            if (inside)
+                finish8<T, kLanes, true>(e, split, m0 + wm * TM + 32 * i + row, n0 + wn * TN + col, v);
+            else
+                finish8<T, kLanes, false>(e, split, m0 + wm * TM + 32 * i + row, n0 + wn * TN + col, v);
         }
         wave_lds_sync();
     }
@@ -420,7 +525,7 @@ __global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, E
     for (int o = 1; o < KW; ++o)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += part[o][row][col + j];
-    finish8<T, kLanes>(e, 0, m0 + row, n0 + col, v);
+    finish8<T, kLanes, false>(e, 0, m0 + row, n0 + col, v);
 }
 
 // ---- layouts -------------------------------------------------------------------
@@ -522,8 +627,10 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
         if (a.act != CHIMERA_ACT_NONE && count > 0) {
             float z[8];
             load8(static_cast<const T*>(a.saved) + m * a.saved_stride + n0, whole && a.saved_vec, count, z);
+            float slope[8];
+            slope8(z, slope, a.act);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = j < count ? g[j] * activation_slope(z[j], a.act) : 0.0f;
+            for (int j = 0; j < 8; ++j) g[j] = j < count ? g[j] * slope[j] : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += g[j];
@@ -683,6 +790,8 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     e.residual_vec = rows_aligned(a.residual, a.residual_stride, sizeof(T));
     e.y_vec = rows_aligned(a.y, a.y_stride, out);
     e.saved_vec = rows_aligned(a.saved, a.saved_stride, sizeof(T));
+    e.bias_vec = rows_aligned(a.bias, 0, sizeof(T));
+    e.vec = e.y_vec && e.bias_vec && (!a.residual || e.residual_vec) && (!a.saved || e.saved_vec);
     Product p = {};
     p.m = s.rows;
     p.n = s.out_features;
@@ -720,11 +829,11 @@ struct BackwardPlan {
 };
 
 // Parts of dW's sum over the rows: enough blocks of 128 x 128 for the GPU,
-// eight steps of 64 rows a part at least.
+// sixteen steps of 64 bytes a part at least.
 int dweight_splits(const chimera_linear_shape& s) {
     const int64_t tiles = ceil_div(s.out_features, 128) * ceil_div(s.in_features, 128);
     const int64_t steps = ceil_div(round_up(s.rows, 64) * type_bytes(s.type), kStepBytes);
-    return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(512, tiles), steps / 8)));
+    return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(512, tiles), steps / 16)));
 }
 
 size_t carve_backward(const chimera_linear_shape& s, void* base, BackwardPlan* plan) {
@@ -810,6 +919,7 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
             e.partial = plan.parts;
             e.y_vec = cols % 4 == 0;
         }
+        e.vec = e.y_vec;
         launch_tiles<T>(st, p, e, splits);
         if (splits > 1) {
             const int64_t steps = ceil_div(p.k_bytes, kStepBytes);
