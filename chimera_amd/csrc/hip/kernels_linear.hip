@@ -8,6 +8,7 @@
 #include "operators.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace chimera {
 
@@ -42,10 +43,32 @@ __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
     return z < 0.0f ? tail : 1.0f - tail;
 }
 
+// Phi(z) for values that are rounded to 16 bits: 1/2 + z P(z^2), a minimax
+// fit on [-4, 4] held to 0 and 1 at its ends (and, clamped, beyond), within
+// 3.4e-5 of Phi, so that gelu is within 1.4e-4: a thirtieth of a bf16 step at
+// 1, half an fp16 rounding. 11 full-rate instructions where the exact form
+// takes 20 and two quarter-rate ones: 65,536 x 4096 outputs took 200 us with
+// that form, a third of the layer's products.
+__device__ __forceinline__ float normal_cdf_16(float z) {
+    const float c = __builtin_amdgcn_fmed3f(z, -4.0f, 4.0f);
+    const float t = c * c;
+    float p = fmaf(-1.2773050395153973e-09f, t, 1.0440346898121788e-07f);
+    p = fmaf(p, t, -3.708714984895778e-06f);
+    p = fmaf(p, t, 7.617972005391493e-05f);
+    p = fmaf(p, t, -1.020980766043067e-03f);
+    p = fmaf(p, t, 9.581183083355427e-03f);
+    p = fmaf(p, t, -6.606381386518478e-02f);
+    p = fmaf(p, t, 0.3988054394721985f);
+    return __builtin_amdgcn_fmed3f(fmaf(p, c, 0.5f), 0.0f, 1.0f);
+}
+
+// T: the type that the result is rounded to or that the layer works in.
+template <typename T>
 __device__ __forceinline__ float activation(float z, int act) {
     switch (act) {
         case CHIMERA_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
         case CHIMERA_ACT_GELU: {
+            if constexpr (sizeof(T) == 2) return z * normal_cdf_16(z);
             float gauss;
             return z * normal_cdf(z, &gauss);
         }
@@ -144,18 +167,20 @@ struct Epilogue {
     bool vec;  // all of them
 };
 
-// act(v) for eight values, one branch for all.
-__device__ __forceinline__ void activate8(float (&v)[8], int act) {
+// act(v) for many values, one branch for all.
+template <typename T, int kRuns>
+__device__ __forceinline__ void activate(float (&v)[kRuns][16], int act) {
+    auto all = [&](auto a) {
+#pragma unroll
+        for (int j = 0; j < kRuns; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[j][r] = activation<T>(v[j][r], decltype(a)::value);
+    };
     switch (act) {
-#define CHIMERA_ACTIVATE(A)                                       \
-    case A:                                                       \
-        _Pragma("unroll") for (int j = 0; j < 8; ++j) v[j] = activation(v[j], A); \
-        break;
-        CHIMERA_ACTIVATE(CHIMERA_ACT_RELU)
-        CHIMERA_ACTIVATE(CHIMERA_ACT_GELU)
-        CHIMERA_ACTIVATE(CHIMERA_ACT_GELU_TANH)
-        CHIMERA_ACTIVATE(CHIMERA_ACT_SILU)
-#undef CHIMERA_ACTIVATE
+        case CHIMERA_ACT_RELU: all(std::integral_constant<int, CHIMERA_ACT_RELU>{}); break;
+        case CHIMERA_ACT_GELU: all(std::integral_constant<int, CHIMERA_ACT_GELU>{}); break;
+        case CHIMERA_ACT_GELU_TANH: all(std::integral_constant<int, CHIMERA_ACT_GELU_TANH>{}); break;
+        case CHIMERA_ACT_SILU: all(std::integral_constant<int, CHIMERA_ACT_SILU>{}); break;
         default: break;
     }
 }
@@ -177,27 +202,23 @@ __device__ __forceinline__ void slope8(const float (&z)[8], float (&v)[8], int a
 
 // The layer's epilogue on eight neighbouring sums of one row; with
 // normalize the row lies in kLanes neighbouring lanes, which all call it.
-// kInside: the eight exist and every matrix takes 16-byte accesses.
-template <typename T, int kLanes, bool kInside>
-__device__ __forceinline__ void finish8(const Epilogue& e, int split, int64_t m, int n0, float (&v)[8]) {
-    const int count = kInside ? 8 : m < e.m ? e.n - n0 : 0;  // may be <= 0
+template <typename T, int kLanes>
+__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n0, float (&v)[8]) {
+    const int count = m < e.m ? e.n - n0 : 0;  // may be <= 0
     const bool whole = count >= 8;
-    if (e.partial) {
-        if (count > 0) store8(e.partial + (split * e.m + m) * e.n + n0, kInside || (whole && e.y_vec), count, v);
-        return;
-    }
     if (count > 0) {
         if (e.bias) {
             float b[8];
-            load8(static_cast<const T*>(e.bias) + n0, kInside || (whole && e.bias_vec), count, b);
+            load8(static_cast<const T*>(e.bias) + n0, whole && e.bias_vec, count, b);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += b[j];
         }
-        if (e.saved) store8(static_cast<T*>(e.saved) + m * e.saved_stride + n0, kInside || (whole && e.saved_vec), count, v);
-        activate8(v, e.act);
+        if (e.saved) store8(static_cast<T*>(e.saved) + m * e.saved_stride + n0, whole && e.saved_vec, count, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = activation<T>(v[j], e.act);
         if (e.residual) {
             float r[8];
-            load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n0, kInside || (whole && e.residual_vec), count, r);
+            load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n0, whole && e.residual_vec, count, r);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += r[j];
         }
@@ -217,9 +238,9 @@ __device__ __forceinline__ void finish8(const Epilogue& e, int split, int64_t m,
     if (count <= 0) return;
     const int64_t at = m * e.y_stride + n0;
     if (e.out_f32)
-        store8(static_cast<float*>(e.y) + at, kInside || (whole && e.y_vec), count, v);
+        store8(static_cast<float*>(e.y) + at, whole && e.y_vec, count, v);
     else
-        store8(static_cast<T*>(e.y) + at, kInside || (whole && e.y_vec), count, v);
+        store8(static_cast<T*>(e.y) + at, whole && e.y_vec, count, v);
 }
 
 // ---- matrix-core steps ---------------------------------------------------------
@@ -282,7 +303,8 @@ struct Product {
 // ---- tiled product -------------------------------------------------------------
 
 constexpr int kStepBytes = 64;  // of the summed axis per step: 32 or 16 values
-constexpr int kSlots = 4;       // steps in LDS: one at work, three on their way
+
+constexpr int kWaitLds = 0xC07F;  // s_waitcnt lgkmcnt(0), the others not waited on
 
 // Waits until at most kLoads of the wave's loads (and no LDS access) are under
 // way, then for the block.
@@ -302,7 +324,7 @@ __device__ __forceinline__ void wait_and_meet() {
 // so that the 16 lanes that follow each other in an LDS read hit different
 // banks. A wave reads the operands of one half of a step while the matrix
 // cores work on the other half.
-template <typename T, int BM, int BN, int WM, int WN>
+template <typename T, int BM, int BN, int WM, int WN, int kSlots>
 __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, Epilogue e) {
     constexpr int W = WM * WN;
     constexpr int TM = BM / WM, TN = BN / WN;
@@ -349,25 +371,29 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     for (int i = 0; i < LB; ++i)
         off_b[i] = static_cast<uint32_t>(min((i * W + w) * 16 + (l >> 2), last_b)) * static_cast<uint32_t>(p.b_stride) +
                    16u * chunk;
-    auto fetch = [&](int s) {
+    auto fetch = [&](int s, auto whole) {
         unsigned char* to = lds + s % kSlots * kSlot;
         const char* a = base_a + static_cast<int64_t>(s) * kStepBytes;
         const char* b = base_b + static_cast<int64_t>(s) * kStepBytes;
-        const int64_t left = p.k_bytes - static_cast<int64_t>(step0 + s) * kStepBytes;
-        const bool zero = 16 * chunk >= left;
+        // in its last step, lanes past the end of the summed axis load zeros
+        // (an offset is chosen, not a load: every lane takes part in each)
+        const bool zero = !whole && 16 * chunk >= p.k_bytes % kStepBytes;
+        const int64_t zero_a = reinterpret_cast<const char*>(g_zero_chunk) - a;
+        const int64_t zero_b = reinterpret_cast<const char*>(g_zero_chunk) - b;
 #pragma unroll
-        for (int i = 0; i < LA; ++i) {
-            const void* src = a + off_a[i];
-            if (left < kStepBytes) src = zero ? static_cast<const void*>(g_zero_chunk) : src;
-            __builtin_amdgcn_global_load_lds(src, lds_at(to + (i * W + w) * 1024), 16, 0, 0);
-        }
+        for (int i = 0; i < LA; ++i)
+            __builtin_amdgcn_global_load_lds(a + (zero ? zero_a : static_cast<int64_t>(off_a[i])),
+                                             lds_at(to + (i * W + w) * 1024), 16, 0, 0);
 #pragma unroll
-        for (int i = 0; i < LB; ++i) {
-            const void* src = b + off_b[i];
-            if (left < kStepBytes) src = zero ? static_cast<const void*>(g_zero_chunk) : src;
-            __builtin_amdgcn_global_load_lds(src, lds_at(to + BM * kStepBytes + (i * W + w) * 1024), 16, 0, 0);
-        }
+        for (int i = 0; i < LB; ++i)
+            __builtin_amdgcn_global_load_lds(b + (zero ? zero_b : static_cast<int64_t>(off_b[i])),
+                                             lds_at(to + BM * kStepBytes + (i * W + w) * 1024), 16, 0, 0);
     };
+    // steps before the one that the axis ends within, if there is one
+    const bool partial = p.k_bytes % kStepBytes != 0 && step0 + steps == p.steps;
+    const int whole = steps - (partial ? 1 : 0);
+    constexpr auto kWhole = std::true_type{};
+    constexpr auto kPartial = std::false_type{};
 
     f32x16_t acc[IM][IN];
 #pragma unroll
@@ -395,7 +421,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
 #pragma unroll
         for (int i = 0; i < IM; ++i)
 #pragma unroll
-            for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(o.a[i], o.b[j], acc[i][j]);
+            for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(o.b[j], o.a[i], acc[i][j]);
     };
 
     constexpr int kLoads = LA + LB;
@@ -404,61 +430,178 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     for (int i = 0; i < IM; ++i) second.a[i] = u32x4_t{0, 0, 0, 0};
 #pragma unroll
     for (int j = 0; j < IN; ++j) second.b[j] = u32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int s = 0; s < kSlots - 1; ++s)
-        if (s < steps) fetch(s);
-    if (steps >= kSlots - 1)
-        wait_and_meet<2 * kLoads>();
-    else
-        wait_and_meet<0>();
-    for (int s = 0; s < steps; ++s) {
-        if (s + 3 < steps) fetch(s + 3);
+    auto step = [&](int s, auto&& more) {
+        more();
         read(s, 0, first);
         __builtin_amdgcn_sched_barrier(0);
         multiply(second);  // the step before's; zeros at first
         __builtin_amdgcn_sched_barrier(0);
+        // the first half is in registers by now; said here, it needs no wait
+        // for the second half's reads below
+        __builtin_amdgcn_s_waitcnt(kWaitLds);
         read(s, 1, second);
         __builtin_amdgcn_sched_barrier(0);
         multiply(first);
         __builtin_amdgcn_sched_barrier(0);
-        if (s + 3 < steps)
-            wait_and_meet<2 * kLoads>();
-        else
-            wait_and_meet<0>();
+    };
+    constexpr int kAhead = kSlots - 1;
+#pragma unroll
+    for (int s = 0; s < kAhead; ++s) {
+        if (s < whole)
+            fetch(s, kWhole);
+        else if (s < steps)
+            fetch(s, kPartial);
+    }
+    if (steps >= kAhead)
+        wait_and_meet<(kAhead - 1) * kLoads>();
+    else
+        wait_and_meet<0>();
+    int s = 0;
+    for (; s + kAhead < whole; ++s) {
+        step(s, [&] { fetch(s + kAhead, kWhole); });
+        wait_and_meet<(kAhead - 1) * kLoads>();
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    for (; s < steps; ++s) {
+        step(s, [&] {
+            if (s + kAhead < steps) fetch(s + kAhead, kPartial);
+        });
+        wait_and_meet<0>();
         __builtin_amdgcn_sched_barrier(0);
     }
     multiply(second);
 
-    // D lane l holds column l % 32, rows 8 (r / 4) + 4 (l / 32) + r % 4: through
-    // LDS into eight neighbouring columns a lane
-    float* stage = reinterpret_cast<float*>(lds) + w * 32 * kPitch;
+    // With W as the first operand, D lane l holds row l % 32 of X and of each
+    // tile the columns 8 (r / 4) + 4 (l / 32) + r % 4: four neighbours at a
+    // time. Bias, activation and length are dealt with there; then the values
+    // go through LDS, in 16 bits where that is all that is left to do, so that
+    // a wave's stores are whole 128-byte lines.
     constexpr int kLanes = TN / 8, kRows = kWave / kLanes;
     const bool inside = m0 + BM <= p.m && n0 + BN <= p.n && e.vec;
-#pragma unroll
-    for (int i = 0; i < IM; ++i) {
+    const int half = l >> 5;
+    const int col0 = n0 + wn * TN;
+    unsigned char* stage = lds + w * 32 * kPitch * 4;
+    auto put = [&](const float(&v)[IN][16], auto type) {
+        using S = decltype(type);
+        S* to = reinterpret_cast<S*>(stage + (l & 31) * (TN * sizeof(S) + 16)) + 4 * half;
 #pragma unroll
         for (int j = 0; j < IN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r)
-                stage[(8 * (r >> 2) + 4 * (l >> 5) + (r & 3)) * kPitch + 32 * j + (l & 31)] = acc[i][j][r];
+            for (int q = 0; q < 4; ++q) {
+                S t[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) t[r] = from_float<S>(v[j][4 * q + r]);
+                if constexpr (sizeof(S) == 4)
+                    *reinterpret_cast<u32x4_t*>(to + 32 * j + 8 * q) = *reinterpret_cast<const u32x4_t*>(t);
+                else
+                    *reinterpret_cast<u32x2_t*>(to + 32 * j + 8 * q) = *reinterpret_cast<const u32x2_t*>(t);
+            }
         wave_lds_sync();
-#pragma unroll 1
+    };
+    // each(row of the 32, first of eight columns, its place in LDS) for the rows put
+    auto each_row = [&](auto type, auto&& each) {
+        using S = decltype(type);
+#pragma unroll
         for (int q = 0; q < 32 / kRows; ++q) {
             const int row = q * kRows + l / kLanes, col = l % kLanes * 8;
-            float v[8];
-            const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(stage + row * kPitch + col);
-            const f32x4_t hi = *reinterpret_cast<const f32x4_t*>(stage + row * kPitch + col + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = lo[j];
-                v[4 + j] = hi[j];
-            }
-            if (inside)
-                finish8<T, kLanes, true>(e, split, m0 + wm * TM + 32 * i + row, n0 + wn * TN + col, v);
-            else
-                finish8<T, kLanes, false>(e, split, m0 + wm * TM + 32 * i + row, n0 + wn * TN + col, v);
+            each(row, col, reinterpret_cast<const S*>(stage + row * (TN * sizeof(S) + 16)) + col);
         }
         wave_lds_sync();
+    };
+    // the rows put in T, as they are, to a matrix of T
+    auto copy_out = [&](void* to, int64_t stride, bool vec, int64_t m_first) {
+        each_row(T{}, [&](int row, int col, const T* from) {
+            const int64_t m = m_first + row;
+            const int n = col0 + col;
+            const int count = inside ? 8 : m < e.m ? e.n - n : 0;
+            T* dst = static_cast<T*>(to) + m * stride + n;
+            if (inside || (vec && count >= 8)) {
+#pragma unroll
+                for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h)
+                    reinterpret_cast<u32x4_t*>(dst)[h] = reinterpret_cast<const u32x4_t*>(from)[h];
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    if (j < count) dst[j] = from[j];
+            }
+        });
+    };
+    float bias[IN][16];
+#pragma unroll
+    for (int j = 0; j < IN; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int n = col0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
+            bias[j][r] = e.bias && n < e.n ? to_float(static_cast<const T*>(e.bias)[n]) : 0.0f;
+        }
+    // what is left to do after LDS: nothing, or something in 32 bits
+    const bool narrow = sizeof(T) == 2 && !e.out_f32 && !e.partial && (!e.residual || e.normalize);
+#pragma unroll
+    for (int i = 0; i < IM; ++i) {
+        const int64_t m_first = m0 + wm * TM + 32 * i;
+        float v[IN][16];
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) v[j][r] = acc[i][j][r] + bias[j][r];
+        if (e.saved) {
+            put(v, T{});
+            copy_out(e.saved, e.saved_stride, e.saved_vec, m_first);
+        }
+        activate<T>(v, e.act);
+        if (e.normalize) {
+            const int64_t m = m_first + (l & 31);
+            float s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int n = col0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
+                    if (e.residual && m < e.m && n < e.n)
+                        v[j][r] += to_float(static_cast<const T*>(e.residual)[m * e.residual_stride + n]);
+                    s = n < e.n ? fmaf(v[j][r], v[j][r], s) : s;
+                }
+            s += __shfl_xor(s, 32, kWave);
+            const float norm = sqrtf(s);
+            const float held = norm < kLeastNorm ? kLeastNorm : norm;  // NaN stays
+            const float inv = 1.0f / held;
+#pragma unroll
+            for (int j = 0; j < IN; ++j)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) v[j][r] *= inv;
+            if (e.norms && half == 0 && m < e.m) e.norms[m] = held;
+        }
+        if (narrow) {
+            put(v, T{});
+            copy_out(e.y, e.y_stride, e.y_vec, m_first);
+            continue;
+        }
+        put(v, 0.0f);
+        each_row(0.0f, [&](int row, int col, const float* from) {
+            const int64_t m = m_first + row;
+            const int n = col0 + col;
+            const int count = inside ? 8 : m < e.m ? e.n - n : 0;
+            if (count <= 0) return;
+            const bool whole = count >= 8;
+            float u[8];
+            load8(from, true, 8, u);
+            if (e.partial) {
+                store8(e.partial + (split * e.m + m) * e.n + n, inside || (whole && e.y_vec), count, u);
+                return;
+            }
+            if (e.residual && !e.normalize) {
+                float r[8];
+                load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n, inside || (whole && e.residual_vec),
+                      count, r);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) u[j] += r[j];
+            }
+            const int64_t at = m * e.y_stride + n;
+            if (e.out_f32)
+                store8(static_cast<float*>(e.y) + at, inside || (whole && e.y_vec), count, u);
+            else
+                store8(static_cast<T*>(e.y) + at, inside || (whole && e.y_vec), count, u);
+        });
     }
 }
 
@@ -525,7 +668,7 @@ __global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, E
     for (int o = 1; o < KW; ++o)
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += part[o][row][col + j];
-    finish8<T, kLanes, false>(e, 0, m0 + row, n0 + col, v);
+    finish8<T, kLanes>(e, m0 + row, n0 + col, v);
 }
 
 // ---- layouts -------------------------------------------------------------------
@@ -721,16 +864,16 @@ void launch_tiles(hipStream_t st, Product p, Epilogue e, int splits) {
     };
     if (e.normalize) {
         const dim3 grid = plan(128, 128);
-        hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, 1>), grid, dim3(256), 0, st, p, e);
+        hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, 1, 4>), grid, dim3(256), 0, st, p, e);
         return;
     }
     if (ceil_div(p.m, 256) * ceil_div(p.n, 256) * splits >= 256) {
         const dim3 grid = plan(256, 256);
-        hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4>), grid, dim3(512), 0, st, p, e);
+        hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4, 4>), grid, dim3(512), 0, st, p, e);
         return;
     }
     const dim3 grid = plan(128, 128);
-    hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2>), grid, dim3(256), 0, st, p, e);
+    hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2, 4>), grid, dim3(256), 0, st, p, e);
 }
 
 // A matrix as a product reads it: as it lies where its rows start at
