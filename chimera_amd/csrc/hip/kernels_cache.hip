@@ -5,6 +5,7 @@
 #include "operators.hpp"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace chimera {
 
@@ -231,7 +232,15 @@ struct MaxsimArgs {
     int64_t num_docs, num_page_entries;
     int nq, query_len, cap;
     int split_tokens, splits, max_tokens;
+    int items;  // parts of documents a wave takes, 1..64
+    bool query_vec;  // query rows start at multiples of 16 bytes
 };
+
+// The query row whose maximum lane l ends up with (maxima_to_rows).
+__device__ __forceinline__ int row_of_lane(int l) {
+    const int r = ((l >> 4) & 1) * 8 + ((l >> 3) & 1) * 4 + ((l >> 2) & 1) * 2 + ((l >> 1) & 1);
+    return 8 * (r >> 2) + 4 * (l >> 5) + (r & 3);
+}
 
 // One query tile of 32 tokens as matrix operand (rows: query tokens), in fp16
 // parts after a power of two per token that brings its largest value to
@@ -240,19 +249,21 @@ struct MaxsimArgs {
 template <typename T, int kFormat, int kParts>
 struct QueryTile {
     f16x8_t part[kParts][4][2];
-    float back;  // 2^e of the row that maxima_to_rows leaves in this lane
+    float back;  // 2^e of row_of_lane's row; 0 in the lanes that do not count it
 
-    __device__ __forceinline__ void load(const T* q, int rows, int dim, int l) {
+    __device__ __forceinline__ void load(const T* q, int rows, int dim, bool vec, int l) {
         const int row = l & 31, half = l >> 5;
-        float x[4][16];
+        float x[4][2][8];
         float most = 0.0f;
 #pragma unroll
         for (int g = 0; g < 4; ++g)
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                const int at = 32 * g + 16 * half + j;
-                x[g][j] = row < rows && at < dim ? to_float(q[static_cast<int64_t>(row) * dim + at]) : 0.0f;
-                most = fmaxf(most, fabsf(x[g][j]));
+            for (int h = 0; h < 2; ++h) {
+                const int at = 32 * g + 16 * half + 8 * h;
+                const int count = row < rows ? dim - at : 0;
+                load8(q + static_cast<int64_t>(row) * dim + at, vec && count >= 8, count, x[g][h]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[g][h][j]));
             }
         most = fmaxf(most, __shfl_xor(most, 32, kWave));
         int e = 0;
@@ -265,75 +276,176 @@ struct QueryTile {
             for (int h = 0; h < 2; ++h)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float v = x[g][8 * h + code_order<kFormat>(j)] * to;
+                    const float v = x[g][h][code_order<kFormat>(j)] * to;
                     const _Float16 hi = static_cast<_Float16>(v);
                     part[0][g][h][j] = hi;
                     if constexpr (kParts == 2) part[1][g][h][j] = static_cast<_Float16>(v - static_cast<float>(hi));
                 }
-        back = __shfl(ldexpf(1.0f, e), row_of(l), kWave);
-    }
-    // The query row whose maximum lane l ends up with.
-    static __device__ __forceinline__ int row_of(int l) {
-        const int r = ((l >> 4) & 1) * 8 + ((l >> 3) & 1) * 4 + ((l >> 2) & 1) * 2 + ((l >> 1) & 1);
-        return 8 * (r >> 2) + 4 * (l >> 5) + (r & 3);
+        back = __shfl(ldexpf(1.0f, e), row_of_lane(l), kWave);
+        if ((l & 1) != 0 || row_of_lane(l) >= rows) back = 0.0f;
     }
 };
 
-template <typename T, int kFormat>
+template <int kCtrl>
+__device__ __forceinline__ float lane_move(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kCtrl, 0xF, 0xF, false));
+}
+constexpr int kRotate8 = 0x128, kMirror8 = 0x141, kSwap2 = 0x4E, kSwap1 = 0xB1;  // of a row of 16 lanes
+
+// Maxima over the 32 lanes of each half of the wave of 16 values a lane: each
+// step leaves a lane half of the values, the last one all lanes of a pair the
+// same one (lane bits 4 to 1 choose it). All in the vector unit.
+__device__ __forceinline__ float maxima_to_rows(float (&v)[16], int l) {
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[r]), __float_as_uint(v[r + 8]), false, false);
+        v[r] = fmaxf(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    }
+    auto step = [&](int bit, int keep, auto ctrl) {
+        const bool upper = (l & bit) != 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (r >= keep) continue;
+            const float mine = upper ? v[r + keep] : v[r], theirs = upper ? v[r] : v[r + keep];
+            v[r] = fmaxf(mine, lane_move<decltype(ctrl)::value>(theirs));
+        }
+    };
+    step(8, 4, std::integral_constant<int, kRotate8>{});
+    step(4, 2, std::integral_constant<int, kMirror8>{});
+    step(2, 1, std::integral_constant<int, kSwap2>{});
+    return fmaxf(v[0], lane_move<kSwap1>(v[0]));
+}
+// Sum over the wave, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+    v += lane_move<kSwap1>(v);
+    v += lane_move<kSwap2>(v);
+    v += lane_move<kMirror8>(v);
+    v += lane_move<kRotate8>(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// A wave scores `items` parts of documents (whole documents unless they are
+// split) against one query, tile after tile of 32 tokens (matrix columns)
+// with no break between documents: the codes of the next tile and the page
+// numbers of the one after it are on their way while a tile is multiplied.
+// Lane l holds of token l % 32 and each run of 32 values the 16 from
+// 16 (l / 32) on; a tile's scores are 16 query rows a lane, of one token, so
+// that the token's scale and the running maxima need no exchange before the
+// document's end. Lanes past a document's last token take that token again;
+// an absent token has NaN for its scale, which the maxima pass over.
+// kOneScale: one scale a row, applied to the sum.
+template <typename T, int kFormat, bool kOneScale>
 __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
     constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
+    constexpr int kScales = kOneScale ? 1 : 4;
     const int l = lane_id();
     const int q = static_cast<int>(blockIdx.y);
-    const int item = static_cast<int>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(wave_id());
-    const int j = item / a.splits, split = item - j * a.splits;
-    if (j >= a.cap) return;
-    const int64_t at = static_cast<int64_t>(q) * a.cap + j;
-    const int count = a.cand_counts ? a.cand_counts[q] : a.cap;
-    const int doc = j < count ? a.cand_ids[at] : -1;
-    int len = 0;
-    int64_t first = 0;
-    if (doc >= 0 && doc < a.num_docs) {
-        len = min(a.doc_lens[doc], a.max_tokens);
-        first = a.page_start[doc];
+    const int w = __builtin_amdgcn_readfirstlane(wave_id());
+    const int64_t first_item = static_cast<int64_t>(blockIdx.x) * 4 * a.items + w;
+    const int64_t total = static_cast<int64_t>(a.cap) * a.splits;
+
+    // lane i: the wave's i-th item, number first_item + 4 i
+    int my_begin = 0, my_end = 0, my_first_lo = 0, my_first_hi = 0;
+    const int64_t my_item = first_item + 4 * l;
+    bool scored = false;  // a score that is not -inf is still to come
+    if (l < a.items && my_item < total) {
+        const int j = static_cast<int>(my_item / a.splits), split = static_cast<int>(my_item - static_cast<int64_t>(j) * a.splits);
+        const int64_t at = static_cast<int64_t>(q) * a.cap + j;
+        const int count = a.cand_counts ? a.cand_counts[q] : a.cap;
+        const int doc = j < count ? a.cand_ids[at] : -1;
+        if (doc >= 0 && doc < a.num_docs) {
+            const int len = min(a.doc_lens[doc], a.max_tokens);
+            const int64_t first = a.page_start[doc];
+            my_begin = split * a.split_tokens;
+            my_end = min(len, my_begin + a.split_tokens);
+            my_first_lo = static_cast<int>(first);
+            my_first_hi = static_cast<int>(first >> 32);
+            scored = my_begin < my_end;
+        }
+        if (!scored && a.splits == 1) a.scores[at] = -INFINITY;
     }
-    const int t_begin = split * a.split_tokens, t_end = min(len, t_begin + a.split_tokens);
+    const uint64_t work = __ballot(scored);
+    if (work == 0) return;
     const int q_len = a.query_lens ? min(max(a.query_lens[q], 0), a.query_len) : a.query_len;
     const int groups = (a.c.dim + 31) / 32;
+    const int shift = a.c.group_log2 - 5;
     const int half = l >> 5;
     const int rows_padded = (a.query_len + 31) / 32 * 32;
-    float total = 0.0f;
+
+    struct Cursor {
+        uint64_t left;  // items from this one on
+        int item, t, end;
+        int64_t first;
+    };
+    auto enter = [&](Cursor& c) {
+        c.item = c.left ? __builtin_ctzll(c.left) : c.item;  // past the end: the last item again
+        c.t = __builtin_amdgcn_readlane(my_begin, c.item);
+        c.end = __builtin_amdgcn_readlane(my_end, c.item);
+        c.first = (static_cast<int64_t>(__builtin_amdgcn_readlane(my_first_hi, c.item)) << 32) |
+                  static_cast<uint32_t>(__builtin_amdgcn_readlane(my_first_lo, c.item));
+    };
+    auto advance = [&](Cursor& c) {
+        c.t += 32;
+        if (c.t < c.end) return;
+        c.left &= c.left - 1;
+        enter(c);
+    };
+    // the token's page number, -1 for none
+    auto load_page = [&](const Cursor& c) {
+        const int64_t entry = c.first + (min(c.t + (l & 31), c.end - 1) >> a.c.page_log2);
+        return entry >= 0 && entry < a.num_page_entries ? a.pages[entry] : -1;
+    };
+    struct Tile {
+        u32x4_t codes[kFormat == CHIMERA_CACHE_INT4 ? 2 : 4];
+        float scale[kScales];
+    };
+    auto load_codes = [&](const Cursor& c, int page, Tile& tile) {
+        const int t = min(c.t + (l & 31), c.end - 1);
+        const bool in = page >= 0 && page < a.c.num_pages;
+        const int64_t slot = in ? (static_cast<int64_t>(page) << a.c.page_log2) + (t & ((1 << a.c.page_log2) - 1)) : 0;
+        const uint8_t* codes = a.c.codes + slot * a.c.row_bytes;
+        if constexpr (kFormat == CHIMERA_CACHE_INT4) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (g < groups) {
+                    const u32x2_t u = *reinterpret_cast<const u32x2_t*>(codes + 16 * g + 8 * half);
+                    tile.codes[g / 2][2 * (g % 2)] = u[0];
+                    tile.codes[g / 2][2 * (g % 2) + 1] = u[1];
+                }
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                if (g < groups) tile.codes[g] = *reinterpret_cast<const u32x4_t*>(codes + 32 * g + 16 * half);
+        }
+        const float* scales = a.c.scales + slot * a.c.row_scales;
+#pragma unroll
+        for (int i = 0; i < kScales; ++i)
+            if (i < a.c.row_scales) tile.scale[i] = in ? scales[i] : NAN;
+    };
+
     for (int q0 = 0; q0 < rows_padded; q0 += 32) {
         if (q0 >= q_len && q0 > 0) break;
         QueryTile<T, kFormat, kParts> qt;
         qt.load(static_cast<const T*>(a.queries) + (static_cast<int64_t>(q) * a.query_len + q0) * a.c.dim, q_len - q0,
-                a.c.dim, l);
+                a.c.dim, a.query_vec, l);
         float best[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) best[r] = -INFINITY;
-        for (int t0 = t_begin; t0 < t_end; t0 += 32) {
-            const int t = t0 + (l & 31);
-            const int64_t entry = first + (t >> a.c.page_log2);
-            int64_t slot = -1;
-            if (t < t_end && entry >= 0 && entry < a.num_page_entries) {
-                const int page = a.pages[entry];
-                if (page >= 0 && page < a.c.num_pages)
-                    slot = (static_cast<int64_t>(page) << a.c.page_log2) + (t & ((1 << a.c.page_log2) - 1));
-            }
-            const bool in = slot >= 0;
-            const int64_t from = in ? slot : 0;
-            const uint8_t* codes = a.c.codes + from * a.c.row_bytes;
-            const float* scales = a.c.scales + from * a.c.row_scales;
+
+        auto multiply = [&](const Tile& tile) {
             f32x16_t sum = {}, acc = {};
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 if (g >= groups) break;
                 f16x8_t v0, v1;
                 if constexpr (kFormat == CHIMERA_CACHE_INT4) {
-                    const u32x2_t u = *reinterpret_cast<const u32x2_t*>(codes + 16 * g + 8 * half);
-                    v0 = int4_values(u[0]);
-                    v1 = int4_values(u[1]);
+                    v0 = int4_values(tile.codes[g / 2][2 * (g % 2)]);
+                    v1 = int4_values(tile.codes[g / 2][2 * (g % 2) + 1]);
                 } else {
-                    const u32x4_t u = *reinterpret_cast<const u32x4_t*>(codes + 32 * g + 16 * half);
+                    const u32x4_t u = tile.codes[g];
                     v0 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[0], u[1]}) : fp8_values(u32x2_t{u[0], u[1]});
                     v1 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[2], u[3]}) : fp8_values(u32x2_t{u[2], u[3]});
                 }
@@ -343,42 +455,60 @@ __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qt.part[s][g][1], v1, acc, 0, 0, 0);
                 }
                 // the end of a scale's group
-                if (((g + 1) & ((1 << (a.c.group_log2 - 5)) - 1)) == 0 || g + 1 == groups) {
-                    const float scale = scales[g >> (a.c.group_log2 - 5)];
+                if constexpr (!kOneScale) {
+                    if (((g + 1) & ((1 << shift) - 1)) == 0 || g + 1 == groups) {
+                        const float scale = shift == 0 ? tile.scale[g] : tile.scale[g / 2];
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {
-                        sum[r] = fmaf(acc[r], scale, sum[r]);
-                        acc[r] = 0.0f;
+                        for (int r = 0; r < 16; ++r) sum[r] = fmaf(acc[r], scale, sum[r]);
+                        acc = f32x16_t{};
                     }
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) best[r] = fmaxf(best[r], in ? sum[r] : -INFINITY);
-        }
-        // the maxima over the 32 tokens of the lanes, each step leaving a lane
-        // half of the rows
+            for (int r = 0; r < 16; ++r) best[r] = fmaxf(best[r], kOneScale ? acc[r] * tile.scale[0] : sum[r]);
+        };
+        // after an item's last tile
+        auto finish = [&](const Cursor& c) {
+            const float top = maxima_to_rows(best, l);
 #pragma unroll
-        for (int o = 16, keep = 8; o >= 2; o >>= 1, keep >>= 1) {
-            const bool upper = (l & o) != 0;
-#pragma unroll
-            for (int r = 0; r < keep; ++r) {
-                const float mine = upper ? best[r + keep] : best[r], theirs = upper ? best[r] : best[r + keep];
-                best[r] = fmaxf(mine, __shfl_xor(theirs, o, kWave));
+            for (int r = 0; r < 16; ++r) best[r] = -INFINITY;
+            const float v = qt.back > 0.0f ? top * qt.back : 0.0f;
+            const int64_t item = first_item + 4 * c.item;
+            if (a.splits > 1) {
+                if ((l & 1) == 0)
+                    a.parts[(static_cast<int64_t>(q) * total + item) * rows_padded + q0 + row_of_lane(l)] = v;
+                return;
             }
+            float s = wave_sum(v);
+            float* score = a.scores + static_cast<int64_t>(q) * a.cap + item;
+            if (l == 0) *score = q0 > 0 ? *score + s : s;
+        };
+
+        Cursor now{work, 0, 0, 0, 0};
+        enter(now);
+        Cursor next = now;
+        advance(next);
+        Cursor after = next;
+        advance(after);
+        Tile t0, t1;
+        load_codes(now, load_page(now), t0);
+        int page = load_page(next);
+        auto round = [&](Tile& mine, Tile& other) {
+            load_codes(next, page, other);
+            page = load_page(after);
+            multiply(mine);
+            if (next.item != now.item || next.left == 0) finish(now);
+            now = next;
+            next = after;
+            advance(after);
+        };
+        while (true) {
+            round(t0, t1);
+            if (now.left == 0) break;
+            round(t1, t0);
+            if (now.left == 0) break;
         }
-        best[0] = fmaxf(best[0], __shfl_xor(best[0], 1, kWave)) * qt.back;
-        const int row = QueryTile<T, kFormat, kParts>::row_of(l);
-        if (a.splits > 1) {
-            if ((l & 1) == 0) a.parts[(at * a.splits + split) * rows_padded + q0 + row] = best[0];
-            continue;
-        }
-        float s = (l & 1) == 0 && q0 + row < q_len ? best[0] : 0.0f;
-#pragma unroll
-        for (int o = 2; o < kWave; o <<= 1) s += __shfl_xor(s, o, kWave);
-        total += s;
     }
-    if (a.splits > 1) return;
-    if (l == 0) a.scores[at] = len > 0 ? total : -INFINITY;
 }
 
 // The parts of split documents: a wave a candidate, a lane a query token.
@@ -450,6 +580,9 @@ Split split_of(const chimera_cache_maxsim& m) {
     s.count = static_cast<int>(ceil_div(longest, s.tokens));
     return s;
 }
+
+// Parts of documents a wave takes: as many as leave 8,192 waves, at most 16.
+int items_of(int64_t parts) { return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(parts / 8192, 16))); }
 
 template <typename Call>
 hipError_t by_format(int format, int type, Call&& call) {
@@ -524,11 +657,19 @@ hipError_t launch_cache_maxsim(hipStream_t st, const chimera_cache& c, const chi
     a.cap = m.cand_cap;
     a.split_tokens = s.tokens;
     a.splits = s.count;
-    a.max_tokens = m.max_doc_tokens;
-    const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<int64_t>(m.cand_cap) * s.count, 4)),
-                    static_cast<unsigned>(m.nq));
+    // without pages every token is absent, and no slot may be read
+    a.max_tokens = c.num_pages > 0 && m.num_page_entries > 0 ? m.max_doc_tokens : 0;
+    const int64_t parts = static_cast<int64_t>(m.cand_cap) * s.count;
+    a.items = items_of(m.nq * parts);
+    a.query_vec = aligned16(m.queries, c.dim, type_bytes(m.type));
+    const dim3 grid(static_cast<unsigned>(ceil_div(parts, 4 * a.items)), static_cast<unsigned>(m.nq));
     hipError_t e = by_format(c.format, m.type, [&](auto f, auto t) {
-        hipLaunchKernelGGL((cache_maxsim_kernel<decltype(t), decltype(f)::value>), grid, dim3(256), 0, st, a);
+        using T = decltype(t);
+        constexpr int kFormat = decltype(f)::value;
+        if (a.c.row_scales == 1)
+            hipLaunchKernelGGL((cache_maxsim_kernel<T, kFormat, true>), grid, dim3(256), 0, st, a);
+        else
+            hipLaunchKernelGGL((cache_maxsim_kernel<T, kFormat, false>), grid, dim3(256), 0, st, a);
     });
     if (e != hipSuccess) return e;
     if (s.count > 1) hipLaunchKernelGGL(cache_maxsim_join_kernel, dim3(static_cast<unsigned>(ceil_div(m.cand_cap, 4)), static_cast<unsigned>(m.nq)),

@@ -99,51 +99,6 @@ __device__ __forceinline__ float activation_slope(float z, int act) {
     }
 }
 
-// ---- eight neighbouring values of a row ----------------------------------------
-
-// `vec`: the eight lie within the row and at a multiple of 16 bytes (of 8
-// values of T); otherwise the first `count` of them one by one.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int count, float (&v)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = a[j];
-                v[4 + j] = b[j];
-            }
-        } else {
-            T t[8];
-            *reinterpret_cast<u32x4_t*>(t) = *reinterpret_cast<const u32x4_t*>(p);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.0f;
-}
-
-template <typename T>
-__device__ __forceinline__ void store8(T* p, bool vec, int count, const float (&v)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
-        } else {
-            T t[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
-            *reinterpret_cast<u32x4_t*>(p) = *reinterpret_cast<const u32x4_t*>(t);
-        }
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-        if (j < count) p[j] = from_float<T>(v[j]);
-}
-
 // Whether rows of `stride` elements from p all start at multiples of 16 bytes.
 bool rows_aligned(const void* p, int64_t stride, size_t elem) {
     return (reinterpret_cast<uintptr_t>(p) | (static_cast<uint64_t>(stride) * elem)) % 16 == 0;
