@@ -3,11 +3,12 @@
 //   Z = X W^T + b,  H = act(Z) + R,  Y = H or H / max(|H|, 1e-12)
 //   dH = dY or (dY - Y <Y, dY>) / norm,  dZ = dH act'(Z),
 //   dX = dZ W,  dW = dZ^T X,  db = sum of dZ's rows,  dR = dH
-// All three products are C = A B^T with both operands' rows along the summed
-// axis; the backward pass lays W, X and dZ out that way (transposed) first.
+// The products read X, W and dZ as they lie, with rows along the summed axis
+// or across it.
 #include "operators.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace chimera {
@@ -241,18 +242,33 @@ __device__ __forceinline__ __attribute__((address_space(3))) void* lds_at(void* 
     return (__attribute__((address_space(3))) void*)(p);
 }
 
+// 16 bytes a lane from memory straight to LDS, lane after lane from `to` on.
+__device__ __forceinline__ void load_to_lds(const void* from, void* to) {
+    __builtin_amdgcn_global_load_lds(from, lds_at(to), 16, 0, 0);
+}
+// Of each 16 lanes, lane s gives the address of four 16-bit values, columns
+// 4 (s % 4) on of row s / 4 of a block of 4 x 16; lane i gets column i.
+__device__ __forceinline__ u32x2_t read_transposed(const void* from) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                           (__attribute__((address_space(3))) s16x4*)(from)));
+}
+
 // What lanes past the end of the summed axis load.
 __device__ __align__(256) unsigned char g_zero_chunk[256];
 
+// C [m, n] = the sum over k < sum of A[., k] B[., k]. A matrix lies with its
+// rows along the sum ("[m, sum]"), or across it ("[sum, m]", as X and dZ lie
+// for dW).
 struct Product {
-    const void* a;  // [m, k]
-    const void* b;  // [n, k]
-    int64_t a_stride, b_stride;  // bytes; rows at multiples of 16 bytes
+    const void* a;
+    const void* b;
+    int64_t a_stride, b_stride;  // bytes between rows, multiples of 16 as is the first row's address
     int64_t m;
     int n;
-    int64_t k_bytes;  // of a row, a multiple of 16
+    int64_t sum;  // with rows along it, whole 16-byte chunks; so are m and n with rows across it
     int tiles_m, tiles_n;
-    int steps, steps_per_split;  // of kStepBytes
+    int steps, steps_per_split;  // of kStepBytes along the sum
 };
 
 // ---- tiled product -------------------------------------------------------------
@@ -271,22 +287,139 @@ __device__ __forceinline__ void wait_and_meet() {
     asm volatile("" ::: "memory");
 }
 
-// C tile of BM x BN by WM x WN waves. The rows of A and B, 64 bytes of the
-// summed axis a step, go straight from memory to a ring of four LDS slots:
-// with three steps on their way the loads' latency is covered at full rate
-// (256 x 256 tiles read 16 KB of LDS-bound data in the 512 cycles that a
-// step's products take a wave). Chunk c of row r lies at place c ^ (r / 4 % 4),
-// so that the 16 lanes that follow each other in an LDS read hit different
-// banks. A wave reads the operands of one half of a step while the matrix
-// cores work on the other half.
-template <typename T, int BM, int BN, int WM, int WN, int kSlots>
+// One operand of a tile: 64 bytes of the summed axis of kRows of its rows (or
+// columns, kAcross) a step, B of them in all, loaded by W waves.
+//
+// Rows along the sum: a step is 64 bytes of each row; chunk c of row r lies at
+// place c ^ (r / 4 % 4), so that the lanes that follow each other in an LDS
+// read of 16 bytes hit different banks.
+// Rows across the sum: a step is 32 (or 16, of 32 bits) rows of B values. For
+// 16-bit values the LDS's transposing read gives 16 lanes four values of a
+// column each from four rows of 32 bytes; chunk c of row r lies at place
+// c ^ 2 (r % 4), which puts those four rows in different banks. 32-bit values
+// are read one by one, neighbouring columns in neighbouring lanes.
+template <typename T, int B, int W, bool kAcross>
+struct Side {
+    static constexpr int kBytes = B * kStepBytes;
+    static constexpr int kRowBytes = kAcross ? B * static_cast<int>(sizeof(T)) : kStepBytes;
+    static constexpr int kPieces = kBytes / 1024;                   // one load instruction of a wave each
+    static constexpr int kLoads = (kPieces + W - 1) / W;            // of each wave; some load the same piece
+    static constexpr int kStepRows = kStepBytes / sizeof(T);        // values of the sum a step
+    static constexpr int kPer = 16 / sizeof(T);
+    static constexpr int kTiles = B / 32;
+    const char* base;
+    int64_t step_bytes;  // between steps
+    uint32_t off[kLoads];
+    int at;  // first value of the sum in this lane's chunk (or its row), within a step
+    uint32_t piece[kLoads];
+
+    __device__ __forceinline__ void init(const void* p, int64_t stride, int64_t first, int64_t count, int step0, int w, int l) {
+        const int last = static_cast<int>(min(count - first, static_cast<int64_t>(B))) - 1;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            piece[i] = static_cast<uint32_t>((i * W + w) % kPieces) * 1024u;
+            const int byte = static_cast<int>(piece[i]) + 16 * l;
+            const int row = byte / kRowBytes, place = byte % kRowBytes / 16;
+            if constexpr (kAcross) {
+                const int chunk = sizeof(T) == 2 ? place ^ ((row & 3) << 1) : place;
+                // columns past the end load the last ones
+                off[i] = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) +
+                         16u * static_cast<uint32_t>(min(chunk, last / kPer));
+            } else {
+                const int chunk = place ^ ((row >> 2) & 3);
+                off[i] = static_cast<uint32_t>(min(row, last)) * static_cast<uint32_t>(stride) + 16u * chunk;
+            }
+        }
+        if constexpr (kAcross) {
+            base = static_cast<const char*>(p) + first * static_cast<int64_t>(sizeof(T));
+            step_bytes = kStepRows * stride;
+        } else {
+            // the same chunk for every piece: 16 rows each
+            at = ((l & 3) ^ (l >> 4)) * kPer;
+            base = static_cast<const char*>(p) + first * stride;
+            step_bytes = kStepBytes;
+        }
+        base += step0 * step_bytes;
+    }
+    // `left` values of the sum are left in a step that it ends within; lanes
+    // past them load zeros (an offset is chosen, not a load: every lane takes
+    // part in each).
+    __device__ __forceinline__ void fetch(int s, unsigned char* to, bool whole, int left, int l) const {
+        const char* from = base + s * step_bytes;
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            int64_t o = off[i];
+            if (!whole) {
+                const int first = kAcross ? (static_cast<int>(piece[i]) + 16 * l) / kRowBytes : at;
+                const int64_t zero = reinterpret_cast<const char*>(g_zero_chunk) - from;
+                o = first >= left ? zero : o;
+            }
+            load_to_lds(from + o, to + piece[i]);
+        }
+    }
+};
+
+// The operands of one wave: kCount tiles of 32 rows (or columns) from `first`
+// on, half a step at a time (two 16-byte chunks of the sum, one for each half
+// of the wave).
+template <typename T, int kCount, bool kAcross, int kRowBytes>
+struct Reader {
+    uint32_t off[kAcross && sizeof(T) == 2 ? kCount : 1];
+
+    __device__ __forceinline__ void init(int first, int l) {
+        if constexpr (!kAcross) {
+            off[0] = static_cast<uint32_t>(first + (l & 31)) * kStepBytes + (((l >> 5) ^ ((l >> 2) & 3)) << 4);
+        } else if constexpr (sizeof(T) == 4) {
+            off[0] = static_cast<uint32_t>(4 * (l >> 5)) * kRowBytes + 4u * static_cast<uint32_t>(first + (l & 31));
+        } else {
+            const int row = 8 * (l >> 5) + ((l & 15) >> 2);
+#pragma unroll
+            for (int i = 0; i < kCount; ++i) {
+                const int col = first + 32 * i + 16 * ((l >> 4) & 1) + 4 * (l & 3);
+                off[i] = static_cast<uint32_t>(row) * kRowBytes + (((col >> 3) ^ ((row & 3) << 1)) << 4) + (col & 7) * 2u;
+            }
+        }
+    }
+    __device__ __forceinline__ void read(const unsigned char* from, int half, u32x4_t (&o)[kCount]) const {
+#pragma unroll
+        for (int i = 0; i < kCount; ++i) {
+            if constexpr (!kAcross) {
+                o[i] = *reinterpret_cast<const u32x4_t*>(from + i * 32 * kStepBytes + (off[0] ^ (half << 5)));
+            } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    o[i][j] = *reinterpret_cast<const uint32_t*>(from + (8 * half + j) * kRowBytes + 128 * i + off[0]);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    const u32x2_t u = read_transposed(from + (16 * half + 4 * t) * kRowBytes + off[i]);
+                    o[i][2 * t] = u[0];
+                    o[i][2 * t + 1] = u[1];
+                }
+            }
+        }
+    }
+};
+
+// C tile of BM x BN by WM x WN waves. The operands go straight from memory to
+// a ring of four LDS slots: with three steps on their way the loads' latency
+// is covered at full rate (a step's products take a wave of the 256 x 256 tile
+// 512 cycles). A wave reads the operands of one half of a step while the
+// matrix cores work on the other half.
+// kEnd: the sums are stored, or go through the layer's epilogue, without or
+// with the division by the rows' length (a tile then has all their columns).
+enum End { kSums, kPlainLayer, kNormalizedLayer };
+template <typename T, int BM, int BN, int WM, int WN, bool kAcrossA, bool kAcrossB, End kEnd>
 __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, Epilogue e) {
+    constexpr bool kLayer = kEnd != kSums;
+    constexpr bool kNormalize = kEnd == kNormalizedLayer;
+    constexpr int kSlots = 4;
     constexpr int W = WM * WN;
     constexpr int TM = BM / WM, TN = BN / WN;
     constexpr int IM = TM / 32, IN = TN / 32;
-    constexpr int LA = BM / 16 / W, LB = BN / 16 / W;  // loads of 16 rows per wave and step
-    static_assert(LA * 16 * W == BM && LB * 16 * W == BN, "every wave loads the same number of rows");
-    constexpr int kSlot = (BM + BN) * kStepBytes;
+    using SideA = Side<T, BM, W, kAcrossA>;
+    using SideB = Side<T, BN, W, kAcrossB>;
+    constexpr int kSlot = SideA::kBytes + SideB::kBytes;
     constexpr int kPitch = TN + 4;
     constexpr int kStage = W * 32 * kPitch * 4;
     __shared__ __align__(1024) unsigned char lds[kSlots * kSlot > kStage ? kSlots * kSlot : kStage];
@@ -311,66 +444,35 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     const int step0 = split * p.steps_per_split;
     const int steps = min(p.steps_per_split, p.steps - step0);
 
-    // lane l loads chunk (l % 4) ^ (l / 16) of row l / 4 of its sixteen rows;
-    // rows past the end load the last row
-    const int chunk = (l & 3) ^ (l >> 4);
-    const char* base_a = static_cast<const char*>(p.a) + m0 * p.a_stride + static_cast<int64_t>(step0) * kStepBytes;
-    const char* base_b = static_cast<const char*>(p.b) + n0 * p.b_stride + static_cast<int64_t>(step0) * kStepBytes;
-    uint32_t off_a[LA], off_b[LB];
-    const int last_a = static_cast<int>(min(p.m - m0, static_cast<int64_t>(BM))) - 1, last_b = min(p.n - n0, BN) - 1;
-#pragma unroll
-    for (int i = 0; i < LA; ++i)
-        off_a[i] = static_cast<uint32_t>(min((i * W + w) * 16 + (l >> 2), last_a)) * static_cast<uint32_t>(p.a_stride) +
-                   16u * chunk;
-#pragma unroll
-    for (int i = 0; i < LB; ++i)
-        off_b[i] = static_cast<uint32_t>(min((i * W + w) * 16 + (l >> 2), last_b)) * static_cast<uint32_t>(p.b_stride) +
-                   16u * chunk;
-    auto fetch = [&](int s, auto whole) {
+    SideA side_a;
+    SideB side_b;
+    side_a.init(p.a, p.a_stride, m0, p.m, step0, w, l);
+    side_b.init(p.b, p.b_stride, n0, p.n, step0, w, l);
+    Reader<T, IM, kAcrossA, SideA::kRowBytes> reader_a;
+    Reader<T, IN, kAcrossB, SideB::kRowBytes> reader_b;
+    reader_a.init(wm * TM, l);
+    reader_b.init(wn * TN, l);
+    // steps before the one that the sum ends within, if there is one
+    const int left = static_cast<int>(p.sum % SideA::kStepRows);
+    const int whole = steps - (left != 0 && step0 + steps == p.steps ? 1 : 0);
+    auto fetch = [&](int s, auto is_whole) {
         unsigned char* to = lds + s % kSlots * kSlot;
-        const char* a = base_a + static_cast<int64_t>(s) * kStepBytes;
-        const char* b = base_b + static_cast<int64_t>(s) * kStepBytes;
-        // in its last step, lanes past the end of the summed axis load zeros
-        // (an offset is chosen, not a load: every lane takes part in each)
-        const bool zero = !whole && 16 * chunk >= p.k_bytes % kStepBytes;
-        const int64_t zero_a = reinterpret_cast<const char*>(g_zero_chunk) - a;
-        const int64_t zero_b = reinterpret_cast<const char*>(g_zero_chunk) - b;
-#pragma unroll
-        for (int i = 0; i < LA; ++i)
-            __builtin_amdgcn_global_load_lds(a + (zero ? zero_a : static_cast<int64_t>(off_a[i])),
-                                             lds_at(to + (i * W + w) * 1024), 16, 0, 0);
-#pragma unroll
-        for (int i = 0; i < LB; ++i)
-            __builtin_amdgcn_global_load_lds(b + (zero ? zero_b : static_cast<int64_t>(off_b[i])),
-                                             lds_at(to + BM * kStepBytes + (i * W + w) * 1024), 16, 0, 0);
+        side_a.fetch(s, to, is_whole, left, l);
+        side_b.fetch(s, to + SideA::kBytes, is_whole, left, l);
     };
-    // steps before the one that the axis ends within, if there is one
-    const bool partial = p.k_bytes % kStepBytes != 0 && step0 + steps == p.steps;
-    const int whole = steps - (partial ? 1 : 0);
-    constexpr auto kWhole = std::true_type{};
-    constexpr auto kPartial = std::false_type{};
 
     f32x16_t acc[IM][IN];
 #pragma unroll
     for (int i = 0; i < IM; ++i)
 #pragma unroll
         for (int j = 0; j < IN; ++j) acc[i][j] = f32x16_t{};
-
-    // halves of a step: chunks 0, 1 and 2, 3
-    const uint32_t place = (((l >> 5) ^ ((l >> 2) & 3)) << 4);
-    const uint32_t row_a = (wm * TM + (l & 31)) * kStepBytes + place;
-    const uint32_t row_b = BM * kStepBytes + (wn * TN + (l & 31)) * kStepBytes + place;
     struct Operands {
         u32x4_t a[IM], b[IN];
     };
     auto read = [&](int s, int half, Operands& o) {
         const unsigned char* from = lds + s % kSlots * kSlot;
-#pragma unroll
-        for (int i = 0; i < IM; ++i)
-            o.a[i] = *reinterpret_cast<const u32x4_t*>(from + i * 32 * kStepBytes + (row_a ^ (half << 5)));
-#pragma unroll
-        for (int j = 0; j < IN; ++j)
-            o.b[j] = *reinterpret_cast<const u32x4_t*>(from + j * 32 * kStepBytes + (row_b ^ (half << 5)));
+        reader_a.read(from, half, o.a);
+        reader_b.read(from + SideA::kBytes, half, o.b);
     };
     auto multiply = [&](const Operands& o) {
 #pragma unroll
@@ -379,7 +481,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
             for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(o.b[j], o.a[i], acc[i][j]);
     };
 
-    constexpr int kLoads = LA + LB;
+    constexpr int kLoads = SideA::kLoads + SideB::kLoads;
     Operands first, second;
 #pragma unroll
     for (int i = 0; i < IM; ++i) second.a[i] = u32x4_t{0, 0, 0, 0};
@@ -400,6 +502,8 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
         __builtin_amdgcn_sched_barrier(0);
     };
     constexpr int kAhead = kSlots - 1;
+    constexpr auto kWhole = std::true_type{};
+    constexpr auto kPartial = std::false_type{};
 #pragma unroll
     for (int s = 0; s < kAhead; ++s) {
         if (s < whole)
@@ -482,15 +586,17 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
         });
     };
     float bias[IN][16];
+    if constexpr (kLayer) {
 #pragma unroll
-    for (int j = 0; j < IN; ++j)
+        for (int j = 0; j < IN; ++j)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int n = col0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
-            bias[j][r] = e.bias && n < e.n ? to_float(static_cast<const T*>(e.bias)[n]) : 0.0f;
-        }
+            for (int r = 0; r < 16; ++r) {
+                const int n = col0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
+                bias[j][r] = e.bias && n < e.n ? to_float(static_cast<const T*>(e.bias)[n]) : 0.0f;
+            }
+    }
     // what is left to do after LDS: nothing, or something in 32 bits
-    const bool narrow = sizeof(T) == 2 && !e.out_f32 && !e.partial && (!e.residual || e.normalize);
+    const bool narrow = sizeof(T) == 2 && !e.out_f32 && !e.partial && (!kLayer || kNormalize || !e.residual);
 #pragma unroll
     for (int i = 0; i < IM; ++i) {
         const int64_t m_first = m0 + wm * TM + 32 * i;
@@ -498,33 +604,46 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
 #pragma unroll
         for (int j = 0; j < IN; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) v[j][r] = acc[i][j][r] + bias[j][r];
-        if (e.saved) {
-            put(v, T{});
-            copy_out(e.saved, e.saved_stride, e.saved_vec, m_first);
-        }
-        activate<T>(v, e.act);
-        if (e.normalize) {
-            const int64_t m = m_first + (l & 31);
-            float s = 0.0f;
+            for (int r = 0; r < 16; ++r) v[j][r] = kLayer ? acc[i][j][r] + bias[j][r] : acc[i][j][r];
+        if constexpr (kLayer) {
+            if (e.saved) {
+                put(v, T{});
+                copy_out(e.saved, e.saved_stride, e.saved_vec, m_first);
+            }
+            activate<T>(v, e.act);
+            if constexpr (kNormalize) {
+                const int64_t m = m_first + (l & 31);
+                float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < IN; ++j)
+                for (int j = 0; j < IN; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int n = col0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
-                    if (e.residual && m < e.m && n < e.n)
-                        v[j][r] += to_float(static_cast<const T*>(e.residual)[m * e.residual_stride + n]);
-                    s = n < e.n ? fmaf(v[j][r], v[j][r], s) : s;
+                    for (int r = 0; r < 16; ++r) {
+                        const int n = col0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
+                        if (e.residual && m < e.m && n < e.n)
+                            v[j][r] += to_float(static_cast<const T*>(e.residual)[m * e.residual_stride + n]);
+                        sum = n < e.n ? fmaf(v[j][r], v[j][r], sum) : sum;
+                    }
+                sum += __shfl_xor(sum, 32, kWave);
+                if constexpr (WN > 1) {
+                    static_assert(IM == 1, "one exchange of the waves' sums");
+                    float* sums = reinterpret_cast<float*>(lds);
+                    __syncthreads();
+                    if (half == 0) sums[w * 32 + l] = sum;
+                    __syncthreads();
+                    sum = 0.0f;
+#pragma unroll
+                    for (int o = 0; o < WN; ++o) sum += sums[(wm * WN + o) * 32 + (l & 31)];
+                    __syncthreads();  // the rows go through the same LDS next
                 }
-            s += __shfl_xor(s, 32, kWave);
-            const float norm = sqrtf(s);
-            const float held = norm < kLeastNorm ? kLeastNorm : norm;  // NaN stays
-            const float inv = 1.0f / held;
+                const float norm = sqrtf(sum);
+                const float held = norm < kLeastNorm ? kLeastNorm : norm;  // NaN stays
+                const float inv = 1.0f / held;
 #pragma unroll
-            for (int j = 0; j < IN; ++j)
+                for (int j = 0; j < IN; ++j)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) v[j][r] *= inv;
-            if (e.norms && half == 0 && m < e.m) e.norms[m] = held;
+                    for (int r = 0; r < 16; ++r) v[j][r] *= inv;
+                if (e.norms && wn == 0 && half == 0 && m < e.m) e.norms[m] = held;
+            }
         }
         if (narrow) {
             put(v, T{});
@@ -544,7 +663,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
                 store8(e.partial + (split * e.m + m) * e.n + n, inside || (whole && e.y_vec), count, u);
                 return;
             }
-            if (e.residual && !e.normalize) {
+            if (kLayer && !kNormalize && e.residual) {
                 float r[8];
                 load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n, inside || (whole && e.residual_vec),
                       count, r);
@@ -646,25 +765,6 @@ __global__ __launch_bounds__(256) void linear_align_kernel(const T* __restrict__
     }
 }
 
-// dst [cols][dst_cols] = src^T, zeros from column `rows` on; dst_cols a
-// multiple of 64. A block takes 64 x 64 values.
-template <typename T>
-__global__ __launch_bounds__(256) void linear_transpose_kernel(const T* __restrict__ src, int64_t src_stride,
-                                                               int64_t rows, int cols, T* __restrict__ dst,
-                                                               int64_t dst_cols) {
-    __shared__ T tile[64][65];
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * 64;
-    const int c0 = static_cast<int>(blockIdx.y) * 64;
-    const int x = static_cast<int>(threadIdx.x) & 63, y = static_cast<int>(threadIdx.x) >> 6;
-#pragma unroll 4
-    for (int i = y; i < 64; i += 4)
-        tile[i][x] = r0 + i < rows && c0 + x < cols ? src[(r0 + i) * src_stride + c0 + x] : from_float<T>(0.0f);
-    __syncthreads();
-#pragma unroll 4
-    for (int i = y; i < 64; i += 4)
-        if (c0 + i < cols) dst[static_cast<int64_t>(c0 + i) * dst_cols + r0 + x] = tile[x][i];
-}
-
 // ---- the gradient before the products ------------------------------------------
 
 struct GradArgs {
@@ -673,30 +773,28 @@ struct GradArgs {
     const void* saved;
     const float* norms;
     void* dresidual;
-    void* g;    // dZ [m][g_cols], zeros from column n on, or NULL
-    void* gt;   // dZ^T [n][gt_cols], zeros from column m on, or NULL
-    float* sums;  // column sums of dZ by blocks of 64 rows [blocks][n], or NULL
-    int64_t dy_stride, y_stride, saved_stride, dresidual_stride, gt_cols;
+    void* g;      // dZ [m][g_cols], zeros from column n on, or NULL
+    float* sums;  // column sums of dZ by blocks of rows [blocks][n], or NULL
+    int64_t dy_stride, y_stride, saved_stride, dresidual_stride;
     int64_t m;
     int n, g_cols, act;
+    int block_rows;  // a multiple of 16
     bool out_f32, normalize, dy_vec, y_vec, saved_vec, dresidual_vec;
 };
 
-// 64 rows x 128 columns a block, eight neighbouring columns of four rows a
-// thread: with normalize (n <= 128) a row is 16 neighbouring lanes.
+// 16 rows x 128 columns at a time, eight neighbouring columns a thread: with
+// normalize (n <= 128) a row is 16 neighbouring lanes. Bound by memory.
 template <typename T>
 __global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
-    __shared__ T tile[64][129];
     __shared__ float sums[16][129];
     const int tid = static_cast<int>(threadIdx.x);
     const int col = tid % 16 * 8, n0 = static_cast<int>(blockIdx.y) * 128 + col;
-    const int64_t m0 = static_cast<int64_t>(blockIdx.x) * 64;
+    const int64_t m_end = min((blockIdx.x + int64_t{1}) * a.block_rows, a.m);
     float sum[8] = {};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int row = tid / 16 + 16 * i;
-        const int64_t m = m0 + row;
-        const int count = m < a.m ? a.n - n0 : 0;
+#pragma unroll 2
+    for (int64_t m0 = static_cast<int64_t>(blockIdx.x) * a.block_rows; m0 < m_end; m0 += 16) {
+        const int64_t m = m0 + tid / 16;
+        const int count = m < m_end ? a.n - n0 : 0;
         const bool whole = count >= 8;
         float g[8] = {};
         auto load = [&](const void* p, int64_t stride, bool vec, float(&v)[8]) {
@@ -723,61 +821,76 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
         if (a.dresidual && count > 0)
             store8(static_cast<T*>(a.dresidual) + m * a.dresidual_stride + n0, whole && a.dresidual_vec, count, g);
         if (a.act != CHIMERA_ACT_NONE && count > 0) {
-            float z[8];
+            float z[8], slope[8];
             load8(static_cast<const T*>(a.saved) + m * a.saved_stride + n0, whole && a.saved_vec, count, z);
-            float slope[8];
             slope8(z, slope, a.act);
 #pragma unroll
             for (int j = 0; j < 8; ++j) g[j] = j < count ? g[j] * slope[j] : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += g[j];
-        if (a.g && m < a.m && n0 < a.g_cols) store8(static_cast<T*>(a.g) + m * a.g_cols + n0, true, 8, g);
-        if (a.gt) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) tile[row][col + j] = from_float<T>(g[j]);
-        }
+        if (a.g && m < m_end && n0 < a.g_cols) store8(static_cast<T*>(a.g) + m * a.g_cols + n0, true, 8, g);
     }
-    if (a.sums) {
+    if (!a.sums) return;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sums[tid / 16][col + j] = sum[j];
-    }
+    for (int j = 0; j < 8; ++j) sums[tid / 16][col + j] = sum[j];
     __syncthreads();
     const int nb = static_cast<int>(blockIdx.y) * 128;
-    if (a.sums && tid < 128 && nb + tid < a.n) {
+    if (tid < 128 && nb + tid < a.n) {
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) s += sums[i][tid];
         a.sums[static_cast<int64_t>(blockIdx.x) * a.n + nb + tid] = s;
     }
-    if (a.gt) {
-        for (int i = tid; i < 128 * 64; i += 256) {
-            const int c = i / 64, r = i % 64;
-            if (nb + c < a.n) static_cast<T*>(a.gt)[static_cast<int64_t>(nb + c) * a.gt_cols + m0 + r] = tile[r][c];
-        }
-    }
 }
 
-// dst[i] = sum over s of src[s][i], in order, for i < count: the parts of a
-// split product (rows of `cols` values to rows of dst_stride) or the blocks'
-// column sums. Four waves share the parts of 64 values.
+// db[n] = the sum of the blocks' column sums, in order: 16 waves share the
+// blocks, a lane a column.
 template <typename T>
-__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ src, int64_t parts, int64_t count,
-                                                          int cols, T* __restrict__ dst, int64_t dst_stride) {
-    __shared__ float sums[4][kWave];
+__global__ __launch_bounds__(1024) void linear_sums_kernel(const float* __restrict__ src, int parts, int n,
+                                                           T* __restrict__ dst) {
+    __shared__ float sums[16][kWave];
     const int l = lane_id(), w = wave_id();
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * kWave + l;
-    const int64_t share = (parts + 3) / 4;
+    const int i = static_cast<int>(blockIdx.x) * kWave + l;
+    const int share = (parts + 15) / 16;
     float s = 0.0f;
-    if (i < count) {
-        const int64_t end = min(parts, (w + 1) * share);
-        for (int64_t k = w * share; k < end; ++k) s += src[k * count + i];
+    if (i < n) {
+        const int end = min(parts, (w + 1) * share);
+#pragma unroll 8
+        for (int k = w * share; k < end; ++k) s += src[static_cast<int64_t>(k) * n + i];
     }
     sums[w][l] = s;
     __syncthreads();
-    if (w != 0 || i >= count) return;
-    s = ((sums[0][l] + sums[1][l]) + sums[2][l]) + sums[3][l];
-    dst[i / cols * dst_stride + i % cols] = from_float<T>(s);
+    if (w != 0 || i >= n) return;
+    s = 0.0f;
+#pragma unroll
+    for (int o = 0; o < 16; ++o) s += sums[o][l];
+    dst[i] = from_float<T>(s);
+}
+
+// dst (rows of `cols` values at dst_stride) = the sum over s of src[s], the
+// parts of a split product, in order; kPer neighbouring values a thread.
+template <typename T, int kPer>
+__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ src, int parts, int64_t count,
+                                                          int cols, T* __restrict__ dst, int64_t dst_stride) {
+    const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * kPer;
+    if (i >= count) return;
+    float s[kPer] = {};
+#pragma unroll 4
+    for (int k = 0; k < parts; ++k) {
+        const float* p = src + k * count + i;
+        if constexpr (kPer == 4) {
+            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(p);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += v[j];
+        } else {
+            s[0] += p[0];
+        }
+    }
+    const int64_t row = i / cols;
+    T* to = dst + row * dst_stride + (i - row * cols);
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) to[j] = from_float<T>(s[j]);
 }
 
 template <typename T>
@@ -803,32 +916,96 @@ struct Carve {
     }
 };
 
-constexpr int kNormalizeCols = 128;
 // Rows up to which a product without a split goes by 16 rows a block.
 constexpr int64_t kFewRows = 64;
 
-template <typename T>
-void launch_tiles(hipStream_t st, Product p, Epilogue e, int splits) {
-    p.steps = static_cast<int>(ceil_div(p.k_bytes, kStepBytes));
+constexpr int kCus = 256;
+
+// Which tile a product takes: the one with the least of
+//   (tiles that the busiest of the 256 CUs gets) x (area) / (rate)
+// with the rate of a CU on that tile, relative to the largest (16-bit
+// operands: 65,536 x 1024 -> 4096 takes 590 us on tiles of 256, 700 of 128;
+// 32-bit operands are bound by the matrix cores on any of them).
+struct TileChoice {
+    int size;
+    double rate16, rate32;
+};
+constexpr TileChoice kTileChoices[3] = {{256, 1.0, 1.0}, {128, 0.8, 0.95}, {64, 0.45, 0.85}};
+
+struct TilePlan {
+    int size, splits;
+};
+
+// With splits allowed, parts of the sum (16 steps at least) go to blocks of
+// their own where there are few tiles; the parts' bytes are written and read
+// once more at 4 TB/s, and the join is a launch of its own.
+TilePlan tile_plan(int64_t m, int64_t n, int64_t sum, size_t elem, bool may_split) {
+    const int64_t steps = ceil_div(sum * static_cast<int64_t>(elem), kStepBytes);
+    const double cu_rate = elem == 4 ? 0.5e6 : 4.5e6;  // operations a microsecond
+    TilePlan best = {256, 1};
+    double least = 0.0;
+    for (const TileChoice& c : kTileChoices) {
+        const double tiles = static_cast<double>(ceil_div(m, c.size)) * static_cast<double>(ceil_div(n, c.size));
+        const double tile_us = 2.0 * c.size * c.size * static_cast<double>(sum) / (cu_rate * (elem == 4 ? c.rate32 : c.rate16));
+        for (int64_t splits = 1; splits == 1 || (may_split && splits <= 256 && steps / splits >= 16); splits *= 2) {
+            double us = std::ceil(tiles * static_cast<double>(splits) / kCus) * tile_us / static_cast<double>(splits);
+            if (splits > 1) us += 3.0 + static_cast<double>(splits * m * n) * 8.0 / 4e6;
+            if ((c.size == 256 && splits == 1) || us < least) {
+                least = us;
+                best = {c.size, static_cast<int>(splits)};
+            }
+        }
+    }
+    return best;
+}
+
+template <typename T, bool kAcrossA, bool kAcrossB, End kEnd>
+void launch_tiles(hipStream_t st, Product p, const Epilogue& e, TilePlan plan) {
+    int splits = plan.splits;
+    p.steps = static_cast<int>(ceil_div(p.sum * static_cast<int64_t>(sizeof(T)), kStepBytes));
     p.steps_per_split = static_cast<int>(ceil_div(p.steps, splits));
     splits = static_cast<int>(ceil_div(p.steps, p.steps_per_split));
-    auto plan = [&](int bm, int bn) {
-        p.tiles_m = static_cast<int>(ceil_div(p.m, bm));
-        p.tiles_n = static_cast<int>(ceil_div(p.n, bn));
-        return dim3(static_cast<unsigned>(p.tiles_m * p.tiles_n), static_cast<unsigned>(splits));
+    auto launch = [&](auto bm, auto bn, auto wm, auto wn) {
+        constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
+        p.tiles_m = static_cast<int>(ceil_div(p.m, BM));
+        p.tiles_n = static_cast<int>(ceil_div(p.n, BN));
+        const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), static_cast<unsigned>(splits));
+        hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, kAcrossA, kAcrossB, kEnd>), grid, dim3(WM * WN * kWave),
+                           0, st, p, e);
     };
-    if (e.normalize) {
-        const dim3 grid = plan(128, 128);
-        hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 4, 1, 4>), grid, dim3(256), 0, st, p, e);
+    using std::integral_constant;
+    if constexpr (kEnd == kNormalizedLayer) {
+        // a block has whole rows: 32 of them where 128 leave CUs idle
+        if (ceil_div(ceil_div(p.m, 32), kCus) * 32 < ceil_div(ceil_div(p.m, 128), kCus) * 128)
+            launch(integral_constant<int, 32>{}, integral_constant<int, 128>{}, integral_constant<int, 1>{},
+                   integral_constant<int, 4>{});
+        else
+            launch(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{},
+                   integral_constant<int, 1>{});
         return;
+    } else {
+    switch (plan.size) {
+        case 256:
+            launch(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{},
+                   integral_constant<int, 4>{});
+            break;
+        case 128:
+            launch(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{},
+                   integral_constant<int, 2>{});
+            break;
+        default:
+            launch(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
+                   integral_constant<int, 2>{});
     }
-    if (ceil_div(p.m, 256) * ceil_div(p.n, 256) * splits >= 256) {
-        const dim3 grid = plan(256, 256);
-        hipLaunchKernelGGL((linear_tile_kernel<T, 256, 256, 2, 4, 4>), grid, dim3(512), 0, st, p, e);
-        return;
     }
-    const dim3 grid = plan(128, 128);
-    hipLaunchKernelGGL((linear_tile_kernel<T, 128, 128, 2, 2, 4>), grid, dim3(256), 0, st, p, e);
+}
+
+// Whether a product's loads can take a matrix as it lies: rows that start at
+// multiples of 16 bytes and end at one, a tile's rows within 32-bit offsets.
+template <typename T>
+bool takes_loads(const void* p, int64_t stride, int64_t cols) {
+    return rows_aligned(p, stride, sizeof(T)) && cols * static_cast<int64_t>(sizeof(T)) % 16 == 0 &&
+           stride * static_cast<int64_t>(sizeof(T)) <= (int64_t{1} << 22);
 }
 
 // A matrix as a product reads it: as it lies where its rows start at
@@ -836,12 +1013,10 @@ void launch_tiles(hipStream_t st, Product p, Epilogue e, int splits) {
 // (rows x round_up(cols, 64)).
 template <typename T>
 void aligned_rows(hipStream_t st, const void* src, int64_t stride, int64_t rows, int cols, void* copy, const void** p,
-                  int64_t* stride_bytes, int64_t* k_bytes) {
-    constexpr int64_t kMostStride = int64_t{1} << 22;  // a tile's rows within 32-bit offsets
-    if (rows_aligned(src, stride, sizeof(T)) && cols * sizeof(T) % 16 == 0 && stride * static_cast<int64_t>(sizeof(T)) <= kMostStride) {
+                  int64_t* stride_bytes) {
+    if (takes_loads<T>(src, stride, cols)) {
         *p = src;
         *stride_bytes = stride * static_cast<int64_t>(sizeof(T));
-        *k_bytes = cols * static_cast<int64_t>(sizeof(T));
         return;
     }
     const int wide = static_cast<int>(round_up(cols, 64));
@@ -851,7 +1026,6 @@ void aligned_rows(hipStream_t st, const void* src, int64_t stride, int64_t rows,
                        cols, static_cast<T*>(copy), wide);
     *p = copy;
     *stride_bytes = wide * static_cast<int64_t>(sizeof(T));
-    *k_bytes = *stride_bytes;
 }
 
 struct ForwardPlan {
@@ -910,43 +1084,41 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     }
     ForwardPlan plan;
     (void)carve_forward(s, a.workspace, &plan);
-    int64_t k_x = 0, k_w = 0;
-    aligned_rows<T>(st, a.x, a.x_stride, s.rows, s.in_features, plan.x, &p.a, &p.a_stride, &k_x);
-    aligned_rows<T>(st, a.weight, a.weight_stride, s.out_features, s.in_features, plan.weight, &p.b, &p.b_stride, &k_w);
-    p.k_bytes = std::min(k_x, k_w);
-    launch_tiles<T>(st, p, e, 1);
+    aligned_rows<T>(st, a.x, a.x_stride, s.rows, s.in_features, plan.x, &p.a, &p.a_stride);
+    aligned_rows<T>(st, a.weight, a.weight_stride, s.out_features, s.in_features, plan.weight, &p.b, &p.b_stride);
+    // whole chunks: as the matrices lie, or both laid out again with zeros
+    p.sum = round_up(s.in_features, 16 / sizeof(T));
+    const TilePlan tiles = tile_plan(p.m, p.n, p.sum, sizeof(T), false);
+    if (e.normalize)
+        launch_tiles<T, false, false, kNormalizedLayer>(st, p, e, tiles);
+    else
+        launch_tiles<T, false, false, kPlainLayer>(st, p, e, tiles);
     return hipGetLastError();
 }
 
 struct BackwardPlan {
-    int64_t m_pad;
     int n_pad;
-    int splits;
-    void *g, *gt, *xt, *wt;
+    int block_rows;  // of the gradient kernel
+    TilePlan dweight;
+    void *g, *x, *weight;
     float *sums, *parts;
 };
-
-// Parts of dW's sum over the rows: enough blocks of 128 x 128 for the GPU,
-// sixteen steps of 64 bytes a part at least.
-int dweight_splits(const chimera_linear_shape& s) {
-    const int64_t tiles = ceil_div(s.out_features, 128) * ceil_div(s.in_features, 128);
-    const int64_t steps = ceil_div(round_up(s.rows, 64) * type_bytes(s.type), kStepBytes);
-    return static_cast<int>(std::max<int64_t>(1, std::min(ceil_div(512, tiles), steps / 16)));
-}
 
 size_t carve_backward(const chimera_linear_shape& s, void* base, BackwardPlan* plan) {
     Carve c{static_cast<char*>(base)};
     const size_t e = type_bytes(s.type);
-    plan->m_pad = round_up(s.rows, 64);
-    plan->n_pad = static_cast<int>(round_up(s.out_features, 64));
-    plan->splits = dweight_splits(s);
     const size_t k = static_cast<size_t>(s.in_features), n = static_cast<size_t>(s.out_features);
+    const size_t wide = round_up(s.in_features, 64) * e;
+    plan->n_pad = static_cast<int>(round_up(s.out_features, 64));
+    // about 1,024 blocks of 16 to 512 rows
+    plan->block_rows = static_cast<int>(std::max<int64_t>(
+        16, std::min<int64_t>(512, round_up(ceil_div(s.rows * ceil_div(s.out_features, 128), 1024), 16))));
+    plan->dweight = tile_plan(s.out_features, s.in_features, s.rows, e, true);
     plan->g = c.take(static_cast<size_t>(s.rows) * plan->n_pad * e);
-    plan->gt = c.take(n * plan->m_pad * e);
-    plan->xt = c.take(k * plan->m_pad * e);
-    plan->wt = c.take(k * plan->n_pad * e);
-    plan->sums = static_cast<float*>(c.take(static_cast<size_t>(plan->m_pad / 64) * n * 4));
-    plan->parts = static_cast<float*>(c.take(plan->splits > 1 ? plan->splits * n * k * 4 : 0));
+    plan->x = c.take(static_cast<size_t>(s.rows) * wide);
+    plan->weight = c.take(n * wide);
+    plan->sums = static_cast<float*>(c.take(static_cast<size_t>(ceil_div(s.rows, plan->block_rows)) * n * 4));
+    plan->parts = static_cast<float*>(c.take(plan->dweight.splits > 1 ? plan->dweight.splits * n * k * 4 : 0));
     return c.off;
 }
 
@@ -966,75 +1138,85 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
     }
     BackwardPlan plan;
     (void)carve_backward(s, a.workspace, &plan);
-    const size_t out = s.out_type == CHIMERA_F32 ? 4 : sizeof(T);
-    const unsigned row_blocks = static_cast<unsigned>(plan.m_pad / 64);
+    const size_t out = type_bytes(s.out_type);
+    // where dZ is dY as it lies, the products read dY
+    const bool as_it_is = s.activation == CHIMERA_ACT_NONE && !s.normalize && out == sizeof(T) &&
+                          takes_loads<T>(a.dy, a.dy_stride, n);
+    const bool products = a.dx || a.dweight;
     GradArgs g = {};
     g.dy = a.dy;
     g.y = a.y;
     g.saved = a.saved;
     g.norms = a.norms;
     g.dresidual = a.dresidual;
-    g.g = a.dx ? plan.g : nullptr;
-    g.gt = a.dweight ? plan.gt : nullptr;
+    g.g = products && !as_it_is ? plan.g : nullptr;
     g.sums = a.dbias ? plan.sums : nullptr;
     g.dy_stride = a.dy_stride;
     g.y_stride = a.y_stride;
     g.saved_stride = a.saved_stride;
     g.dresidual_stride = a.dresidual_stride;
-    g.gt_cols = plan.m_pad;
     g.m = s.rows;
     g.n = n;
     g.g_cols = plan.n_pad;
     g.act = s.activation;
+    g.block_rows = plan.block_rows;
     g.out_f32 = out == 4;
     g.normalize = s.normalize != 0;
     g.dy_vec = rows_aligned(a.dy, a.dy_stride, out);
     g.y_vec = rows_aligned(a.y, a.y_stride, out);
     g.saved_vec = rows_aligned(a.saved, a.saved_stride, sizeof(T));
     g.dresidual_vec = rows_aligned(a.dresidual, a.dresidual_stride, sizeof(T));
-    hipLaunchKernelGGL((linear_grad_kernel<T>), dim3(row_blocks, static_cast<unsigned>(ceil_div(n, 128))), dim3(256), 0, st, g);
-    auto join = [&](const float* src, int64_t parts, int64_t count, int cols, void* dst, int64_t stride) {
-        hipLaunchKernelGGL((linear_join_kernel<T>), dim3(static_cast<unsigned>(ceil_div(count, kWave))), dim3(256), 0, st,
-                           src, parts, count, cols, static_cast<T*>(dst), stride);
-    };
-    if (a.dbias) join(plan.sums, row_blocks, n, n, a.dbias, n);
-    auto product = [&](const void* pa, int64_t m, int64_t sum, const void* pb, int cols, void* dst, int64_t stride,
-                       int splits) {
-        Product p = {};
-        p.a = pa;
-        p.b = pb;
-        p.a_stride = p.b_stride = p.k_bytes = sum * static_cast<int64_t>(sizeof(T));
-        p.m = m;
-        p.n = cols;
-        Epilogue e = {};
+    const int64_t blocks = ceil_div(s.rows, plan.block_rows);
+    if (g.g || g.sums || g.dresidual)
+        hipLaunchKernelGGL((linear_grad_kernel<T>),
+                           dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(ceil_div(n, 128))), dim3(256), 0, st, g);
+    if (a.dbias)
+        hipLaunchKernelGGL((linear_sums_kernel<T>), dim3(static_cast<unsigned>(ceil_div(n, kWave))), dim3(1024), 0, st,
+                           plan.sums, static_cast<int>(blocks), n, static_cast<T*>(a.dbias));
+    const void* dz = as_it_is ? a.dy : plan.g;
+    const int64_t dz_stride = (as_it_is ? a.dy_stride : plan.n_pad) * static_cast<int64_t>(sizeof(T));
+    auto product_to = [&](Product& p, Epilogue& e, int64_t m, int cols, int64_t sum, void* dst, int64_t stride) {
+        p.m = e.m = m;
+        p.n = e.n = cols;
+        p.sum = sum;
         e.y = dst;
         e.y_stride = stride;
-        e.m = m;
-        e.n = cols;
         e.out_f32 = sizeof(T) == 4;
-        e.y_vec = rows_aligned(dst, stride, sizeof(T));
-        if (splits > 1) {
-            e.partial = plan.parts;
-            e.y_vec = cols % 4 == 0;
-        }
-        e.vec = e.y_vec;
-        launch_tiles<T>(st, p, e, splits);
-        if (splits > 1) {
-            const int64_t steps = ceil_div(p.k_bytes, kStepBytes);
-            join(plan.parts, ceil_div(steps, ceil_div(steps, splits)), m * cols, cols, dst, stride);
-        }
+        e.vec = e.y_vec = rows_aligned(dst, stride, sizeof(T));
     };
     if (a.dx) {
-        hipLaunchKernelGGL((linear_transpose_kernel<T>),
-                           dim3(static_cast<unsigned>(plan.n_pad / 64), static_cast<unsigned>(ceil_div(k, 64))), dim3(256),
-                           0, st, static_cast<const T*>(a.weight), a.weight_stride, static_cast<int64_t>(n), k,
-                           static_cast<T*>(plan.wt), static_cast<int64_t>(plan.n_pad));
-        product(plan.g, s.rows, plan.n_pad, plan.wt, k, a.dx, a.dx_stride, 1);
+        Product p = {};
+        Epilogue e = {};
+        product_to(p, e, s.rows, k, n, a.dx, a.dx_stride);
+        p.a = dz;
+        p.a_stride = dz_stride;
+        aligned_rows<T>(st, a.weight, a.weight_stride, n, k, plan.weight, &p.b, &p.b_stride);
+        launch_tiles<T, false, true, kSums>(st, p, e, tile_plan(p.m, p.n, p.sum, sizeof(T), false));
     }
     if (a.dweight) {
-        hipLaunchKernelGGL((linear_transpose_kernel<T>), dim3(row_blocks, static_cast<unsigned>(ceil_div(k, 64))), dim3(256),
-                           0, st, static_cast<const T*>(a.x), a.x_stride, s.rows, k, static_cast<T*>(plan.xt), plan.m_pad);
-        product(plan.gt, n, plan.m_pad, plan.xt, k, a.dweight, a.dweight_stride, plan.splits);
+        Product p = {};
+        Epilogue e = {};
+        product_to(p, e, n, k, s.rows, a.dweight, a.dweight_stride);
+        p.a = dz;
+        p.a_stride = dz_stride;
+        aligned_rows<T>(st, a.x, a.x_stride, s.rows, k, plan.x, &p.b, &p.b_stride);
+        const int splits = plan.dweight.splits;
+        if (splits > 1) {
+            e.partial = plan.parts;
+            e.vec = e.y_vec = k % 4 == 0;
+        }
+        launch_tiles<T, true, true, kSums>(st, p, e, plan.dweight);
+        if (splits > 1) {
+            const int64_t steps = ceil_div(s.rows * static_cast<int64_t>(sizeof(T)), kStepBytes);
+            const int parts = static_cast<int>(ceil_div(steps, ceil_div(steps, splits)));
+            const int64_t count = static_cast<int64_t>(n) * k;
+            if (k % 4 == 0)
+                hipLaunchKernelGGL((linear_join_kernel<T, 4>), dim3(static_cast<unsigned>(ceil_div(count, 1024))), dim3(256),
+                                   0, st, plan.parts, parts, count, k, static_cast<T*>(a.dweight), a.dweight_stride);
+            else
+                hipLaunchKernelGGL((linear_join_kernel<T, 1>), dim3(static_cast<unsigned>(ceil_div(count, 256))), dim3(256),
+                                   0, st, plan.parts, parts, count, k, static_cast<T*>(a.dweight), a.dweight_stride);
+        }
     }
     return hipGetLastError();
 }
