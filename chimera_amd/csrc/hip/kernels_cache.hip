@@ -511,12 +511,13 @@ __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
     }
 }
 
-// The parts of split documents: a wave a candidate, a lane a query token.
-__global__ __launch_bounds__(256) void cache_maxsim_join_kernel(MaxsimArgs a) {
+// The parts of split documents: a block a candidate, a lane a query token
+// (half a wave's lanes each of 32 tokens), the half waves share the parts.
+__global__ __launch_bounds__(512) void cache_maxsim_join_kernel(MaxsimArgs a) {
+    __shared__ float best[16][32];
     const int l = lane_id();
-    const int q = static_cast<int>(blockIdx.y);
-    const int j = static_cast<int>(blockIdx.x) * 4 + wave_id();
-    if (j >= a.cap) return;
+    const int row = l & 31, group = static_cast<int>(threadIdx.x) / 32;
+    const int q = static_cast<int>(blockIdx.y), j = static_cast<int>(blockIdx.x);
     const int64_t at = static_cast<int64_t>(q) * a.cap + j;
     const int count = a.cand_counts ? a.cand_counts[q] : a.cap;
     const int doc = j < count ? a.cand_ids[at] : -1;
@@ -524,15 +525,24 @@ __global__ __launch_bounds__(256) void cache_maxsim_join_kernel(MaxsimArgs a) {
     const int q_len = a.query_lens ? min(max(a.query_lens[q], 0), a.query_len) : a.query_len;
     const int rows_padded = (a.query_len + 31) / 32 * 32;
     const int parts = (len + a.split_tokens - 1) / a.split_tokens;
-    float s = 0.0f;
-    for (int i = l; i < q_len; i += kWave) {
-        float best = -INFINITY;
-        for (int p = 0; p < parts; ++p) best = fmaxf(best, a.parts[(at * a.splits + p) * rows_padded + i]);
-        s += best;
-    }
+    float total = 0.0f;
+    for (int q0 = 0; q0 < q_len; q0 += 32) {
+        float m = -INFINITY;
+#pragma unroll 4
+        for (int p = group; p < parts; p += 16) m = fmaxf(m, a.parts[(at * a.splits + p) * rows_padded + q0 + row]);
+        best[group][row] = m;
+        __syncthreads();
+        if (threadIdx.x < 32) {
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) s += __shfl_xor(s, o, kWave);
-    if (l == 0) a.scores[at] = parts > 0 ? s : -INFINITY;
+            for (int g = 1; g < 16; ++g) m = fmaxf(m, best[g][row]);
+            total += q0 + row < q_len ? m : 0.0f;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x >= 32) return;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) total += __shfl_xor(total, o, kWave);
+    if (threadIdx.x == 0) a.scores[at] = parts > 0 ? total : -INFINITY;
 }
 
 // The best k candidates of a query by score, ties to the larger id: one block
@@ -672,8 +682,8 @@ hipError_t launch_cache_maxsim(hipStream_t st, const chimera_cache& c, const chi
             hipLaunchKernelGGL((cache_maxsim_kernel<T, kFormat, false>), grid, dim3(256), 0, st, a);
     });
     if (e != hipSuccess) return e;
-    if (s.count > 1) hipLaunchKernelGGL(cache_maxsim_join_kernel, dim3(static_cast<unsigned>(ceil_div(m.cand_cap, 4)), static_cast<unsigned>(m.nq)),
-                       dim3(256), 0, st, a);
+    if (s.count > 1) hipLaunchKernelGGL(cache_maxsim_join_kernel, dim3(static_cast<unsigned>(m.cand_cap), static_cast<unsigned>(m.nq)),
+                       dim3(512), 0, st, a);
     if (m.k > 0) {
         // at least one key per thread of the block's merge sort
         int sort_cap = 1024;

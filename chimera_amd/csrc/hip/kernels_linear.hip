@@ -717,16 +717,17 @@ __global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, E
         return v;
     };
     f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    for (int s = kw * share; s < s_end; s += 4) {
-        u32x4_t a[4], b[4];
+    constexpr int kAtOnce = 8;  // steps whose loads are under way together
+    for (int s = kw * share; s < s_end; s += kAtOnce) {
+        u32x4_t a[kAtOnce], b[kAtOnce];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < kAtOnce; ++u) {
             const bool in = s + u < s_end;
             a[u] = in ? chunk(wt, s + u) : u32x4_t{0, 0, 0, 0};
             b[u] = in ? chunk(x, s + u) : u32x4_t{0, 0, 0, 0};
         }
 #pragma unroll
-        for (int u = 0; u < 4; ++u) acc = mma16<T>(a[u], b[u], acc);
+        for (int u = 0; u < kAtOnce; ++u) acc = mma16<T>(a[u], b[u], acc);
     }
     // D lane l holds row l % 16 of X, columns 4 (l / 16) .. + 3 of the tile
     *reinterpret_cast<f32x4_t*>(&part[kw][l & 15][nt * 16 + 4 * (l >> 4)]) = acc;
@@ -921,41 +922,62 @@ constexpr int64_t kFewRows = 64;
 
 constexpr int kCus = 256;
 
-// Which tile a product takes: the one with the least of
-//   (tiles that the busiest of the 256 CUs gets) x (area) / (rate)
-// with the rate of a CU on that tile, relative to the largest (16-bit
-// operands: 65,536 x 1024 -> 4096 takes 590 us on tiles of 256, 700 of 128;
-// 32-bit operands are bound by the matrix cores on any of them).
-struct TileChoice {
+// Which tile a product takes, and into how many parts its sum is split (where
+// that is allowed): the least of an estimate in microseconds,
+//   3 + steps x (step time of the busiest CU) + (parts written and read back).
+// A step (64 bytes of the sum) takes a CU that has one tile `alone`, and `full`
+// for each tile where it has several or all CUs work. Fitted to products of
+// 64 to 65,536 rows; measured / estimated, us, 16-bit operands:
+//                                      256 x 256   128 x 128    64 x 64
+//     1024 x 1024, sum 1024            25 / 26     10 / 11      7 / 7
+//     4096 x 1024, sum 1024            28 / 29     13 / 14      18 / 20
+//     10007 x 1024, sum 1024           34 / 38     33 / 35      46 / 43
+//     16384 x 1024, sum 1024           39 / 38     48 / 50      76 / 68
+//     65536 x 4096, sum 1024           597 / 566   690 / 751    1039 / 1029
+// With rows across the sum the data come from beyond the L2 and one tile a CU
+// waits for them: 1024 x 1024 of 16,384 rows takes 222 us in 256 tiles of 64,
+// 66 in four parts of the sum each; 300 in 64 tiles of 128, 85 in four parts,
+// 56 in eight. 32-bit operands are bound by the matrix cores, which small
+// tiles keep busy more evenly: 6001 x 1024, sum 768 takes 111 us on tiles of
+// 128, 89 of 64.
+struct TileCost {
     int size;
-    double rate16, rate32;
+    double alone, alone_across, full;  // us
 };
-constexpr TileChoice kTileChoices[3] = {{256, 1.0, 1.0}, {128, 0.8, 0.95}, {64, 0.45, 0.85}};
+constexpr TileCost kCosts16[] = {{256, 0.70, 1.00, 1.10}, {128, 0.225, 0.60, 0.365}, {64, 0.115, 0.42, 0.125}};
+constexpr TileCost kCosts32[] = {{128, 1.00, 1.05, 1.15}, {64, 0.31, 0.31, 0.32}};
 
 struct TilePlan {
     int size, splits;
 };
 
-// With splits allowed, parts of the sum (16 steps at least) go to blocks of
-// their own where there are few tiles; the parts' bytes are written and read
-// once more at 4 TB/s, and the join is a launch of its own.
-TilePlan tile_plan(int64_t m, int64_t n, int64_t sum, size_t elem, bool may_split) {
-    const int64_t steps = ceil_div(sum * static_cast<int64_t>(elem), kStepBytes);
-    const double cu_rate = elem == 4 ? 0.5e6 : 4.5e6;  // operations a microsecond
-    TilePlan best = {256, 1};
+TilePlan tile_plan(int64_t m, int64_t n, int64_t sum, size_t elem, bool across, bool may_split) {
+    const int64_t all_steps = ceil_div(sum * static_cast<int64_t>(elem), kStepBytes);
+    TilePlan best = {0, 1};
     double least = 0.0;
-    for (const TileChoice& c : kTileChoices) {
+    auto consider = [&](const TileCost& c) {
         const double tiles = static_cast<double>(ceil_div(m, c.size)) * static_cast<double>(ceil_div(n, c.size));
-        const double tile_us = 2.0 * c.size * c.size * static_cast<double>(sum) / (cu_rate * (elem == 4 ? c.rate32 : c.rate16));
-        for (int64_t splits = 1; splits == 1 || (may_split && splits <= 256 && steps / splits >= 16); splits *= 2) {
-            double us = std::ceil(tiles * static_cast<double>(splits) / kCus) * tile_us / static_cast<double>(splits);
-            if (splits > 1) us += 3.0 + static_cast<double>(splits * m * n) * 8.0 / 4e6;
-            if ((c.size == 256 && splits == 1) || us < least) {
+        for (int64_t splits = 1; splits == 1 || (may_split && splits <= 256 && all_steps / splits >= 8); splits *= 2) {
+            const double share = tiles * static_cast<double>(splits) / kCus;  // tiles a CU
+            const double alone = across ? c.alone_across : c.alone;
+            // CUs hold one tile of 256 at a time, two of 128, four of 64
+            const double rounds = c.size == 256   ? std::ceil(share)
+                                  : c.size == 128 ? (share + std::ceil(share)) / 2
+                                                  : share + 0.25;
+            const double step = share <= 1.0 ? alone + std::max(0.0, c.full - alone) * share
+                                             : std::max(alone, c.full * rounds);
+            double us = 3.0 + static_cast<double>(ceil_div(all_steps, splits)) * step;
+            if (splits > 1) us += 3.0 + static_cast<double>(splits * m * n) * 8.0 / 4.5e6;
+            if (best.size == 0 || us < least) {
                 least = us;
                 best = {c.size, static_cast<int>(splits)};
             }
         }
-    }
+    };
+    if (elem == 4)
+        for (const TileCost& c : kCosts32) consider(c);
+    else
+        for (const TileCost& c : kCosts16) consider(c);
     return best;
 }
 
@@ -973,30 +995,35 @@ void launch_tiles(hipStream_t st, Product p, const Epilogue& e, TilePlan plan) {
         hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, kAcrossA, kAcrossB, kEnd>), grid, dim3(WM * WN * kWave),
                            0, st, p, e);
     };
-    using std::integral_constant;
+    constexpr std::integral_constant<int, 1> k1;
+    constexpr std::integral_constant<int, 2> k2;
+    constexpr std::integral_constant<int, 3> k3;
+    constexpr std::integral_constant<int, 4> k4;
+    constexpr std::integral_constant<int, 32> k32;
+    constexpr std::integral_constant<int, 64> k64;
+    constexpr std::integral_constant<int, 96> k96;
+    constexpr std::integral_constant<int, 128> k128;
+    constexpr std::integral_constant<int, 256> k256;
     if constexpr (kEnd == kNormalizedLayer) {
-        // a block has whole rows: 32 of them where 128 leave CUs idle
-        if (ceil_div(ceil_div(p.m, 32), kCus) * 32 < ceil_div(ceil_div(p.m, 128), kCus) * 128)
-            launch(integral_constant<int, 32>{}, integral_constant<int, 128>{}, integral_constant<int, 1>{},
-                   integral_constant<int, 4>{});
+        // a block has whole rows: 32 of them where 128 leave CUs idle, the
+        // columns in waves of 32
+        const bool many = ceil_div(ceil_div(p.m, 32), kCus) * 32 >= ceil_div(ceil_div(p.m, 128), kCus) * 128;
+        if (sizeof(T) == 2 && many)
+            launch(k128, k128, k4, k1);
+        else if (p.n > 96)
+            launch(k32, k128, k1, k4);
+        else if (p.n > 64)
+            launch(k32, k96, k1, k3);
         else
-            launch(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 4>{},
-                   integral_constant<int, 1>{});
-        return;
+            launch(k64, k64, k2, k2);
     } else {
-    switch (plan.size) {
-        case 256:
-            launch(integral_constant<int, 256>{}, integral_constant<int, 256>{}, integral_constant<int, 2>{},
-                   integral_constant<int, 4>{});
-            break;
-        case 128:
-            launch(integral_constant<int, 128>{}, integral_constant<int, 128>{}, integral_constant<int, 2>{},
-                   integral_constant<int, 2>{});
-            break;
-        default:
-            launch(integral_constant<int, 64>{}, integral_constant<int, 64>{}, integral_constant<int, 2>{},
-                   integral_constant<int, 2>{});
-    }
+        if constexpr (sizeof(T) == 2) {
+            if (plan.size == 256) return launch(k256, k256, k2, k4);
+        }
+        if (plan.size == 128)
+            launch(k128, k128, k2, k2);
+        else
+            launch(k64, k64, k2, k2);
     }
 }
 
@@ -1088,7 +1115,7 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     aligned_rows<T>(st, a.weight, a.weight_stride, s.out_features, s.in_features, plan.weight, &p.b, &p.b_stride);
     // whole chunks: as the matrices lie, or both laid out again with zeros
     p.sum = round_up(s.in_features, 16 / sizeof(T));
-    const TilePlan tiles = tile_plan(p.m, p.n, p.sum, sizeof(T), false);
+    const TilePlan tiles = tile_plan(p.m, p.n, p.sum, sizeof(T), false, false);
     if (e.normalize)
         launch_tiles<T, false, false, kNormalizedLayer>(st, p, e, tiles);
     else
@@ -1113,7 +1140,7 @@ size_t carve_backward(const chimera_linear_shape& s, void* base, BackwardPlan* p
     // about 1,024 blocks of 16 to 512 rows
     plan->block_rows = static_cast<int>(std::max<int64_t>(
         16, std::min<int64_t>(512, round_up(ceil_div(s.rows * ceil_div(s.out_features, 128), 1024), 16))));
-    plan->dweight = tile_plan(s.out_features, s.in_features, s.rows, e, true);
+    plan->dweight = tile_plan(s.out_features, s.in_features, s.rows, e, true, true);
     plan->g = c.take(static_cast<size_t>(s.rows) * plan->n_pad * e);
     plan->x = c.take(static_cast<size_t>(s.rows) * wide);
     plan->weight = c.take(n * wide);
@@ -1191,7 +1218,7 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
         p.a = dz;
         p.a_stride = dz_stride;
         aligned_rows<T>(st, a.weight, a.weight_stride, n, k, plan.weight, &p.b, &p.b_stride);
-        launch_tiles<T, false, true, kSums>(st, p, e, tile_plan(p.m, p.n, p.sum, sizeof(T), false));
+        launch_tiles<T, false, true, kSums>(st, p, e, tile_plan(p.m, p.n, p.sum, sizeof(T), true, false));
     }
     if (a.dweight) {
         Product p = {};
