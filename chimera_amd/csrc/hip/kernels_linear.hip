@@ -273,7 +273,7 @@ struct Product {
 
 // ---- tiled product -------------------------------------------------------------
 
-constexpr int kStepBytes = 64;  // of the summed axis per step: 32 or 16 values
+constexpr int kStepBytes = 128;  // of the summed axis per step: 64 or 32 values
 
 constexpr int kWaitLds = 0xC07F;  // s_waitcnt lgkmcnt(0), the others not waited on
 
@@ -287,13 +287,15 @@ __device__ __forceinline__ void wait_and_meet() {
     asm volatile("" ::: "memory");
 }
 
-// One operand of a tile: 64 bytes of the summed axis of kRows of its rows (or
-// columns, kAcross) a step, B of them in all, loaded by W waves.
+// One operand of a tile: 128 bytes of the summed axis of its B rows (or
+// columns, kAcross) a step, loaded by W waves.
 //
-// Rows along the sum: a step is 64 bytes of each row; chunk c of row r lies at
-// place c ^ (r / 4 % 4), so that the lanes that follow each other in an LDS
-// read of 16 bytes hit different banks.
-// Rows across the sum: a step is 32 (or 16, of 32 bits) rows of B values. For
+// Rows along the sum: a step is 128 bytes of each row, whole lines (with 64
+// bytes a CU loads 60 GB/s into LDS, with 128 it loads 125; the largest tile
+// needs 75 at the matrix cores' rate); chunk c of row r lies at place
+// c ^ (r % 8), so that the lanes that follow each other in an LDS read of 16
+// bytes hit different banks.
+// Rows across the sum: a step is 64 (or 32, of 32 bits) rows of B values. For
 // 16-bit values the LDS's transposing read gives 16 lanes four values of a
 // column each from four rows of 32 bytes; chunk c of row r lies at place
 // c ^ 2 (r % 4), which puts those four rows in different banks. 32-bit values
@@ -326,7 +328,7 @@ struct Side {
                 off[i] = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) +
                          16u * static_cast<uint32_t>(min(chunk, last / kPer));
             } else {
-                const int chunk = place ^ ((row >> 2) & 3);
+                const int chunk = place ^ (row & 7);
                 off[i] = static_cast<uint32_t>(min(row, last)) * static_cast<uint32_t>(stride) + 16u * chunk;
             }
         }
@@ -334,8 +336,8 @@ struct Side {
             base = static_cast<const char*>(p) + first * static_cast<int64_t>(sizeof(T));
             step_bytes = kStepRows * stride;
         } else {
-            // the same chunk for every piece: 16 rows each
-            at = ((l & 3) ^ (l >> 4)) * kPer;
+            // the same chunk for every piece: 8 rows each
+            at = ((l & 7) ^ (l >> 3)) * kPer;
             base = static_cast<const char*>(p) + first * stride;
             step_bytes = kStepBytes;
         }
@@ -360,15 +362,15 @@ struct Side {
 };
 
 // The operands of one wave: kCount tiles of 32 rows (or columns) from `first`
-// on, half a step at a time (two 16-byte chunks of the sum, one for each half
-// of the wave).
+// on, a quarter of a step at a time (two 16-byte chunks of the sum, one for
+// each half of the wave).
 template <typename T, int kCount, bool kAcross, int kRowBytes>
 struct Reader {
     uint32_t off[kAcross && sizeof(T) == 2 ? kCount : 1];
 
     __device__ __forceinline__ void init(int first, int l) {
         if constexpr (!kAcross) {
-            off[0] = static_cast<uint32_t>(first + (l & 31)) * kStepBytes + (((l >> 5) ^ ((l >> 2) & 3)) << 4);
+            off[0] = static_cast<uint32_t>(first + (l & 31)) * kStepBytes + (((l >> 5) ^ (l & 7)) << 4);
         } else if constexpr (sizeof(T) == 4) {
             off[0] = static_cast<uint32_t>(4 * (l >> 5)) * kRowBytes + 4u * static_cast<uint32_t>(first + (l & 31));
         } else {
@@ -380,19 +382,19 @@ struct Reader {
             }
         }
     }
-    __device__ __forceinline__ void read(const unsigned char* from, int half, u32x4_t (&o)[kCount]) const {
+    __device__ __forceinline__ void read(const unsigned char* from, int quarter, u32x4_t (&o)[kCount]) const {
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
             if constexpr (!kAcross) {
-                o[i] = *reinterpret_cast<const u32x4_t*>(from + i * 32 * kStepBytes + (off[0] ^ (half << 5)));
+                o[i] = *reinterpret_cast<const u32x4_t*>(from + i * 32 * kStepBytes + (off[0] ^ (quarter << 5)));
             } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    o[i][j] = *reinterpret_cast<const uint32_t*>(from + (8 * half + j) * kRowBytes + 128 * i + off[0]);
+                    o[i][j] = *reinterpret_cast<const uint32_t*>(from + (8 * quarter + j) * kRowBytes + 128 * i + off[0]);
             } else {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const u32x2_t u = read_transposed(from + (16 * half + 4 * t) * kRowBytes + off[i]);
+                    const u32x2_t u = read_transposed(from + (16 * quarter + 4 * t) * kRowBytes + off[i]);
                     o[i][2 * t] = u[0];
                     o[i][2 * t + 1] = u[1];
                 }
@@ -402,27 +404,28 @@ struct Reader {
 };
 
 // C tile of BM x BN by WM x WN waves. The operands go straight from memory to
-// a ring of four LDS slots: with three steps on their way the loads' latency
-// is covered at full rate (a step's products take a wave of the 256 x 256 tile
-// 512 cycles). A wave reads the operands of one half of a step while the
-// matrix cores work on the other half.
+// rings of LDS slots, one step each: kSlotsA of A, kSlotsB of B. Three and two
+// fill the LDS with one tile of 256 (two of 128, four of 64) a CU, and leave
+// half of a step's loads two steps to arrive and half of them one. A wave
+// reads the operands of a quarter step while the matrix cores work on the
+// quarter before it; once all waves have read a step's last quarter, its slots
+// take new loads, before that quarter is multiplied. One meeting a step.
 // kEnd: the sums are stored, or go through the layer's epilogue, without or
 // with the division by the rows' length (a tile then has all their columns).
 enum End { kSums, kPlainLayer, kNormalizedLayer };
-template <typename T, int BM, int BN, int WM, int WN, bool kAcrossA, bool kAcrossB, End kEnd>
+template <typename T, int BM, int BN, int WM, int WN, int kSlotsA, int kSlotsB, bool kAcrossA, bool kAcrossB, End kEnd>
 __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, Epilogue e) {
     constexpr bool kLayer = kEnd != kSums;
     constexpr bool kNormalize = kEnd == kNormalizedLayer;
-    constexpr int kSlots = 4;
     constexpr int W = WM * WN;
     constexpr int TM = BM / WM, TN = BN / WN;
     constexpr int IM = TM / 32, IN = TN / 32;
     using SideA = Side<T, BM, W, kAcrossA>;
     using SideB = Side<T, BN, W, kAcrossB>;
-    constexpr int kSlot = SideA::kBytes + SideB::kBytes;
+    constexpr int kRings = kSlotsA * SideA::kBytes + kSlotsB * SideB::kBytes;
     constexpr int kPitch = TN + 4;
     constexpr int kStage = W * 32 * kPitch * 4;
-    __shared__ __align__(1024) unsigned char lds[kSlots * kSlot > kStage ? kSlots * kSlot : kStage];
+    __shared__ __align__(1024) unsigned char lds[kRings > kStage ? kRings : kStage];
 
     const int l = lane_id();
     const int w = __builtin_amdgcn_readfirstlane(wave_id());
@@ -455,10 +458,21 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     // steps before the one that the sum ends within, if there is one
     const int left = static_cast<int>(p.sum % SideA::kStepRows);
     const int whole = steps - (left != 0 && step0 + steps == p.steps ? 1 : 0);
-    auto fetch = [&](int s, auto is_whole) {
-        unsigned char* to = lds + s % kSlots * kSlot;
-        side_a.fetch(s, to, is_whole, left, l);
-        side_b.fetch(s, to + SideA::kBytes, is_whole, left, l);
+    unsigned char* const ring_b = lds + kSlotsA * SideA::kBytes;
+    // the operands' parts of step s, if there is one
+    auto fetch_a = [&](int s) {
+        unsigned char* to = lds + s % kSlotsA * SideA::kBytes;
+        if (s < whole)
+            side_a.fetch(s, to, true, left, l);
+        else if (s < steps)
+            side_a.fetch(s, to, false, left, l);
+    };
+    auto fetch_b = [&](int s) {
+        unsigned char* to = ring_b + s % kSlotsB * SideB::kBytes;
+        if (s < whole)
+            side_b.fetch(s, to, true, left, l);
+        else if (s < steps)
+            side_b.fetch(s, to, false, left, l);
     };
 
     f32x16_t acc[IM][IN];
@@ -469,10 +483,10 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     struct Operands {
         u32x4_t a[IM], b[IN];
     };
-    auto read = [&](int s, int half, Operands& o) {
-        const unsigned char* from = lds + s % kSlots * kSlot;
-        reader_a.read(from, half, o.a);
-        reader_b.read(from + SideA::kBytes, half, o.b);
+    auto read = [&](int s, int quarter, Operands& o) {
+        reader_a.read(lds + s % kSlotsA * SideA::kBytes, quarter, o.a);
+        reader_b.read(ring_b + s % kSlotsB * SideB::kBytes, quarter, o.b);
+        __builtin_amdgcn_sched_barrier(0);
     };
     auto multiply = [&](const Operands& o) {
 #pragma unroll
@@ -481,54 +495,61 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
             for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(o.b[j], o.a[i], acc[i][j]);
     };
 
-    constexpr int kLoads = SideA::kLoads + SideB::kLoads;
-    Operands first, second;
-#pragma unroll
-    for (int i = 0; i < IM; ++i) second.a[i] = u32x4_t{0, 0, 0, 0};
-#pragma unroll
-    for (int j = 0; j < IN; ++j) second.b[j] = u32x4_t{0, 0, 0, 0};
-    auto step = [&](int s, auto&& more) {
-        more();
-        read(s, 0, first);
+    Operands even, odd;
+    // the first three quarters of step s, whose first one is in `even`
+    auto quarters = [&](int s) {
+        read(s, 1, odd);
+        multiply(even);
         __builtin_amdgcn_sched_barrier(0);
-        multiply(second);  // the step before's; zeros at first
+        __builtin_amdgcn_s_waitcnt(kWaitLds);  // said before the next reads, it does not wait for them
+        read(s, 2, even);
+        multiply(odd);
         __builtin_amdgcn_sched_barrier(0);
-        // the first half is in registers by now; said here, it needs no wait
-        // for the second half's reads below
         __builtin_amdgcn_s_waitcnt(kWaitLds);
-        read(s, 1, second);
-        __builtin_amdgcn_sched_barrier(0);
-        multiply(first);
+        read(s, 3, odd);
+        multiply(even);
         __builtin_amdgcn_sched_barrier(0);
     };
-    constexpr int kAhead = kSlots - 1;
-    constexpr auto kWhole = std::true_type{};
-    constexpr auto kPartial = std::false_type{};
+    // in the order that the loop goes on with: B and then A of a step, with A
+    // kSlotsA - kSlotsB steps ahead
+    static_assert(kSlotsA >= kSlotsB && kSlotsB >= 2, "");
+    constexpr int kLead = kSlotsA - kSlotsB;
 #pragma unroll
-    for (int s = 0; s < kAhead; ++s) {
-        if (s < whole)
-            fetch(s, kWhole);
-        else if (s < steps)
-            fetch(s, kPartial);
+    for (int s = 0; s < kLead; ++s) fetch_a(s);
+#pragma unroll
+    for (int s = 0; s < kSlotsB; ++s) {
+        fetch_b(s);
+        fetch_a(s + kLead);
     }
-    if (steps >= kAhead)
-        wait_and_meet<(kAhead - 1) * kLoads>();
+    // at a step's meeting the next step's parts have to be there: of what is
+    // under way, all up to B's part of it, or A's where that comes after
+    constexpr int kPair = SideA::kLoads + SideB::kLoads;
+    constexpr int kUnderWay = (kLead > 0 ? SideA::kLoads : 0) + (kSlotsB - 2) * kPair;
+    if (steps >= kSlotsA)
+        wait_and_meet<kUnderWay + kPair>();
     else
         wait_and_meet<0>();
+    read(0, 0, even);
     int s = 0;
-    for (; s + kAhead < whole; ++s) {
-        step(s, [&] { fetch(s + kAhead, kWhole); });
-        wait_and_meet<(kAhead - 1) * kLoads>();
+    for (; s + kSlotsA < whole; ++s) {
+        quarters(s);
+        wait_and_meet<kUnderWay>();
+        side_b.fetch(s + kSlotsB, ring_b + s % kSlotsB * SideB::kBytes, true, left, l);
+        side_a.fetch(s + kSlotsA, lds + s % kSlotsA * SideA::kBytes, true, left, l);
+        read(s + 1, 0, even);
+        multiply(odd);
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(kWaitLds);
     }
     for (; s < steps; ++s) {
-        step(s, [&] {
-            if (s + kAhead < steps) fetch(s + kAhead, kPartial);
-        });
+        quarters(s);
         wait_and_meet<0>();
+        fetch_b(s + kSlotsB);
+        fetch_a(s + kSlotsA);
+        if (s + 1 < steps) read(s + 1, 0, even);
+        multiply(odd);
         __builtin_amdgcn_sched_barrier(0);
     }
-    multiply(second);
 
     // With W as the first operand, D lane l holds row l % 32 of X and of each
     // tile the columns 8 (r / 4) + 4 (l / 32) + r % 4: four neighbours at a
@@ -683,9 +704,11 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
 
 // 16 rows of X against NT tiles of 16 rows of W; KW waves share the summed
 // axis of each tile and join in LDS. Every row of W is read by one wave
-// straight into registers, with no barrier before the join.
-template <typename T, int NT, int KW>
-__global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, Epilogue e, int k, bool aligned) {
+// straight into registers, eight steps' loads under way together, with no
+// barrier before the join: what bounds a call of few rows is the way to memory
+// and back. kAligned: rows start at multiples of 16 bytes and end at one.
+template <typename T, int NT, int KW, bool kAligned>
+__global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, Epilogue e) {
     constexpr int kCols = NT * 16;
     constexpr int kPitch = kCols + 4;
     __shared__ __align__(16) float part[KW][16][kPitch];
@@ -694,41 +717,60 @@ __global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, E
     const int nt = w % NT, kw = w / NT;
     const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16;
     const int n0 = static_cast<int>(blockIdx.x) * kCols;
+    const int k = static_cast<int>(p.sum);
+    // rows past the end are the last row again
     const int64_t row_x = min(m0 + (l & 15), p.m - 1);
     const int row_w = min(n0 + nt * 16 + (l & 15), p.n - 1);
-    const char* x = static_cast<const char*>(p.a) + row_x * p.a_stride;
-    const char* wt = static_cast<const char*>(p.b) + row_w * p.b_stride;
-    constexpr int kPer = 16 / sizeof(T);  // values of a chunk
+    const T* x = reinterpret_cast<const T*>(static_cast<const char*>(p.a) + row_x * p.a_stride);
+    const T* wt = reinterpret_cast<const T*>(static_cast<const char*>(p.b) + row_w * p.b_stride);
+    constexpr int kPer = 16 / sizeof(T);  // values of a chunk; four chunks a step
     const int steps = (k + 4 * kPer - 1) / (4 * kPer);
     const int share = (steps + KW - 1) / KW;
     const int s_end = min(steps, (kw + 1) * share);
-    auto chunk = [&](const char* row, int s) {
-        const int at = (4 * s + (l >> 4)) * kPer;  // first value
-        u32x4_t v = {0, 0, 0, 0};
-        if (aligned) {
-            if (at < k) v = *reinterpret_cast<const u32x4_t*>(row + static_cast<int64_t>(at) * sizeof(T));
-        } else {
-            T t[kPer];
-#pragma unroll
-            for (int j = 0; j < kPer; ++j)
-                t[j] = at + j < k ? reinterpret_cast<const T*>(row)[at + j] : from_float<T>(0.0f);
-            v = *reinterpret_cast<const u32x4_t*>(t);
-        }
-        return v;
-    };
+    const int lane_at = (l >> 4) * kPer;
     f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    constexpr int kAtOnce = 8;  // steps whose loads are under way together
-    for (int s = kw * share; s < s_end; s += kAtOnce) {
-        u32x4_t a[kAtOnce], b[kAtOnce];
+    auto batch = [&](int s, auto count, auto inside) {
+        constexpr int kCount = decltype(count)::value;
+        u32x4_t a[kCount], b[kCount];
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) {
-            const bool in = s + u < s_end;
-            a[u] = in ? chunk(wt, s + u) : u32x4_t{0, 0, 0, 0};
-            b[u] = in ? chunk(x, s + u) : u32x4_t{0, 0, 0, 0};
+        for (int u = 0; u < kCount; ++u) {
+            const int at = (s + u) * 4 * kPer + lane_at;
+            if constexpr (kAligned) {
+                // chunks past the end read the row's first, and count as zeros
+                const bool in = decltype(inside)::value || (s + u < s_end && at < k);
+                a[u] = *reinterpret_cast<const u32x4_t*>(wt + (in ? at : 0));
+                b[u] = *reinterpret_cast<const u32x4_t*>(x + (in ? at : 0));
+            } else {
+                T ta[kPer], tb[kPer];
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) {
+                    const bool in = s + u < s_end && at + j < k;
+                    ta[j] = wt[in ? at + j : 0];
+                    tb[j] = x[in ? at + j : 0];
+                    ta[j] = in ? ta[j] : from_float<T>(0.0f);
+                    tb[j] = in ? tb[j] : from_float<T>(0.0f);
+                }
+                a[u] = *reinterpret_cast<const u32x4_t*>(ta);
+                b[u] = *reinterpret_cast<const u32x4_t*>(tb);
+            }
         }
+        __builtin_amdgcn_sched_barrier(0);  // all loads before the first wait
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) acc = mma16<T>(a[u], b[u], acc);
-    }
+        for (int u = 0; u < kCount; ++u) {
+            if constexpr (kAligned && !decltype(inside)::value) {
+                const bool in = s + u < s_end && (s + u) * 4 * kPer + lane_at < k;
+                a[u] = in ? a[u] : u32x4_t{0, 0, 0, 0};
+                b[u] = in ? b[u] : u32x4_t{0, 0, 0, 0};
+            }
+            acc = mma16<T>(a[u], b[u], acc);
+        }
+    };
+    constexpr std::integral_constant<int, kAligned ? 8 : 2> kAtOnce;
+    const int s_whole = min(s_end, k / (4 * kPer));  // steps that end within the rows
+    int s = kw * share;
+    if constexpr (kAligned)
+        for (; s + kAtOnce <= s_whole; s += kAtOnce) batch(s, kAtOnce, std::true_type{});
+    for (; s < s_end; s += kAtOnce) batch(s, kAtOnce, std::false_type{});
     // D lane l holds row l % 16 of X, columns 4 (l / 16) .. + 3 of the tile
     *reinterpret_cast<f32x4_t*>(&part[kw][l & 15][nt * 16 + 4 * (l >> 4)]) = acc;
     __syncthreads();
@@ -925,7 +967,7 @@ constexpr int kCus = 256;
 // Which tile a product takes, and into how many parts its sum is split (where
 // that is allowed): the least of an estimate in microseconds,
 //   3 + steps x (step time of the busiest CU) + (parts written and read back).
-// A step (64 bytes of the sum) takes a CU that has one tile `alone`, and `full`
+// A step (128 bytes of the sum) takes a CU that has one tile `alone`, and `full`
 // for each tile where it has several or all CUs work. Fitted to products of
 // 64 to 65,536 rows; measured / estimated, us, 16-bit operands:
 //                                      256 x 256   128 x 128    64 x 64
@@ -987,12 +1029,12 @@ void launch_tiles(hipStream_t st, Product p, const Epilogue& e, TilePlan plan) {
     p.steps = static_cast<int>(ceil_div(p.sum * static_cast<int64_t>(sizeof(T)), kStepBytes));
     p.steps_per_split = static_cast<int>(ceil_div(p.steps, splits));
     splits = static_cast<int>(ceil_div(p.steps, p.steps_per_split));
-    auto launch = [&](auto bm, auto bn, auto wm, auto wn) {
+    auto launch = [&](auto bm, auto bn, auto wm, auto wn, auto slots_a, auto slots_b) {
         constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
         p.tiles_m = static_cast<int>(ceil_div(p.m, BM));
         p.tiles_n = static_cast<int>(ceil_div(p.n, BN));
         const dim3 grid(static_cast<unsigned>(p.tiles_m * p.tiles_n), static_cast<unsigned>(splits));
-        hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, kAcrossA, kAcrossB, kEnd>), grid, dim3(WM * WN * kWave),
+        hipLaunchKernelGGL((linear_tile_kernel<T, BM, BN, WM, WN, decltype(slots_a)::value, decltype(slots_b)::value, kAcrossA, kAcrossB, kEnd>), grid, dim3(WM * WN * kWave),
                            0, st, p, e);
     };
     constexpr std::integral_constant<int, 1> k1;
@@ -1009,21 +1051,21 @@ void launch_tiles(hipStream_t st, Product p, const Epilogue& e, TilePlan plan) {
         // columns in waves of 32
         const bool many = ceil_div(ceil_div(p.m, 32), kCus) * 32 >= ceil_div(ceil_div(p.m, 128), kCus) * 128;
         if (sizeof(T) == 2 && many)
-            launch(k128, k128, k4, k1);
+            launch(k128, k128, k4, k1, k3, k2);
         else if (p.n > 96)
-            launch(k32, k128, k1, k4);
+            launch(k32, k128, k1, k4, k3, k3);
         else if (p.n > 64)
-            launch(k32, k96, k1, k3);
+            launch(k32, k96, k1, k3, k3, k3);
         else
-            launch(k64, k64, k2, k2);
+            launch(k64, k64, k2, k2, k3, k2);
     } else {
         if constexpr (sizeof(T) == 2) {
-            if (plan.size == 256) return launch(k256, k256, k2, k4);
+            if (plan.size == 256) return launch(k256, k256, k2, k4, k3, k2);
         }
         if (plan.size == 128)
-            launch(k128, k128, k2, k2);
+            launch(k128, k128, k2, k2, k3, k2);
         else
-            launch(k64, k64, k2, k2);
+            launch(k64, k64, k2, k2, k3, k2);
     }
 }
 
@@ -1101,12 +1143,20 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
         p.b_stride = a.weight_stride * static_cast<int64_t>(sizeof(T));
         const bool aligned = rows_aligned(a.x, a.x_stride, sizeof(T)) && rows_aligned(a.weight, a.weight_stride, sizeof(T)) &&
                              s.in_features * sizeof(T) % 16 == 0;
+        p.sum = s.in_features;
         const unsigned by = static_cast<unsigned>(ceil_div(s.rows, 16));
-        if (e.normalize)
-            hipLaunchKernelGGL((linear_rows_kernel<T, 8, 2>), dim3(1, by), dim3(1024), 0, st, p, e, s.in_features, aligned);
+        auto launch = [&](auto is_aligned) {
+            constexpr bool kAligned = decltype(is_aligned)::value;
+            if (e.normalize)
+                hipLaunchKernelGGL((linear_rows_kernel<T, 8, 2, kAligned>), dim3(1, by), dim3(1024), 0, st, p, e);
+            else
+                hipLaunchKernelGGL((linear_rows_kernel<T, 1, 8, kAligned>),
+                                   dim3(static_cast<unsigned>(ceil_div(s.out_features, 16)), by), dim3(512), 0, st, p, e);
+        };
+        if (aligned)
+            launch(std::true_type{});
         else
-            hipLaunchKernelGGL((linear_rows_kernel<T, 1, 8>), dim3(static_cast<unsigned>(ceil_div(s.out_features, 16)), by),
-                               dim3(512), 0, st, p, e, s.in_features, aligned);
+            launch(std::false_type{});
         return hipGetLastError();
     }
     ForwardPlan plan;
