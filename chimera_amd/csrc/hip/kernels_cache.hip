@@ -286,12 +286,6 @@ struct QueryTile {
     }
 };
 
-template <int kCtrl>
-__device__ __forceinline__ float lane_move(float v) {
-    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kCtrl, 0xF, 0xF, false));
-}
-constexpr int kRotate8 = 0x128, kMirror8 = 0x141, kSwap2 = 0x4E, kSwap1 = 0xB1;  // of a row of 16 lanes
-
 // Maxima over the 32 lanes of each half of the wave of 16 values a lane: each
 // step leaves a lane half of the values, the last one all lanes of a pair the
 // same one (lane bits 4 to 1 choose it). All in the vector unit.
@@ -315,18 +309,6 @@ __device__ __forceinline__ float maxima_to_rows(float (&v)[16], int l) {
     step(2, 1, std::integral_constant<int, kSwap2>{});
     return fmaxf(v[0], lane_move<kSwap1>(v[0]));
 }
-// Sum over the wave, in every lane.
-__device__ __forceinline__ float wave_sum(float v) {
-    v += lane_move<kSwap1>(v);
-    v += lane_move<kSwap2>(v);
-    v += lane_move<kMirror8>(v);
-    v += lane_move<kRotate8>(v);
-    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
-
 // A wave scores `items` parts of documents (whole documents unless they are
 // split) against one query, tile after tile of 32 tokens (matrix columns)
 // with no break between documents: the codes of the next tile and the page

@@ -156,49 +156,6 @@ __device__ __forceinline__ void slope8(const float (&z)[8], float (&v)[8], int a
     }
 }
 
-// The layer's epilogue on eight neighbouring sums of one row; with
-// normalize the row lies in kLanes neighbouring lanes, which all call it.
-template <typename T, int kLanes>
-__device__ __forceinline__ void finish8(const Epilogue& e, int64_t m, int n0, float (&v)[8]) {
-    const int count = m < e.m ? e.n - n0 : 0;  // may be <= 0
-    const bool whole = count >= 8;
-    if (count > 0) {
-        if (e.bias) {
-            float b[8];
-            load8(static_cast<const T*>(e.bias) + n0, whole && e.bias_vec, count, b);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += b[j];
-        }
-        if (e.saved) store8(static_cast<T*>(e.saved) + m * e.saved_stride + n0, whole && e.saved_vec, count, v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = activation<T>(v[j], e.act);
-        if (e.residual) {
-            float r[8];
-            load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n0, whole && e.residual_vec, count, r);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] += r[j];
-        }
-    }
-    if (e.normalize) {
-        float s = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s = j < count ? fmaf(v[j], v[j], s) : s;
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) s += __shfl_xor(s, o, kWave);
-        const float norm = sqrtf(s);
-        const float held = norm < kLeastNorm ? kLeastNorm : norm;  // NaN stays
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = v[j] / held;
-        if (e.norms && n0 == 0 && count > 0) e.norms[m] = held;
-    }
-    if (count <= 0) return;
-    const int64_t at = m * e.y_stride + n0;
-    if (e.out_f32)
-        store8(static_cast<float*>(e.y) + at, whole && e.y_vec, count, v);
-    else
-        store8(static_cast<T*>(e.y) + at, whole && e.y_vec, count, v);
-}
-
 // ---- matrix-core steps ---------------------------------------------------------
 
 // One 16-byte chunk of a row of A and of B per lane: a 32 x 32 tile's product
@@ -221,23 +178,6 @@ __device__ __forceinline__ f32x16_t mma32(u32x4_t a, u32x4_t b, f32x16_t c) {
                                                        __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
     }
 }
-// The same for a 16 x 16 tile over 64 bytes (lane / 16 is the chunk).
-template <typename T>
-__device__ __forceinline__ f32x4_t mma16(u32x4_t a, u32x4_t b, f32x4_t c) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0, 0, 0);
-        return c;
-    } else if constexpr (__is_same(T, _Float16)) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
-                                                      0, 0, 0);
-    } else {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a),
-                                                       __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-    }
-}
-
 __device__ __forceinline__ __attribute__((address_space(3))) void* lds_at(void* p) {
     return (__attribute__((address_space(3))) void*)(p);
 }
@@ -702,90 +642,67 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
 
 // ---- few rows ------------------------------------------------------------------
 
-// 16 rows of X against NT tiles of 16 rows of W; KW waves share the summed
-// axis of each tile and join in LDS. Every row of W is read by one wave
-// straight into registers, eight steps' loads under way together, with no
-// barrier before the join: what bounds a call of few rows is the way to memory
-// and back. kAligned: rows start at multiples of 16 bytes and end at one.
-template <typename T, int NT, int KW, bool kAligned>
-__global__ __launch_bounds__(NT* KW* kWave) void linear_rows_kernel(Product p, Epilogue e) {
-    constexpr int kCols = NT * 16;
-    constexpr int kPitch = kCols + 4;
-    __shared__ __align__(16) float part[KW][16][kPitch];
+constexpr int kFewRows = 4;     // rows of X that go this way
+constexpr int kWaveOutputs = 4; // rows of W a wave
+
+// Up to four rows of X (kRows) against W, bound by reading W once: a wave
+// takes four rows of W, a kilobyte of each at a time over its lanes, and sums
+// the products in 32 bits on the vector unit; no matrix tile is worth filling
+// for so few rows (one row, 1024 -> 4096: 4 us, on tiles of 64 7).
+template <typename T, int kRows>
+__global__ __launch_bounds__(256) void linear_vector_kernel(Product p, Epilogue e, bool x_vec, bool w_vec) {
     const int l = lane_id();
-    const int w = __builtin_amdgcn_readfirstlane(wave_id());
-    const int nt = w % NT, kw = w / NT;
-    const int64_t m0 = static_cast<int64_t>(blockIdx.y) * 16;
-    const int n0 = static_cast<int>(blockIdx.x) * kCols;
+    const int n0 = (static_cast<int>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(wave_id())) * kWaveOutputs;
+    if (n0 >= p.n) return;
     const int k = static_cast<int>(p.sum);
-    // rows past the end are the last row again
-    const int64_t row_x = min(m0 + (l & 15), p.m - 1);
-    const int row_w = min(n0 + nt * 16 + (l & 15), p.n - 1);
-    const T* x = reinterpret_cast<const T*>(static_cast<const char*>(p.a) + row_x * p.a_stride);
-    const T* wt = reinterpret_cast<const T*>(static_cast<const char*>(p.b) + row_w * p.b_stride);
-    constexpr int kPer = 16 / sizeof(T);  // values of a chunk; four chunks a step
-    const int steps = (k + 4 * kPer - 1) / (4 * kPer);
-    const int share = (steps + KW - 1) / KW;
-    const int s_end = min(steps, (kw + 1) * share);
-    const int lane_at = (l >> 4) * kPer;
-    f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto batch = [&](int s, auto count, auto inside) {
-        constexpr int kCount = decltype(count)::value;
-        u32x4_t a[kCount], b[kCount];
+    const T* w[kWaveOutputs];
 #pragma unroll
-        for (int u = 0; u < kCount; ++u) {
-            const int at = (s + u) * 4 * kPer + lane_at;
-            if constexpr (kAligned) {
-                // chunks past the end read the row's first, and count as zeros
-                const bool in = decltype(inside)::value || (s + u < s_end && at < k);
-                a[u] = *reinterpret_cast<const u32x4_t*>(wt + (in ? at : 0));
-                b[u] = *reinterpret_cast<const u32x4_t*>(x + (in ? at : 0));
-            } else {
-                T ta[kPer], tb[kPer];
+    for (int o = 0; o < kWaveOutputs; ++o)
+        w[o] = reinterpret_cast<const T*>(static_cast<const char*>(p.b) + min(n0 + o, p.n - 1) * p.b_stride);
+    float sums[kRows][kWaveOutputs] = {};
+    constexpr int kAtOnce = 2;  // 8 values a lane each
+    for (int k0 = 8 * l; k0 < k; k0 += kAtOnce * 8 * kWave) {
+        float x[kAtOnce][kRows][8], v[kAtOnce][kWaveOutputs][8];
 #pragma unroll
-                for (int j = 0; j < kPer; ++j) {
-                    const bool in = s + u < s_end && at + j < k;
-                    ta[j] = wt[in ? at + j : 0];
-                    tb[j] = x[in ? at + j : 0];
-                    ta[j] = in ? ta[j] : from_float<T>(0.0f);
-                    tb[j] = in ? tb[j] : from_float<T>(0.0f);
-                }
-                a[u] = *reinterpret_cast<const u32x4_t*>(ta);
-                b[u] = *reinterpret_cast<const u32x4_t*>(tb);
-            }
+        for (int u = 0; u < kAtOnce; ++u) {
+            const int at = k0 + u * 8 * kWave;
+            const int count = k - at;
+#pragma unroll
+            for (int o = 0; o < kWaveOutputs; ++o) load8(w[o] + at, w_vec && count >= 8, count, v[u][o]);
+#pragma unroll
+            for (int m = 0; m < kRows; ++m)
+                load8(reinterpret_cast<const T*>(static_cast<const char*>(p.a) + m * p.a_stride) + at, x_vec && count >= 8,
+                      count, x[u][m]);
         }
-        __builtin_amdgcn_sched_barrier(0);  // all loads before the first wait
 #pragma unroll
-        for (int u = 0; u < kCount; ++u) {
-            if constexpr (kAligned && !decltype(inside)::value) {
-                const bool in = s + u < s_end && (s + u) * 4 * kPer + lane_at < k;
-                a[u] = in ? a[u] : u32x4_t{0, 0, 0, 0};
-                b[u] = in ? b[u] : u32x4_t{0, 0, 0, 0};
-            }
-            acc = mma16<T>(a[u], b[u], acc);
+        for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+            for (int m = 0; m < kRows; ++m)
+#pragma unroll
+                for (int o = 0; o < kWaveOutputs; ++o)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) sums[m][o] = fmaf(x[u][m][j], v[u][o][j], sums[m][o]);
+    }
+    // lane m * kWaveOutputs + o finishes that sum
+    float z = 0.0f;
+#pragma unroll
+    for (int m = 0; m < kRows; ++m)
+#pragma unroll
+        for (int o = 0; o < kWaveOutputs; ++o) {
+            const float s = wave_sum(sums[m][o]);
+            z = l == m * kWaveOutputs + o ? s : z;
         }
-    };
-    constexpr std::integral_constant<int, kAligned ? 8 : 2> kAtOnce;
-    const int s_whole = min(s_end, k / (4 * kPer));  // steps that end within the rows
-    int s = kw * share;
-    if constexpr (kAligned)
-        for (; s + kAtOnce <= s_whole; s += kAtOnce) batch(s, kAtOnce, std::true_type{});
-    for (; s < s_end; s += kAtOnce) batch(s, kAtOnce, std::false_type{});
-    // D lane l holds row l % 16 of X, columns 4 (l / 16) .. + 3 of the tile
-    *reinterpret_cast<f32x4_t*>(&part[kw][l & 15][nt * 16 + 4 * (l >> 4)]) = acc;
-    __syncthreads();
-    constexpr int kLanes = kCols / 8;
-    const int tid = static_cast<int>(threadIdx.x);
-    if (tid >= 16 * kLanes) return;
-    const int row = tid / kLanes, col = tid % kLanes * 8;
-    float v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = part[0][row][col + j];
-#pragma unroll
-    for (int o = 1; o < KW; ++o)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += part[o][row][col + j];
-    finish8<T, kLanes>(e, m0 + row, n0 + col, v);
+    const int64_t m = l / kWaveOutputs;
+    const int n = n0 + l % kWaveOutputs;
+    if (m >= kRows || n >= p.n) return;
+    if (e.bias) z += to_float(static_cast<const T*>(e.bias)[n]);
+    if (e.saved) static_cast<T*>(e.saved)[m * e.saved_stride + n] = from_float<T>(z);
+    float h = activation<T>(z, e.act);
+    if (e.residual) h += to_float(static_cast<const T*>(e.residual)[m * e.residual_stride + n]);
+    if (e.out_f32)
+        static_cast<float*>(e.y)[m * e.y_stride + n] = h;
+    else
+        static_cast<T*>(e.y)[m * e.y_stride + n] = from_float<T>(h);
 }
 
 // ---- layouts -------------------------------------------------------------------
@@ -958,9 +875,6 @@ struct Carve {
         return p;
     }
 };
-
-// Rows up to which a product without a split goes by 16 rows a block.
-constexpr int64_t kFewRows = 64;
 
 constexpr int kCus = 256;
 
@@ -1136,27 +1050,21 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     Product p = {};
     p.m = s.rows;
     p.n = s.out_features;
-    if (s.rows <= kFewRows) {
+    if (s.rows <= kFewRows && !e.normalize) {
         p.a = a.x;
         p.b = a.weight;
         p.a_stride = a.x_stride * static_cast<int64_t>(sizeof(T));
         p.b_stride = a.weight_stride * static_cast<int64_t>(sizeof(T));
-        const bool aligned = rows_aligned(a.x, a.x_stride, sizeof(T)) && rows_aligned(a.weight, a.weight_stride, sizeof(T)) &&
-                             s.in_features * sizeof(T) % 16 == 0;
         p.sum = s.in_features;
-        const unsigned by = static_cast<unsigned>(ceil_div(s.rows, 16));
-        auto launch = [&](auto is_aligned) {
-            constexpr bool kAligned = decltype(is_aligned)::value;
-            if (e.normalize)
-                hipLaunchKernelGGL((linear_rows_kernel<T, 8, 2, kAligned>), dim3(1, by), dim3(1024), 0, st, p, e);
-            else
-                hipLaunchKernelGGL((linear_rows_kernel<T, 1, 8, kAligned>),
-                                   dim3(static_cast<unsigned>(ceil_div(s.out_features, 16)), by), dim3(512), 0, st, p, e);
-        };
-        if (aligned)
-            launch(std::true_type{});
-        else
-            launch(std::false_type{});
+        const bool x_vec = rows_aligned(a.x, a.x_stride, sizeof(T));
+        const bool w_vec = rows_aligned(a.weight, a.weight_stride, sizeof(T));
+        const dim3 grid(static_cast<unsigned>(ceil_div(s.out_features, 4 * kWaveOutputs)));
+        switch (s.rows) {
+            case 1: hipLaunchKernelGGL((linear_vector_kernel<T, 1>), grid, dim3(256), 0, st, p, e, x_vec, w_vec); break;
+            case 2: hipLaunchKernelGGL((linear_vector_kernel<T, 2>), grid, dim3(256), 0, st, p, e, x_vec, w_vec); break;
+            case 3: hipLaunchKernelGGL((linear_vector_kernel<T, 3>), grid, dim3(256), 0, st, p, e, x_vec, w_vec); break;
+            default: hipLaunchKernelGGL((linear_vector_kernel<T, 4>), grid, dim3(256), 0, st, p, e, x_vec, w_vec);
+        }
         return hipGetLastError();
     }
     ForwardPlan plan;

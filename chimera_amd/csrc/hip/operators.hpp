@@ -76,6 +76,25 @@ __device__ __forceinline__ void store8(T* p, bool vec, int count, const float (&
         if (j < count) p[j] = from_float<T>(v[j]);
 }
 
+// A value from another lane by a DPP control.
+template <int kCtrl>
+__device__ __forceinline__ float lane_move(float v) {
+    return __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), kCtrl, 0xF, 0xF, false));
+}
+constexpr int kRotate8 = 0x128, kMirror8 = 0x141, kSwap2 = 0x4E, kSwap1 = 0xB1;  // of a row of 16 lanes
+
+// Sum over the wave, in every lane.
+__device__ __forceinline__ float wave_sum(float v) {
+    v += lane_move<kSwap1>(v);
+    v += lane_move<kSwap2>(v);
+    v += lane_move<kMirror8>(v);
+    v += lane_move<kRotate8>(v);
+    const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
 // ---- dense layer (kernels_linear.hip) ----
 
 struct LinearForward {
