@@ -51,27 +51,13 @@ CacheView view_of(const chimera_cache& c) {
 // neighbouring lanes.
 template <typename T, int kFormat>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, const T* __restrict__ rows, int64_t stride,
-                                                          const int64_t* __restrict__ slots, int64_t n, bool vec) {
+                                                          const int64_t* __restrict__ slots, int64_t n) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
     const int col = static_cast<int>(threadIdx.x) % 16 * 8;
     const int64_t slot = i < n ? slots[i] : -1;
     const bool in = slot >= 0 && slot < c.slots;
     float x[8] = {};
-    if (in) {
-        const T* src = rows + i * stride + col;
-        if (vec && col + 8 <= c.dim) {
-            T t[8];
-#pragma unroll
-            for (int j = 0; j < 8 * static_cast<int>(sizeof(T)) / 16; ++j)
-                reinterpret_cast<u32x4_t*>(t)[j] = reinterpret_cast<const u32x4_t*>(src)[j];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = to_float(t[j]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (col + j < c.dim) x[j] = to_float(src[j]);
-        }
-    }
+    if (in && col < c.dim) load8(rows + i * stride + col, c.dim - col, x);
     float most = 0.0f;
     bool bad = false;
 #pragma unroll
@@ -126,7 +112,7 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, const T* 
 
 template <typename T, int kFormat>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, const int64_t* __restrict__ slots, int64_t n,
-                                                         T* __restrict__ out, int64_t stride, bool vec) {
+                                                         T* __restrict__ out, int64_t stride) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 16 + threadIdx.x / 16;
     const int col = static_cast<int>(threadIdx.x) % 16 * 8;
     if (i >= n || col >= c.dim) return;
@@ -152,19 +138,7 @@ __global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, const int6
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= scale;
     }
-    T t[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
-    T* dst = out + i * stride + col;
-    if (vec && col + 8 <= c.dim) {
-#pragma unroll
-        for (int j = 0; j < 8 * static_cast<int>(sizeof(T)) / 16; ++j)
-            reinterpret_cast<u32x4_t*>(dst)[j] = reinterpret_cast<const u32x4_t*>(t)[j];
-    } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (col + j < c.dim) dst[j] = t[j];
-    }
+    store8(out + i * stride + col, c.dim - col, v);
 }
 
 // ---- late interaction ----------------------------------------------------------
@@ -233,7 +207,6 @@ struct MaxsimArgs {
     int nq, query_len, cap;
     int split_tokens, splits, max_tokens;
     int items;  // parts of documents a wave takes, 1..64
-    bool query_vec;  // query rows start at multiples of 16 bytes
 };
 
 // The query row whose maximum lane l ends up with (maxima_to_rows).
@@ -251,7 +224,7 @@ struct QueryTile {
     f16x8_t part[kParts][4][2];
     float back;  // 2^e of row_of_lane's row; 0 in the lanes that do not count it
 
-    __device__ __forceinline__ void load(const T* q, int rows, int dim, bool vec, int l) {
+    __device__ __forceinline__ void load(const T* q, int rows, int dim, int l) {
         const int row = l & 31, half = l >> 5;
         float x[4][2][8];
         float most = 0.0f;
@@ -261,7 +234,7 @@ struct QueryTile {
             for (int h = 0; h < 2; ++h) {
                 const int at = 32 * g + 16 * half + 8 * h;
                 const int count = row < rows ? dim - at : 0;
-                load8(q + static_cast<int64_t>(row) * dim + at, vec && count >= 8, count, x[g][h]);
+                load8(q + static_cast<int64_t>(row) * dim + at, count, x[g][h]);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(x[g][h][j]));
             }
@@ -412,7 +385,7 @@ __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
         if (q0 >= q_len && q0 > 0) break;
         QueryTile<T, kFormat, kParts> qt;
         qt.load(static_cast<const T*>(a.queries) + (static_cast<int64_t>(q) * a.query_len + q0) * a.c.dim, q_len - q0,
-                a.c.dim, a.query_vec, l);
+                a.c.dim, l);
         float best[16];
 #pragma unroll
         for (int r = 0; r < 16; ++r) best[r] = -INFINITY;
@@ -593,21 +566,16 @@ hipError_t by_format(int format, int type, Call&& call) {
     return hipGetLastError();
 }
 
-bool aligned16(const void* p, int64_t stride, size_t elem) {
-    return (reinterpret_cast<uintptr_t>(p) | static_cast<uint64_t>(stride) * elem) % 16 == 0;
-}
-
 }  // namespace
 
 hipError_t launch_cache_write(hipStream_t st, const chimera_cache& c, const void* rows, int type, int64_t stride,
                               const int64_t* slots, int64_t n) {
     const CacheView v = view_of(c);
     const unsigned blocks = static_cast<unsigned>(ceil_div(n, 16));
-    const bool vec = aligned16(rows, stride, type_bytes(type));
     return by_format(c.format, type, [&](auto f, auto t) {
         using T = decltype(t);
         hipLaunchKernelGGL((cache_write_kernel<T, decltype(f)::value>), dim3(blocks), dim3(256), 0, st, v,
-                           static_cast<const T*>(rows), stride, slots, n, vec);
+                           static_cast<const T*>(rows), stride, slots, n);
     });
 }
 
@@ -615,11 +583,10 @@ hipError_t launch_cache_read(hipStream_t st, const chimera_cache& c, const int64
                              int type, int64_t stride) {
     const CacheView v = view_of(c);
     const unsigned blocks = static_cast<unsigned>(ceil_div(n, 16));
-    const bool vec = aligned16(out, stride, type_bytes(type));
     return by_format(c.format, type, [&](auto f, auto t) {
         using T = decltype(t);
         hipLaunchKernelGGL((cache_read_kernel<T, decltype(f)::value>), dim3(blocks), dim3(256), 0, st, v, slots, n,
-                           static_cast<T*>(out), stride, vec);
+                           static_cast<T*>(out), stride);
     });
 }
 
@@ -653,7 +620,6 @@ hipError_t launch_cache_maxsim(hipStream_t st, const chimera_cache& c, const chi
     a.max_tokens = c.num_pages > 0 && m.num_page_entries > 0 ? m.max_doc_tokens : 0;
     const int64_t parts = static_cast<int64_t>(m.cand_cap) * s.count;
     a.items = items_of(m.nq * parts);
-    a.query_vec = aligned16(m.queries, c.dim, type_bytes(m.type));
     const dim3 grid(static_cast<unsigned>(ceil_div(parts, 4 * a.items)), static_cast<unsigned>(m.nq));
     hipError_t e = by_format(c.format, m.type, [&](auto f, auto t) {
         using T = decltype(t);

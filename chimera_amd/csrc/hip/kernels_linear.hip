@@ -119,8 +119,6 @@ struct Epilogue {
     int n;
     int act;
     bool out_f32, normalize;
-    bool bias_vec, residual_vec, y_vec, saved_vec;
-    bool vec;  // all of them
 };
 
 // act(v) for many values, one branch for all.
@@ -497,7 +495,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     // go through LDS, in 16 bits where that is all that is left to do, so that
     // a wave's stores are whole 128-byte lines.
     constexpr int kLanes = TN / 8, kRows = kWave / kLanes;
-    const bool inside = m0 + BM <= p.m && n0 + BN <= p.n && e.vec;
+    const bool inside = m0 + BM <= p.m && n0 + BN <= p.n;
     const int half = l >> 5;
     const int col0 = n0 + wn * TN;
     unsigned char* stage = lds + w * 32 * kPitch * 4;
@@ -529,16 +527,18 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
         wave_lds_sync();
     };
     // the rows put in T, as they are, to a matrix of T
-    auto copy_out = [&](void* to, int64_t stride, bool vec, int64_t m_first) {
+    auto copy_out = [&](void* to, int64_t stride, int64_t m_first) {
         each_row(T{}, [&](int row, int col, const T* from) {
             const int64_t m = m_first + row;
             const int n = col0 + col;
             const int count = inside ? 8 : m < e.m ? e.n - n : 0;
             T* dst = static_cast<T*>(to) + m * stride + n;
-            if (inside || (vec && count >= 8)) {
+            if (count >= 8) {
 #pragma unroll
-                for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h)
-                    reinterpret_cast<u32x4_t*>(dst)[h] = reinterpret_cast<const u32x4_t*>(from)[h];
+                for (int h = 0; h < static_cast<int>(sizeof(T)) / 2; ++h) {
+                    const u32x4_t t = reinterpret_cast<const u32x4_t*>(from)[h];
+                    __builtin_memcpy(dst + h * (16 / sizeof(T)), &t, 16);
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
@@ -569,7 +569,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
         if constexpr (kLayer) {
             if (e.saved) {
                 put(v, T{});
-                copy_out(e.saved, e.saved_stride, e.saved_vec, m_first);
+                copy_out(e.saved, e.saved_stride, m_first);
             }
             activate<T>(v, e.act);
             if constexpr (kNormalize) {
@@ -608,7 +608,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
         }
         if (narrow) {
             put(v, T{});
-            copy_out(e.y, e.y_stride, e.y_vec, m_first);
+            copy_out(e.y, e.y_stride, m_first);
             continue;
         }
         put(v, 0.0f);
@@ -617,25 +617,23 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
             const int n = col0 + col;
             const int count = inside ? 8 : m < e.m ? e.n - n : 0;
             if (count <= 0) return;
-            const bool whole = count >= 8;
             float u[8];
-            load8(from, true, 8, u);
+            load8(static_cast<const float*>(__builtin_assume_aligned(from, 16)), 8, u);
             if (e.partial) {
-                store8(e.partial + (split * e.m + m) * e.n + n, inside || (whole && e.y_vec), count, u);
+                store8(e.partial + (split * e.m + m) * e.n + n, count, u);
                 return;
             }
             if (kLayer && !kNormalize && e.residual) {
                 float r[8];
-                load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n, inside || (whole && e.residual_vec),
-                      count, r);
+                load8(static_cast<const T*>(e.residual) + m * e.residual_stride + n, count, r);
 #pragma unroll
                 for (int j = 0; j < 8; ++j) u[j] += r[j];
             }
             const int64_t at = m * e.y_stride + n;
             if (e.out_f32)
-                store8(static_cast<float*>(e.y) + at, inside || (whole && e.y_vec), count, u);
+                store8(static_cast<float*>(e.y) + at, count, u);
             else
-                store8(static_cast<T*>(e.y) + at, inside || (whole && e.y_vec), count, u);
+                store8(static_cast<T*>(e.y) + at, count, u);
         });
     }
 }
@@ -650,7 +648,7 @@ constexpr int kWaveOutputs = 4; // rows of W a wave
 // the products in 32 bits on the vector unit; no matrix tile is worth filling
 // for so few rows (one row, 1024 -> 4096: 4 us, on tiles of 64 7).
 template <typename T, int kRows>
-__global__ __launch_bounds__(256) void linear_vector_kernel(Product p, Epilogue e, bool x_vec, bool w_vec) {
+__global__ __launch_bounds__(256) void linear_vector_kernel(Product p, Epilogue e) {
     const int l = lane_id();
     const int n0 = (static_cast<int>(blockIdx.x) * 4 + __builtin_amdgcn_readfirstlane(wave_id())) * kWaveOutputs;
     if (n0 >= p.n) return;
@@ -668,11 +666,10 @@ __global__ __launch_bounds__(256) void linear_vector_kernel(Product p, Epilogue 
             const int at = k0 + u * 8 * kWave;
             const int count = k - at;
 #pragma unroll
-            for (int o = 0; o < kWaveOutputs; ++o) load8(w[o] + at, w_vec && count >= 8, count, v[u][o]);
+            for (int o = 0; o < kWaveOutputs; ++o) load8(w[o] + at, count, v[u][o]);
 #pragma unroll
             for (int m = 0; m < kRows; ++m)
-                load8(reinterpret_cast<const T*>(static_cast<const char*>(p.a) + m * p.a_stride) + at, x_vec && count >= 8,
-                      count, x[u][m]);
+                load8(reinterpret_cast<const T*>(static_cast<const char*>(p.a) + m * p.a_stride) + at, count, x[u][m]);
         }
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u)
@@ -718,9 +715,14 @@ __global__ __launch_bounds__(256) void linear_align_kernel(const T* __restrict__
     for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
         const int64_t r = i / chunks;
         const int c = static_cast<int>(i - r * chunks) * kPer;
+        const T* from = src + r * src_stride + c;
         T t[kPer];
+        if (c + kPer <= cols) {
+            __builtin_memcpy(t, from, 16);  // at any alignment of elements
+        } else {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) t[j] = c + j < cols ? src[r * src_stride + c + j] : from_float<T>(0.0f);
+            for (int j = 0; j < kPer; ++j) t[j] = c + j < cols ? from[j] : from_float<T>(0.0f);
+        }
         *reinterpret_cast<u32x4_t*>(dst + r * dst_cols + c) = *reinterpret_cast<const u32x4_t*>(t);
     }
 }
@@ -739,7 +741,7 @@ struct GradArgs {
     int64_t m;
     int n, g_cols, act;
     int block_rows;  // a multiple of 16
-    bool out_f32, normalize, dy_vec, y_vec, saved_vec, dresidual_vec;
+    bool out_f32, normalize;
 };
 
 // 16 rows x 128 columns at a time, eight neighbouring columns a thread: with
@@ -755,18 +757,17 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
     for (int64_t m0 = static_cast<int64_t>(blockIdx.x) * a.block_rows; m0 < m_end; m0 += 16) {
         const int64_t m = m0 + tid / 16;
         const int count = m < m_end ? a.n - n0 : 0;
-        const bool whole = count >= 8;
         float g[8] = {};
-        auto load = [&](const void* p, int64_t stride, bool vec, float(&v)[8]) {
+        auto load = [&](const void* p, int64_t stride, float(&v)[8]) {
             if (a.out_f32)
-                load8(static_cast<const float*>(p) + m * stride + n0, whole && vec, count, v);
+                load8(static_cast<const float*>(p) + m * stride + n0, count, v);
             else
-                load8(static_cast<const T*>(p) + m * stride + n0, whole && vec, count, v);
+                load8(static_cast<const T*>(p) + m * stride + n0, count, v);
         };
-        if (count > 0) load(a.dy, a.dy_stride, a.dy_vec, g);
+        if (count > 0) load(a.dy, a.dy_stride, g);
         if (a.normalize) {
             float y[8] = {};
-            if (count > 0) load(a.y, a.y_stride, a.y_vec, y);
+            if (count > 0) load(a.y, a.y_stride, y);
             float dot = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) dot = fmaf(y[j], g[j], dot);
@@ -779,17 +780,17 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
             for (int j = 0; j < 8; ++j) g[j] = fmaf(-y[j], dot, g[j]) / norm;
         }
         if (a.dresidual && count > 0)
-            store8(static_cast<T*>(a.dresidual) + m * a.dresidual_stride + n0, whole && a.dresidual_vec, count, g);
+            store8(static_cast<T*>(a.dresidual) + m * a.dresidual_stride + n0, count, g);
         if (a.act != CHIMERA_ACT_NONE && count > 0) {
             float z[8], slope[8];
-            load8(static_cast<const T*>(a.saved) + m * a.saved_stride + n0, whole && a.saved_vec, count, z);
+            load8(static_cast<const T*>(a.saved) + m * a.saved_stride + n0, count, z);
             slope8(z, slope, a.act);
 #pragma unroll
             for (int j = 0; j < 8; ++j) g[j] = j < count ? g[j] * slope[j] : 0.0f;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) sum[j] += g[j];
-        if (a.g && m < m_end && n0 < a.g_cols) store8(static_cast<T*>(a.g) + m * a.g_cols + n0, true, 8, g);
+        if (a.g && m < m_end && n0 < a.g_cols) store8(static_cast<T*>(a.g) + m * a.g_cols + n0, 8, g);
     }
     if (!a.sums) return;
 #pragma unroll
@@ -1042,11 +1043,6 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     e.act = s.activation;
     e.out_f32 = out == 4;
     e.normalize = s.normalize != 0;
-    e.residual_vec = rows_aligned(a.residual, a.residual_stride, sizeof(T));
-    e.y_vec = rows_aligned(a.y, a.y_stride, out);
-    e.saved_vec = rows_aligned(a.saved, a.saved_stride, sizeof(T));
-    e.bias_vec = rows_aligned(a.bias, 0, sizeof(T));
-    e.vec = e.y_vec && e.bias_vec && (!a.residual || e.residual_vec) && (!a.saved || e.saved_vec);
     Product p = {};
     p.m = s.rows;
     p.n = s.out_features;
@@ -1056,14 +1052,12 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
         p.a_stride = a.x_stride * static_cast<int64_t>(sizeof(T));
         p.b_stride = a.weight_stride * static_cast<int64_t>(sizeof(T));
         p.sum = s.in_features;
-        const bool x_vec = rows_aligned(a.x, a.x_stride, sizeof(T));
-        const bool w_vec = rows_aligned(a.weight, a.weight_stride, sizeof(T));
         const dim3 grid(static_cast<unsigned>(ceil_div(s.out_features, 4 * kWaveOutputs)));
         switch (s.rows) {
-            case 1: hipLaunchKernelGGL((linear_vector_kernel<T, 1>), grid, dim3(256), 0, st, p, e, x_vec, w_vec); break;
-            case 2: hipLaunchKernelGGL((linear_vector_kernel<T, 2>), grid, dim3(256), 0, st, p, e, x_vec, w_vec); break;
-            case 3: hipLaunchKernelGGL((linear_vector_kernel<T, 3>), grid, dim3(256), 0, st, p, e, x_vec, w_vec); break;
-            default: hipLaunchKernelGGL((linear_vector_kernel<T, 4>), grid, dim3(256), 0, st, p, e, x_vec, w_vec);
+            case 1: hipLaunchKernelGGL((linear_vector_kernel<T, 1>), grid, dim3(256), 0, st, p, e); break;
+            case 2: hipLaunchKernelGGL((linear_vector_kernel<T, 2>), grid, dim3(256), 0, st, p, e); break;
+            case 3: hipLaunchKernelGGL((linear_vector_kernel<T, 3>), grid, dim3(256), 0, st, p, e); break;
+            default: hipLaunchKernelGGL((linear_vector_kernel<T, 4>), grid, dim3(256), 0, st, p, e);
         }
         return hipGetLastError();
     }
@@ -1147,10 +1141,6 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
     g.block_rows = plan.block_rows;
     g.out_f32 = out == 4;
     g.normalize = s.normalize != 0;
-    g.dy_vec = rows_aligned(a.dy, a.dy_stride, out);
-    g.y_vec = rows_aligned(a.y, a.y_stride, out);
-    g.saved_vec = rows_aligned(a.saved, a.saved_stride, sizeof(T));
-    g.dresidual_vec = rows_aligned(a.dresidual, a.dresidual_stride, sizeof(T));
     const int64_t blocks = ceil_div(s.rows, plan.block_rows);
     if (g.g || g.sums || g.dresidual)
         hipLaunchKernelGGL((linear_grad_kernel<T>),
@@ -1167,8 +1157,7 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
         e.y = dst;
         e.y_stride = stride;
         e.out_f32 = sizeof(T) == 4;
-        e.vec = e.y_vec = rows_aligned(dst, stride, sizeof(T));
-    };
+        };
     if (a.dx) {
         Product p = {};
         Epilogue e = {};
@@ -1188,8 +1177,7 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
         const int splits = plan.dweight.splits;
         if (splits > 1) {
             e.partial = plan.parts;
-            e.vec = e.y_vec = k % 4 == 0;
-        }
+                }
         launch_tiles<T, true, true, kSums>(st, p, e, plan.dweight);
         if (splits > 1) {
             const int64_t steps = ceil_div(s.rows * static_cast<int64_t>(sizeof(T)), kStepBytes);

@@ -32,24 +32,20 @@ __device__ __forceinline__ float to_float(T v) {
     return static_cast<float>(v);
 }
 
-// Eight neighbouring values of a row.
-// `vec`: the eight lie within the row and at a multiple of 16 bytes (of 8
-// values of T); otherwise the first `count` of them one by one.
+// Eight neighbouring values of a row, of which the first `count` (8 or more:
+// all) exist. Addresses need the alignment of T only: global memory takes
+// 16-byte accesses at any, a little slower where they cross lines.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int count, float (&v)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            const f32x4_t a = *reinterpret_cast<const f32x4_t*>(p), b = *reinterpret_cast<const f32x4_t*>(p + 4);
+__device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
+    if (count >= 8) {
+        typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int kPer = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = a[j];
-                v[4 + j] = b[j];
-            }
-        } else {
-            T t[8];
-            *reinterpret_cast<u32x4_t*>(t) = *reinterpret_cast<const u32x4_t*>(p);
+        for (int h = 0; h < 8 / kPer; ++h) {
+            vec_t t;
+            __builtin_memcpy(&t, p + h * kPer, 16);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = to_float(t[j]);
+            for (int j = 0; j < kPer; ++j) v[h * kPer + j] = to_float(static_cast<T>(t[j]));
         }
         return;
     }
@@ -58,16 +54,16 @@ __device__ __forceinline__ void load8(const T* p, bool vec, int count, float (&v
 }
 
 template <typename T>
-__device__ __forceinline__ void store8(T* p, bool vec, int count, const float (&v)[8]) {
-    if (vec) {
-        if constexpr (sizeof(T) == 4) {
-            *reinterpret_cast<f32x4_t*>(p) = f32x4_t{v[0], v[1], v[2], v[3]};
-            *reinterpret_cast<f32x4_t*>(p + 4) = f32x4_t{v[4], v[5], v[6], v[7]};
-        } else {
-            T t[8];
+__device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
+    if (count >= 8) {
+        typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
+        constexpr int kPer = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = from_float<T>(v[j]);
-            *reinterpret_cast<u32x4_t*>(p) = *reinterpret_cast<const u32x4_t*>(t);
+        for (int h = 0; h < 8 / kPer; ++h) {
+            vec_t t;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) t[j] = from_float<T>(v[h * kPer + j]);
+            __builtin_memcpy(p + h * kPer, &t, 16);
         }
         return;
     }
