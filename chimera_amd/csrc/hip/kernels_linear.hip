@@ -213,6 +213,7 @@ struct Product {
 
 constexpr int kStepBytes = 128;  // of the summed axis per step: 64 or 32 values
 
+constexpr int kSchedMfma = 0x008, kSchedLdsRead = 0x100;  // instruction groups of the scheduler
 constexpr int kWaitLds = 0xC07F;  // s_waitcnt lgkmcnt(0), the others not waited on
 
 // Waits until at most kLoads of the wave's loads (and no LDS access) are under
@@ -304,6 +305,7 @@ struct Side {
 // each half of the wave).
 template <typename T, int kCount, bool kAcross, int kRowBytes>
 struct Reader {
+    static constexpr int kReads = !kAcross ? 1 : sizeof(T) == 4 ? 4 : 2;  // of a tile's quarter step
     uint32_t off[kAcross && sizeof(T) == 2 ? kCount : 1];
 
     __device__ __forceinline__ void init(int first, int l) {
@@ -424,13 +426,24 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     auto read = [&](int s, int quarter, Operands& o) {
         reader_a.read(lds + s % kSlotsA * SideA::kBytes, quarter, o.a);
         reader_b.read(ring_b + s % kSlotsB * SideB::kBytes, quarter, o.b);
-        __builtin_amdgcn_sched_barrier(0);
     };
+    // The products of a quarter, with the LDS reads before it spread between
+    // them (issued all at once they held up the first products: 8192 x 8192 x
+    // 8192 took 950 us, 880 so).
+    constexpr int kMfmas = IM * IN * (sizeof(T) == 4 ? 4 : 1);
+    constexpr int kReads = IM * decltype(reader_a)::kReads + IN * decltype(reader_b)::kReads;
+    constexpr int kBetween = (kReads + kMfmas - 1) / kMfmas;
     auto multiply = [&](const Operands& o) {
 #pragma unroll
         for (int i = 0; i < IM; ++i)
 #pragma unroll
             for (int j = 0; j < IN; ++j) acc[i][j] = mma32<T>(o.b[j], o.a[i], acc[i][j]);
+#pragma unroll
+        for (int g = 0; g < kReads / kBetween; ++g) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, kBetween, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     Operands even, odd;
@@ -438,15 +451,12 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     auto quarters = [&](int s) {
         read(s, 1, odd);
         multiply(even);
-        __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(kWaitLds);  // said before the next reads, it does not wait for them
         read(s, 2, even);
         multiply(odd);
-        __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(kWaitLds);
         read(s, 3, odd);
         multiply(even);
-        __builtin_amdgcn_sched_barrier(0);
     };
     // in the order that the loop goes on with: B and then A of a step, with A
     // kSlotsA - kSlotsB steps ahead
@@ -476,7 +486,6 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
         side_a.fetch(s + kSlotsA, lds + s % kSlotsA * SideA::kBytes, true, left, l);
         read(s + 1, 0, even);
         multiply(odd);
-        __builtin_amdgcn_sched_barrier(0);
         __builtin_amdgcn_s_waitcnt(kWaitLds);
     }
     for (; s < steps; ++s) {
@@ -486,7 +495,6 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
         fetch_a(s + kSlotsA);
         if (s + 1 < steps) read(s + 1, 0, even);
         multiply(odd);
-        __builtin_amdgcn_sched_barrier(0);
     }
 
     // With W as the first operand, D lane l holds row l % 32 of X and of each
@@ -886,23 +894,23 @@ constexpr int kCus = 256;
 // for each tile where it has several or all CUs work. Fitted to products of
 // 64 to 65,536 rows; measured / estimated, us, 16-bit operands:
 //                                      256 x 256   128 x 128    64 x 64
-//     1024 x 1024, sum 1024            25 / 26     10 / 11      7 / 7
-//     4096 x 1024, sum 1024            28 / 29     13 / 14      18 / 20
-//     10007 x 1024, sum 1024           34 / 38     33 / 35      46 / 43
-//     16384 x 1024, sum 1024           39 / 38     48 / 50      76 / 68
-//     65536 x 4096, sum 1024           597 / 566   690 / 751    1039 / 1029
+//     1024 x 1024, sum 1024            25 / 25     12 / 12      8 / 7
+//     4096 x 1024, sum 1024            27 / 27     14 / 13      17 / 18
+//     10007 x 1024, sum 1024           32 / 36     31 / 30      39 / 38
+//     16384 x 1024, sum 1024           37 / 36     43 / 43      66 / 60
+//     65536 x 4096, sum 1024           527 / 528   619 / 638    859 / 905
 // With rows across the sum the data come from beyond the L2 and one tile a CU
-// waits for them: 1024 x 1024 of 16,384 rows takes 222 us in 256 tiles of 64,
-// 66 in four parts of the sum each; 300 in 64 tiles of 128, 85 in four parts,
-// 56 in eight. 32-bit operands are bound by the matrix cores, which small
-// tiles keep busy more evenly: 6001 x 1024, sum 768 takes 111 us on tiles of
-// 128, 89 of 64.
+// waits for them: 1024 x 1024 of 16,384 rows takes 160 us in 256 tiles of 64,
+// 61 in four parts of the sum each; 226 in 64 tiles of 128, 69 in four parts,
+// 50 in eight. 32-bit operands are bound by the matrix cores, which small
+// tiles keep busy more evenly: 6001 x 1024, sum 768 takes 102 us on tiles of
+// 128, 86 of 64.
 struct TileCost {
     int size;
     double alone, alone_across, full;  // us
 };
-constexpr TileCost kCosts16[] = {{256, 0.70, 1.00, 1.10}, {128, 0.225, 0.60, 0.365}, {64, 0.115, 0.42, 0.125}};
-constexpr TileCost kCosts32[] = {{128, 1.00, 1.05, 1.15}, {64, 0.31, 0.31, 0.32}};
+constexpr TileCost kCosts16[] = {{256, 1.33, 1.55, 2.05}, {128, 0.51, 0.87, 0.62}, {64, 0.26, 0.60, 0.22}};
+constexpr TileCost kCosts32[] = {{128, 2.00, 2.20, 2.20}, {64, 0.62, 0.62, 0.60}};
 
 struct TilePlan {
     int size, splits;

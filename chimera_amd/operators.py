@@ -55,11 +55,18 @@ class CacheMaxsim(C.Structure):
                 ("top_counts", P), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 
+_NUMPY = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int32): "int32",
+          np.dtype(np.int64): "int64", np.dtype(np.uint8): "uint8"}
+
+
 def _type_name(a) -> str:
+    d = a.dtype
+    if d.__class__ is str:
+        return _NAMES.get(d, d)
     if getattr(a, "bf16", False):
         return "bf16"
-    name = a.dtype if isinstance(a.dtype, str) else np.dtype(a.dtype).name
-    return _NAMES.get(name, name)
+    d = np.dtype(d)
+    return _NUMPY.get(d) or d.name
 
 
 def _type(a, what: str) -> int:
@@ -70,10 +77,19 @@ def _type(a, what: str) -> int:
 
 
 def _expect(a, what: str, shape: tuple, type_name: str) -> None:
-    if tuple(a.shape) != shape:
+    if a.shape != shape and tuple(a.shape) != shape:
         raise ValueError(f"{what} must have shape {shape}, not {tuple(a.shape)}")
     if _type_name(a) != type_name:
         raise ValueError(f"{what} must be {type_name}, not {_type_name(a)}")
+
+
+def _function(name: str, *argtypes):
+    """An entry point with its argument types set: plain integers and struct
+    references go through without wrapping."""
+    f = capi.lib()[name]
+    f.argtypes = argtypes
+    f.restype = C.c_int
+    return f
 
 
 def _stride(a) -> int:
@@ -109,6 +125,10 @@ class Linear:
         self._shape = LinearShape(0, self.in_features, self.out_features, t, t, ACTIVATIONS[activation], int(normalize))
         self._forward = LinearForward(weight=weight.ptr, bias=_ptr(bias), weight_stride=_stride(weight))
         self._backward = LinearBackward(weight=weight.ptr, weight_stride=_stride(weight))
+        self._shape_ref = C.byref(self._shape)
+        self._forward_ref, self._backward_ref = C.byref(self._forward), C.byref(self._backward)
+        self._call_forward = _function("chimera_linear_forward_device", P, P, P)
+        self._call_backward = _function("chimera_linear_backward_device", P, P, P)
         self._workspace = None
         need = C.c_size_t()
         self._shape.rows = max_rows
@@ -155,7 +175,7 @@ class Linear:
         if norms is not None:
             _expect(norms, "norms", (rows,), "f32")
             a.norms = norms.ptr
-        check(capi.lib().chimera_linear_forward_device(self.ctx.handle, C.byref(self._shape), C.byref(a)))
+        check(self._call_forward(self.ctx.handle, self._shape_ref, self._forward_ref))
 
     def backward(self, x, dy, saved=None, y=None, norms=None, dx=None, dweight=None, dbias=None,
                  dresidual=None) -> None:
@@ -178,7 +198,7 @@ class Linear:
                 if len(shape) == 2:
                     setattr(a, name + "_stride", _stride(v))
             setattr(a, name, _ptr(v))
-        check(capi.lib().chimera_linear_backward_device(self.ctx.handle, C.byref(self._shape), C.byref(a)))
+        check(self._call_backward(self.ctx.handle, self._shape_ref, self._backward_ref))
 
 
 def cache_row(format: str, dim: int, group: int) -> tuple[int, int]:
@@ -211,9 +231,14 @@ class TokenCache:
         self.format, self.dim, self.group, self.page_tokens = format, dim, group, page_tokens
         self.slots = slots
         self._desc = CacheDesc(FORMATS[format], dim, group, page_tokens, slots // page_tokens, codes.ptr, scales.ptr)
+        self._desc_ref = C.byref(self._desc)
+        self._call_write = _function("chimera_cache_write_device", P, P, P, C.c_int32, C.c_int64, P, C.c_int64)
+        self._call_read = _function("chimera_cache_read_device", P, P, P, C.c_int64, P, C.c_int32, C.c_int64)
+        self._call_maxsim = _function("chimera_cache_maxsim_device", P, P, P)
         self._workspace = None
         self._sizes = None
         self._args = CacheMaxsim()
+        self._args_ref = C.byref(self._args)
 
     def close(self) -> None:
         if getattr(self, "_workspace", None) is not None:
@@ -234,9 +259,7 @@ class TokenCache:
         if tuple(rows.shape) != (n, self.dim):
             raise ValueError(f"rows must be [n, {self.dim}]")
         _expect(slots, "slots", (n,), "int64")
-        check(capi.lib().chimera_cache_write_device(self.ctx.handle, C.byref(self._desc), P(rows.ptr),
-                                                    _type(rows, "rows"), C.c_int64(_stride(rows)), P(slots.ptr),
-                                                    C.c_int64(n)))
+        check(self._call_write(self.ctx.handle, self._desc_ref, rows.ptr, _type(rows, "rows"), _stride(rows), slots.ptr, n))
 
     def read(self, slots, out) -> None:
         """out [n, dim] = the values in slots [n], zeros for a slot outside
@@ -245,8 +268,7 @@ class TokenCache:
         if tuple(out.shape) != (n, self.dim):
             raise ValueError(f"out must be [n, {self.dim}]")
         _expect(slots, "slots", (n,), "int64")
-        check(capi.lib().chimera_cache_read_device(self.ctx.handle, C.byref(self._desc), P(slots.ptr), C.c_int64(n),
-                                                   P(out.ptr), _type(out, "out"), C.c_int64(_stride(out))))
+        check(self._call_read(self.ctx.handle, self._desc_ref, slots.ptr, n, out.ptr, _type(out, "out"), _stride(out)))
 
     def maxsim(self, queries, page_start, doc_lens, pages, max_doc_tokens: int, cand_ids, scores, query_lens=None,
                cand_counts=None, k: int = 0, top_ids=None, top_scores=None, top_counts=None) -> None:
@@ -261,16 +283,27 @@ class TokenCache:
         docs, cap = doc_lens.shape[0], cand_ids.shape[1]
         a = self._args
         t = _type(queries, "queries")
-        for name, v, shape, kind in (("page_start", page_start, (docs,), "int64"), ("doc_lens", doc_lens, (docs,), "int32"),
-                                     ("pages", pages, (pages.shape[0],), "int32"),
-                                     ("cand_ids", cand_ids, (nq, cap), "int32"), ("scores", scores, (nq, cap), "f32"),
-                                     ("query_lens", query_lens, (nq,), "int32"),
-                                     ("cand_counts", cand_counts, (nq,), "int32"), ("top_ids", top_ids, (nq, k), "int64"),
-                                     ("top_scores", top_scores, (nq, k), "f32"),
-                                     ("top_counts", top_counts, (nq,), "int32")):
-            if v is not None:
-                _expect(v, name, shape, kind)
-            setattr(a, name, _ptr(v))
+        _expect(page_start, "page_start", (docs,), "int64")
+        _expect(doc_lens, "doc_lens", (docs,), "int32")
+        _expect(pages, "pages", (pages.shape[0],), "int32")
+        _expect(cand_ids, "cand_ids", (nq, cap), "int32")
+        _expect(scores, "scores", (nq, cap), "f32")
+        a.page_start, a.doc_lens, a.pages = page_start.ptr, doc_lens.ptr, pages.ptr
+        a.cand_ids, a.scores = cand_ids.ptr, scores.ptr
+        a.query_lens = a.cand_counts = a.top_ids = a.top_scores = a.top_counts = None
+        if query_lens is not None:
+            _expect(query_lens, "query_lens", (nq,), "int32")
+            a.query_lens = query_lens.ptr
+        if cand_counts is not None:
+            _expect(cand_counts, "cand_counts", (nq,), "int32")
+            a.cand_counts = cand_counts.ptr
+        if k:
+            for name, v, shape, kind in (("top_ids", top_ids, (nq, k), "int64"),
+                                         ("top_scores", top_scores, (nq, k), "f32"),
+                                         ("top_counts", top_counts, (nq,), "int32")):
+                if v is not None:
+                    _expect(v, name, shape, kind)
+                    setattr(a, name, v.ptr)
         a.queries, a.type, a.nq, a.query_len = queries.ptr, t, nq, query_len
         a.num_docs, a.num_page_entries, a.max_doc_tokens = docs, pages.shape[0], max_doc_tokens
         a.cand_cap, a.k = cap, k
@@ -283,4 +316,4 @@ class TokenCache:
                 self._workspace = self.ctx.empty(need.value, np.uint8)
                 a.workspace, a.workspace_bytes = self._workspace.ptr, need.value
             self._sizes = sizes
-        check(capi.lib().chimera_cache_maxsim_device(self.ctx.handle, C.byref(self._desc), C.byref(a)))
+        check(self._call_maxsim(self.ctx.handle, self._desc_ref, self._args_ref))
