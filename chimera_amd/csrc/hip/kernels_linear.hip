@@ -353,8 +353,16 @@ struct Reader {
 // kEnd: the sums are stored, or go through the layer's epilogue, without or
 // with the division by the rows' length (a tile then has all their columns).
 enum End { kSums, kPlainLayer, kNormalizedLayer };
+
+// LDS of a tile: the rings, or the rows on their way out.
+template <int BM, int BN, int WM, int WN, int kSlotsA, int kSlotsB>
+constexpr int tile_lds() {
+    const int rings = (kSlotsA * BM + kSlotsB * BN) * kStepBytes, rows = WM * WN * 32 * (BN / WN + 4) * 4;
+    return rings > rows ? rings : rows;
+}
+
 template <typename T, int BM, int BN, int WM, int WN, int kSlotsA, int kSlotsB, bool kAcrossA, bool kAcrossB, End kEnd>
-__global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, Epilogue e) {
+__device__ __forceinline__ void tile_product(unsigned char* lds, const Product& p, const Epilogue& e, int id, int split) {
     constexpr bool kLayer = kEnd != kSums;
     constexpr bool kNormalize = kEnd == kNormalizedLayer;
     constexpr int W = WM * WN;
@@ -362,10 +370,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     constexpr int IM = TM / 32, IN = TN / 32;
     using SideA = Side<T, BM, W, kAcrossA>;
     using SideB = Side<T, BN, W, kAcrossB>;
-    constexpr int kRings = kSlotsA * SideA::kBytes + kSlotsB * SideB::kBytes;
     constexpr int kPitch = TN + 4;
-    constexpr int kStage = W * 32 * kPitch * 4;
-    __shared__ __align__(1024) unsigned char lds[kRings > kStage ? kRings : kStage];
 
     const int l = lane_id();
     const int w = __builtin_amdgcn_readfirstlane(wave_id());
@@ -374,7 +379,6 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     // blocks go round the 8 XCDs; each XCD takes a run of tiles, in bands of
     // 8 tiles of rows, so that its L2 serves a band's rows and columns
     const int tiles = p.tiles_m * p.tiles_n;
-    const int id = static_cast<int>(blockIdx.x);
     const int per = tiles / 8, rest = tiles % 8, xcd = id % 8;
     const int t = xcd * per + (xcd < rest ? xcd : rest) + id / 8;
     constexpr int kBand = 8;
@@ -383,7 +387,6 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     const int in_band = t - band * kBand * p.tiles_n;
     const int64_t m0 = static_cast<int64_t>(band * kBand + in_band % height) * BM;
     const int n0 = in_band / height * BN;
-    const int split = static_cast<int>(blockIdx.y);
     const int step0 = split * p.steps_per_split;
     const int steps = min(p.steps_per_split, p.steps - step0);
 
@@ -646,6 +649,25 @@ __global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, E
     }
 }
 
+template <typename T, int BM, int BN, int WM, int WN, int kSlotsA, int kSlotsB, bool kAcrossA, bool kAcrossB, End kEnd>
+__global__ __launch_bounds__(WM* WN* kWave) void linear_tile_kernel(Product p, Epilogue e) {
+    __shared__ __align__(1024) unsigned char lds[tile_lds<BM, BN, WM, WN, kSlotsA, kSlotsB>()];
+    tile_product<T, BM, BN, WM, WN, kSlotsA, kSlotsB, kAcrossA, kAcrossB, kEnd>(lds, p, e, static_cast<int>(blockIdx.x),
+                                                                                static_cast<int>(blockIdx.y));
+}
+
+// dW (its parts first, the longer blocks) and dX on tiles of 64 in one launch:
+// neither alone fills the GPU where both take such tiles.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_gradients_kernel(Product pw, Epilogue ew, int splits, Product px, Epilogue ex) {
+    __shared__ __align__(1024) unsigned char lds[tile_lds<64, 64, 2, 2, 3, 2>()];
+    const int id = static_cast<int>(blockIdx.x), tiles = pw.tiles_m * pw.tiles_n;
+    if (id < tiles * splits)
+        tile_product<T, 64, 64, 2, 2, 3, 2, true, true, kSums>(lds, pw, ew, id % tiles, id / tiles);
+    else
+        tile_product<T, 64, 64, 2, 2, 3, 2, false, true, kSums>(lds, px, ex, id - tiles * splits, 0);
+}
+
 // ---- few rows ------------------------------------------------------------------
 
 constexpr int kFewRows = 4;     // rows of X that go this way
@@ -712,26 +734,37 @@ __global__ __launch_bounds__(256) void linear_vector_kernel(Product p, Epilogue 
 
 // ---- layouts -------------------------------------------------------------------
 
-// dst [rows][dst_stride] = src, zeros from column `cols` on: rows of any
+// dst [rows][dst_cols] = src, zeros from column `cols` on: rows of any
 // alignment laid out at multiples of 16 bytes.
+struct AlignJob {
+    const void* src;
+    void* dst;
+    int64_t src_stride, rows;
+    int cols, dst_cols, blocks;
+};
+// Two matrices a launch: the first job's blocks, then the second's.
 template <typename T>
-__global__ __launch_bounds__(256) void linear_align_kernel(const T* __restrict__ src, int64_t src_stride, int64_t rows,
-                                                           int cols, T* __restrict__ dst, int dst_cols) {
+__global__ __launch_bounds__(256) void linear_align_kernel(AlignJob first, AlignJob second) {
     constexpr int kPer = 16 / sizeof(T);
-    const int chunks = dst_cols / kPer;
-    const int64_t total = rows * chunks;
-    for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const bool one = static_cast<int>(blockIdx.x) < first.blocks;
+    const AlignJob job = one ? first : second;
+    const int block = static_cast<int>(blockIdx.x) - (one ? 0 : first.blocks);
+    const int chunks = job.dst_cols / kPer;
+    const int64_t total = job.rows * chunks;
+    for (int64_t i = block * 256ll + threadIdx.x; i < total; i += job.blocks * 256ll) {
         const int64_t r = i / chunks;
         const int c = static_cast<int>(i - r * chunks) * kPer;
-        const T* from = src + r * src_stride + c;
-        T t[kPer];
-        if (c + kPer <= cols) {
-            __builtin_memcpy(t, from, 16);  // at any alignment of elements
+        const T* from = static_cast<const T*>(job.src) + r * job.src_stride + c;
+        u32x4_t t;
+        if (c + kPer <= job.cols) {
+            __builtin_memcpy(&t, from, 16);  // at any alignment of elements
         } else {
+            T v[kPer];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) t[j] = c + j < cols ? from[j] : from_float<T>(0.0f);
+            for (int j = 0; j < kPer; ++j) v[j] = c + j < job.cols ? from[j] : from_float<T>(0.0f);
+            __builtin_memcpy(&t, v, 16);
         }
-        *reinterpret_cast<u32x4_t*>(dst + r * dst_cols + c) = *reinterpret_cast<const u32x4_t*>(t);
+        *reinterpret_cast<u32x4_t*>(static_cast<T*>(job.dst) + r * job.dst_cols + c) = t;
     }
 }
 
@@ -813,53 +846,57 @@ __global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
     }
 }
 
-// db[n] = the sum of the blocks' column sums, in order: 16 waves share the
-// blocks, a lane a column.
+// What is left to sum, in order: dst[rows][cols] = the sum over the parts of
+// src [parts][rows * cols] - the parts of dW's product, or db's column sums.
+struct Join {
+    const float* src;
+    void* dst;
+    int64_t dst_stride, count;
+    int parts, cols;
+};
+
+// Blocks of 512 threads: the first take 2,048 values of dW each, four
+// neighbours a thread (one, where rows are not multiples of four), then the
+// others 64 columns of db each, a lane a column, the parts over eight waves.
 template <typename T>
-__global__ __launch_bounds__(1024) void linear_sums_kernel(const float* __restrict__ src, int parts, int n,
-                                                           T* __restrict__ dst) {
-    __shared__ float sums[16][kWave];
-    const int l = lane_id(), w = wave_id();
-    const int i = static_cast<int>(blockIdx.x) * kWave + l;
-    const int share = (parts + 15) / 16;
-    float s = 0.0f;
-    if (i < n) {
-        const int end = min(parts, (w + 1) * share);
-#pragma unroll 8
-        for (int k = w * share; k < end; ++k) s += src[static_cast<int64_t>(k) * n + i];
+__global__ __launch_bounds__(512) void linear_join_kernel(Join w, int w_blocks, Join b) {
+    __shared__ float sums[8][kWave];
+    if (static_cast<int>(blockIdx.x) < w_blocks) {
+        const bool four = w.cols % 4 == 0;
+        const int64_t i = (blockIdx.x * 512ll + threadIdx.x) * (four ? 4 : 1);
+        if (i >= w.count) return;
+        const int64_t row = i / w.cols;
+        T* to = static_cast<T*>(w.dst) + row * w.dst_stride + (i - row * w.cols);
+        if (four) {
+            f32x4_t s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for (int k = 0; k < w.parts; ++k) s += *reinterpret_cast<const f32x4_t*>(w.src + k * w.count + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[j] = from_float<T>(s[j]);
+        } else {
+            float s = 0.0f;
+#pragma unroll 4
+            for (int k = 0; k < w.parts; ++k) s += w.src[k * w.count + i];
+            to[0] = from_float<T>(s);
+        }
+        return;
     }
-    sums[w][l] = s;
+    const int l = lane_id(), wave = wave_id();
+    const int i = (static_cast<int>(blockIdx.x) - w_blocks) * kWave + l;
+    const int share = (b.parts + 7) / 8;
+    float s = 0.0f;
+    if (i < b.cols) {
+        const int end = min(b.parts, (wave + 1) * share);
+#pragma unroll 8
+        for (int k = wave * share; k < end; ++k) s += b.src[static_cast<int64_t>(k) * b.cols + i];
+    }
+    sums[wave][l] = s;
     __syncthreads();
-    if (w != 0 || i >= n) return;
+    if (wave != 0 || i >= b.cols) return;
     s = 0.0f;
 #pragma unroll
-    for (int o = 0; o < 16; ++o) s += sums[o][l];
-    dst[i] = from_float<T>(s);
-}
-
-// dst (rows of `cols` values at dst_stride) = the sum over s of src[s], the
-// parts of a split product, in order; kPer neighbouring values a thread.
-template <typename T, int kPer>
-__global__ __launch_bounds__(256) void linear_join_kernel(const float* __restrict__ src, int parts, int64_t count,
-                                                          int cols, T* __restrict__ dst, int64_t dst_stride) {
-    const int64_t i = (blockIdx.x * 256ll + threadIdx.x) * kPer;
-    if (i >= count) return;
-    float s[kPer] = {};
-#pragma unroll 4
-    for (int k = 0; k < parts; ++k) {
-        const float* p = src + k * count + i;
-        if constexpr (kPer == 4) {
-            const f32x4_t v = *reinterpret_cast<const f32x4_t*>(p);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += v[j];
-        } else {
-            s[0] += p[0];
-        }
-    }
-    const int64_t row = i / cols;
-    T* to = dst + row * dst_stride + (i - row * cols);
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) to[j] = from_float<T>(s[j]);
+    for (int o = 0; o < 8; ++o) s += sums[o][l];
+    static_cast<T*>(b.dst)[i] = from_float<T>(s);
 }
 
 template <typename T>
@@ -946,12 +983,19 @@ TilePlan tile_plan(int64_t m, int64_t n, int64_t sum, size_t elem, bool across, 
     return best;
 }
 
-template <typename T, bool kAcrossA, bool kAcrossB, End kEnd>
-void launch_tiles(hipStream_t st, Product p, const Epilogue& e, TilePlan plan) {
-    int splits = plan.splits;
+// Sets a product's steps for about `splits` parts of its sum; returns how many
+// parts that makes.
+template <typename T>
+int split_steps(Product& p, int splits) {
+    if (p.sum == 0) return 0;
     p.steps = static_cast<int>(ceil_div(p.sum * static_cast<int64_t>(sizeof(T)), kStepBytes));
     p.steps_per_split = static_cast<int>(ceil_div(p.steps, splits));
-    splits = static_cast<int>(ceil_div(p.steps, p.steps_per_split));
+    return static_cast<int>(ceil_div(p.steps, p.steps_per_split));
+}
+
+template <typename T, bool kAcrossA, bool kAcrossB, End kEnd>
+void launch_tiles(hipStream_t st, Product p, const Epilogue& e, TilePlan plan) {
+    const int splits = split_steps<T>(p, plan.splits);
     auto launch = [&](auto bm, auto bn, auto wm, auto wn, auto slots_a, auto slots_b) {
         constexpr int BM = decltype(bm)::value, BN = decltype(bn)::value, WM = decltype(wm)::value, WN = decltype(wn)::value;
         p.tiles_m = static_cast<int>(ceil_div(p.m, BM));
@@ -1000,12 +1044,11 @@ bool takes_loads(const void* p, int64_t stride, int64_t cols) {
            stride * static_cast<int64_t>(sizeof(T)) <= (int64_t{1} << 22);
 }
 
-// A matrix as a product reads it: as it lies where its rows start at
-// multiples of 16 bytes and end at one, else laid out again in `copy`
-// (rows x round_up(cols, 64)).
+// A matrix as a product reads it: as it lies where its loads can take it, else
+// laid out again in `copy` (rows x round_up(cols, 64)) by a job added to jobs.
 template <typename T>
-void aligned_rows(hipStream_t st, const void* src, int64_t stride, int64_t rows, int cols, void* copy, const void** p,
-                  int64_t* stride_bytes) {
+void aligned_rows(const void* src, int64_t stride, int64_t rows, int cols, void* copy, const void** p,
+                  int64_t* stride_bytes, AlignJob* jobs, int* count) {
     if (takes_loads<T>(src, stride, cols)) {
         *p = src;
         *stride_bytes = stride * static_cast<int64_t>(sizeof(T));
@@ -1013,11 +1056,19 @@ void aligned_rows(hipStream_t st, const void* src, int64_t stride, int64_t rows,
     }
     const int wide = static_cast<int>(round_up(cols, 64));
     const int64_t chunks = rows * (wide * static_cast<int64_t>(sizeof(T)) / 16);
-    const unsigned blocks = static_cast<unsigned>(std::min<int64_t>(ceil_div(chunks, 256), 65536));
-    hipLaunchKernelGGL((linear_align_kernel<T>), dim3(blocks), dim3(256), 0, st, static_cast<const T*>(src), stride, rows,
-                       cols, static_cast<T*>(copy), wide);
+    jobs[(*count)++] = AlignJob{src, copy, stride, rows, cols, wide,
+                                static_cast<int>(std::min<int64_t>(ceil_div(chunks, 256), 65536))};
     *p = copy;
     *stride_bytes = wide * static_cast<int64_t>(sizeof(T));
+}
+
+template <typename T>
+void launch_align(hipStream_t st, const AlignJob* jobs, int count) {
+    if (count == 0) return;
+    const AlignJob none = {};
+    const AlignJob& second = count > 1 ? jobs[1] : none;
+    hipLaunchKernelGGL((linear_align_kernel<T>), dim3(static_cast<unsigned>(jobs[0].blocks + second.blocks)), dim3(256), 0, st,
+                       jobs[0], second);
 }
 
 struct ForwardPlan {
@@ -1071,8 +1122,11 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     }
     ForwardPlan plan;
     (void)carve_forward(s, a.workspace, &plan);
-    aligned_rows<T>(st, a.x, a.x_stride, s.rows, s.in_features, plan.x, &p.a, &p.a_stride);
-    aligned_rows<T>(st, a.weight, a.weight_stride, s.out_features, s.in_features, plan.weight, &p.b, &p.b_stride);
+    AlignJob jobs[2];
+    int njobs = 0;
+    aligned_rows<T>(a.x, a.x_stride, s.rows, s.in_features, plan.x, &p.a, &p.a_stride, jobs, &njobs);
+    aligned_rows<T>(a.weight, a.weight_stride, s.out_features, s.in_features, plan.weight, &p.b, &p.b_stride, jobs, &njobs);
+    launch_align<T>(st, jobs, njobs);
     // whole chunks: as the matrices lie, or both laid out again with zeros
     p.sum = round_up(s.in_features, 16 / sizeof(T));
     const TilePlan tiles = tile_plan(p.m, p.n, p.sum, sizeof(T), false, false);
@@ -1153,52 +1207,61 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
     if (g.g || g.sums || g.dresidual)
         hipLaunchKernelGGL((linear_grad_kernel<T>),
                            dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(ceil_div(n, 128))), dim3(256), 0, st, g);
-    if (a.dbias)
-        hipLaunchKernelGGL((linear_sums_kernel<T>), dim3(static_cast<unsigned>(ceil_div(n, kWave))), dim3(1024), 0, st,
-                           plan.sums, static_cast<int>(blocks), n, static_cast<T*>(a.dbias));
     const void* dz = as_it_is ? a.dy : plan.g;
     const int64_t dz_stride = (as_it_is ? a.dy_stride : plan.n_pad) * static_cast<int64_t>(sizeof(T));
     auto product_to = [&](Product& p, Epilogue& e, int64_t m, int cols, int64_t sum, void* dst, int64_t stride) {
+        p.a = dz;
+        p.a_stride = dz_stride;
         p.m = e.m = m;
         p.n = e.n = cols;
         p.sum = sum;
         e.y = dst;
         e.y_stride = stride;
         e.out_f32 = sizeof(T) == 4;
-        };
+    };
+    Product px = {}, pw = {};
+    Epilogue ex = {}, ew = {};
+    TilePlan tiles_x = {};
+    AlignJob jobs[2];
+    int njobs = 0;
     if (a.dx) {
-        Product p = {};
-        Epilogue e = {};
-        product_to(p, e, s.rows, k, n, a.dx, a.dx_stride);
-        p.a = dz;
-        p.a_stride = dz_stride;
-        aligned_rows<T>(st, a.weight, a.weight_stride, n, k, plan.weight, &p.b, &p.b_stride);
-        launch_tiles<T, false, true, kSums>(st, p, e, tile_plan(p.m, p.n, p.sum, sizeof(T), true, false));
+        product_to(px, ex, s.rows, k, n, a.dx, a.dx_stride);
+        tiles_x = tile_plan(px.m, px.n, px.sum, sizeof(T), true, false);
+        aligned_rows<T>(a.weight, a.weight_stride, n, k, plan.weight, &px.b, &px.b_stride, jobs, &njobs);
     }
     if (a.dweight) {
-        Product p = {};
-        Epilogue e = {};
-        product_to(p, e, n, k, s.rows, a.dweight, a.dweight_stride);
-        p.a = dz;
-        p.a_stride = dz_stride;
-        aligned_rows<T>(st, a.x, a.x_stride, s.rows, k, plan.x, &p.b, &p.b_stride);
-        const int splits = plan.dweight.splits;
-        if (splits > 1) {
-            e.partial = plan.parts;
-                }
-        launch_tiles<T, true, true, kSums>(st, p, e, plan.dweight);
-        if (splits > 1) {
-            const int64_t steps = ceil_div(s.rows * static_cast<int64_t>(sizeof(T)), kStepBytes);
-            const int parts = static_cast<int>(ceil_div(steps, ceil_div(steps, splits)));
-            const int64_t count = static_cast<int64_t>(n) * k;
-            if (k % 4 == 0)
-                hipLaunchKernelGGL((linear_join_kernel<T, 4>), dim3(static_cast<unsigned>(ceil_div(count, 1024))), dim3(256),
-                                   0, st, plan.parts, parts, count, k, static_cast<T*>(a.dweight), a.dweight_stride);
-            else
-                hipLaunchKernelGGL((linear_join_kernel<T, 1>), dim3(static_cast<unsigned>(ceil_div(count, 256))), dim3(256),
-                                   0, st, plan.parts, parts, count, k, static_cast<T*>(a.dweight), a.dweight_stride);
-        }
+        product_to(pw, ew, n, k, s.rows, a.dweight, a.dweight_stride);
+        aligned_rows<T>(a.x, a.x_stride, s.rows, k, plan.x, &pw.b, &pw.b_stride, jobs, &njobs);
+        if (plan.dweight.splits > 1) ew.partial = plan.parts;
     }
+    launch_align<T>(st, jobs, njobs);
+    const int parts = split_steps<T>(pw, plan.dweight.splits);
+    if (a.dx && a.dweight && tiles_x.size == 64 && plan.dweight.size == 64) {
+        split_steps<T>(px, 1);
+        for (Product* p : {&pw, &px}) {
+            p->tiles_m = static_cast<int>(ceil_div(p->m, 64));
+            p->tiles_n = static_cast<int>(ceil_div(p->n, 64));
+        }
+        const int64_t blocks = static_cast<int64_t>(pw.tiles_m) * pw.tiles_n * parts + static_cast<int64_t>(px.tiles_m) * px.tiles_n;
+        hipLaunchKernelGGL((linear_gradients_kernel<T>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, st, pw, ew, parts,
+                           px, ex);
+    } else {
+        if (a.dx) launch_tiles<T, false, true, kSums>(st, px, ex, tiles_x);
+        if (a.dweight) launch_tiles<T, true, true, kSums>(st, pw, ew, plan.dweight);
+    }
+    Join jw = {}, jb = {};
+    int64_t w_blocks = 0, b_blocks = 0;
+    if (ew.partial) {
+        jw = Join{plan.parts, a.dweight, a.dweight_stride, static_cast<int64_t>(n) * k, parts, k};
+        w_blocks = ceil_div(jw.count, k % 4 == 0 ? 2048 : 512);
+    }
+    if (a.dbias) {
+        jb = Join{plan.sums, a.dbias, n, n, static_cast<int>(blocks), n};
+        b_blocks = ceil_div(n, kWave);
+    }
+    if (w_blocks + b_blocks > 0)
+        hipLaunchKernelGGL((linear_join_kernel<T>), dim3(static_cast<unsigned>(w_blocks + b_blocks)), dim3(512), 0, st, jw,
+                           static_cast<int>(w_blocks), jb);
     return hipGetLastError();
 }
 
