@@ -35,15 +35,17 @@ __device__ __forceinline__ float to_float(T v) {
 // Eight neighbouring values of a row, of which the first `count` (8 or more:
 // all) exist. Addresses need the alignment of T only: global memory takes
 // 16-byte accesses at any, a little slower where they cross lines.
-template <typename T>
+// kOnce: past the caches, for data that are not needed again soon.
+template <typename T, bool kOnce = false>
 __device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
     if (count >= 8) {
         typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
         constexpr int kPer = 16 / static_cast<int>(sizeof(T));
 #pragma unroll
         for (int h = 0; h < 8 / kPer; ++h) {
-            vec_t t;
-            __builtin_memcpy(&t, p + h * kPer, 16);
+            typedef vec_t any_t __attribute__((aligned(sizeof(T))));
+            const any_t* from = reinterpret_cast<const any_t*>(p + h * kPer);
+            const vec_t t = kOnce ? __builtin_nontemporal_load(from) : *from;
 #pragma unroll
             for (int j = 0; j < kPer; ++j) v[h * kPer + j] = to_float(static_cast<T>(t[j]));
         }
@@ -53,7 +55,7 @@ __device__ __forceinline__ void load8(const T* p, int count, float (&v)[8]) {
     for (int j = 0; j < 8; ++j) v[j] = j < count ? to_float(p[j]) : 0.0f;
 }
 
-template <typename T>
+template <typename T, bool kOnce = false>
 __device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
     if (count >= 8) {
         typedef T vec_t __attribute__((ext_vector_type(16 / sizeof(T))));
@@ -63,7 +65,12 @@ __device__ __forceinline__ void store8(T* p, int count, const float (&v)[8]) {
             vec_t t;
 #pragma unroll
             for (int j = 0; j < kPer; ++j) t[j] = from_float<T>(v[h * kPer + j]);
-            __builtin_memcpy(p + h * kPer, &t, 16);
+            typedef vec_t any_t __attribute__((aligned(sizeof(T))));
+            any_t* to = reinterpret_cast<any_t*>(p + h * kPer);
+            if constexpr (kOnce)
+                __builtin_nontemporal_store(t, to);
+            else
+                *to = t;
         }
         return;
     }
