@@ -161,30 +161,35 @@ __device__ __forceinline__ f16x8_t int8_values(u32x2_t u) {
     return v;
 }
 __device__ __forceinline__ f16x8_t int4_values(uint32_t u) {
-    const f16x2_t bias = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
+    // the bits of a stored code are that many times fp16's least value, 2^-24;
+    // code - 8 of them is exact, and code_unit brings the sums back
+    const f16x2_t eight = __builtin_bit_cast(f16x2_t, 0x00080008u);
     f16x8_t v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const f16x2_t p = __builtin_bit_cast(f16x2_t, ((u >> (4 * j)) & 0x000F000Fu) | 0x64006400u) - bias;
+        const f16x2_t p = __builtin_bit_cast(f16x2_t, (u >> (4 * j)) & 0x000F000Fu) - eight;
         v[2 * j] = p[0];
         v[2 * j + 1] = p[1];
     }
     return v;
 }
 __device__ __forceinline__ f16x8_t fp8_values(u32x2_t u) {
-    // e4m3 bits under fp16's exponent are the value times 2^-8, also below
-    // the least normal one; 2^8 brings it back exactly
-    const f16x2_t up = {static_cast<_Float16>(256.0f), static_cast<_Float16>(256.0f)};
     f16x8_t v;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const uint32_t x = u[j / 2] >> (16 * (j % 2));
-        const uint32_t pair = ((x & 0x7Fu) << 7) | ((x & 0x80u) << 8) | ((x & 0x7F00u) << 15) | ((x & 0x8000u) << 16);
-        const f16x2_t p = __builtin_bit_cast(f16x2_t, pair) * up;
-        v[2 * j] = p[0];
-        v[2 * j + 1] = p[1];
+    for (int j = 0; j < 2; ++j) {
+        const auto lo = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u[j], 1.0f, false);
+        const auto hi = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(u[j], 1.0f, true);
+        v[4 * j] = lo[0];
+        v[4 * j + 1] = lo[1];
+        v[4 * j + 2] = hi[0];
+        v[4 * j + 3] = hi[1];
     }
     return v;
+}
+// What a code's value is multiplied with to give the code.
+template <int kFormat>
+constexpr float code_unit() {
+    return kFormat == CHIMERA_CACHE_INT4 ? 0x1p24f : 1.0f;
 }
 // Which of eight neighbouring values the j-th one is.
 template <int kFormat>
@@ -241,7 +246,7 @@ struct QueryTile {
         most = fmaxf(most, __shfl_xor(most, 32, kWave));
         int e = 0;
         frexpf(most > 0.0f ? most : 1.0f, &e);
-        e = min(max(e, -126), 126);  // both powers of two are normal numbers
+        e = min(max(e, -100), 100);  // all powers of two here are normal numbers
         const float to = ldexpf(1.0f, -e);
 #pragma unroll
         for (int g = 0; g < 4; ++g)
@@ -254,7 +259,7 @@ struct QueryTile {
                     part[0][g][h][j] = hi;
                     if constexpr (kParts == 2) part[1][g][h][j] = static_cast<_Float16>(v - static_cast<float>(hi));
                 }
-        back = __shfl(ldexpf(1.0f, e), row_of_lane(l), kWave);
+        back = __shfl(ldexpf(1.0f, e) * code_unit<kFormat>(), row_of_lane(l), kWave);
         if ((l & 1) != 0 || row_of_lane(l) >= rows) back = 0.0f;
     }
 };
@@ -291,11 +296,11 @@ __device__ __forceinline__ float maxima_to_rows(float (&v)[16], int l) {
 // that the token's scale and the running maxima need no exchange before the
 // document's end. Lanes past a document's last token take that token again;
 // an absent token has NaN for its scale, which the maxima pass over.
-// kOneScale: one scale a row, applied to the sum.
-template <typename T, int kFormat, bool kOneScale>
+// kRuns: runs of 32 values that share a scale: 1, 2, or 4 for one scale a row.
+template <typename T, int kFormat, int kRuns>
 __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
     constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
-    constexpr int kScales = kOneScale ? 1 : 4;
+    constexpr int kScales = 4 / kRuns;
     const int l = lane_id();
     const int q = static_cast<int>(blockIdx.y);
     const int w = __builtin_amdgcn_readfirstlane(wave_id());
@@ -326,7 +331,6 @@ __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
     if (work == 0) return;
     const int q_len = a.query_lens ? min(max(a.query_lens[q], 0), a.query_len) : a.query_len;
     const int groups = (a.c.dim + 31) / 32;
-    const int shift = a.c.group_log2 - 5;
     const int half = l >> 5;
     const int rows_padded = (a.query_len + 31) / 32 * 32;
 
@@ -390,37 +394,37 @@ __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) best[r] = -INFINITY;
 
-        auto multiply = [&](const Tile& tile) {
-            f32x16_t sum = {}, acc = {};
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                if (g >= groups) break;
-                f16x8_t v0, v1;
-                if constexpr (kFormat == CHIMERA_CACHE_INT4) {
-                    v0 = int4_values(tile.codes[g / 2][2 * (g % 2)]);
-                    v1 = int4_values(tile.codes[g / 2][2 * (g % 2) + 1]);
-                } else {
-                    const u32x4_t u = tile.codes[g];
-                    v0 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[0], u[1]}) : fp8_values(u32x2_t{u[0], u[1]});
-                    v1 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[2], u[3]}) : fp8_values(u32x2_t{u[2], u[3]});
-                }
-#pragma unroll
-                for (int s = 0; s < kParts; ++s) {
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qt.part[s][g][0], v0, acc, 0, 0, 0);
-                    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qt.part[s][g][1], v1, acc, 0, 0, 0);
-                }
-                // the end of a scale's group
-                if constexpr (!kOneScale) {
-                    if (((g + 1) & ((1 << shift) - 1)) == 0 || g + 1 == groups) {
-                        const float scale = shift == 0 ? tile.scale[g] : tile.scale[g / 2];
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) sum[r] = fmaf(acc[r], scale, sum[r]);
-                        acc = f32x16_t{};
-                    }
-                }
+        auto run = [&](const Tile& tile, int g, f32x16_t acc) {
+            f16x8_t v0, v1;
+            if constexpr (kFormat == CHIMERA_CACHE_INT4) {
+                v0 = int4_values(tile.codes[g / 2][2 * (g % 2)]);
+                v1 = int4_values(tile.codes[g / 2][2 * (g % 2) + 1]);
+            } else {
+                const u32x4_t u = tile.codes[g];
+                v0 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[0], u[1]}) : fp8_values(u32x2_t{u[0], u[1]});
+                v1 = kFormat == CHIMERA_CACHE_INT8 ? int8_values(u32x2_t{u[2], u[3]}) : fp8_values(u32x2_t{u[2], u[3]});
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) best[r] = fmaxf(best[r], kOneScale ? acc[r] * tile.scale[0] : sum[r]);
+            for (int s = 0; s < kParts; ++s) {
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qt.part[s][g][0], v0, acc, 0, 0, 0);
+                acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(qt.part[s][g][1], v1, acc, 0, 0, 0);
+            }
+            return acc;
+        };
+        auto multiply = [&](const Tile& tile) {
+            f32x16_t sum;
+#pragma unroll
+            for (int i = 0; i < kScales; ++i) {
+                if (i > 0 && i * kRuns >= groups) break;
+                f32x16_t acc = run(tile, i * kRuns, f32x16_t{});
+#pragma unroll
+                for (int g = 1; g < kRuns; ++g)
+                    if (i * kRuns + g < groups) acc = run(tile, i * kRuns + g, acc);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sum[r] = i == 0 ? acc[r] * tile.scale[0] : fmaf(acc[r], tile.scale[i], sum[r]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) best[r] = fmaxf(best[r], sum[r]);
         };
         // after an item's last tile
         auto finish = [&](const Cursor& c) {
@@ -640,10 +644,10 @@ hipError_t launch_cache_maxsim(hipStream_t st, const chimera_cache& c, const chi
     hipError_t e = by_format(c.format, m.type, [&](auto f, auto t) {
         using T = decltype(t);
         constexpr int kFormat = decltype(f)::value;
-        if (a.c.row_scales == 1)
-            hipLaunchKernelGGL((cache_maxsim_kernel<T, kFormat, true>), grid, dim3(256), 0, st, a);
-        else
-            hipLaunchKernelGGL((cache_maxsim_kernel<T, kFormat, false>), grid, dim3(256), 0, st, a);
+        auto* kernel = a.c.row_scales == 1   ? cache_maxsim_kernel<T, kFormat, 4>
+                       : a.c.group_log2 == 6 ? cache_maxsim_kernel<T, kFormat, 2>
+                                             : cache_maxsim_kernel<T, kFormat, 1>;
+        hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, a);
     });
     if (e != hipSuccess) return e;
     if (s.count > 1) hipLaunchKernelGGL(cache_maxsim_join_kernel, dim3(static_cast<unsigned>(m.cand_cap), static_cast<unsigned>(m.nq)),
