@@ -21,8 +21,10 @@ bool known_type(int type) { return type == CHIMERA_F32 || type == CHIMERA_F16 ||
 
 constexpr int kMostFeatures = 65536;
 constexpr int kMostNormalized = 128;
-// blocks of 512 threads that one launch may have, in tiles of 128 x 128
-constexpr int64_t kMostTiles = int64_t{1} << 22;
+// tiles of 128 x 128 that one launch may have (blocks of 32 rows stay within
+// 2^32 threads), and values of a weight
+constexpr int64_t kMostTiles = int64_t{1} << 21;
+constexpr int64_t kMostWeights = int64_t{1} << 30;
 constexpr int kMostCandidates = 8192;  // the top-k sorts a query's candidates in LDS
 
 int check_shape(const chimera_linear_shape* s) {
@@ -37,7 +39,9 @@ int check_shape(const chimera_linear_shape* s) {
     if (s->normalize && s->out_features > kMostNormalized) return invalid("normalized rows have at most 128 features");
     const int64_t widest = s->in_features > s->out_features ? s->in_features : s->out_features;
     if (s->rows > (int64_t{1} << 31) || (s->rows + 127) / 128 * ((widest + 127) / 128) > kMostTiles)
-        return invalid("too many rows for one call: rows * features / 16384 must not pass 2^22");
+        return invalid("too many rows for one call: rows * features / 16384 must not pass 2^21");
+    if (static_cast<int64_t>(s->in_features) * s->out_features > kMostWeights)
+        return invalid("a weight has at most 2^30 values");
     return CHIMERA_OK;
 }
 
@@ -49,6 +53,37 @@ int check_matrix(const char* name, const void* p, int64_t stride, int64_t cols, 
     return CHIMERA_OK;
 }
 int check_vector(const char* name, const void* p, size_t elem) { return check_matrix(name, p, 0, 0, elem); }
+
+// What a call reads or writes, for the check that outputs lie apart.
+struct Region {
+    const char* name;
+    const void* p;
+    int64_t rows, row_bytes, stride_bytes;
+};
+Region region(const char* name, const void* p, int64_t rows, int64_t cols, int64_t stride, size_t elem) {
+    return Region{name, p, rows, cols * static_cast<int64_t>(elem), stride * static_cast<int64_t>(elem)};
+}
+// Whether two matrices share a byte. Rows of the same stride may interleave
+// (columns of one wider matrix); otherwise the ranges have to be apart.
+bool overlap(const Region& a, const Region& b) {
+    if (!a.p || !b.p || a.rows == 0 || b.rows == 0) return false;
+    const char *pa = static_cast<const char*>(a.p), *pb = static_cast<const char*>(b.p);
+    const char *ea = pa + (a.rows - 1) * a.stride_bytes + a.row_bytes, *eb = pb + (b.rows - 1) * b.stride_bytes + b.row_bytes;
+    if (ea <= pb || eb <= pa) return false;
+    if (a.stride_bytes != b.stride_bytes || a.stride_bytes == 0) return true;
+    const int64_t apart = ((pb - pa) % a.stride_bytes + a.stride_bytes) % a.stride_bytes;
+    return apart < a.row_bytes || apart + b.row_bytes > a.stride_bytes;
+}
+template <size_t kOut, size_t kIn>
+int check_apart(const Region (&outs)[kOut], const Region (&ins)[kIn]) {
+    for (size_t i = 0; i < kOut; ++i) {
+        for (const Region& in : ins)
+            if (overlap(outs[i], in)) return invalid(std::string(outs[i].name) + " overlaps " + in.name);
+        for (size_t j = i + 1; j < kOut; ++j)
+            if (overlap(outs[i], outs[j])) return invalid(std::string(outs[i].name) + " overlaps " + outs[j].name);
+    }
+    return CHIMERA_OK;
+}
 
 int check_workspace(const void* p, size_t have, size_t need) {
     if (need == 0) return CHIMERA_OK;
@@ -127,7 +162,18 @@ int chimera_linear_forward_device(chimera_ctx* ctx, const chimera_linear_shape* 
     if (args->saved) CK(check_matrix("saved", args->saved, args->saved_stride, shape->out_features, e));
     if (args->norms) CK(check_vector("norms", args->norms, 4));
     if (args->norms && !shape->normalize) return invalid("norms are an output of normalized layers");
-    CK(check_workspace(args->workspace, args->workspace_bytes, linear_forward_workspace(*shape)));
+    const size_t need = linear_forward_workspace(*shape);
+    CK(check_workspace(args->workspace, args->workspace_bytes, need));
+    const int64_t m = shape->rows, k = shape->in_features, n = shape->out_features, bytes = static_cast<int64_t>(need);
+    const Region outs[] = {region("y", args->y, m, n, args->y_stride, out),
+                           region("saved", args->saved, m, n, args->saved_stride, e),
+                           region("norms", args->norms, 1, m, m, 4),
+                           region("the workspace", args->workspace, 1, bytes, bytes, 1)};
+    const Region ins[] = {region("x", args->x, m, k, args->x_stride, e),
+                          region("weight", args->weight, n, k, args->weight_stride, e),
+                          region("bias", args->bias, 1, n, n, e),
+                          region("residual", args->residual, m, n, args->residual_stride, e)};
+    CK(check_apart(outs, ins));
     return launched(launch_linear_forward(st, LinearForward{*shape, *args}), "linear forward kernels");
 }
 
@@ -155,7 +201,22 @@ int chimera_linear_backward_device(chimera_ctx* ctx, const chimera_linear_shape*
         }
         if (args->dresidual)
             CK(check_matrix("dresidual", args->dresidual, args->dresidual_stride, shape->out_features, e));
-        CK(check_workspace(args->workspace, args->workspace_bytes, linear_backward_workspace(*shape)));
+        const size_t need = linear_backward_workspace(*shape);
+        CK(check_workspace(args->workspace, args->workspace_bytes, need));
+        const int64_t m = shape->rows, k = shape->in_features, n = shape->out_features, bytes = static_cast<int64_t>(need);
+        const bool act = shape->activation != CHIMERA_ACT_NONE, norm = shape->normalize != 0;
+        const Region outs[] = {region("dx", args->dx, m, k, args->dx_stride, e),
+                               region("dweight", args->dweight, n, k, args->dweight_stride, e),
+                               region("dbias", args->dbias, 1, n, n, e),
+                               region("dresidual", args->dresidual, m, n, args->dresidual_stride, e),
+                               region("the workspace", args->workspace, 1, bytes, bytes, 1)};
+        const Region ins[] = {region("x", args->dweight ? args->x : nullptr, m, k, args->x_stride, e),
+                              region("weight", args->dx ? args->weight : nullptr, n, k, args->weight_stride, e),
+                              region("dy", args->dy, m, n, args->dy_stride, out),
+                              region("saved", act ? args->saved : nullptr, m, n, args->saved_stride, e),
+                              region("y", norm ? args->y : nullptr, m, n, args->y_stride, out),
+                              region("norms", norm ? args->norms : nullptr, 1, m, m, 4)};
+        CK(check_apart(outs, ins));
     }
     return launched(launch_linear_backward(st, LinearBackward{*shape, *args}), "linear backward kernels");
 }

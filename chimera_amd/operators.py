@@ -106,7 +106,7 @@ class Linear:
     length with `normalize` (at most 128 outputs). weight [out, in] and bias
     [out] stay the caller's arrays and may change between calls. The object
     holds the workspace for calls of up to max_rows rows, and with `training`
-    for the backward pass."""
+    for the backward pass; close it before its context."""
 
     def __init__(self, ctx: capi.Context, weight, bias=None, activation: str = "none", normalize: bool = False,
                  max_rows: int = 1, training: bool = False):
@@ -215,7 +215,8 @@ class TokenCache:
     """Quantised token embeddings in pages of page_tokens slots: codes [slots,
     row bytes] uint8 and scales [slots, scales] f32, the caller's arrays. A
     call's workspace is kept for the next one and grows as needed (a call that
-    needs a larger one waits for the work before it)."""
+    needs a larger one waits for the work before it). Close the cache before
+    its context."""
 
     def __init__(self, ctx: capi.Context, codes, scales, format: str = "int8", dim: int = 128, group: int = 128,
                  page_tokens: int = 16):

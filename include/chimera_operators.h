@@ -49,10 +49,11 @@ extern "C" {
  * are held in 32 bits and rounded once. Matrices are row-major with a row
  * stride in elements; any stride of at least the row's length and any
  * alignment of whole elements will do, rows that start at multiples of 16
- * bytes are the fast ones. Outputs overlap neither inputs nor each other. */
+ * bytes are the fast ones. Outputs and workspace overlap neither inputs nor
+ * each other (columns of one wider matrix do not overlap). */
 typedef struct {
-    int64_t rows;         /* >= 0 */
-    int32_t in_features;  /* 1..65536 */
+    int64_t rows;         /* >= 0; rows * features at most 2^35 */
+    int32_t in_features;  /* 1..65536, in_features * out_features at most 2^30 */
     int32_t out_features; /* 1..65536; at most 128 with normalize */
     int32_t type;         /* CHIMERA_F32, _F16 or _BF16 */
     int32_t out_type;     /* type or CHIMERA_F32 */

@@ -307,3 +307,54 @@ def test_absent_tokens_and_empty_queries():
     for v in (rows, at, c, *dev):
         v.free()
     ctx.close()
+
+
+def test_graph_of_writing_reading_and_scoring():
+    """Captured calls replay with the eager results, with eager work between
+    the replays."""
+    import ctypes as C
+
+    from chimera_amd import capi
+
+    hip = C.CDLL("libamdhip64.so.7")
+    rng = np.random.default_rng(3)
+    ctx = context()
+    page, dim = 16, 128
+    lens = np.array([700, 30, 5], np.int32)  # split: two launches
+    start, pages, slots, total = corpus(rng, lens, page)
+    c = Cache(ctx, total * page, "int8", dim, 128, page)
+    x = rng.standard_normal((total * page, dim)).astype(np.float32)
+    rows, at, out = Matrix(ctx, x, "f32"), Array(ctx, np.arange(total * page)), Matrix(ctx, None, "f32", shape=x.shape)
+    q = Matrix(ctx, rng.standard_normal((2, 32, dim)), "f32")
+    dev = [Array(ctx, v) for v in (start, lens, pages, np.tile(np.arange(3, dtype=np.int32), (2, 1)))]
+    scores = Matrix(ctx, None, "f32", shape=(2, 3))
+    top = [Array(ctx, np.zeros((2, 2), np.int64)), Array(ctx, np.zeros((2, 2), np.float32)), Array(ctx, np.zeros(2, np.int32))]
+
+    def step():
+        c.cache.write(rows, at)
+        c.cache.read(at, out)
+        c.cache.maxsim(q, dev[0], dev[1], dev[2], 700, dev[3], scores, k=2, top_ids=top[0], top_scores=top[1],
+                       top_counts=top[2])
+
+    def results():
+        return [out.values(), scores.values(), c.codes.numpy(), c.scales.numpy(), *(t.numpy() for t in top)]
+
+    step()
+    want = results()
+    stream, graph, run = C.c_void_p(), C.c_void_p(), C.c_void_p()
+    capi.check(capi.lib().chimera_stream(ctx.handle, C.byref(stream)))
+    assert hip.hipStreamBeginCapture(stream, 0) == 0
+    step()
+    assert hip.hipStreamEndCapture(stream, C.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(C.byref(run), graph, None, None, C.c_size_t(0)) == 0
+    for _ in range(3):
+        assert hip.hipGraphLaunch(run, stream) == 0
+        ctx.synchronize()
+        assert all(np.array_equal(a, b) for a, b in zip(results(), want))
+        step()
+        ctx.synchronize()
+    hip.hipGraphExecDestroy(run)
+    hip.hipGraphDestroy(graph)
+    for v in (rows, at, out, q, *dev, scores, *top, c):
+        v.free()
+    ctx.close()

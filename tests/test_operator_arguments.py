@@ -61,6 +61,24 @@ for field in ("dy", "x", "weight", "saved", "y", "norms"):
 for field, v in (("dy_stride", 31), ("dx_stride", 63), ("dweight_stride", 63), ("dresidual_stride", 31)):
     refuses(bwd, b, field, v, "row stride of " + field[:-7])
 refuses(bwd, b, "workspace_bytes", need.value // 1000, "workspace", 4)
+# outputs lie apart from inputs and each other; columns of one matrix do
+refuses(fwd, f, "y", M, "y overlaps x")
+refuses(fwd, f, "saved", 2 * M + 512, "saved overlaps weight")
+refuses(fwd, f, "norms", 5 * M + 64, "y overlaps norms")
+refuses(fwd, f, "workspace", 4 * M, "the workspace overlaps residual")
+refuses(bwd, b, "dx", 3 * M, "dx overlaps dy")
+refuses(bwd, b, "dweight", 7 * M + 128, "dx overlaps dweight")
+refuses(bwd, b, "dbias", 4 * M, "dbias overlaps saved")
+for y, stride, code in ((M + 128, 64, 0), (M + 124, 64, 1), (M + 128, 63, 1), (M + 64, 64, 1)):
+    wide = op.LinearForward.from_buffer_copy(f)
+    wide.x_stride, wide.y, wide.y_stride = 128, y, stride  # rows of 256 bytes: x in 128, y in 128
+    got = L.chimera_linear_forward_device(ctx.handle, C.byref(s), C.byref(wide))
+    assert got == code, (stride, y, got, L.chimera_last_error())
+hip.host_hip_reset_launches()
+refuses(fwd, s, "in_features", 65536, "row stride")
+s2 = op.LinearShape(1, 65536, 65536, 2, 2, 0, 0)
+rc(1, "2^30", L.chimera_linear_workspace, C.byref(s2), 0, C.byref(need))
+assert L.chimera_linear_workspace(C.byref(s), 1, C.byref(need)) == 0
 rc(1, "null context", L.chimera_linear_forward_device, None, C.byref(s), C.byref(f))
 rc(1, "null", L.chimera_linear_forward_device, ctx.handle, None, C.byref(f))
 rc(1, "null", L.chimera_linear_forward_device, ctx.handle, C.byref(s), None)
