@@ -161,13 +161,14 @@ __device__ __forceinline__ f16x8_t int8_values(u32x2_t u) {
     return v;
 }
 __device__ __forceinline__ f16x8_t int4_values(uint32_t u) {
-    // the bits of a stored code are that many times fp16's least value, 2^-24;
-    // code - 8 of them is exact, and code_unit brings the sums back
-    const f16x2_t eight = __builtin_bit_cast(f16x2_t, 0x00080008u);
+    // a stored code below the exponent of 1024 is 1032 + code. (Its bits alone,
+    // multiples of fp16's least value, cost as much and the products of such
+    // values lost four bits in the matrix instruction's sums.)
+    const f16x2_t bias = {static_cast<_Float16>(1032.0f), static_cast<_Float16>(1032.0f)};
     f16x8_t v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const f16x2_t p = __builtin_bit_cast(f16x2_t, (u >> (4 * j)) & 0x000F000Fu) - eight;
+        const f16x2_t p = __builtin_bit_cast(f16x2_t, ((u >> (4 * j)) & 0x000F000Fu) | 0x64006400u) - bias;
         v[2 * j] = p[0];
         v[2 * j + 1] = p[1];
     }
@@ -185,11 +186,6 @@ __device__ __forceinline__ f16x8_t fp8_values(u32x2_t u) {
         v[4 * j + 3] = hi[1];
     }
     return v;
-}
-// What a code's value is multiplied with to give the code.
-template <int kFormat>
-constexpr float code_unit() {
-    return kFormat == CHIMERA_CACHE_INT4 ? 0x1p24f : 1.0f;
 }
 // Which of eight neighbouring values the j-th one is.
 template <int kFormat>
@@ -259,7 +255,7 @@ struct QueryTile {
                     part[0][g][h][j] = hi;
                     if constexpr (kParts == 2) part[1][g][h][j] = static_cast<_Float16>(v - static_cast<float>(hi));
                 }
-        back = __shfl(ldexpf(1.0f, e) * code_unit<kFormat>(), row_of_lane(l), kWave);
+        back = __shfl(ldexpf(1.0f, e), row_of_lane(l), kWave);
         if ((l & 1) != 0 || row_of_lane(l) >= rows) back = 0.0f;
     }
 };

@@ -275,6 +275,36 @@ def test_maxsim(format, dim, group, page, type, nq, q_len, lens, cap):
     ctx.close()
 
 
+@pytest.mark.parametrize("format", ["int8", "int4", "fp8"])
+@pytest.mark.parametrize("type", ["f32", "f16"])
+def test_maxsim_keeps_32_bits(format, type):
+    """Single tokens against single documents of one token: the error is that
+    of a sum of 128 products in 32 bits in about eight joins, and of a query in
+    two halves of 11 bits. Both are near 2^-24 of a sum's size; 2^-22 over the
+    mean square."""
+    rng = np.random.default_rng(17)
+    n, dim = 2048, 128
+    start, pages, slots, total = corpus(rng, np.ones(n, np.int32), 8)
+    ctx = context()
+    c = Cache(ctx, total * 8, format, dim, 32, 8)
+    x = rng.standard_normal((total * 8, dim)).astype(np.float32)
+    rows, at = Matrix(ctx, x, "f32"), Array(ctx, np.arange(total * 8))
+    c.cache.write(rows, at)
+    _, s, value = quantise(x, format, 32)
+    tokens = spread(value, s, 32, dim).astype(np.float64)
+    q = to_type(rng.standard_normal((2, 1, dim)), type)
+    ids = np.tile(np.arange(n, dtype=np.int32), (2, 1))
+    dev = {"q": Matrix(ctx, q, type), "start": Array(ctx, start), "lens": Array(ctx, np.ones(n, np.int32)),
+           "pages": Array(ctx, pages), "ids": Array(ctx, ids), "scores": Matrix(ctx, None, "f32", shape=(2, n))}
+    c.cache.maxsim(dev["q"], dev["start"], dev["lens"], dev["pages"], 1, dev["ids"], dev["scores"])
+    have = dev["scores"].values()
+    want = reference(q, np.ones(2, np.int64), tokens, slots, ids, np.full(2, n))
+    assert np.sqrt(np.square(have - want).mean()) <= 2.0**-22 * np.sqrt(np.square(want).mean())
+    for v in (c, *dev.values(), rows, at):
+        v.free()
+    ctx.close()
+
+
 def test_absent_tokens_and_empty_queries():
     """Pages outside the cache or the list and tokens past max_doc_tokens are
     absent; a query without tokens scores 0."""
