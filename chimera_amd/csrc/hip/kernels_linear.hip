@@ -44,35 +44,33 @@ __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
     return z < 0.0f ? tail : 1.0f - tail;
 }
 
-// Phi(z) for values that are rounded to 16 bits: 1/2 + z P(z^2), a minimax
-// fit on [-4, 4] held to 0 and 1 at its ends (and, clamped, beyond), within
-// 3.4e-5 of Phi, so that gelu is within 1.4e-4: a thirtieth of a bf16 step at
-// 1, half an fp16 rounding. 11 full-rate instructions where the exact form
-// takes 20 and two quarter-rate ones: 65,536 x 4096 outputs took 200 us with
-// that form, a third of the layer's products.
-__device__ __forceinline__ float normal_cdf_16(float z) {
-    const float c = __builtin_amdgcn_fmed3f(z, -4.0f, 4.0f);
-    const float t = c * c;
-    float p = fmaf(-1.2773050395153973e-09f, t, 1.0440346898121788e-07f);
-    p = fmaf(p, t, -3.708714984895778e-06f);
-    p = fmaf(p, t, 7.617972005391493e-05f);
-    p = fmaf(p, t, -1.020980766043067e-03f);
-    p = fmaf(p, t, 9.581183083355427e-03f);
-    p = fmaf(p, t, -6.606381386518478e-02f);
-    p = fmaf(p, t, 0.3988054394721985f);
-    return __builtin_amdgcn_fmed3f(fmaf(p, c, 0.5f), 0.0f, 1.0f);
+// z Phi(z) for results that are rounded to 16 bits: Phi(-a) = 2^P(a) for
+// a >= 0 with P a minimax fit on [0, 6], so that results are within 1.9e-4 of
+// their size above 4e-5 (half a rounding of fp16) and within 3e-5 everywhere;
+// P falls to -infinity beyond. 10 full-rate instructions and one quarter-rate
+// one where the exact form takes 20 and two: 65,536 x 4096 outputs took 200 us
+// with that form, a third of the layer's products.
+__device__ __forceinline__ float gelu_16(float z) {
+    const float a = fabsf(z);
+    float p = fmaf(-2.4950269e-4f, a, 5.092669e-3f);
+    p = fmaf(p, a, -4.5601506e-2f);
+    p = fmaf(p, a, -0.46793399f);
+    p = fmaf(p, a, -1.147275f);
+    p = fmaf(p, a, -1.000271f);
+    const float tail = __builtin_amdgcn_exp2f(p);
+    return z * (z > 0.0f ? 1.0f - tail : tail);
 }
 
-// T: the type that the result is rounded to or that the layer works in.
-template <typename T>
+constexpr int kRoundedGelu = -1;  // gelu_16 for CHIMERA_ACT_GELU
+
 __device__ __forceinline__ float activation(float z, int act) {
     switch (act) {
         case CHIMERA_ACT_RELU: return z > 0.0f ? z : (z != z ? z : 0.0f);
         case CHIMERA_ACT_GELU: {
-            if constexpr (sizeof(T) == 2) return z * normal_cdf_16(z);
             float gauss;
             return z * normal_cdf(z, &gauss);
         }
+        case kRoundedGelu: return gelu_16(z);
         case CHIMERA_ACT_GELU_TANH:  // (1 + tanh u) / 2 is the sigmoid of 2 u
             return z * sigmoid(2.0f * kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
         case CHIMERA_ACT_SILU: return z * sigmoid(z);
@@ -128,11 +126,14 @@ __device__ __forceinline__ void activate(float (&v)[kRuns][16], int act) {
 #pragma unroll
         for (int j = 0; j < kRuns; ++j)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) v[j][r] = activation<T>(v[j][r], decltype(a)::value);
+            for (int r = 0; r < 16; ++r) v[j][r] = activation(v[j][r], decltype(a)::value);
     };
     switch (act) {
         case CHIMERA_ACT_RELU: all(std::integral_constant<int, CHIMERA_ACT_RELU>{}); break;
         case CHIMERA_ACT_GELU: all(std::integral_constant<int, CHIMERA_ACT_GELU>{}); break;
+        case kRoundedGelu:
+            if constexpr (sizeof(T) == 2) all(std::integral_constant<int, kRoundedGelu>{});
+            break;
         case CHIMERA_ACT_GELU_TANH: all(std::integral_constant<int, CHIMERA_ACT_GELU_TANH>{}); break;
         case CHIMERA_ACT_SILU: all(std::integral_constant<int, CHIMERA_ACT_SILU>{}); break;
         default: break;
@@ -724,7 +725,7 @@ __global__ __launch_bounds__(256) void linear_vector_kernel(Product p, Epilogue 
     if (m >= kRows || n >= p.n) return;
     if (e.bias) z += to_float(static_cast<const T*>(e.bias)[n]);
     if (e.saved) static_cast<T*>(e.saved)[m * e.saved_stride + n] = from_float<T>(z);
-    float h = activation<T>(z, e.act);
+    float h = activation(z, e.act);
     if (e.residual) h += to_float(static_cast<const T*>(e.residual)[m * e.residual_stride + n]);
     if (e.out_f32)
         static_cast<float*>(e.y)[m * e.y_stride + n] = h;
@@ -1099,7 +1100,7 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     e.saved_stride = a.saved_stride;
     e.m = s.rows;
     e.n = s.out_features;
-    e.act = s.activation;
+    e.act = s.activation == CHIMERA_ACT_GELU && out == 2 ? kRoundedGelu : s.activation;
     e.out_f32 = out == 4;
     e.normalize = s.normalize != 0;
     Product p = {};

@@ -303,3 +303,30 @@ def test_graph_of_a_training_step():
     hip.hipGraphDestroy(graph)
     release(ctx, layer, {**d, **g})
     ctx.close()
+
+
+@pytest.mark.parametrize("type,out", [("f32", "f32"), ("f16", "f32"), ("bf16", "f32"), ("f16", "f16"), ("bf16", "bf16")])
+@pytest.mark.parametrize("rows", [1, 40])
+def test_gelu_over_its_range(type, out, rows):
+    """Sums that are the weights themselves. Results in 32 bits are within
+    2^-20 of 1 + |z|, and below zero, where they are small, within 2^-8 of
+    their size to -6; those rounded to 16 bits within 2^-12 of their size to -4
+    and 2^-8 to -6, before the rounding; infinities and NaN as in the formula."""
+    z = to_type(np.concatenate([np.linspace(-12, 12, 4001), [0.0, 1e-3, -1e-3, 60000.0, -60000.0]])[None], type)
+    special = to_type(np.array([[np.inf, -np.inf, np.nan]]), type)
+    w = np.concatenate([z, special], axis=1).T
+    x = np.ones((rows, 1))
+    ctx = context()
+    layer, d = run_forward(ctx, x, w, None, None, type, out, "gelu", False)
+    have = d["y"].values()[-1]
+    want = linear(x[:1], z.T, None, None, "gelu", False)[4][0]
+    z = z[0]
+    size = np.abs(want)
+    off = 2.0**-20 * (1 + np.abs(z)) if out == "f32" else 2.0**-12 * size
+    close = np.where(z < -6, 3e-8, np.where(z < -4, 2.0**-8 * size, np.maximum(2.0**-12 * size, off)))
+    close = np.where((out == "f32") & (z < 0), np.minimum(off, np.maximum(2.0**-8 * size, 3e-8)), close)
+    least = 2.0**-25 if out == "f16" else 0.0
+    assert (np.abs(have[:-3] - want) <= close + 2.0**-BITS[out] * size + least).all()
+    assert have[-3] == np.inf and np.isnan(have[-2:]).all()
+    release(ctx, layer, d)
+    ctx.close()
