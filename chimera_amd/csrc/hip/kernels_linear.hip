@@ -988,13 +988,14 @@ struct TilePlan {
     int size, splits;
 };
 
-TilePlan tile_plan(int64_t m, int64_t n, int64_t sum, size_t elem, bool across, bool may_split) {
+// The least estimate among tiles, and among parts of the sum up to most_splits.
+TilePlan tile_plan(int64_t m, int64_t n, int64_t sum, size_t elem, bool across, int64_t most_splits) {
     const int64_t all_steps = ceil_div(sum * static_cast<int64_t>(elem), kStepBytes);
     TilePlan best = {0, 1};
     double least = 0.0;
     auto consider = [&](const TileCost& c) {
         const double tiles = static_cast<double>(ceil_div(m, c.size)) * static_cast<double>(ceil_div(n, c.size));
-        for (int64_t splits = 1; splits == 1 || (may_split && splits <= 256 && all_steps / splits >= 8); splits *= 2) {
+        for (int64_t splits = 1; splits == 1 || (splits <= most_splits && all_steps / splits >= 8); splits *= 2) {
             const double share = tiles * static_cast<double>(splits) / kCus;  // tiles a CU
             const double alone = across ? c.alone_across : c.alone;
             // CUs hold one tile of 256 at a time, two of 128, four of 64
@@ -1164,7 +1165,7 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     launch_align<T>(st, jobs, njobs);
     // whole chunks: as the matrices lie, or both laid out again with zeros
     p.sum = round_up(s.in_features, 16 / sizeof(T));
-    const TilePlan tiles = tile_plan(p.m, p.n, p.sum, sizeof(T), false, false);
+    const TilePlan tiles = tile_plan(p.m, p.n, p.sum, sizeof(T), false, 1);
     if (e.normalize)
         launch_tiles<T, false, false, kNormalizedLayer>(st, p, e, tiles);
     else
@@ -1180,6 +1181,21 @@ struct BackwardPlan {
     float *sums, *parts;
 };
 
+// Parts that dW's sum may have, and that the workspace has room for: those of
+// a few tiles of 64 a CU (64 MB), or as many as take the room of X and dZ laid
+// out again where that is more. Grows with the rows only, so that a workspace
+// sized for some rows serves fewer; the least estimate without a bound lies
+// beyond it for 2 of 60,000 random shapes, where it costs 1 and 3 %.
+int64_t most_parts(int64_t rows, int64_t n, int64_t k, size_t elem) {
+    const int64_t e = static_cast<int64_t>(elem);
+    const int64_t tiles = ceil_div(n, 64) * ceil_div(k, 64);
+    const int64_t most = std::min<int64_t>(
+        {256, std::max<int64_t>(16 * kCus / tiles, rows * e * (n + k) / (4 * n * k)), ceil_div(rows * e, kStepBytes) / 8});
+    int64_t parts = 1;
+    while (parts * 2 <= most) parts *= 2;
+    return parts;
+}
+
 size_t carve_backward(const chimera_linear_shape& s, void* base, BackwardPlan* plan) {
     Carve c{static_cast<char*>(base)};
     const size_t e = type_bytes(s.type);
@@ -1189,12 +1205,16 @@ size_t carve_backward(const chimera_linear_shape& s, void* base, BackwardPlan* p
     // about 1,024 blocks of 16 to 512 rows
     plan->block_rows = static_cast<int>(std::max<int64_t>(
         16, std::min<int64_t>(512, round_up(ceil_div(s.rows * ceil_div(s.out_features, 128), 1024), 16))));
-    plan->dweight = tile_plan(s.out_features, s.in_features, s.rows, e, true, true);
+    const int64_t most = most_parts(s.rows, s.out_features, s.in_features, e);
+    plan->dweight = tile_plan(s.out_features, s.in_features, s.rows, e, true, most);
+    // blocks of any number of rows up to these
+    const int64_t most_blocks = std::min<int64_t>(
+        ceil_div(s.rows, 16), std::max<int64_t>(ceil_div(1024, ceil_div(s.out_features, 128)), ceil_div(s.rows, 512)));
     plan->g = c.take(static_cast<size_t>(s.rows) * plan->n_pad * e);
     plan->x = c.take(static_cast<size_t>(s.rows) * wide);
     plan->weight = c.take(n * wide);
-    plan->sums = static_cast<float*>(c.take(static_cast<size_t>(ceil_div(s.rows, plan->block_rows)) * n * 4));
-    plan->parts = static_cast<float*>(c.take(plan->dweight.splits > 1 ? plan->dweight.splits * n * k * 4 : 0));
+    plan->sums = static_cast<float*>(c.take(static_cast<size_t>(most_blocks) * n * 4));
+    plan->parts = static_cast<float*>(c.take(most > 1 ? static_cast<size_t>(most) * n * k * 4 : 0));
     return c.off;
 }
 
@@ -1261,7 +1281,7 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
     int njobs = 0;
     if (a.dx) {
         product_to(px, ex, s.rows, k, n, a.dx, a.dx_stride);
-        tiles_x = tile_plan(px.m, px.n, px.sum, sizeof(T), true, false);
+        tiles_x = tile_plan(px.m, px.n, px.sum, sizeof(T), true, 1);
         aligned_rows<T>(a.weight, a.weight_stride, n, k, plan.weight, &px.b, &px.b_stride, jobs, &njobs);
     }
     if (a.dweight) {
