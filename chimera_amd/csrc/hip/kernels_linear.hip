@@ -45,18 +45,24 @@ __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
 }
 
 // z Phi(z) for results that are rounded to 16 bits: Phi(-a) = 2^P(a) for
-// a >= 0 with P a minimax fit on [0, 6], so that results are within 1.9e-4 of
-// their size above 4e-5 (half a rounding of fp16) and within 3e-5 everywhere;
-// P falls to -infinity beyond. 10 full-rate instructions and one quarter-rate
-// one where the exact form takes 20 and two: 65,536 x 4096 outputs took 200 us
-// with that form, a third of the layer's products.
+// a >= 0 with P a minimax fit on [0, 6] (2.5e-7 of the size), so that results
+// are within 3e-6 of their size there, most of which is P's own rounding, and
+// within 6e-9 below -6, where P falls to -infinity. 14 full-rate instructions
+// and one quarter-rate one. (Five coefficients less give 1.9e-4, which is seen
+// in the rounding: 8 % of fp16 results were not the nearest value. They took
+// 65,536 x 4096 outputs 630 us instead of 672.)
 __device__ __forceinline__ float gelu_16(float z) {
     const float a = fabsf(z);
-    float p = fmaf(-2.4950269e-4f, a, 5.092669e-3f);
-    p = fmaf(p, a, -4.5601506e-2f);
-    p = fmaf(p, a, -0.46793399f);
-    p = fmaf(p, a, -1.147275f);
-    p = fmaf(p, a, -1.000271f);
+    float p = fmaf(-1.2316869e-8f, a, 4.1466188e-7f);
+    p = fmaf(p, a, -5.9383565e-6f);
+    p = fmaf(p, a, 4.5272715e-5f);
+    p = fmaf(p, a, -1.6424450e-4f);
+    p = fmaf(p, a, -2.6072026e-4f);
+    p = fmaf(p, a, 7.2999932e-3f);
+    p = fmaf(p, a, -5.2711684e-2f);
+    p = fmaf(p, a, -4.5911723e-1f);
+    p = fmaf(p, a, -1.1511194f);
+    p = fmaf(p, a, -0.99999964f);
     const float tail = __builtin_amdgcn_exp2f(p);
     return z * (z > 0.0f ? 1.0f - tail : tail);
 }
@@ -352,7 +358,7 @@ struct Reader {
 // take new loads, before that quarter is multiplied. One meeting a step.
 // Bound by the matrix cores and the LDS and loads that feed them: 8192 x 8192 x
 // 8192 bf16 takes 880 us (1.25 PFLOP/s), 65,536 x 1024 -> 4096 with bias and
-// GELU 630 (0.87; the same sums without the epilogue 530). Four waves of
+// GELU 672 (0.82; the same sums without the epilogue 530). Four waves of
 // 128 x 128, two blocks a CU on 128 x 256, deeper rings and a whole step in
 // registers were all slower.
 // kEnd: the sums are stored, or go through the layer's epilogue, without or
