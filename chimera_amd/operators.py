@@ -139,7 +139,10 @@ class Linear:
                 args.workspace, args.workspace_bytes = self._workspace.ptr, need.value
 
     def close(self) -> None:
+        """Frees the workspace; calls after it are refused."""
         if getattr(self, "_workspace", None) is not None:
+            for args in (self._forward, self._backward):
+                args.workspace, args.workspace_bytes = None, 0
             self.ctx.synchronize()
             self._workspace.free()
             self._workspace = None
@@ -237,12 +240,19 @@ class TokenCache:
         self._call_read = _function("chimera_cache_read_device", P, P, P, C.c_int64, P, C.c_int32, C.c_int64)
         self._call_maxsim = _function("chimera_cache_maxsim_device", P, P, P)
         self._workspace = None
-        self._sizes = None
+        self._closed = False
+        self._sizes = None  # of the call that the workspace was last found large enough for
         self._args = CacheMaxsim()
         self._args_ref = C.byref(self._args)
 
     def close(self) -> None:
+        """Frees the workspace; calls after it that need one are refused."""
+        self._closed = True
+        self._drop_workspace()
+
+    def _drop_workspace(self) -> None:
         if getattr(self, "_workspace", None) is not None:
+            self._args.workspace, self._args.workspace_bytes = None, 0
             self.ctx.synchronize()
             self._workspace.free()
             self._workspace = None
@@ -309,12 +319,13 @@ class TokenCache:
         a.num_docs, a.num_page_entries, a.max_doc_tokens = docs, pages.shape[0], max_doc_tokens
         a.cand_cap, a.k = cap, k
         sizes = (nq, query_len, cap, max_doc_tokens)
-        if sizes != self._sizes:
+        if sizes != self._sizes and not self._closed:
             need = C.c_size_t()
             check(capi.lib().chimera_cache_maxsim_workspace(C.byref(a), C.byref(need)))
             if need.value > (0 if self._workspace is None else self._workspace.nbytes):
-                self.close()
-                self._workspace = self.ctx.empty(need.value, np.uint8)
-                a.workspace, a.workspace_bytes = self._workspace.ptr, need.value
+                larger = self.ctx.empty(need.value, np.uint8)  # where it fails the present one stays
+                self._drop_workspace()
+                self._workspace = larger
+                a.workspace, a.workspace_bytes = larger.ptr, need.value
             self._sizes = sizes
         check(self._call_maxsim(self.ctx.handle, self._desc_ref, self._args_ref))
