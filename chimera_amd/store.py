@@ -59,10 +59,19 @@ class TokenStore:
         if not 0 <= doc < len(self._docs) or self._docs[doc] is None:
             raise KeyError(f"no document {doc}")
 
-    def _slots(self, doc: int, begin: int, end: int) -> np.ndarray:
-        pages = np.asarray(self._docs[doc], np.int64)
+    def _slots(self, pages: list[int], begin: int, end: int) -> np.ndarray:
         t = np.arange(begin, end)
-        return pages[t // self.page_tokens] * self.page_tokens + t % self.page_tokens
+        return np.asarray(pages, np.int64)[t // self.page_tokens] * self.page_tokens + t % self.page_tokens
+
+    def _next_pages(self, count: int) -> list[int]:
+        """The pages that the next document gets; they stay free until they
+        are taken."""
+        if count > len(self._free):
+            raise MemoryError(f"{count} pages are needed, {len(self._free)} are free")
+        return self._free[len(self._free) - count:][::-1]
+
+    def _take(self, pages: list[int]) -> None:
+        del self._free[len(self._free) - len(pages):]
 
     def _write(self, embeddings, slots: np.ndarray) -> None:
         if slots.size == 0:
@@ -84,23 +93,26 @@ class TokenStore:
         after the other's (a numpy array or a device array), and the number of
         tokens of each. Returns their numbers."""
         lens = [int(n) for n in doc_lens]
-        if any(n < 0 for n in lens) or sum(lens) != embeddings.shape[0] or embeddings.shape[1] != self.dim:
+        if len(embeddings.shape) != 2 or embeddings.shape[1] != self.dim or any(n < 0 for n in lens) or \
+                sum(lens) != embeddings.shape[0]:
             raise ValueError(f"the lengths must add up to the rows of embeddings [tokens, {self.dim}]")
-        need = sum(-(-n // self.page_tokens) for n in lens)
-        if need > len(self._free):
-            raise MemoryError(f"{need} pages are needed, {len(self._free)} are free")
+        owned = [-(-n // self.page_tokens) for n in lens]
+        pages = self._next_pages(sum(owned))
+        ends = np.cumsum([0, *owned]).tolist()
+        per_doc = [pages[a:b] for a, b in zip(ends, ends[1:])]
+        slots = [self._slots(p, 0, n) for p, n in zip(per_doc, lens)]
+        self._write(embeddings, np.concatenate(slots).astype(np.int64) if slots else np.zeros(0, np.int64))
+        # nothing has changed up to here, so a refused write leaves the store as it was
+        self._take(pages)
         ids = []
-        for n in lens:
+        for p, n in zip(per_doc, lens):
             doc = self._unused.pop() if self._unused else len(self._docs)
             if doc == len(self._docs):
                 self._docs.append(None)
                 self._lens.append(0)
-            self._docs[doc] = [self._free.pop() for _ in range(-(-n // self.page_tokens))]
-            self._lens[doc] = n
+            self._docs[doc], self._lens[doc] = p, n
             ids.append(doc)
         self._drop_tables()
-        slots = [self._slots(doc, 0, n) for doc, n in zip(ids, lens)]
-        self._write(embeddings, np.concatenate(slots).astype(np.int64) if slots else np.zeros(0, np.int64))
         return ids
 
     def append(self, doc: int, embeddings) -> None:
@@ -109,13 +121,12 @@ class TokenStore:
         if len(embeddings.shape) != 2 or embeddings.shape[1] != self.dim:
             raise ValueError(f"embeddings must be [tokens, {self.dim}]")
         begin, end = self._lens[doc], self._lens[doc] + embeddings.shape[0]
-        more = -(-end // self.page_tokens) - len(self._docs[doc])
-        if more > len(self._free):
-            raise MemoryError(f"{more} pages are needed, {len(self._free)} are free")
-        self._docs[doc].extend(self._free.pop() for _ in range(more))
+        pages = self._next_pages(-(-end // self.page_tokens) - len(self._docs[doc]))
+        self._write(embeddings, self._slots(self._docs[doc] + pages, begin, end).astype(np.int64))
+        self._take(pages)
+        self._docs[doc] = self._docs[doc] + pages
         self._lens[doc] = end
         self._drop_tables()
-        self._write(embeddings, self._slots(doc, begin, end).astype(np.int64))
 
     def remove(self, doc: int) -> None:
         self._check(doc)
@@ -130,7 +141,7 @@ class TokenStore:
         n = self._lens[doc]
         if n == 0:
             return np.zeros((0, self.dim), np.float32)
-        slots = self.ctx.to_device(self._slots(doc, 0, n).astype(np.int64))
+        slots = self.ctx.to_device(self._slots(self._docs[doc], 0, n).astype(np.int64))
         out = self.ctx.empty((n, self.dim), np.float32)
         try:
             self.cache.read(slots, out)

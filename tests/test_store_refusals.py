@@ -1,0 +1,54 @@
+"""What calls that fail leave of a TokenStore, on the CPU: the library runs on
+a model of the HIP runtime with failing allocations."""
+from host_hip_child import host_hip  # noqa: F401
+
+SETUP = """
+from chimera_amd.store import TokenStore
+
+ctx = context()
+store = TokenStore(ctx, num_pages=20, dim=64, group=64, page_tokens=8)
+
+def rows(n):
+    return np.ones((n, 64), np.float32)
+
+def state():
+    docs = range(len(store._docs))
+    return (store.free_tokens, list(store._free), [store._docs[d] and list(store._docs[d]) for d in docs],
+            list(store._lens), list(store._unused), hip.host_hip_used())
+
+def leaves_all(kind, call, *args):
+    before = state()
+    try:
+        call(*args)
+    except kind:
+        assert state() == before, (before, state())
+        return
+    raise AssertionError("not refused")
+"""
+
+
+def test_a_write_that_fails_leaves_the_documents(host_hip):  # noqa: F811
+    host_hip(SETUP + """
+a, b, c = store.add(rows(3 + 17 + 8), [3, 17, 8])
+store.remove(b)
+whole = ctx.empty((5, 64), np.int32)  # not an element type
+five = ctx.empty((5, 64), np.float32)
+store.tables()
+leaves_all(ValueError, store.append, a, whole)
+leaves_all(ValueError, store.add, whole, [5])
+leaves_all(ValueError, store.add, whole, [2, 3])
+leaves_all(ValueError, store.add, np.ones(64, np.float32), [1])
+assert store.doc_len(a) == 3
+# no memory for the slots
+hip.host_hip_refuse_malloc(C.c_size_t(40), C.c_size_t(40))
+leaves_all(capi.ChimeraError, store.append, a, five)
+leaves_all(capi.ChimeraError, store.add, five, [5])
+leaves_all(capi.ChimeraError, store.append, c, five)
+hip.host_hip_refuse_malloc(C.c_size_t(0), C.c_size_t(0))
+store.append(a, five)
+(d,) = store.add(five, [5])
+assert d == b and store.doc_len(a) == 8 and store.doc_len(d) == 5
+# pages are not given twice
+held = [p for pages in store._docs if pages for p in pages] + store._free
+assert sorted(held) == list(range(20))
+""")
