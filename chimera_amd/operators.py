@@ -6,7 +6,9 @@ go on top of the cache.
 Arrays are device arrays: capi.DeviceArray, or any object with `ptr`, `shape`
 and `dtype` ("f32", "f16", "bf16", a numpy dtype or its name) and, for a
 matrix whose rows lie apart, `stride` in elements. Calls are asynchronous on
-the context's stream.
+the context's stream. An object keeps the arguments of its calls, so threads
+that share one take turns; calls can be captured into a graph, which stays good
+until the object is closed.
 """
 from __future__ import annotations
 
@@ -217,9 +219,11 @@ def cache_row(format: str, dim: int, group: int) -> tuple[int, int]:
 class TokenCache:
     """Quantised token embeddings in pages of page_tokens slots: codes [slots,
     row bytes] uint8 and scales [slots, scales] f32, the caller's arrays. A
-    call's workspace is kept for the next one and grows as needed (a call that
-    needs a larger one waits for the work before it). Close the cache before
-    its context."""
+    call's workspace is kept for the next one; where one needs a larger one, it
+    allocates (so it cannot be captured: make a call of that size first), and
+    the smaller ones stay until close() for the graphs that hold their
+    addresses. Each is at least twice the one before it, the last below 32 MiB.
+    Close the cache before its context."""
 
     def __init__(self, ctx: capi.Context, codes, scales, format: str = "int8", dim: int = 128, group: int = 128,
                  page_tokens: int = 16):
@@ -239,23 +243,25 @@ class TokenCache:
         self._call_write = _function("chimera_cache_write_device", P, P, P, C.c_int32, C.c_int64, P, C.c_int64)
         self._call_read = _function("chimera_cache_read_device", P, P, P, C.c_int64, P, C.c_int32, C.c_int64)
         self._call_maxsim = _function("chimera_cache_maxsim_device", P, P, P)
-        self._workspace = None
+        self._workspaces = []  # the last one is in use
         self._closed = False
         self._sizes = None  # of the call that the workspace was last found large enough for
         self._args = CacheMaxsim()
         self._args_ref = C.byref(self._args)
 
     def close(self) -> None:
-        """Frees the workspace; calls after it that need one are refused."""
+        """Frees the workspaces; calls after it that need one are refused."""
         self._closed = True
-        self._drop_workspace()
-
-    def _drop_workspace(self) -> None:
-        if getattr(self, "_workspace", None) is not None:
+        workspaces = getattr(self, "_workspaces", None)
+        if workspaces:
             self._args.workspace, self._args.workspace_bytes = None, 0
             self.ctx.synchronize()
-            self._workspace.free()
-            self._workspace = None
+            while workspaces:
+                workspaces.pop().free()
+
+    @property
+    def _workspace(self):
+        return self._workspaces[-1] if self._workspaces else None
 
     def __del__(self):
         try:
@@ -322,10 +328,10 @@ class TokenCache:
         if sizes != self._sizes and not self._closed:
             need = C.c_size_t()
             check(capi.lib().chimera_cache_maxsim_workspace(C.byref(a), C.byref(need)))
-            if need.value > (0 if self._workspace is None else self._workspace.nbytes):
-                larger = self.ctx.empty(need.value, np.uint8)  # where it fails the present one stays
-                self._drop_workspace()
-                self._workspace = larger
-                a.workspace, a.workspace_bytes = larger.ptr, need.value
+            have = 0 if self._workspace is None else self._workspace.nbytes
+            if need.value > have:
+                larger = self.ctx.empty(max(need.value, 2 * have), np.uint8)
+                self._workspaces.append(larger)
+                a.workspace, a.workspace_bytes = larger.ptr, larger.nbytes
             self._sizes = sizes
         check(self._call_maxsim(self.ctx.handle, self._desc_ref, self._args_ref))

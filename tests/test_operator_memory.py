@@ -69,3 +69,19 @@ assert "workspace" in fails(layer.forward, x, y)
 assert "workspace" in fails(layer.backward, x, y, dx=ctx.empty((10, 64), "bf16"))
 assert hip.host_hip_launches(b"linear") == 0 and held(layer, layer._forward) == held(layer, layer._backward) == 0
 """)
+
+
+def test_outgrown_workspaces_stay_for_graphs(host_hip):  # noqa: F811
+    """A captured call's workspace stays allocated while later calls take
+    larger ones, up to close()."""
+    host_hip(SETUP + """
+begin = hip.host_hip_used()
+kept = {}
+for tokens in (600, 1000, 3000, 20_000, 60_000, 200_000):
+    maxsim(ctx, cache, tokens)
+    kept[cache._args.workspace] = -(-cache._workspace.nbytes // 4096) * 4096
+    assert hip.host_hip_used() - begin == sum(kept.values())
+assert len(kept) > 2 and sum(kept.values()) <= 2 * held(cache, cache._args) + 4096 * len(kept)
+cache.close()
+assert hip.host_hip_used() == begin
+""")
