@@ -85,12 +85,11 @@ def test_workspaces_grow_with_the_rows(host_hip):  # noqa: F811
     those take."""
     host_hip(SETUP + """
 rng = np.random.default_rng(3)
-for _ in range(4000):
-    k, n = (int(2 ** rng.uniform(0, 13)) for _ in range(2))
-    type, training = int(rng.integers(3)), int(rng.integers(2))
-    rows = np.sort(np.exp2(rng.uniform(0, 18, 2)).astype(np.int64))
-    if rng.random() < 0.3:
-        rows[0] = rows[1] - 1
+for i in range(30_000):
+    k, n = (int(2 ** rng.uniform(5, 13)) for _ in range(2))
+    type, training = int(rng.integers(3)), int(i % 8 != 0)
+    rows = np.exp2(rng.uniform(0, 18)) * np.array([rng.uniform(0.4, 1), 1])  # near each other: parts change between them
+    rows = np.maximum(1, rows.astype(np.int64))
     need = [C.c_size_t(), C.c_size_t()]
     for r, v in zip(rows, need):
         s = op.LinearShape(int(r), k, n, type, type, 0, 0)
