@@ -248,7 +248,9 @@ struct QueryTile {
         most = fmaxf(most, __shfl_xor(most, 32, kWave));
         int e = 0;
         frexpf(most > 0.0f ? most : 1.0f, &e);
-        e = min(max(e, -100), 100);  // all powers of two here are normal numbers
+        // 2^e and 2^-e are normal numbers; the largest queries come to [2, 4) and
+        // those below the normal numbers, which have fewer bits, to less than 0.5
+        e = min(max(e, -126), 126);
         const float to = ldexpf(1.0f, -e);
 #pragma unroll
         for (int g = 0; g < 4; ++g)
