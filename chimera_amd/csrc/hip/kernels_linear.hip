@@ -1067,12 +1067,13 @@ void launch_tiles(hipStream_t st, Product p, const Epilogue& e, TilePlan plan) {
     constexpr std::integral_constant<int, 128> k128;
     constexpr std::integral_constant<int, 256> k256;
     if constexpr (kEnd == kNormalizedLayer) {
-        // a block has whole rows: 32 of them where 128 leave CUs idle, the
-        // columns in waves of 32
-        const bool many = ceil_div(ceil_div(p.m, 32), kCus) * 32 >= ceil_div(ceil_div(p.m, 128), kCus) * 128;
-        if (sizeof(T) == 2 && many)
-            launch(k128, k128, k4, k1, k3, k2);
-        else if (p.n > 96)
+        // a block has whole rows: 32 of them where 128 leave CUs idle (and
+        // always of 32 bits), the columns in waves of 32
+        if constexpr (sizeof(T) == 2) {
+            const bool many = ceil_div(ceil_div(p.m, 32), kCus) * 32 >= ceil_div(ceil_div(p.m, 128), kCus) * 128;
+            if (many) return launch(k128, k128, k4, k1, k3, k2);
+        }
+        if (p.n > 96)
             launch(k32, k128, k1, k4, k3, k3);
         else if (p.n > 64)
             launch(k32, k96, k1, k3, k3, k3);
