@@ -85,6 +85,18 @@ def _expect(a, what: str, shape: tuple, type_name: str) -> None:
         raise ValueError(f"{what} must be {type_name}, not {_type_name(a)}")
 
 
+def _expect_whole(a, what: str, shape: tuple, type_name: str) -> None:
+    _expect(a, what, shape, type_name)
+    _whole(a, what)
+
+
+def _whole(a, what: str) -> None:
+    """Refuses rows that lie apart where the call takes no stride."""
+    s = getattr(a, "stride", None)
+    if s is not None and s != a.shape[-1] and len(a.shape) > 1 and any(n != 1 for n in a.shape[:-1]):
+        raise ValueError(f"the rows of {what} must follow each other")
+
+
 def _function(name: str, *argtypes):
     """An entry point with its argument types set: plain integers and struct
     references go through without wrapping."""
@@ -233,6 +245,8 @@ class TokenCache:
             raise ValueError(f"the cache needs codes [slots, {row}] and scales [slots, {groups}]")
         if _type_name(codes) != "uint8" or _type_name(scales) != "f32":
             raise ValueError("codes must be uint8 and scales f32")
+        _whole(codes, "codes")
+        _whole(scales, "scales")
         if page_tokens < 1 or slots % page_tokens:
             raise ValueError("the slots must fill whole pages")
         self.ctx, self.codes, self.scales = ctx, codes, scales
@@ -300,11 +314,12 @@ class TokenCache:
         docs, cap = doc_lens.shape[0], cand_ids.shape[1]
         a = self._args
         t = _type(queries, "queries")
+        _whole(queries, "queries")
         _expect(page_start, "page_start", (docs,), "int64")
         _expect(doc_lens, "doc_lens", (docs,), "int32")
         _expect(pages, "pages", (pages.shape[0],), "int32")
-        _expect(cand_ids, "cand_ids", (nq, cap), "int32")
-        _expect(scores, "scores", (nq, cap), "f32")
+        _expect_whole(cand_ids, "cand_ids", (nq, cap), "int32")
+        _expect_whole(scores, "scores", (nq, cap), "f32")
         a.page_start, a.doc_lens, a.pages = page_start.ptr, doc_lens.ptr, pages.ptr
         a.cand_ids, a.scores = cand_ids.ptr, scores.ptr
         a.query_lens = a.cand_counts = a.top_ids = a.top_scores = a.top_counts = None
@@ -319,7 +334,7 @@ class TokenCache:
                                          ("top_scores", top_scores, (nq, k), "f32"),
                                          ("top_counts", top_counts, (nq,), "int32")):
                 if v is not None:
-                    _expect(v, name, shape, kind)
+                    _expect_whole(v, name, shape, kind)
                     setattr(a, name, v.ptr)
         a.queries, a.type, a.nq, a.query_len = queries.ptr, t, nq, query_len
         a.num_docs, a.num_page_entries, a.max_doc_tokens = docs, pages.shape[0], max_doc_tokens
