@@ -218,13 +218,21 @@ class Linear:
         check(self._call_backward(self.ctx.handle, self._shape_ref, self._backward_ref))
 
 
-def cache_row(format: str, dim: int, group: int) -> tuple[int, int]:
+def _int32(value: int, what: str) -> int:
+    """The value, which ctypes would cut to 32 bits without a word."""
+    if not -(1 << 31) <= value < 1 << 31:
+        raise ValueError(f"{what} must fit 32 bits, not {value}")
+    return value
+
+
+def cache_row(format: str, dim: int, group: int, page_tokens: int = 1) -> tuple[int, int]:
     """(bytes of codes, number of scales) of one slot of a cache."""
     if format not in FORMATS:
         raise ValueError(f"unknown cache format {format!r}")
     row, scales = C.c_int32(), C.c_int32()
-    check(capi.lib().chimera_cache_row(C.byref(CacheDesc(FORMATS[format], dim, group, 1, 0, None, None)),
-                                       C.byref(row), C.byref(scales)))
+    desc = CacheDesc(FORMATS[format], _int32(dim, "dim"), _int32(group, "group"), _int32(page_tokens, "page_tokens"), 0,
+                     None, None)
+    check(capi.lib().chimera_cache_row(C.byref(desc), C.byref(row), C.byref(scales)))
     return row.value, scales.value
 
 
@@ -249,6 +257,7 @@ class TokenCache:
         _whole(scales, "scales")
         if page_tokens < 1 or slots % page_tokens:
             raise ValueError("the slots must fill whole pages")
+        cache_row(format, dim, group, page_tokens)
         self.ctx, self.codes, self.scales = ctx, codes, scales
         self.format, self.dim, self.group, self.page_tokens = format, dim, group, page_tokens
         self.slots = slots
@@ -337,8 +346,8 @@ class TokenCache:
                     _expect_whole(v, name, shape, kind)
                     setattr(a, name, v.ptr)
         a.queries, a.type, a.nq, a.query_len = queries.ptr, t, nq, query_len
-        a.num_docs, a.num_page_entries, a.max_doc_tokens = docs, pages.shape[0], max_doc_tokens
-        a.cand_cap, a.k = cap, k
+        a.num_docs, a.num_page_entries = docs, pages.shape[0]
+        a.max_doc_tokens, a.cand_cap, a.k = _int32(max_doc_tokens, "max_doc_tokens"), cap, _int32(k, "k")
         sizes = (nq, query_len, cap, max_doc_tokens)
         if sizes != self._sizes and not self._closed:
             need = C.c_size_t()

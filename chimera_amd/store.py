@@ -18,7 +18,7 @@ class TokenStore:
 
     def __init__(self, ctx: capi.Context, num_pages: int, dim: int = 128, format: str = "int8", group: int = 128,
                  page_tokens: int = 16):
-        row, scales = cache_row(format, dim, group)
+        row, scales = cache_row(format, dim, group, page_tokens)
         if num_pages < 1:
             raise ValueError("a store needs pages")
         self.ctx, self.dim, self.page_tokens = ctx, dim, page_tokens
