@@ -166,13 +166,14 @@ class TokenStore:
         queries [nq, query_len, dim]: (scores of all candidates [nq, cap], ids
         [nq, k], scores [nq, k], counts [nq])."""
         q = np.ascontiguousarray(queries, np.float32)
-        ids = np.ascontiguousarray(cand_ids, np.int32)
+        ids = np.asarray(cand_ids).astype(np.int64)
+        ids = np.where((ids >= -(1 << 31)) & (ids < 1 << 31), ids, -1).astype(np.int32)  # past 32 bits: no document's
         nq, cap = ids.shape
         start, lens, pages, longest = self.tables()
         bufs = [self.ctx.to_device(q), self.ctx.to_device(ids), self.ctx.empty((nq, cap), np.float32),
                 self.ctx.empty((nq, k), np.int64), self.ctx.empty((nq, k), np.float32), self.ctx.empty((nq,), np.int32)]
         if query_lens is not None:
-            bufs.append(self.ctx.to_device(np.ascontiguousarray(query_lens, np.int32)))
+            bufs.append(self.ctx.to_device(np.clip(query_lens, 0, q.shape[1]).astype(np.int32)))
         try:
             d_q, d_ids, d_scores, d_top, d_top_scores, d_counts = bufs[:6]
             self.cache.maxsim(d_q, start, lens, pages, longest, d_ids, d_scores,

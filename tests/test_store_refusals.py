@@ -52,3 +52,24 @@ assert d == b and store.doc_len(a) == 8 and store.doc_len(d) == 5
 held = [p for pages in store._docs if pages for p in pages] + store._free
 assert sorted(held) == list(range(20))
 """)
+
+
+def test_ids_and_lengths_past_32_bits(host_hip):  # noqa: F811
+    """64-bit ids, as a search returns them: those that are no document's
+    are absent, not cut to another document's."""
+    host_hip(SETUP + """
+store.add(rows(24), [8, 8, 8])
+seen = {}
+
+def maxsim(q, start, lens, pages, longest, ids, scores, query_lens=None, **kw):
+    seen.update(ids=ids.numpy(), lens=query_lens.numpy())
+
+store.cache.maxsim = maxsim
+big = 1 << 32
+ids = np.array([[0, 2, -1, 1 << 31, big, big + 1, -big, 2**63 - 1]], np.int64)
+store.rescore(np.zeros((1, 4, 64), np.float32), ids, 2, query_lens=np.array([big + 1], np.int64))
+assert seen["ids"].tolist() == [[0, 2, -1, -1, -1, -1, -1, -1]], seen
+assert seen["lens"].tolist() == [4]
+store.rescore(np.zeros((1, 4, 64), np.float32), ids.astype(np.uint64), 2, query_lens=np.array([-big - 3], np.int64))
+assert seen["ids"].tolist() == [[0, 2, -1, -1, -1, -1, -1, -1]] and seen["lens"].tolist() == [0]
+""")
