@@ -5,10 +5,18 @@ candidates (of an index's search, or all documents) on them.
 """
 from __future__ import annotations
 
+from contextlib import ExitStack
+
 import numpy as np
 
 from . import capi
 from .operators import TokenCache, cache_row
+
+
+def _freed(stack: ExitStack, array: capi.DeviceArray) -> capi.DeviceArray:
+    """The array, which the stack frees."""
+    stack.callback(array.free)
+    return array
 
 
 class TokenStore:
@@ -22,9 +30,11 @@ class TokenStore:
         if num_pages < 1:
             raise ValueError("a store needs pages")
         self.ctx, self.dim, self.page_tokens = ctx, dim, page_tokens
-        self._codes = ctx.empty((num_pages * page_tokens, row), np.uint8)
-        self._scales = ctx.empty((num_pages * page_tokens, scales), np.float32)
-        self.cache = TokenCache(ctx, self._codes, self._scales, format, dim, group, page_tokens)
+        with ExitStack() as made:
+            self._codes = _freed(made, ctx.empty((num_pages * page_tokens, row), np.uint8))
+            self._scales = _freed(made, ctx.empty((num_pages * page_tokens, scales), np.float32))
+            self.cache = TokenCache(ctx, self._codes, self._scales, format, dim, group, page_tokens)
+            made.pop_all()
         self._free = list(range(num_pages - 1, -1, -1))
         self._docs: list[list[int] | None] = []  # pages of each document, None: removed
         self._lens: list[int] = []
@@ -76,17 +86,11 @@ class TokenStore:
     def _write(self, embeddings, slots: np.ndarray) -> None:
         if slots.size == 0:
             return
-        own = None
-        if isinstance(embeddings, np.ndarray):
-            own = embeddings = self.ctx.to_device(np.ascontiguousarray(embeddings, np.float32))
-        d_slots = self.ctx.to_device(slots)
-        try:
-            self.cache.write(embeddings, d_slots)
+        with ExitStack() as bufs:
+            if isinstance(embeddings, np.ndarray):
+                embeddings = _freed(bufs, self.ctx.to_device(np.ascontiguousarray(embeddings, np.float32)))
+            self.cache.write(embeddings, _freed(bufs, self.ctx.to_device(slots)))
             self.ctx.synchronize()
-        finally:
-            d_slots.free()
-            if own is not None:
-                own.free()
 
     def add(self, embeddings, doc_lens) -> list[int]:
         """Adds documents: embeddings [tokens, dim], one document's tokens
@@ -141,14 +145,11 @@ class TokenStore:
         n = self._lens[doc]
         if n == 0:
             return np.zeros((0, self.dim), np.float32)
-        slots = self.ctx.to_device(self._slots(self._docs[doc], 0, n).astype(np.int64))
-        out = self.ctx.empty((n, self.dim), np.float32)
-        try:
+        with ExitStack() as bufs:
+            slots = _freed(bufs, self.ctx.to_device(self._slots(self._docs[doc], 0, n).astype(np.int64)))
+            out = _freed(bufs, self.ctx.empty((n, self.dim), np.float32))
             self.cache.read(slots, out)
             return out.numpy()
-        finally:
-            slots.free()
-            out.free()
 
     def tables(self):
         """(page_start, doc_lens, pages) on the device and the longest
@@ -157,8 +158,11 @@ class TokenStore:
             owned = [d or [] for d in self._docs]
             start = np.concatenate([[0], np.cumsum([len(d) for d in owned], dtype=np.int64)])[:-1]
             pages = np.array([p for d in owned for p in d] or [0], np.int32)
-            self._tables = [self.ctx.to_device(a) for a in (start.astype(np.int64) if len(owned) else np.zeros(1, np.int64),
-                                                            np.array(self._lens or [0], np.int32), pages)]
+            with ExitStack() as made:
+                self._tables = [_freed(made, self.ctx.to_device(a))
+                                for a in (start.astype(np.int64) if len(owned) else np.zeros(1, np.int64),
+                                          np.array(self._lens or [0], np.int32), pages)]
+                made.pop_all()
         return (*self._tables, max(self._lens, default=0))
 
     def rescore(self, queries: np.ndarray, cand_ids: np.ndarray, k: int, query_lens=None):
@@ -170,16 +174,14 @@ class TokenStore:
         ids = np.where((ids >= -(1 << 31)) & (ids < 1 << 31), ids, -1).astype(np.int32)  # past 32 bits: no document's
         nq, cap = ids.shape
         start, lens, pages, longest = self.tables()
-        bufs = [self.ctx.to_device(q), self.ctx.to_device(ids), self.ctx.empty((nq, cap), np.float32),
-                self.ctx.empty((nq, k), np.int64), self.ctx.empty((nq, k), np.float32), self.ctx.empty((nq,), np.int32)]
-        if query_lens is not None:
-            bufs.append(self.ctx.to_device(np.clip(query_lens, 0, q.shape[1]).astype(np.int32)))
-        try:
-            d_q, d_ids, d_scores, d_top, d_top_scores, d_counts = bufs[:6]
-            self.cache.maxsim(d_q, start, lens, pages, longest, d_ids, d_scores,
-                              query_lens=bufs[6] if query_lens is not None else None, k=k, top_ids=d_top,
+        with ExitStack() as bufs:
+            d_q, d_ids = (_freed(bufs, self.ctx.to_device(v)) for v in (q, ids))
+            d_scores, d_top, d_top_scores, d_counts = (
+                _freed(bufs, self.ctx.empty(shape, dtype))
+                for shape, dtype in (((nq, cap), np.float32), ((nq, k), np.int64), ((nq, k), np.float32), ((nq,), np.int32)))
+            d_lens = None
+            if query_lens is not None:
+                d_lens = _freed(bufs, self.ctx.to_device(np.clip(query_lens, 0, q.shape[1]).astype(np.int32)))
+            self.cache.maxsim(d_q, start, lens, pages, longest, d_ids, d_scores, query_lens=d_lens, k=k, top_ids=d_top,
                               top_scores=d_top_scores, top_counts=d_counts)
             return d_scores.numpy(), d_top.numpy(), d_top_scores.numpy(), d_counts.numpy()
-        finally:
-            for b in bufs:
-                b.free()

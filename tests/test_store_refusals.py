@@ -73,3 +73,54 @@ assert seen["lens"].tolist() == [4]
 store.rescore(np.zeros((1, 4, 64), np.float32), ids.astype(np.uint64), 2, query_lens=np.array([-big - 3], np.int64))
 assert seen["ids"].tolist() == [[0, 2, -1, -1, -1, -1, -1, -1]] and seen["lens"].tolist() == [0]
 """)
+
+
+def test_allocations_that_fail_leave_no_memory(host_hip):  # noqa: F811
+    """Every allocation of every call in turn."""
+    host_hip(SETUP + """
+empty, left = ctx.empty, [0]
+
+def counted(shape, dtype):
+    left[0] -= 1
+    if left[0] < 0:
+        raise capi.ChimeraError(2, "out of memory")
+    return empty(shape, dtype)
+
+def to_device(a, bf16=False):
+    a = np.ascontiguousarray(a)
+    d = counted(a.shape, a.dtype)
+    capi.check(capi.lib().chimera_copy_to_device(ctx.handle, capi.P(d.ptr), capi._ptr(a), C.c_size_t(a.nbytes)))
+    return d
+
+def each(call, least):
+    \"\"\"Lets the first, second, ... allocation of the call fail, until it ends.\"\"\"
+    for n in range(100):
+        left[0] = n
+        used = hip.host_hip_used()
+        ctx.empty, ctx.to_device = counted, to_device
+        try:
+            call()
+        except capi.ChimeraError:
+            assert hip.host_hip_used() == used, (call, n)
+            continue
+        finally:
+            ctx.empty, ctx.to_device = empty, type(ctx).to_device.__get__(ctx)
+        assert n >= least, n
+        return
+    raise AssertionError("does not end")
+
+each(lambda: TokenStore(ctx, 8).close(), 2)
+each(lambda: store.add(rows(11), [3, 8]), 2)
+each(lambda: store.append(0, rows(9)), 2)
+each(lambda: store.read(0), 2)
+store.append(0, rows(1))
+each(lambda: store.tables(), 3)
+q = np.zeros((2, 4, 64), np.float32)
+each(lambda: store.rescore(q, np.zeros((2, 5), np.int64), 2, query_lens=[1, 2]), 7)
+# one document of 600 tokens, so that the cache takes a workspace
+store.close()
+store = TokenStore(ctx, num_pages=100, dim=64, group=64, page_tokens=8)
+store.add(rows(600), [600])
+store.tables()
+each(lambda: store.rescore(q, np.zeros((2, 5), np.int64), 2), 7)  # the cache's too
+""")
