@@ -105,7 +105,9 @@ __device__ __forceinline__ float activation_slope(float z, int act) {
         }
         case CHIMERA_ACT_GELU_TANH: {
             const float g = sigmoid(2.0f * kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
-            return fmaf(2.0f * kGeluTanhC * z * g * (1.0f - g), fmaf(3.0f * kGeluTanhA * z, z, 1.0f), g);
+            // g (1 - g) is zero long before z or its square overflow in this
+            const float near = fminf(fmaxf(z, -1e6f), 1e6f);
+            return fmaf(2.0f * kGeluTanhC * near * g * (1.0f - g), fmaf(3.0f * kGeluTanhA * near, near, 1.0f), g);
         }
         case CHIMERA_ACT_SILU: {
             const float g = sigmoid(z);
