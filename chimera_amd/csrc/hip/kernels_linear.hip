@@ -632,7 +632,9 @@ __device__ __forceinline__ void tile_product(unsigned char* lds, const Product& 
             activate<T>(v, e.act);
             if constexpr (kNormalize) {
                 const int64_t m = m_first + (l & 31);
-                float sum = 0.0f;
+                // the squares' sum, and that of the values times 2^-72 for rows
+                // whose squares overflow (a length from 1.8e19 on)
+                float sum = 0.0f, low_sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < IN; ++j)
 #pragma unroll
@@ -640,28 +642,36 @@ __device__ __forceinline__ void tile_product(unsigned char* lds, const Product& 
                         const int n = col0 + 32 * j + 8 * (r >> 2) + 4 * half + (r & 3);
                         if (e.residual && m < e.m && n < e.n)
                             v[j][r] += to_float(static_cast<const T*>(e.residual)[m * e.residual_stride + n]);
+                        const float low = v[j][r] * 0x1p-72f;
                         sum = n < e.n ? fmaf(v[j][r], v[j][r], sum) : sum;
+                        low_sum = n < e.n ? fmaf(low, low, low_sum) : low_sum;
                     }
                 sum += __shfl_xor(sum, 32, kWave);
+                low_sum += __shfl_xor(low_sum, 32, kWave);
                 if constexpr (WN > 1) {
                     static_assert(IM == 1, "one exchange of the waves' sums");
-                    float* sums = reinterpret_cast<float*>(lds);
+                    f32x2_t* sums = reinterpret_cast<f32x2_t*>(lds);
                     __syncthreads();
-                    if (half == 0) sums[w * 32 + l] = sum;
+                    if (half == 0) sums[w * 32 + l] = f32x2_t{sum, low_sum};
                     __syncthreads();
-                    sum = 0.0f;
+                    sum = low_sum = 0.0f;
 #pragma unroll
-                    for (int o = 0; o < WN; ++o) sum += sums[(wm * WN + o) * 32 + (l & 31)];
+                    for (int o = 0; o < WN; ++o) {
+                        const f32x2_t t = sums[(wm * WN + o) * 32 + (l & 31)];
+                        sum += t[0];
+                        low_sum += t[1];
+                    }
                     __syncthreads();  // the rows go through the same LDS next
                 }
-                const float norm = sqrtf(sum);
-                const float held = norm < kLeastNorm ? kLeastNorm : norm;  // NaN stays
-                const float inv = 1.0f / held;
+                const bool large = sum == INFINITY;
+                const float norm = sqrtf(large ? low_sum : sum);  // times 2^-72 where large
+                const float held = norm < kLeastNorm && !large ? kLeastNorm : norm;  // NaN stays
+                const float inv = 1.0f / held, before = large ? 0x1p-72f : 1.0f;
 #pragma unroll
                 for (int j = 0; j < IN; ++j)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) v[j][r] *= inv;
-                if (e.norms && wn == 0 && half == 0 && m < e.m) e.norms[m] = held;
+                    for (int r = 0; r < 16; ++r) v[j][r] = v[j][r] * before * inv;
+                if (e.norms && wn == 0 && half == 0 && m < e.m) e.norms[m] = large ? held * 0x1p72f : held;
             }
         }
         if (narrow) {

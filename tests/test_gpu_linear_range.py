@@ -26,3 +26,39 @@ def test_activations_of_large_sums(type, act, rows):
     assert np.array_equal(np.abs(g["dw"].values()[:, 0]), (z[0] > 0).astype(float))
     release(ctx, layer, {**d, **g})
     ctx.close()
+
+
+@pytest.mark.parametrize("type,k,n,rows", [("f32", 8, 128, 40), ("f32", 8, 70, 5), ("f32", 8, 40, 70), ("bf16", 8, 128, 24_600),
+                                           ("bf16", 8, 100, 300)])
+def test_rows_of_any_length(type, k, n, rows):
+    """Rows of length one from sums near 1e-10 to 1e38, whose squares leave
+    32 bits; the lengths, and the gradient of the residual, come with them.
+    The sums are the inputs' products with whole numbers: k roundings of 2^-24
+    of terms that are at most 8 times the sum's size here, the length's and the
+    division's of 2^-23 each."""
+    rng = np.random.default_rng(n + rows)
+    size = np.exp(rng.uniform(np.log(1e-9), np.log(1e36), rows))
+    size[:4] = 3e36, 1e19, 2e19, 1e-8
+    x = to_type(rng.integers(1, 9, (rows, k)) * size[:, None], type)
+    w = rng.integers(1, 5, (n, k)).astype(np.float64)
+    ctx = context()
+    layer, d = run_forward(ctx, x, w, None, None, type, "f32", "none", True, training=True)
+    h = x @ w.T
+    norm = np.sqrt(np.square(h / size[:, None]).sum(1)) * size
+    y = h / norm[:, None]
+    off = (k + 8) * 2.0**-23
+    fits = (np.abs(x) @ np.abs(w).T).max(1) < 3.4e38  # a sum past the 32-bit range is infinite
+    assert fits[1:].sum() > rows // 2 and not np.isnan(d["y"].values()[fits]).any()
+    assert (np.abs(d["y"].values() - y) <= off * np.abs(y))[fits].all()
+    representable = fits & (norm < 3.4e38)
+    assert (np.abs(d["norms"].values() / norm - 1)[representable] <= off).all()
+    dy = rng.standard_normal((rows, n))
+    g = {"dy": Matrix(ctx, dy, "f32"), "dr": Matrix(ctx, None, type, shape=(rows, n))}
+    layer.backward(d["x"], g["dy"], y=d["y"], norms=d["norms"], dresidual=g["dr"])
+    dy = g["dy"].values()
+    want = (dy - y * (y * dy).sum(1, keepdims=True)) / norm[:, None]
+    terms = (np.abs(dy) + np.abs(y) * np.abs(y * dy).sum(1, keepdims=True)) / norm[:, None]
+    bound = (3 * off + n * 2.0**-23) * terms + 2.0**-BITS[type] * np.abs(want) + 2.0**-126
+    assert (np.abs(g["dr"].values() - want) <= bound)[representable].all()
+    release(ctx, layer, {**d, **g})
+    ctx.close()
