@@ -1141,13 +1141,16 @@ struct ForwardPlan {
     void* x;
     void* weight;
 };
-size_t carve_forward(const chimera_linear_shape& s, void* base, ForwardPlan* plan) {
+// Room for `rows` rows of X laid out again, and for W.
+size_t carve_forward(const chimera_linear_shape& s, int64_t rows, void* base, ForwardPlan* plan) {
     Carve c{static_cast<char*>(base)};
     const size_t wide = round_up(s.in_features, 64) * type_bytes(s.type);
-    plan->x = c.take(static_cast<size_t>(s.rows) * wide);
     plan->weight = c.take(static_cast<size_t>(s.out_features) * wide);
+    plan->x = c.take(static_cast<size_t>(rows) * wide);
     return c.off;
 }
+
+bool few_rows(const chimera_linear_shape& s) { return s.rows <= kFewRows && !s.normalize; }
 
 template <typename T>
 hipError_t forward(hipStream_t st, const LinearForward& f) {
@@ -1171,7 +1174,7 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
     Product p = {};
     p.m = s.rows;
     p.n = s.out_features;
-    if (s.rows <= kFewRows && !e.normalize) {
+    if (few_rows(s)) {
         p.a = a.x;
         p.b = a.weight;
         p.a_stride = a.x_stride * static_cast<int64_t>(sizeof(T));
@@ -1187,7 +1190,7 @@ hipError_t forward(hipStream_t st, const LinearForward& f) {
         return hipGetLastError();
     }
     ForwardPlan plan;
-    (void)carve_forward(s, a.workspace, &plan);
+    (void)carve_forward(s, s.rows, a.workspace, &plan);  // X's room comes last: it is not there where X needs none
     AlignJob jobs[2];
     int njobs = 0;
     aligned_rows<T>(a.x, a.x_stride, s.rows, s.in_features, plan.x, &p.a, &p.a_stride, jobs, &njobs);
@@ -1351,7 +1354,7 @@ hipError_t backward(hipStream_t st, const LinearBackward& b) {
 }
 
 template <typename Call>
-hipError_t by_type(int type, Call&& call) {
+auto by_type(int type, Call&& call) {
     switch (type) {
         case CHIMERA_F32: return call(float{});
         case CHIMERA_F16: return call(_Float16{});
@@ -1363,7 +1366,12 @@ hipError_t by_type(int type, Call&& call) {
 
 size_t linear_forward_workspace(const chimera_linear_shape& s) {
     ForwardPlan plan;
-    return carve_forward(s, nullptr, &plan);
+    return carve_forward(s, s.rows, nullptr, &plan);
+}
+size_t linear_forward_workspace(const LinearForward& f) {
+    const bool taken = by_type(f.s.type, [&](auto t) { return takes_loads<decltype(t)>(f.a.x, f.a.x_stride, f.s.in_features); });
+    ForwardPlan plan;
+    return carve_forward(f.s, taken || few_rows(f.s) ? 0 : f.s.rows, nullptr, &plan);
 }
 size_t linear_backward_workspace(const chimera_linear_shape& s) {
     BackwardPlan plan;

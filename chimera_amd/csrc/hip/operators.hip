@@ -162,7 +162,7 @@ int chimera_linear_forward_device(chimera_ctx* ctx, const chimera_linear_shape* 
     if (args->saved) CK(check_matrix("saved", args->saved, args->saved_stride, shape->out_features, e));
     if (args->norms) CK(check_vector("norms", args->norms, 4));
     if (args->norms && !shape->normalize) return invalid("norms are an output of normalized layers");
-    const size_t need = linear_forward_workspace(*shape);
+    const size_t need = linear_forward_workspace(LinearForward{*shape, *args});
     CK(check_workspace(args->workspace, args->workspace_bytes, need));
     const int64_t m = shape->rows, k = shape->in_features, n = shape->out_features, bytes = static_cast<int64_t>(need);
     const Region outs[] = {region("y", args->y, m, n, args->y_stride, out),

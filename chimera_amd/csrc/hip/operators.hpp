@@ -110,7 +110,8 @@ struct LinearBackward {
     chimera_linear_backward a;
 };
 
-size_t linear_forward_workspace(const chimera_linear_shape& s);
+size_t linear_forward_workspace(const chimera_linear_shape& s);  // of any call of the shape
+size_t linear_forward_workspace(const LinearForward& f);         // of this one
 size_t linear_backward_workspace(const chimera_linear_shape& s);
 hipError_t launch_linear_forward(hipStream_t st, const LinearForward& f);
 hipError_t launch_linear_backward(hipStream_t st, const LinearBackward& b);

@@ -22,6 +22,7 @@ from .capi import P, check
 TYPES = {"f32": 0, "f16": 1, "bf16": 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 FORMATS = {"int8": 0, "int4": 1, "fp8": 2}
+_CAPACITY = 4  # CHIMERA_ERR_CAPACITY
 _NAMES = {"f32": "f32", "f16": "f16", "bf16": "bf16", "float32": "f32", "float16": "f16", "bfloat16": "bf16"}
 
 
@@ -120,7 +121,10 @@ class Linear:
     length with `normalize` (at most 128 outputs). weight [out, in] and bias
     [out] stay the caller's arrays and may change between calls. The object
     holds the workspace for calls of up to max_rows rows, and with `training`
-    for the backward pass; close it before its context."""
+    for the backward pass; close it before its context. Where in_features fill
+    whole 16 bytes it allocates the room to lay out x again, without `training`,
+    at the first call whose rows do not start at multiples of 16 bytes: make
+    one before such a call is captured into a graph."""
 
     def __init__(self, ctx: capi.Context, weight, bias=None, activation: str = "none", normalize: bool = False,
                  max_rows: int = 1, training: bool = False):
@@ -143,23 +147,44 @@ class Linear:
         self._forward_ref, self._backward_ref = C.byref(self._forward), C.byref(self._backward)
         self._call_forward = _function("chimera_linear_forward_device", P, P, P)
         self._call_backward = _function("chimera_linear_backward_device", P, P, P)
-        self._workspace = None
+        self._workspaces = []  # the last one is in use, and holds `capacity` bytes when a call needed them
+        self.max_rows = max_rows
+        self._capacity = self._need(max_rows, training)
+        # rows that do not end at a multiple of 16 bytes are always laid out again
+        whole = self.in_features * (4 if self.type == "f32" else 2) % 16 == 0
+        self._allocate(self._need(0, False) if whole and not training else self._capacity)
+
+    def _need(self, rows: int, training: bool) -> int:
         need = C.c_size_t()
-        self._shape.rows = max_rows
-        check(capi.lib().chimera_linear_workspace(C.byref(self._shape), int(training), C.byref(need)))
-        if need.value:
-            self._workspace = ctx.empty(need.value, np.uint8)
-            for args in (self._forward, self._backward):
-                args.workspace, args.workspace_bytes = self._workspace.ptr, need.value
+        self._shape.rows = rows
+        check(capi.lib().chimera_linear_workspace(self._shape_ref, int(training), C.byref(need)))
+        return need.value
+
+    @property
+    def _workspace(self):
+        return self._workspaces[-1] if self._workspaces else None
+
+    def _allocate(self, nbytes: int) -> None:
+        self._workspaces.append(self.ctx.empty(nbytes, np.uint8))
+        for args in (self._forward, self._backward):
+            args.workspace, args.workspace_bytes = self._workspace.ptr, nbytes
+
+    def _run(self, call, args) -> None:
+        code = call(self.ctx.handle, self._shape_ref, args)
+        if code == _CAPACITY and self._workspaces and self._workspace.nbytes < self._capacity:
+            self._allocate(self._capacity)
+            code = call(self.ctx.handle, self._shape_ref, args)
+        check(code)
 
     def close(self) -> None:
         """Frees the workspace; calls after it are refused."""
-        if getattr(self, "_workspace", None) is not None:
+        workspaces = getattr(self, "_workspaces", None)
+        if workspaces:
             for args in (self._forward, self._backward):
                 args.workspace, args.workspace_bytes = None, 0
             self.ctx.synchronize()
-            self._workspace.free()
-            self._workspace = None
+            while workspaces:
+                workspaces.pop().free()
 
     def __del__(self):
         try:
@@ -167,8 +192,12 @@ class Linear:
         except Exception:
             pass
 
-    def _rows(self, x, y, what: str) -> int:
+    def _rows(self, x, y, what: str, training: bool) -> int:
         rows = x.shape[0]
+        if rows > self.max_rows:
+            need = self._need(rows, training)
+            if need > self._capacity:
+                raise capi.ChimeraError(_CAPACITY, f"the workspace is for {self.max_rows} rows, the call has {rows}")
         if tuple(y.shape) != (rows, self.out_features):
             raise ValueError(f"{what} must have shape {(rows, self.out_features)}, not {tuple(y.shape)}")
         self._shape.rows, self._shape.out_type = rows, _type(y, what)
@@ -178,7 +207,7 @@ class Linear:
         """y [rows, out] (the layer's type or f32) from x [rows, in]. For the
         backward pass, `saved` [rows, out] gets the sums before the activation
         and `norms` [rows] f32 the lengths."""
-        rows = self._rows(x, y, "y")
+        rows = self._rows(x, y, "y", False)
         _expect(x, "x", (rows, self.in_features), self.type)
         a = self._forward
         a.x, a.x_stride, a.y, a.y_stride = x.ptr, _stride(x), y.ptr, _stride(y)
@@ -192,7 +221,7 @@ class Linear:
         if norms is not None:
             _expect(norms, "norms", (rows,), "f32")
             a.norms = norms.ptr
-        check(self._call_forward(self.ctx.handle, self._shape_ref, self._forward_ref))
+        self._run(self._call_forward, self._forward_ref)
 
     def backward(self, x, dy, saved=None, y=None, norms=None, dx=None, dweight=None, dbias=None,
                  dresidual=None) -> None:
@@ -201,7 +230,7 @@ class Linear:
         forward() left them."""
         if not self.training:
             raise ValueError("the layer was made without training")
-        rows = self._rows(x, dy, "dy")
+        rows = self._rows(x, dy, "dy", True)
         n, k, t = self.out_features, self.in_features, self.type
         _expect(x, "x", (rows, k), t)
         a = self._backward
@@ -215,7 +244,7 @@ class Linear:
                 if len(shape) == 2:
                     setattr(a, name + "_stride", _stride(v))
             setattr(a, name, _ptr(v))
-        check(self._call_backward(self.ctx.handle, self._shape_ref, self._backward_ref))
+        self._run(self._call_backward, self._backward_ref)
 
 
 def _int32(value: int, what: str) -> int:

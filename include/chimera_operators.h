@@ -70,7 +70,7 @@ typedef struct {
     void* saved;          /* Z [rows, out_features] for the backward pass, or NULL */
     float* norms;         /* max(|H|, 1e-12) [rows] for the backward pass, or NULL */
     int64_t x_stride, weight_stride, residual_stride, y_stride, saved_stride;
-    void* workspace;      /* chimera_linear_workspace bytes, 256-byte aligned; NULL if 0 */
+    void* workspace;      /* chimera_linear_workspace bytes, 256-byte aligned */
     size_t workspace_bytes;
 } chimera_linear_forward;
 
@@ -99,7 +99,10 @@ typedef struct {
 
 /* Bytes of workspace for calls of this shape (any strides and alignment):
  * the forward pass, or with training the larger of both passes. Grows with
- * rows, so that of the largest call serves all. Host arithmetic only. */
+ * rows, so that of the largest call serves all. Most of the forward pass's is
+ * for X laid out again: a call whose rows of X start and end at multiples of
+ * 16 bytes, with a stride of at most 4 MiB, or one of up to four rows without
+ * normalize, needs no more than for rows = 0. Host arithmetic only. */
 int chimera_linear_workspace(const chimera_linear_shape* shape, int32_t training, size_t* bytes);
 
 int chimera_linear_forward_device(chimera_ctx* ctx, const chimera_linear_shape* shape,
