@@ -45,14 +45,17 @@ int check_shape(const chimera_linear_shape* s) {
     return CHIMERA_OK;
 }
 
-// A matrix argument: aligned to its elements, rows that do not overlap.
-int check_matrix(const char* name, const void* p, int64_t stride, int64_t cols, size_t elem) {
+// A matrix argument: aligned to its elements, rows that do not overlap and
+// whose offsets fit 62 bits.
+int check_matrix(const char* name, const void* p, int64_t rows, int64_t cols, int64_t stride, size_t elem) {
     if (!p) return invalid(std::string("null argument: ") + name);
     if (reinterpret_cast<uintptr_t>(p) % elem) return invalid(std::string(name) + " is not aligned to its elements");
     if (stride < cols) return invalid(std::string("the row stride of ") + name + " is less than a row");
+    if (stride > (int64_t{1} << 62) / (rows * static_cast<int64_t>(elem)))
+        return invalid(std::string("the row stride of ") + name + " is too large");
     return CHIMERA_OK;
 }
-int check_vector(const char* name, const void* p, size_t elem) { return check_matrix(name, p, 0, 0, elem); }
+int check_vector(const char* name, const void* p, size_t elem) { return check_matrix(name, p, 1, 0, 0, elem); }
 
 // What a call reads or writes, for the check that outputs lie apart.
 struct Region {
@@ -154,12 +157,12 @@ int chimera_linear_forward_device(chimera_ctx* ctx, const chimera_linear_shape* 
     if (!args) return invalid("null argument");
     if (shape->rows == 0) return CHIMERA_OK;
     const size_t e = type_bytes(shape->type), out = type_bytes(shape->out_type);
-    CK(check_matrix("x", args->x, args->x_stride, shape->in_features, e));
-    CK(check_matrix("weight", args->weight, args->weight_stride, shape->in_features, e));
-    CK(check_matrix("y", args->y, args->y_stride, shape->out_features, out));
+    CK(check_matrix("x", args->x, shape->rows, shape->in_features, args->x_stride, e));
+    CK(check_matrix("weight", args->weight, shape->out_features, shape->in_features, args->weight_stride, e));
+    CK(check_matrix("y", args->y, shape->rows, shape->out_features, args->y_stride, out));
     if (args->bias) CK(check_vector("bias", args->bias, e));
-    if (args->residual) CK(check_matrix("residual", args->residual, args->residual_stride, shape->out_features, e));
-    if (args->saved) CK(check_matrix("saved", args->saved, args->saved_stride, shape->out_features, e));
+    if (args->residual) CK(check_matrix("residual", args->residual, shape->rows, shape->out_features, args->residual_stride, e));
+    if (args->saved) CK(check_matrix("saved", args->saved, shape->rows, shape->out_features, args->saved_stride, e));
     if (args->norms) CK(check_vector("norms", args->norms, 4));
     if (args->norms && !shape->normalize) return invalid("norms are an output of normalized layers");
     const size_t need = linear_forward_workspace(LinearForward{*shape, *args});
@@ -184,23 +187,23 @@ int chimera_linear_backward_device(chimera_ctx* ctx, const chimera_linear_shape*
     CK(check_shape(shape));
     if (!args) return invalid("null argument");
     const size_t e = type_bytes(shape->type), out = type_bytes(shape->out_type);
-    if (args->dweight) CK(check_matrix("dweight", args->dweight, args->dweight_stride, shape->in_features, e));
+    if (args->dweight) CK(check_matrix("dweight", args->dweight, shape->out_features, shape->in_features, args->dweight_stride, e));
     if (args->dbias) CK(check_vector("dbias", args->dbias, e));
     if (shape->rows > 0) {
-        CK(check_matrix("dy", args->dy, args->dy_stride, shape->out_features, out));
-        if (args->dweight) CK(check_matrix("x", args->x, args->x_stride, shape->in_features, e));
+        CK(check_matrix("dy", args->dy, shape->rows, shape->out_features, args->dy_stride, out));
+        if (args->dweight) CK(check_matrix("x", args->x, shape->rows, shape->in_features, args->x_stride, e));
         if (args->dx) {
-            CK(check_matrix("weight", args->weight, args->weight_stride, shape->in_features, e));
-            CK(check_matrix("dx", args->dx, args->dx_stride, shape->in_features, e));
+            CK(check_matrix("weight", args->weight, shape->out_features, shape->in_features, args->weight_stride, e));
+            CK(check_matrix("dx", args->dx, shape->rows, shape->in_features, args->dx_stride, e));
         }
         if (shape->activation != CHIMERA_ACT_NONE)
-            CK(check_matrix("saved", args->saved, args->saved_stride, shape->out_features, e));
+            CK(check_matrix("saved", args->saved, shape->rows, shape->out_features, args->saved_stride, e));
         if (shape->normalize) {
-            CK(check_matrix("y", args->y, args->y_stride, shape->out_features, out));
+            CK(check_matrix("y", args->y, shape->rows, shape->out_features, args->y_stride, out));
             CK(check_vector("norms", args->norms, 4));
         }
         if (args->dresidual)
-            CK(check_matrix("dresidual", args->dresidual, args->dresidual_stride, shape->out_features, e));
+            CK(check_matrix("dresidual", args->dresidual, shape->rows, shape->out_features, args->dresidual_stride, e));
         const size_t need = linear_backward_workspace(*shape);
         CK(check_workspace(args->workspace, args->workspace_bytes, need));
         const int64_t m = shape->rows, k = shape->in_features, n = shape->out_features, bytes = static_cast<int64_t>(need);
@@ -238,7 +241,7 @@ int chimera_cache_write_device(chimera_ctx* ctx, const chimera_cache* cache, con
     CK(check_rows(n));
     if (!known_type(type)) return invalid("unknown element type");
     if (n == 0) return CHIMERA_OK;
-    CK(check_matrix("rows", d_rows, row_stride, cache->dim, type_bytes(type)));
+    CK(check_matrix("rows", d_rows, n, cache->dim, row_stride, type_bytes(type)));
     CK(check_vector("slots", d_slots, 8));
     return launched(launch_cache_write(st, *cache, d_rows, type, row_stride, d_slots, n), "cache write kernel");
 }
@@ -252,7 +255,7 @@ int chimera_cache_read_device(chimera_ctx* ctx, const chimera_cache* cache, cons
     CK(check_rows(n));
     if (!known_type(type)) return invalid("unknown element type");
     if (n == 0) return CHIMERA_OK;
-    CK(check_matrix("out", d_out, out_stride, cache->dim, type_bytes(type)));
+    CK(check_matrix("out", d_out, n, cache->dim, out_stride, type_bytes(type)));
     CK(check_vector("slots", d_slots, 8));
     return launched(launch_cache_read(st, *cache, d_slots, n, d_out, type, out_stride), "cache read kernel");
 }

@@ -48,3 +48,39 @@ for tokens in (48, 0, 3):
 refuses("page", TokenStore, ctx, 10, page_tokens=8192)
 assert hip.host_hip_used() == used
 """)
+
+
+def test_strides_past_the_address_space(host_hip):  # noqa: F811
+    """A matrix whose last row's offset does not fit 62 bits."""
+    host_hip(SETUP + """
+L = capi.lib()
+M = 1 << 20
+s = op.LinearShape(100, 64, 32, 0, 0, 2, 0)
+need = C.c_size_t()
+capi.check(L.chimera_linear_workspace(C.byref(s), 1, C.byref(need)))
+f = op.LinearForward(M, 2 * M, 3 * M, 4 * M, 5 * M, 6 * M, None, 64, 64, 32, 32, 32, 8 * M, need.value)
+b = op.LinearBackward(M, 2 * M, 3 * M, 4 * M, 5 * M, None, 7 * M, 8 * M, 9 * M, 10 * M, 64, 64, 32, 32, 32, 64, 64,
+                      32, 11 * M, need.value)
+fwd = lambda: L.chimera_linear_forward_device(ctx.handle, C.byref(s), C.byref(f))
+bwd = lambda: L.chimera_linear_backward_device(ctx.handle, C.byref(s), C.byref(b))
+assert fwd() == 0 and bwd() == 0
+hip.host_hip_reset_launches()
+for call, args, names in ((fwd, f, ("x", "weight", "residual", "y", "saved")),
+                          (bwd, b, ("x", "weight", "dy", "saved", "dx", "dweight", "dresidual"))):
+    for name in names:
+        for stride in (1 << 61, (1 << 63) - 1, (1 << 60) // 25):
+            old = getattr(args, name + "_stride")
+            setattr(args, name + "_stride", stride)
+            assert call() == 1 and b"stride of " + name.encode() in L.chimera_last_error(), (name, stride)
+            setattr(args, name + "_stride", old)
+c = op.CacheDesc(0, 128, 128, 16, 6, codes.ptr, scales.ptr)
+for stride in (1 << 61, (1 << 63) - 1):
+    assert L.chimera_cache_write_device(ctx.handle, C.byref(c), C.c_void_p(M), 0, C.c_int64(stride), C.c_void_p(2 * M),
+                                        C.c_int64(9)) == 1
+    assert L.chimera_cache_read_device(ctx.handle, C.byref(c), C.c_void_p(M), C.c_int64(9), C.c_void_p(2 * M), 0,
+                                       C.c_int64(stride)) == 1
+assert hip.host_hip_launches(b"") == 0
+# one row lies where it lies
+s.rows, f.x_stride = 1, 1 << 59
+assert fwd() == 0, L.chimera_last_error()
+""")
