@@ -227,6 +227,13 @@ class Context:
     def handle(self):
         return self._ctx
 
+    @property
+    def stream(self) -> int:
+        """The HIP stream that the context's asynchronous calls run on."""
+        p = P()
+        check(lib().chimera_stream(self._ctx, C.byref(p)))
+        return p.value or 0
+
     def memory_usage(self) -> int:
         v = C.c_uint64()
         check(lib().chimera_memory_usage(self._ctx, C.byref(v)))

@@ -3,7 +3,8 @@ that turn hidden states into token embeddings, a quantised cache of token
 embeddings and late interaction on it, and a store of documents that come and
 go on top of the cache.
 
-Arrays are device arrays: capi.DeviceArray, or any object with `ptr`, `shape`
+Arrays are device arrays: capi.DeviceArray, a PyTorch tensor through
+from_torch(), or any object with `ptr`, `shape`
 and `dtype` ("f32", "f16", "bf16", a numpy dtype or its name) and, for a
 matrix whose rows lie apart, `stride` in elements. Calls are asynchronous on
 the context's stream. An object keeps the arguments of its calls, so threads
@@ -114,6 +115,32 @@ def _stride(a) -> int:
 
 def _ptr(a):
     return None if a is None else a.ptr
+
+
+class TensorArray:
+    """A device array that is a PyTorch tensor's memory (from_torch)."""
+
+    def __init__(self, tensor, ptr: int, shape: tuple, dtype: str, stride: int | None):
+        self.tensor, self.ptr, self.shape, self.dtype, self.stride = tensor, ptr, shape, dtype, stride
+
+
+def from_torch(tensor) -> TensorArray:
+    """A PyTorch tensor as an array that the operators take: its memory, not
+    a copy; rows of a matrix may lie apart. torch has to be imported before
+    this package loads its library, so that both share torch's HIP runtime, and
+    its work is not ordered against the context's stream: run it there
+    (torch.cuda.ExternalStream(ctx.stream)), or synchronize between the two."""
+    if not tensor.is_cuda:
+        raise ValueError("the tensor is not on the device")
+    shape, strides = tuple(tensor.shape), tuple(tensor.stride())
+    follow = 1  # elements from one index to the next without gaps
+    for i in range(len(shape) - 1, -1, -1):
+        rows = len(shape) == 2 and i == 0 and strides[0] >= shape[1]
+        if shape[i] > 1 and strides[i] != follow and not rows:
+            raise ValueError(f"a tensor with strides {strides} is no matrix of rows; call contiguous()")
+        follow *= shape[i]
+    apart = strides[0] if len(shape) == 2 and shape[0] > 1 else None
+    return TensorArray(tensor, tensor.data_ptr(), shape, str(tensor.dtype).rpartition(".")[2], apart)
 
 
 class Linear:
