@@ -550,7 +550,10 @@ __global__ __launch_bounds__(1024) void cache_topk_kernel(const float* __restric
 //     10 candidates of up to 4,000 tokens      11.7 / 14.2 / 20.0
 //     8 of 30,000 to 60,000                    19.2 / 21.0 / 24.8
 //     100 of up to 300                         11.2 / 11.0 / 11.0 (whole)
-// and 1,000 of up to 300 split in two 17.2, whole 13.7.
+// and 1,000 of up to 300 split in two 17.2, whole 13.7. Candidates are counted
+// by their capacity, which the host knows, and not by those that are filled,
+// and from 2,049 on none is split, however long: a call with a few long
+// documents does better with a capacity near their number.
 struct Split {
     int tokens, count;
 };

@@ -61,7 +61,7 @@ __device__ __forceinline__ float normal_cdf(float z, float* gauss) {
 // within 6e-9 below -6, where P falls to -infinity. 14 full-rate instructions
 // and one quarter-rate one. (Five coefficients less give 1.9e-4, which is seen
 // in the rounding: 8 % of fp16 results were not the nearest value. They took
-// 65,536 x 4096 outputs 630 us instead of 672.)
+// 65,536 x 4096 outputs 630 us instead of 657.)
 __device__ __forceinline__ float gelu_16(float z) {
     const float a = fabsf(z);
     float p = fmaf(-1.2316869e-8f, a, 4.1466188e-7f);
@@ -371,7 +371,7 @@ struct Reader {
 // take new loads, before that quarter is multiplied. One meeting a step.
 // Bound by the matrix cores and the LDS and loads that feed them: 8192 x 8192 x
 // 8192 bf16 takes 880 us (1.25 PFLOP/s), 65,536 x 1024 -> 4096 with bias and
-// GELU 672 (0.82; the same sums without the epilogue 530). Four waves of
+// GELU 657 (0.84; the same sums without the epilogue 530). Four waves of
 // 128 x 128, two blocks a CU on 128 x 256, deeper rings and a whole step in
 // registers were all slower.
 // kEnd: the sums are stored, or go through the layer's epilogue, without or
@@ -847,8 +847,8 @@ struct GradArgs {
 
 // 16 rows x 128 columns at a time, eight neighbouring columns a thread: with
 // normalize (n <= 128) a row is 16 neighbouring lanes. Bound by memory: 16,384
-// x 1024 bf16 values with GELU and dR, 134 MB read and written, take 26 us (5.1
-// TB/s).
+// x 1024 bf16 values with GELU and dR, 134 MB read and written, take 28 us (4.8
+// TB/s; the slope to 32 bits is 2 us of it).
 template <typename T>
 __global__ __launch_bounds__(256) void linear_grad_kernel(GradArgs a) {
     __shared__ float sums[16][129];

@@ -22,7 +22,10 @@ def _freed(stack: ExitStack, array: capi.DeviceArray) -> capi.DeviceArray:
 class TokenStore:
     """A cache of num_pages pages and the tables that say which of them a
     document has. Documents are numbered from 0 on; the number of a removed
-    document is used again."""
+    document is used again. The tables are made again and uploaded, all of
+    them, at the first call of rescore() after a change, and rescore() takes
+    and gives back its buffers: where that counts, keep the tables and buffers
+    and call `cache` with tables()."""
 
     def __init__(self, ctx: capi.Context, num_pages: int, dim: int = 128, format: str = "int8", group: int = 128,
                  page_tokens: int = 16):
