@@ -14,6 +14,7 @@ until the object is closed.
 from __future__ import annotations
 
 import ctypes as C
+import math
 
 import numpy as np
 
@@ -95,7 +96,9 @@ def _expect_whole(a, what: str, shape: tuple, type_name: str) -> None:
 def _whole(a, what: str) -> None:
     """Refuses rows that lie apart where the call takes no stride."""
     s = getattr(a, "stride", None)
-    if s is not None and s != a.shape[-1] and len(a.shape) > 1 and any(n != 1 for n in a.shape[:-1]):
+    if s is None or len(a.shape) < 2 or s == a.shape[-1]:
+        return
+    if s != math.prod(a.shape[1:]) and any(n != 1 for n in a.shape[:-1]):  # between first indices, of more than two
         raise ValueError(f"the rows of {what} must follow each other")
 
 

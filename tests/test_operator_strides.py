@@ -43,6 +43,9 @@ def maxsim(**other):
 maxsim()
 for name, word in (("q", "queries"), ("c", "cand_ids"), ("o", "scores"), ("ti", "top_ids"), ("ts", "top_scores")):
     refuses(word, maxsim, **{name: Apart(*arrays[name])})
+whole = Apart(*arrays["q"])
+whole.stride = 32 * 128  # between queries, which follow each other
+maxsim(q=whole)
 # matrices of rows may lie apart, and one row is whole whatever its stride
 cache.write(Apart((3, 128), np.float32), ctx.empty((3,), np.int64))
 cache.read(ctx.empty((3,), np.int64), Apart((3, 128), np.float32))
