@@ -36,6 +36,9 @@ EXPORTED = [
     "chimera_linear_workspace", "chimera_linear_forward_device", "chimera_linear_backward_device",
     "chimera_cache_row", "chimera_cache_write_device", "chimera_cache_read_device",
     "chimera_cache_maxsim_workspace", "chimera_cache_maxsim_device",
+    "chimera_norm_workspace", "chimera_norm_forward_device", "chimera_norm_backward_device",
+    "chimera_mx4_row", "chimera_mx4_quantise_device", "chimera_mx4_read_device", "chimera_mx4_linear_workspace",
+    "chimera_mx4_linear_device", "chimera_orthogonal_workspace", "chimera_orthogonal_update_device",
 ]
 
 # chimera_matrix_core_rate kinds: instruction and operands

@@ -2,6 +2,8 @@
 // checks of their arguments, then the launches.
 #include "operators.hpp"
 
+#include <algorithm>
+#include <cmath>
 #include <string>
 
 #include "capi_internal.hpp"
@@ -102,6 +104,40 @@ int check_workspace(const void* p, size_t have, size_t need) {
         const int r_ = (expr);           \
         if (r_ != CHIMERA_OK) return r_; \
     } while (0)
+
+int check_norm(const chimera_norm_shape* s) {
+    if (!s) return invalid("null shape");
+    if (s->rows < 0) return invalid("negative row count");
+    if (s->rows > (int64_t{1} << 31)) return invalid("at most 2^31 rows per call");
+    if (s->features < 1 || s->features > kMostFeatures) return invalid("features must be in [1, 65536]");
+    if (!known_type(s->type)) return invalid("unknown element type");
+    if (s->out_type != s->type && s->out_type != CHIMERA_F32) return invalid("the output has the norm's type or 32 bits");
+    if (!(s->eps >= 1e-30f) || std::isinf(s->eps)) return invalid("eps must be finite and at least 1e-30");
+    return CHIMERA_OK;
+}
+
+int check_features(int32_t features) {
+    if (features < 1 || features > kMostFeatures) return invalid("features must be in [1, 65536]");
+    return CHIMERA_OK;
+}
+// Codes and scales of rows of 4-bit values.
+int check_mx4(const void* codes, const void* scales) {
+    CK(check_vector("codes", codes, 16));
+    return check_vector("scales", scales, 8);
+}
+
+int check_orthogonal(const chimera_orthogonal_shape* s) {
+    if (!s) return invalid("null shape");
+    if (s->rows < 1 || s->rows > kMostFeatures || s->cols < 1 || s->cols > kMostFeatures)
+        return invalid("rows and columns must be in [1, 65536]");
+    if (static_cast<int64_t>(s->rows) * s->cols > (int64_t{1} << 28)) return invalid("an update has at most 2^28 values");
+    if (std::min(s->rows, s->cols) > 8192) return invalid("the shorter side has at most 8192 values");
+    if (!known_type(s->type)) return invalid("unknown element type");
+    if (s->out_type != s->type && s->out_type != CHIMERA_F32) return invalid("the output has the gradient's type or 32 bits");
+    if (s->steps < 1 || s->steps > 100) return invalid("steps must be in [1, 100]");
+    if (!std::isfinite(s->a) || !std::isfinite(s->b) || !std::isfinite(s->c)) return invalid("coefficients must be finite");
+    return CHIMERA_OK;
+}
 
 int check_cache(const chimera_cache* c) {
     if (!c) return invalid("null cache");
@@ -222,6 +258,195 @@ int chimera_linear_backward_device(chimera_ctx* ctx, const chimera_linear_shape*
         CK(check_apart(outs, ins));
     }
     return launched(launch_linear_backward(st, LinearBackward{*shape, *args}), "linear backward kernels");
+}
+
+int chimera_norm_workspace(const chimera_norm_shape* shape, size_t* bytes) {
+    CK(check_norm(shape));
+    if (!bytes) return invalid("null argument");
+    *bytes = norm_workspace(*shape);
+    return CHIMERA_OK;
+}
+
+int chimera_norm_forward_device(chimera_ctx* ctx, const chimera_norm_shape* shape, const chimera_norm_forward* args) {
+    hipStream_t st;
+    CK(api_enter(ctx, &st));
+    CK(check_norm(shape));
+    if (!args) return invalid("null argument");
+    if (shape->rows == 0) return CHIMERA_OK;
+    const size_t e = type_bytes(shape->type), out = type_bytes(shape->out_type);
+    const int64_t m = shape->rows, n = shape->features;
+    CK(check_matrix("x", args->x, m, n, args->x_stride, e));
+    CK(check_matrix("y", args->y, m, n, args->y_stride, out));
+    if (args->weight) CK(check_vector("weight", args->weight, e));
+    if (args->bias) CK(check_vector("bias", args->bias, e));
+    if (args->mean) CK(check_vector("mean", args->mean, 4));
+    if (args->rstd) CK(check_vector("rstd", args->rstd, 4));
+    const Region outs[] = {region("y", args->y, m, n, args->y_stride, out), region("mean", args->mean, 1, m, m, 4),
+                           region("rstd", args->rstd, 1, m, m, 4)};
+    const Region ins[] = {region("x", args->x, m, n, args->x_stride, e), region("weight", args->weight, 1, n, n, e),
+                          region("bias", args->bias, 1, n, n, e)};
+    CK(check_apart(outs, ins));
+    return launched(launch_norm_forward(st, *shape, *args), "layer norm kernel");
+}
+
+int chimera_norm_backward_device(chimera_ctx* ctx, const chimera_norm_shape* shape, const chimera_norm_backward* args) {
+    hipStream_t st;
+    CK(api_enter(ctx, &st));
+    CK(check_norm(shape));
+    if (!args) return invalid("null argument");
+    const size_t e = type_bytes(shape->type), out = type_bytes(shape->out_type);
+    const int64_t m = shape->rows, n = shape->features;
+    const bool sums = args->dweight || args->dbias;
+    if (args->dweight) CK(check_vector("dweight", args->dweight, e));
+    if (args->dbias) CK(check_vector("dbias", args->dbias, e));
+    if (m > 0) {
+        CK(check_matrix("x", args->x, m, n, args->x_stride, e));
+        CK(check_matrix("dy", args->dy, m, n, args->dy_stride, out));
+        CK(check_vector("mean", args->mean, 4));
+        CK(check_vector("rstd", args->rstd, 4));
+        if (args->weight) CK(check_vector("weight", args->weight, e));
+        if (args->dx) CK(check_matrix("dx", args->dx, m, n, args->dx_stride, e));
+        const size_t need = sums ? norm_workspace(*shape) : 0;
+        CK(check_workspace(args->workspace, args->workspace_bytes, need));
+        const int64_t bytes = static_cast<int64_t>(need);
+        const Region outs[] = {region("dx", args->dx, m, n, args->dx_stride, e), region("dweight", args->dweight, 1, n, n, e),
+                               region("dbias", args->dbias, 1, n, n, e),
+                               region("the workspace", args->workspace, 1, bytes, bytes, 1)};
+        const Region ins[] = {region("x", args->x, m, n, args->x_stride, e), region("weight", args->weight, 1, n, n, e),
+                              region("dy", args->dy, m, n, args->dy_stride, out), region("mean", args->mean, 1, m, m, 4),
+                              region("rstd", args->rstd, 1, m, m, 4)};
+        CK(check_apart(outs, ins));
+    }
+    return launched(launch_norm_backward(st, *shape, *args), "layer norm gradient kernels");
+}
+
+int chimera_mx4_row(int32_t features, int32_t* row_bytes, int32_t* scales) {
+    CK(check_features(features));
+    if (!row_bytes || !scales) return invalid("null argument");
+    *row_bytes = mx4_row_bytes(features);
+    *scales = mx4_row_scales(features);
+    return CHIMERA_OK;
+}
+
+int chimera_mx4_quantise_device(chimera_ctx* ctx, const void* d_rows, int32_t type, int64_t row_stride, int64_t n,
+                                int32_t features, uint8_t* d_codes, uint8_t* d_scales) {
+    hipStream_t st;
+    CK(api_enter(ctx, &st));
+    CK(check_rows(n));
+    CK(check_features(features));
+    if (!known_type(type)) return invalid("unknown element type");
+    if (n == 0) return CHIMERA_OK;
+    const size_t e = type_bytes(type);
+    const int64_t bytes = mx4_row_bytes(features), scales = mx4_row_scales(features);
+    CK(check_matrix("rows", d_rows, n, features, row_stride, e));
+    CK(check_mx4(d_codes, d_scales));
+    const Region outs[] = {region("codes", d_codes, 1, n * bytes, n * bytes, 1),
+                           region("scales", d_scales, 1, n * scales, n * scales, 1)};
+    const Region ins[] = {region("rows", d_rows, n, features, row_stride, e)};
+    CK(check_apart(outs, ins));
+    return launched(launch_mx4_quantise(st, d_rows, type, row_stride, n, features, d_codes, d_scales), "4-bit quantising kernel");
+}
+
+int chimera_mx4_read_device(chimera_ctx* ctx, const uint8_t* d_codes, const uint8_t* d_scales, int64_t n,
+                            int32_t features, void* d_out, int32_t type, int64_t out_stride) {
+    hipStream_t st;
+    CK(api_enter(ctx, &st));
+    CK(check_rows(n));
+    CK(check_features(features));
+    if (!known_type(type)) return invalid("unknown element type");
+    if (n == 0) return CHIMERA_OK;
+    const size_t e = type_bytes(type);
+    const int64_t bytes = mx4_row_bytes(features), scales = mx4_row_scales(features);
+    CK(check_mx4(d_codes, d_scales));
+    CK(check_matrix("out", d_out, n, features, out_stride, e));
+    const Region outs[] = {region("out", d_out, n, features, out_stride, e)};
+    const Region ins[] = {region("codes", d_codes, 1, n * bytes, n * bytes, 1),
+                          region("scales", d_scales, 1, n * scales, n * scales, 1)};
+    CK(check_apart(outs, ins));
+    return launched(launch_mx4_read(st, d_codes, d_scales, n, features, d_out, type, out_stride), "4-bit reading kernel");
+}
+
+int chimera_mx4_linear_workspace(const chimera_linear_shape* shape, size_t* bytes) {
+    CK(check_shape(shape));
+    if (!bytes) return invalid("null argument");
+    *bytes = mx4_linear_workspace(*shape);
+    return CHIMERA_OK;
+}
+
+int chimera_mx4_linear_device(chimera_ctx* ctx, const chimera_linear_shape* shape, const chimera_mx4_linear* args) {
+    hipStream_t st;
+    CK(api_enter(ctx, &st));
+    CK(check_shape(shape));
+    if (!args) return invalid("null argument");
+    if (shape->rows == 0) return CHIMERA_OK;
+    const size_t e = type_bytes(shape->type), out = type_bytes(shape->out_type);
+    const int64_t m = shape->rows, k = shape->in_features, n = shape->out_features;
+    CK(check_matrix("x", args->x, m, k, args->x_stride, e));
+    CK(check_mx4(args->codes, args->scales));
+    CK(check_matrix("y", args->y, m, n, args->y_stride, out));
+    if (args->bias) CK(check_vector("bias", args->bias, e));
+    if (args->residual) CK(check_matrix("residual", args->residual, m, n, args->residual_stride, e));
+    const size_t need = mx4_linear_workspace(*shape);
+    CK(check_workspace(args->workspace, args->workspace_bytes, need));
+    const int64_t bytes = static_cast<int64_t>(need), codes = n * mx4_row_bytes(shape->in_features),
+                  scales = n * mx4_row_scales(shape->in_features);
+    const Region outs[] = {region("y", args->y, m, n, args->y_stride, out),
+                           region("the workspace", args->workspace, 1, bytes, bytes, 1)};
+    const Region ins[] = {region("x", args->x, m, k, args->x_stride, e), region("codes", args->codes, 1, codes, codes, 1),
+                          region("scales", args->scales, 1, scales, scales, 1), region("bias", args->bias, 1, n, n, e),
+                          region("residual", args->residual, m, n, args->residual_stride, e)};
+    CK(check_apart(outs, ins));
+    return launched(launch_mx4_linear(st, *shape, *args), "4-bit layer kernels");
+}
+
+int chimera_orthogonal_workspace(const chimera_orthogonal_shape* shape, size_t* bytes) {
+    CK(check_orthogonal(shape));
+    if (!bytes) return invalid("null argument");
+    *bytes = orthogonal_workspace(*shape);
+    return CHIMERA_OK;
+}
+
+int chimera_orthogonal_update_device(chimera_ctx* ctx, const chimera_orthogonal_shape* shape,
+                                     const chimera_orthogonal_update* args) {
+    hipStream_t st;
+    CK(api_enter(ctx, &st));
+    CK(check_orthogonal(shape));
+    if (!args) return invalid("null argument");
+    const chimera_orthogonal_update& g = *args;
+    const size_t e = type_bytes(shape->type), out = type_bytes(shape->out_type);
+    const int64_t m = shape->rows, n = shape->cols;
+    if (g.nesterov != 0 && g.nesterov != 1) return invalid("nesterov must be 0 or 1");
+    if (!std::isfinite(g.mu) || !std::isfinite(g.rate) || !std::isfinite(g.decay))
+        return invalid("mu, rate and decay must be finite");
+    if (!g.out && !g.weight) return invalid("null argument: out and weight");
+    CK(check_matrix("gradient", g.gradient, m, n, g.gradient_stride, e));
+    if (g.momentum) {
+        CK(check_matrix("momentum", g.momentum, m, n, g.momentum_stride, 4));
+        CK(check_matrix("new_momentum", g.new_momentum, m, n, g.new_momentum_stride, 4));
+    }
+    if (g.out) CK(check_matrix("out", g.out, m, n, g.out_stride, out));
+    if (g.weight) {
+        CK(check_matrix("weight", g.weight, m, n, g.weight_stride, 4));
+        CK(check_matrix("new_weight", g.new_weight, m, n, g.new_weight_stride, 4));
+        if (g.rounded) CK(check_matrix("rounded", g.rounded, m, n, g.rounded_stride, e));
+    }
+    const size_t need = orthogonal_workspace(*shape);
+    CK(check_workspace(g.workspace, g.workspace_bytes, need));
+    // a state that is updated in its place
+    const bool same_momentum = g.momentum && g.momentum == g.new_momentum, same_weight = g.weight && g.weight == g.new_weight;
+    if (same_momentum && g.momentum_stride != g.new_momentum_stride) return invalid("new_momentum overlaps momentum");
+    if (same_weight && g.weight_stride != g.new_weight_stride) return invalid("new_weight overlaps weight");
+    const int64_t bytes = static_cast<int64_t>(need);
+    const Region outs[] = {region("new_momentum", g.momentum ? g.new_momentum : nullptr, m, n, g.new_momentum_stride, 4),
+                           region("out", g.out, m, n, g.out_stride, out),
+                           region("new_weight", g.weight ? g.new_weight : nullptr, m, n, g.new_weight_stride, 4),
+                           region("rounded", g.weight ? g.rounded : nullptr, m, n, g.rounded_stride, e),
+                           region("the workspace", g.workspace, 1, bytes, bytes, 1)};
+    const Region ins[] = {region("gradient", g.gradient, m, n, g.gradient_stride, e),
+                          region("momentum", same_momentum ? nullptr : g.momentum, m, n, g.momentum_stride, 4),
+                          region("weight", same_weight ? nullptr : g.weight, m, n, g.weight_stride, 4)};
+    CK(check_apart(outs, ins));
+    return launched(launch_orthogonal(st, *shape, g), "orthogonal update kernels");
 }
 
 int chimera_cache_row(const chimera_cache* cache, int32_t* row_bytes, int32_t* scales) {

@@ -116,6 +116,29 @@ size_t linear_backward_workspace(const chimera_linear_shape& s);
 hipError_t launch_linear_forward(hipStream_t st, const LinearForward& f);
 hipError_t launch_linear_backward(hipStream_t st, const LinearBackward& b);
 
+// ---- layer norm (kernels_norm.hip) ----
+
+size_t norm_workspace(const chimera_norm_shape& s);
+hipError_t launch_norm_forward(hipStream_t st, const chimera_norm_shape& s, const chimera_norm_forward& f);
+hipError_t launch_norm_backward(hipStream_t st, const chimera_norm_shape& s, const chimera_norm_backward& b);
+
+// ---- microscaled 4-bit floating point (kernels_mx4.hip) ----
+
+inline int mx4_row_bytes(int features) { return (features + 31) / 32 * 16; }
+inline int mx4_row_scales(int features) { return (features + 255) / 256 * 8; }
+
+size_t mx4_linear_workspace(const chimera_linear_shape& s);
+hipError_t launch_mx4_quantise(hipStream_t st, const void* x, int type, int64_t stride, int64_t rows, int cols,
+                               uint8_t* codes, uint8_t* scales);
+hipError_t launch_mx4_read(hipStream_t st, const uint8_t* codes, const uint8_t* scales, int64_t rows, int cols, void* out,
+                           int type, int64_t stride);
+hipError_t launch_mx4_linear(hipStream_t st, const chimera_linear_shape& s, const chimera_mx4_linear& a);
+
+// ---- orthogonal update (kernels_orthogonal.hip) ----
+
+size_t orthogonal_workspace(const chimera_orthogonal_shape& s);
+hipError_t launch_orthogonal(hipStream_t st, const chimera_orthogonal_shape& s, const chimera_orthogonal_update& g);
+
 // ---- quantised cache (kernels_cache.hip) ----
 
 inline int cache_row_bytes(const chimera_cache& c) {

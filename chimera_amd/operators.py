@@ -1,7 +1,8 @@
 """The operators beside the index (include/chimera_operators.h): dense layers
-that turn hidden states into token embeddings, a quantised cache of token
-embeddings and late interaction on it, and a store of documents that come and
-go on top of the cache.
+that turn hidden states into token embeddings, the layer norm between them, the
+update of their weights, layers served in microscaled 4-bit floating point, a
+quantised cache of token embeddings and late interaction on it, and a store of
+documents that come and go on top of the cache.
 
 Arrays are device arrays: capi.DeviceArray, a PyTorch tensor through
 from_torch(), or any object with `ptr`, `shape`
@@ -14,6 +15,7 @@ until the object is closed.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -60,6 +62,39 @@ class CacheMaxsim(C.Structure):
                 ("top_counts", P), ("workspace", P), ("workspace_bytes", C.c_size_t)]
 
 
+class NormShape(C.Structure):
+    _fields_ = [("rows", C.c_int64), ("features", C.c_int32), ("type", C.c_int32), ("out_type", C.c_int32), ("eps", C.c_float)]
+
+
+class NormForward(C.Structure):
+    _fields_ = [("x", P), ("weight", P), ("bias", P), ("y", P), ("mean", P), ("rstd", P), ("x_stride", C.c_int64),
+                ("y_stride", C.c_int64)]
+
+
+class NormBackward(C.Structure):
+    _fields_ = [("x", P), ("weight", P), ("dy", P), ("mean", P), ("rstd", P), ("dx", P), ("dweight", P), ("dbias", P),
+                ("x_stride", C.c_int64), ("dy_stride", C.c_int64), ("dx_stride", C.c_int64), ("workspace", P),
+                ("workspace_bytes", C.c_size_t)]
+
+
+class Mx4LinearArgs(C.Structure):
+    _fields_ = [("x", P), ("codes", P), ("scales", P), ("bias", P), ("residual", P), ("y", P), ("x_stride", C.c_int64),
+                ("residual_stride", C.c_int64), ("y_stride", C.c_int64), ("workspace", P), ("workspace_bytes", C.c_size_t)]
+
+
+class OrthogonalShape(C.Structure):
+    _fields_ = [("rows", C.c_int32), ("cols", C.c_int32), ("type", C.c_int32), ("out_type", C.c_int32), ("steps", C.c_int32),
+                ("a", C.c_float), ("b", C.c_float), ("c", C.c_float)]
+
+
+class OrthogonalArgs(C.Structure):
+    _fields_ = [("gradient", P), ("momentum", P), ("new_momentum", P), ("mu", C.c_float), ("nesterov", C.c_int32), ("out", P),
+                ("weight", P), ("new_weight", P), ("rounded", P), ("rate", C.c_float), ("decay", C.c_float),
+                ("gradient_stride", C.c_int64), ("momentum_stride", C.c_int64), ("new_momentum_stride", C.c_int64),
+                ("out_stride", C.c_int64), ("weight_stride", C.c_int64), ("new_weight_stride", C.c_int64),
+                ("rounded_stride", C.c_int64), ("workspace", P), ("workspace_bytes", C.c_size_t)]
+
+
 _NUMPY = {np.dtype(np.float32): "f32", np.dtype(np.float16): "f16", np.dtype(np.int32): "int32",
           np.dtype(np.int64): "int64", np.dtype(np.uint8): "uint8"}
 
@@ -102,6 +137,7 @@ def _whole(a, what: str) -> None:
         raise ValueError(f"the rows of {what} must follow each other")
 
 
+@functools.lru_cache(maxsize=None)
 def _function(name: str, *argtypes):
     """An entry point with its argument types set: plain integers and struct
     references go through without wrapping."""
@@ -282,6 +318,270 @@ def _int32(value: int, what: str) -> int:
     if not -(1 << 31) <= value < 1 << 31:
         raise ValueError(f"{what} must fit 32 bits, not {value}")
     return value
+
+
+class _Workspace:
+    """What an object's calls need of memory, for calls of up to a number of
+    rows: freed by close(), after which calls that need it are refused."""
+
+    def __init__(self, ctx: capi.Context):
+        self.ctx = ctx
+        self._workspace = None
+
+    def _allocate(self, nbytes: int, *args) -> None:
+        self._holders = args
+        self._bytes = nbytes
+        if nbytes:
+            self._workspace = self.ctx.empty(nbytes, np.uint8)
+        for a in args:
+            a.workspace, a.workspace_bytes = _ptr(self._workspace), nbytes
+
+    def close(self) -> None:
+        """Frees the workspace; calls after it that need it are refused."""
+        workspace, self._workspace = getattr(self, "_workspace", None), None
+        if workspace is not None:
+            for a in self._holders:
+                a.workspace, a.workspace_bytes = None, 0
+            self.ctx.synchronize()
+            workspace.free()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _room(self, rows: int, need) -> None:
+        if rows > self.max_rows and need(rows) > self._bytes:
+            raise capi.ChimeraError(_CAPACITY, f"the workspace is for {self.max_rows} rows, the call has {rows}")
+
+
+class LayerNorm(_Workspace):
+    """y = (x - mean) / sqrt(var + eps) * weight + bias, row by row. weight and
+    bias [features] stay the caller's arrays and may change between calls; a
+    bias of None is zeros. For ones, leave the weight out and give `features`
+    and `type`. With `training` the object holds the workspace for backward
+    passes of up to max_rows rows; close it before its context."""
+
+    def __init__(self, ctx: capi.Context, weight=None, bias=None, eps: float = 1e-5, max_rows: int = 1,
+                 training: bool = False, features: int | None = None, type: str | None = None):
+        super().__init__(ctx)
+        if weight is None and bias is None and (features is None or type is None):
+            raise ValueError("a layer norm without weight and bias needs features and type")
+        given = weight if weight is not None else bias
+        if given is not None:
+            if len(given.shape) != 1:
+                raise ValueError("weight and bias must be [features]")
+            features, type = given.shape[0], _type_name(given)
+        if type not in TYPES:
+            raise ValueError(f"the type must be f32, f16 or bf16, not {type}")
+        for v, what in ((weight, "weight"), (bias, "bias")):
+            if v is not None:
+                _expect(v, what, (features,), type)
+        self.weight, self.bias, self.features, self.type = weight, bias, features, type
+        self.training, self.max_rows = training, max_rows
+        self._shape = NormShape(0, _int32(features, "features"), TYPES[type], TYPES[type], eps)
+        self._forward = NormForward(weight=_ptr(weight), bias=_ptr(bias))
+        self._backward = NormBackward(weight=_ptr(weight))
+        self._shape_ref = C.byref(self._shape)
+        self._forward_ref, self._backward_ref = C.byref(self._forward), C.byref(self._backward)
+        self._call_forward = _function("chimera_norm_forward_device", P, P, P)
+        self._call_backward = _function("chimera_norm_backward_device", P, P, P)
+        need = self._need(max_rows)
+        self._allocate(need if training else 0, self._backward)
+
+    def _need(self, rows: int) -> int:
+        need = C.c_size_t()
+        self._shape.rows, self._shape.out_type = rows, self._shape.type  # a refused call may have left another
+        check(capi.lib().chimera_norm_workspace(self._shape_ref, C.byref(need)))
+        return need.value
+
+    def forward(self, x, y, mean=None, rstd=None) -> None:
+        """y [rows, features] (the norm's type or f32) from x [rows, features].
+        For the backward pass `mean` and `rstd` [rows] f32 get the rows'
+        statistics."""
+        rows = x.shape[0]
+        _expect(x, "x", (rows, self.features), self.type)
+        if tuple(y.shape) != (rows, self.features):
+            raise ValueError(f"y must have shape {(rows, self.features)}, not {tuple(y.shape)}")
+        self._shape.rows, self._shape.out_type = rows, _type(y, "y")
+        a = self._forward
+        a.x, a.x_stride, a.y, a.y_stride = x.ptr, _stride(x), y.ptr, _stride(y)
+        for name, v in (("mean", mean), ("rstd", rstd)):
+            if v is not None:
+                _expect(v, name, (rows,), "f32")
+            setattr(a, name, _ptr(v))
+        check(self._call_forward(self.ctx.handle, self._shape_ref, self._forward_ref))
+
+    def backward(self, x, dy, mean, rstd, dx=None, dweight=None, dbias=None) -> None:
+        """Gradients from dy [rows, features] and what forward() left in `mean`
+        and `rstd`; those left out are not computed. The weight's is that of the
+        factor, also where it is ones."""
+        if not self.training:
+            raise ValueError("the layer norm was made without training")
+        rows, n, t = x.shape[0], self.features, self.type
+        _expect(x, "x", (rows, n), t)
+        if tuple(dy.shape) != (rows, n):
+            raise ValueError(f"dy must have shape {(rows, n)}, not {tuple(dy.shape)}")
+        _expect(mean, "mean", (rows,), "f32")
+        _expect(rstd, "rstd", (rows,), "f32")
+        self._room(rows, self._need)
+        self._shape.rows, self._shape.out_type = rows, _type(dy, "dy")
+        a = self._backward
+        a.x, a.x_stride, a.dy, a.dy_stride, a.mean, a.rstd = x.ptr, _stride(x), dy.ptr, _stride(dy), mean.ptr, rstd.ptr
+        if dx is not None:
+            _expect(dx, "dx", (rows, n), t)
+            a.dx_stride = _stride(dx)
+        a.dx = _ptr(dx)
+        for name, v in (("dweight", dweight), ("dbias", dbias)):
+            if v is not None:
+                _expect(v, name, (n,), t)
+            setattr(a, name, _ptr(v))
+        check(self._call_backward(self.ctx.handle, self._shape_ref, self._backward_ref))
+
+
+def mx4_row(features: int) -> tuple[int, int]:
+    """(bytes of codes, bytes of scales) of a row of 4-bit values."""
+    row, scales = C.c_int32(), C.c_int32()
+    check(capi.lib().chimera_mx4_row(_int32(features, "features"), C.byref(row), C.byref(scales)))
+    return row.value, scales.value
+
+
+def _expect_mx4(codes, scales, rows: int, features: int) -> None:
+    row, blocks = mx4_row(features)
+    _expect_whole(codes, "codes", (rows, row), "uint8")
+    _expect_whole(scales, "scales", (rows, blocks), "uint8")
+
+
+def mx4_quantise(ctx: capi.Context, rows, codes, scales) -> None:
+    """Rows [n, features] as codes of 4 bits [n, row bytes] uint8 and a power of
+    two for each 32 values, scales [n, row scales] uint8 (mx4_row)."""
+    n, features = rows.shape
+    _expect_mx4(codes, scales, n, features)
+    call = _function("chimera_mx4_quantise_device", P, P, C.c_int32, C.c_int64, C.c_int64, C.c_int32, P, P)
+    check(call(ctx.handle, rows.ptr, _type(rows, "rows"), _stride(rows), n, features, codes.ptr, scales.ptr))
+
+
+def mx4_read(ctx: capi.Context, codes, scales, out) -> None:
+    """out [n, features] = the values of rows that mx4_quantise wrote."""
+    n, features = out.shape
+    _expect_mx4(codes, scales, n, features)
+    call = _function("chimera_mx4_read_device", P, P, P, C.c_int64, C.c_int32, P, C.c_int32, C.c_int64)
+    check(call(ctx.handle, codes.ptr, scales.ptr, n, features, out.ptr, _type(out, "out"), _stride(out)))
+
+
+class Mx4Linear(_Workspace):
+    """A dense layer on a weight in microscaled 4-bit floating point, codes
+    [out, row bytes] and scales [out, row scales] as mx4_quantise writes them of
+    a weight [out, in_features]. x is quantised the same way within the call;
+    what follows the product is as in Linear. `type` is that of x, the bias and
+    the residual. The object holds the workspace for calls of up to max_rows
+    rows; close it before its context."""
+
+    def __init__(self, ctx: capi.Context, codes, scales, in_features: int, bias=None, type: str = "bf16",
+                 activation: str = "none", normalize: bool = False, max_rows: int = 1):
+        super().__init__(ctx)
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"unknown activation {activation!r}")
+        if type not in TYPES:
+            raise ValueError(f"the type must be f32, f16 or bf16, not {type}")
+        n = codes.shape[0]
+        _expect_mx4(codes, scales, n, in_features)
+        if bias is not None:
+            _expect(bias, "bias", (n,), type)
+        self.codes, self.scales, self.bias = codes, scales, bias
+        self.in_features, self.out_features, self.type, self.max_rows = in_features, n, type, max_rows
+        t = TYPES[type]
+        self._shape = LinearShape(0, in_features, n, t, t, ACTIVATIONS[activation], int(normalize))
+        self._args = Mx4LinearArgs(codes=codes.ptr, scales=scales.ptr, bias=_ptr(bias))
+        self._shape_ref, self._args_ref = C.byref(self._shape), C.byref(self._args)
+        self._call = _function("chimera_mx4_linear_device", P, P, P)
+        self._allocate(self._need(max_rows), self._args)
+
+    def _need(self, rows: int) -> int:
+        need = C.c_size_t()
+        self._shape.rows, self._shape.out_type = rows, self._shape.type  # a refused call may have left another
+        check(capi.lib().chimera_mx4_linear_workspace(self._shape_ref, C.byref(need)))
+        return need.value
+
+    def forward(self, x, y, residual=None) -> None:
+        """y [rows, out] (the layer's type or f32) from x [rows, in]."""
+        rows = x.shape[0]
+        _expect(x, "x", (rows, self.in_features), self.type)
+        if tuple(y.shape) != (rows, self.out_features):
+            raise ValueError(f"y must have shape {(rows, self.out_features)}, not {tuple(y.shape)}")
+        self._room(rows, self._need)
+        self._shape.rows, self._shape.out_type = rows, _type(y, "y")
+        a = self._args
+        a.x, a.x_stride, a.y, a.y_stride = x.ptr, _stride(x), y.ptr, _stride(y)
+        if residual is not None:
+            _expect(residual, "residual", (rows, self.out_features), self.type)
+            a.residual_stride = _stride(residual)
+        a.residual = _ptr(residual)
+        check(self._call(self.ctx.handle, self._shape_ref, self._args_ref))
+
+
+class OrthogonalUpdate(_Workspace):
+    """The update of a weight [rows, cols]: its gradient (of `type`), with
+    momentum or without, is divided by its size and made near orthogonal by
+    `steps` steps X <- a X + (b A + c A^2) X with A = X X^T. The object holds
+    the workspace; close it before its context."""
+
+    def __init__(self, ctx: capi.Context, rows: int, cols: int, type: str = "f32", steps: int = 5,
+                 coefficients: tuple[float, float, float] = (3.4445, -4.7750, 2.0315)):
+        super().__init__(ctx)
+        if type not in TYPES:
+            raise ValueError(f"the type must be f32, f16 or bf16, not {type}")
+        a, b, c = coefficients
+        self.rows, self.cols, self.type = _int32(rows, "rows"), _int32(cols, "cols"), type
+        self._shape = OrthogonalShape(rows, cols, TYPES[type], TYPES[type], _int32(steps, "steps"), a, b, c)
+        self._args = OrthogonalArgs()
+        self._shape_ref, self._args_ref = C.byref(self._shape), C.byref(self._args)
+        self._call = _function("chimera_orthogonal_update_device", P, P, P)
+        need = C.c_size_t()
+        check(capi.lib().chimera_orthogonal_workspace(self._shape_ref, C.byref(need)))
+        self._allocate(need.value, self._args)
+
+    def _set(self, name: str, v, kind: str) -> None:
+        if v is not None:
+            _expect(v, name, (self.rows, self.cols), kind)
+            setattr(self._args, name + "_stride", _stride(v))
+        setattr(self._args, name, _ptr(v))
+
+    def _run(self, gradient, out, momentum, new_momentum, mu, nesterov) -> None:
+        a = self._args
+        self._set("gradient", gradient, self.type)
+        self._set("momentum", momentum, "f32")
+        self._set("new_momentum", new_momentum if new_momentum is not None else momentum, "f32")
+        if momentum is None and new_momentum is not None:
+            raise ValueError("new_momentum needs momentum")
+        a.mu, a.nesterov = mu, int(nesterov)
+        self._shape.out_type = self._shape.type
+        if out is not None:
+            _expect(out, "out", (self.rows, self.cols), _type_name(out))
+            self._shape.out_type, a.out_stride = _type(out, "out"), _stride(out)
+        a.out = _ptr(out)
+        check(self._call(self.ctx.handle, self._shape_ref, self._args_ref))
+
+    def orthogonalize(self, gradient, out, momentum=None, new_momentum=None, mu: float = 0.95, nesterov: bool = True) -> None:
+        """out [rows, cols] (the gradient's type or f32) = the orthogonal
+        update alone."""
+        for name in ("weight", "new_weight", "rounded"):
+            self._set(name, None, "f32")
+        self._args.rate = self._args.decay = 0.0
+        self._run(gradient, out, momentum, new_momentum, mu, nesterov)
+
+    def step(self, gradient, weight, new_weight=None, rate: float = 0.02, decay: float = 0.0, momentum=None,
+             new_momentum=None, mu: float = 0.95, nesterov: bool = True, rounded=None, out=None) -> None:
+        """new_weight = (1 - decay) weight - rate * update, and the momentum
+        mu * momentum + gradient; weights and momentum are f32 and change in
+        their place where no new array is given. `rounded` gets the weight in
+        the gradient's type, as a 16-bit layer reads it."""
+        self._set("weight", weight, "f32")
+        self._set("new_weight", new_weight if new_weight is not None else weight, "f32")
+        self._set("rounded", rounded, self.type)
+        self._args.rate, self._args.decay = rate, decay
+        self._run(gradient, out, momentum, new_momentum, mu, nesterov)
 
 
 def cache_row(format: str, dim: int, group: int, page_tokens: int = 1) -> tuple[int, int]:

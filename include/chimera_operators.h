@@ -1,8 +1,10 @@
 /*
  * chimera_operators.h - the operators next to an index: dense layers that
  * turn a language model's hidden states into token embeddings (forward and
- * backward), a quantised cache of token embeddings in pages, for documents
- * that come and go, and late interaction (MaxSim) on that cache.
+ * backward), the layer norm between them, the update that turns a weight's
+ * gradient into its next value, dense layers served in microscaled 4-bit
+ * floating point, a quantised cache of token embeddings in pages, for
+ * documents that come and go, and late interaction (MaxSim) on that cache.
  *
  * No counterpart in the reference, which takes embeddings as they are and
  * whose index does not change. Same conventions as chimera_hip.h: a status
@@ -115,6 +117,159 @@ int chimera_linear_forward_device(chimera_ctx* ctx, const chimera_linear_shape* 
                                   const chimera_linear_forward* args);
 int chimera_linear_backward_device(chimera_ctx* ctx, const chimera_linear_shape* shape,
                                    const chimera_linear_backward* args);
+
+/* ---- layer norm ----
+ *
+ *   z = (x - mean) rstd,  rstd = 1 / sqrt(mean of (x - mean)^2 + eps)
+ *   y = z w + b           [rows, features]
+ *
+ * x, w and b have one type, y has it too or is 32-bit; statistics and sums are
+ * held in 32 bits, results rounded once. The mean is corrected by what is left
+ * of a row's sum after it, and rows whose squares pass the 32-bit range are
+ * scaled, so rows of any finite values are normalized; a row with a value that
+ * is not finite becomes NaN. Rows may lie apart and have any alignment of whole
+ * elements, as for dense layers. Outputs and workspace overlap neither inputs
+ * nor each other. */
+typedef struct {
+    int64_t rows;     /* 0..2^31 */
+    int32_t features; /* 1..65536 */
+    int32_t type;     /* CHIMERA_F32, _F16 or _BF16 */
+    int32_t out_type; /* type or CHIMERA_F32 */
+    float eps;        /* 1e-30 or more */
+} chimera_norm_shape;
+
+typedef struct {
+    const void* x;      /* [rows, features] */
+    const void* weight; /* [features] or NULL: ones */
+    const void* bias;   /* [features] or NULL: zeros */
+    void* y;            /* [rows, features], out_type */
+    float* mean;        /* [rows] for the backward pass, or NULL */
+    float* rstd;        /* likewise */
+    int64_t x_stride, y_stride;
+} chimera_norm_forward;
+
+/* Gradients from dY, with g = dY w:
+ *   dx = rstd (g - mean of g - z mean of g z),
+ *   dw = the sum over rows of dY z,  db = the sum over rows of dY,
+ * in a fixed order. With rows = 0, dw and db are zeros. Outputs that are NULL
+ * are not computed. */
+typedef struct {
+    const void* x;
+    const void* weight; /* as in the forward pass */
+    const void* dy;     /* out_type */
+    const float* mean;  /* as the forward pass left them */
+    const float* rstd;
+    void* dx;           /* [rows, features], type, or NULL */
+    void* dweight;      /* [features], type, or NULL */
+    void* dbias;        /* [features], type, or NULL */
+    int64_t x_stride, dy_stride, dx_stride;
+    void* workspace;    /* chimera_norm_workspace bytes, 256-byte aligned; read with dweight or dbias */
+    size_t workspace_bytes;
+} chimera_norm_backward;
+
+/* Bytes of workspace of the backward pass; grows with rows, so that of the
+ * largest call serves all. Host arithmetic only. */
+int chimera_norm_workspace(const chimera_norm_shape* shape, size_t* bytes);
+
+int chimera_norm_forward_device(chimera_ctx* ctx, const chimera_norm_shape* shape, const chimera_norm_forward* args);
+int chimera_norm_backward_device(chimera_ctx* ctx, const chimera_norm_shape* shape, const chimera_norm_backward* args);
+
+/* ---- microscaled 4-bit floating point ----
+ *
+ * A row of features values is codes of 4 bits and, for each 32 neighbours, a
+ * scale of 8 bits that is a power of two: value = code * 2^(scale - 127), with
+ * codes 0, 0.5, 1, 1.5, 2, 3, 4 and 6 (0..7, plus 8 with a minus sign), the
+ * even value in the low half of a byte. Quantising takes
+ *   scale - 127 = the exponent of the largest magnitude - 2, at least -127,
+ *   code = value / 2^(scale - 127) to the nearest, ties to the even code, 6
+ *          at the most.
+ * A block with a value that is not finite has the scale 255 and reads back as
+ * NaN. Rows of codes are padded with zeros to whole blocks (16 bytes each),
+ * rows of scales to a multiple of 8; what the padding's scales hold does not
+ * matter where they are read. */
+
+/* Bytes of a row's codes and of its scales. Host arithmetic only. */
+int chimera_mx4_row(int32_t features, int32_t* row_bytes, int32_t* scales);
+
+/* d_codes [n, row_bytes] (16-byte aligned) and d_scales [n, scales] (8-byte
+ * aligned) of rows [n, features] of `type` (row stride in elements). */
+int chimera_mx4_quantise_device(chimera_ctx* ctx, const void* d_rows, int32_t type, int64_t row_stride, int64_t n,
+                                int32_t features, uint8_t* d_codes, uint8_t* d_scales);
+
+/* d_out [n, features] of `type` = the values, rounded once to the type. */
+int chimera_mx4_read_device(chimera_ctx* ctx, const uint8_t* d_codes, const uint8_t* d_scales, int64_t n,
+                            int32_t features, void* d_out, int32_t type, int64_t out_stride);
+
+/* A dense layer on a weight that is held so,
+ *   Y = act(Q(X) W^T + b) + R, divided row by row by its length with normalize,
+ * with Q(X) the values of X's rows quantised as above. Shape, types, epilogue
+ * and limits are those of the dense layer; products are exact and sums held in
+ * 32 bits. */
+typedef struct {
+    const void* x;           /* [rows, in_features], type */
+    const uint8_t* codes;    /* [out_features, row_bytes of in_features], 16-byte aligned */
+    const uint8_t* scales;   /* [out_features, scales of in_features], 8-byte aligned */
+    const void* bias;        /* [out_features], type, or NULL */
+    const void* residual;    /* [rows, out_features], type, or NULL */
+    void* y;                 /* [rows, out_features], out_type */
+    int64_t x_stride, residual_stride, y_stride;
+    void* workspace;         /* chimera_mx4_linear_workspace bytes, 256-byte aligned; NULL if 0 */
+    size_t workspace_bytes;
+} chimera_mx4_linear;
+
+/* Grows with rows, so that of the largest call serves all. Host arithmetic
+ * only. */
+int chimera_mx4_linear_workspace(const chimera_linear_shape* shape, size_t* bytes);
+
+int chimera_mx4_linear_device(chimera_ctx* ctx, const chimera_linear_shape* shape, const chimera_mx4_linear* args);
+
+/* ---- orthogonal update of a weight ----
+ *
+ *   M' = mu M + G,  U = G without M, G + mu M' with nesterov, else M'
+ *   X = U / |U| (the square root of the sum of squares; zeros stay zeros), then
+ *   X <- a X + (b A + c A^2) X with A = X X^T, `steps` times,
+ *   W' = (1 - decay) W - rate X
+ *
+ * which brings U's singular values near one and keeps its directions: what the
+ * products do to a singular value s is a s + b s^3 + c s^5, step by step. G has
+ * the layer's type, M and W are 32-bit; a 16-bit layer reads the rounded copy.
+ * Products are sums in 32 bits of values that are held to 22 bits; sums of
+ * squares are held in 64. The coefficients should keep singular values below
+ * 100 from step to step (the values 3.4445, -4.7750, 2.0315 keep them below
+ * 1.3): X and b A + c A^2 become infinite from 255 on. A U that is not finite
+ * gives X that is not. */
+typedef struct {
+    int32_t rows, cols; /* 1..65536; rows * cols at most 2^28, the smaller at most 8192 */
+    int32_t type;       /* of the gradient and the rounded copy */
+    int32_t out_type;   /* type or CHIMERA_F32 */
+    int32_t steps;      /* 1..100 */
+    float a, b, c;
+} chimera_orthogonal_shape;
+
+typedef struct {
+    const void* gradient;  /* [rows, cols], type */
+    const float* momentum; /* [rows, cols] or NULL */
+    float* new_momentum;   /* [rows, cols], with momentum; may be momentum */
+    float mu;
+    int32_t nesterov;      /* 0 or 1 */
+    void* out;             /* X [rows, cols], out_type, or NULL */
+    const float* weight;   /* [rows, cols] or NULL */
+    float* new_weight;     /* [rows, cols], with weight; may be weight */
+    void* rounded;         /* W' [rows, cols], type, or NULL */
+    float rate, decay;
+    int64_t gradient_stride, momentum_stride, new_momentum_stride, out_stride;
+    int64_t weight_stride, new_weight_stride, rounded_stride;
+    void* workspace;       /* chimera_orthogonal_workspace bytes, 256-byte aligned */
+    size_t workspace_bytes;
+} chimera_orthogonal_update;
+
+/* Host arithmetic only. */
+int chimera_orthogonal_workspace(const chimera_orthogonal_shape* shape, size_t* bytes);
+
+/* Outputs and workspace overlap neither inputs nor each other, but for
+ * new_momentum = momentum and new_weight = weight with the same stride. */
+int chimera_orthogonal_update_device(chimera_ctx* ctx, const chimera_orthogonal_shape* shape,
+                                     const chimera_orthogonal_update* args);
 
 /* ---- quantised token cache ----
  *
