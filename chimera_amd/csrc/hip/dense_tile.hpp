@@ -100,7 +100,24 @@ __device__ __forceinline__ float gelu_16(float z) {
     return z * (z > 0.0f ? 1.0f - tail : tail);
 }
 
-constexpr int kRoundedGelu = -1;  // gelu_16 for CHIMERA_ACT_GELU
+// The same with P of degree 7, within 2^-17 of the size down to -6: for sums of
+// 4-bit values, whose rounding to 16 bits is seldom another for it (about one
+// fp16 result in a hundred). Three instructions less: 65,536 x 4096 outputs of
+// such a layer 316 -> 302 us.
+__device__ __forceinline__ float gelu_short(float z) {
+    const float a = fabsf(z);
+    float p = fmaf(-1.8348062e-6f, a, 6.1598182e-5f);
+    p = fmaf(p, a, -9.3052391e-4f);
+    p = fmaf(p, a, 8.5078869e-3f);
+    p = fmaf(p, a, -5.3960058e-2f);
+    p = fmaf(p, a, -4.5846441e-1f);
+    p = fmaf(p, a, -1.1512511f);
+    p = fmaf(p, a, -0.99999529f);
+    const float tail = __builtin_amdgcn_exp2f(p);
+    return z * (z > 0.0f ? 1.0f - tail : tail);
+}
+
+constexpr int kRoundedGelu = -1, kShortGelu = -2;  // gelu_16 and gelu_short for CHIMERA_ACT_GELU
 
 __device__ __forceinline__ float activation(float z, int act) {
     switch (act) {
@@ -110,6 +127,7 @@ __device__ __forceinline__ float activation(float z, int act) {
             return z * normal_cdf(z, &gauss);
         }
         case kRoundedGelu: return gelu_16(z);
+        case kShortGelu: return gelu_short(z);
         case CHIMERA_ACT_GELU_TANH:  // (1 + tanh u) / 2 is the sigmoid of 2 u
             return z * sigmoid(2.0f * kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
         case CHIMERA_ACT_SILU: return z * sigmoid(z);
@@ -262,9 +280,9 @@ struct Product {
     int64_t sum;  // with rows along it, whole 16-byte chunks; so are m and n with rows across it
     int tiles_m, tiles_n;
     int steps, steps_per_split;  // of kStepBytes along the sum
-    // of 4-bit operands: a byte for each chunk, eight for each step
+    // of 4-bit operands [steps][m or n][8]: those of a step's chunks 0, 2, 4, 6
+    // and 1, 3, 5, 7, as the halves of a wave take them; zeros past the sum
     const uint8_t *a_scales, *b_scales;
-    int64_t a_scales_stride, b_scales_stride;  // bytes between rows
 };
 
 // ---- tiled product -------------------------------------------------------------
@@ -290,8 +308,9 @@ __device__ __forceinline__ void wait_and_meet() {
 // Rows along the sum: a step is 128 bytes of each row, whole lines (with 64
 // bytes a CU loads 60 GB/s into LDS, with 128 it loads 125; the largest tile
 // needs 75 at the matrix cores' rate); chunk c of row r lies at place
-// c ^ (r % 8), so that the lanes that follow each other in an LDS read of 16
-// bytes hit different banks.
+// c ^ (r / 2 % 8), so that 16 lanes that follow each other in an LDS read of 16
+// bytes, two rows of which fill the banks, hit different ones (with r % 8 half
+// of the reads' cycles were conflicts).
 // Rows across the sum: a step is 64 (or 32, of 32 bits) rows of B values. For
 // 16-bit values the LDS's transposing read gives 16 lanes four values of a
 // column each from four rows of 32 bytes; chunk c of row r lies at place
@@ -308,7 +327,6 @@ struct Side {
     const char* base;
     int64_t step_bytes;  // between steps
     uint32_t off[kLoads];
-    int at;  // first value of the sum in this lane's chunk (or its row), within a step
     uint32_t piece[kLoads];
 
     __device__ __forceinline__ void init(const void* p, int64_t stride, int64_t first, int64_t count, int step0, int w, int l) {
@@ -324,7 +342,7 @@ struct Side {
                 off[i] = static_cast<uint32_t>(row) * static_cast<uint32_t>(stride) +
                          16u * static_cast<uint32_t>(min(chunk, last / kPer));
             } else {
-                const int chunk = place ^ (row & 7);
+                const int chunk = place ^ ((row >> 1) & 7);
                 off[i] = static_cast<uint32_t>(min(row, last)) * static_cast<uint32_t>(stride) + 16u * chunk;
             }
         }
@@ -332,8 +350,6 @@ struct Side {
             base = static_cast<const char*>(p) + first * static_cast<int64_t>(sizeof(T));
             step_bytes = kStepRows * stride;
         } else {
-            // the same chunk for every piece: 8 rows each
-            at = ((l & 7) ^ (l >> 3)) * kPer;
             base = static_cast<const char*>(p) + first * stride;
             step_bytes = kStepBytes;
         }
@@ -348,7 +364,9 @@ struct Side {
         for (int i = 0; i < kLoads; ++i) {
             int64_t o = off[i];
             if (!whole) {
-                const int first = kAcross ? (static_cast<int>(piece[i]) + 16 * l) / kRowBytes : at;
+                const int row = (static_cast<int>(piece[i]) + 16 * l) / kRowBytes;
+                // the first value of the sum in this lane's chunk (or its row), within the step
+                const int first = kAcross ? row : ((l & 7) ^ ((row >> 1) & 7)) * kPer;
                 const int64_t zero = reinterpret_cast<const char*>(g_zero_chunk) - from;
                 o = first >= left ? zero : o;
             }
@@ -359,19 +377,15 @@ struct Side {
 
 // The operands of one wave: kCount tiles of 32 rows (or columns) from `first`
 // on, a quarter of a step at a time (two 16-byte chunks of the sum, one for
-// each half of the wave: neighbours, or of 4-bit values those four apart, so
-// that a half's four scales are neighbours).
+// each half of the wave).
 template <typename T, int kCount, bool kAcross, int kRowBytes>
 struct Reader {
-    static constexpr bool kHalves = sizeof(T) == 1;
     static constexpr int kReads = !kAcross ? 1 : sizeof(T) == 4 ? 4 : 2;  // of a tile's quarter step
     uint32_t off[kAcross && sizeof(T) == 2 ? kCount : 1];
 
     __device__ __forceinline__ void init(int first, int l) {
-        if constexpr (kHalves) {
-            off[0] = static_cast<uint32_t>(first + (l & 31)) * kStepBytes + (((l >> 5 << 2) ^ (l & 7)) << 4);
-        } else if constexpr (!kAcross) {
-            off[0] = static_cast<uint32_t>(first + (l & 31)) * kStepBytes + (((l >> 5) ^ (l & 7)) << 4);
+        if constexpr (!kAcross) {
+            off[0] = static_cast<uint32_t>(first + (l & 31)) * kStepBytes + (((l >> 5) ^ ((l >> 1) & 7)) << 4);
         } else if constexpr (sizeof(T) == 4) {
             off[0] = static_cast<uint32_t>(4 * (l >> 5)) * kRowBytes + 4u * static_cast<uint32_t>(first + (l & 31));
         } else {
@@ -387,7 +401,7 @@ struct Reader {
 #pragma unroll
         for (int i = 0; i < kCount; ++i) {
             if constexpr (!kAcross) {
-                o[i] = *reinterpret_cast<const u32x4_t*>(from + i * 32 * kStepBytes + (off[0] ^ (quarter << (kHalves ? 4 : 5))));
+                o[i] = *reinterpret_cast<const u32x4_t*>(from + i * 32 * kStepBytes + (off[0] ^ (quarter << 5)));
             } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -405,23 +419,25 @@ struct Reader {
 };
 
 // The scales of kCount tiles of 32 rows of 4-bit values: of each step, the
-// four of this lane's row and half of the wave in one word.
+// four of this lane's row and half of the wave in one word. 32 rows' are two
+// lines (where they lay with their rows, each in a line of its own, a step's
+// loads of scales took the caches longer than those of its codes).
 template <int kCount>
 struct RowScales {
     const uint8_t* base;
+    int64_t step_bytes;
     uint32_t off[kCount];
-    __device__ __forceinline__ void init(const uint8_t* p, int64_t stride, int64_t first, int64_t count, int l) {
+    __device__ __forceinline__ void init(const uint8_t* p, int64_t first, int64_t count, int step0, int l) {
         const int64_t from = min(first, count - 1);  // rows past the end take the last one's
-        base = p + from * stride + 4 * (l >> 5);
+        step_bytes = 8 * count;
+        base = p + step0 * step_bytes + 8 * from + 4 * (l >> 5);
 #pragma unroll
-        for (int i = 0; i < kCount; ++i)
-            off[i] = static_cast<uint32_t>(min(first + 32 * i + (l & 31), count - 1) - from) * static_cast<uint32_t>(stride);
+        for (int i = 0; i < kCount; ++i) off[i] = static_cast<uint32_t>(min(first + 32 * i + (l & 31), count - 1) - from) * 8u;
     }
-    // past the end of the sum codes are zeros; scales there, which may be
-    // anything, are taken for zeros too (NaN would reach the sums)
-    __device__ __forceinline__ void load(int s, uint32_t mask, uint32_t (&v)[kCount]) const {
+    __device__ __forceinline__ void load(int s, uint32_t (&v)[kCount]) const {
+        const uint8_t* from = base + s * step_bytes;
 #pragma unroll
-        for (int i = 0; i < kCount; ++i) v[i] = *reinterpret_cast<const uint32_t*>(base + off[i] + 8 * s) & mask;
+        for (int i = 0; i < kCount; ++i) v[i] = *reinterpret_cast<const uint32_t*>(from + off[i]);
     }
 };
 
@@ -525,9 +541,11 @@ __device__ __forceinline__ void tile_product(unsigned char* lds, const Product& 
     constexpr int kMfmas = IM * IN * (sizeof(Op) == 4 ? 4 : 1);
     constexpr int kReads = IM * decltype(reader_a)::kReads + IN * decltype(reader_b)::kReads;
     constexpr int kBetween = (kReads + kMfmas - 1) / kMfmas;
-    // Scales of the step that is multiplied, of the next one and of the one
-    // after it, whose loads are issued before that step's parts, so that they
-    // are there when these are waited for and no wait grows by them.
+    // Scales of the step that is multiplied, of the next one and, on their way,
+    // of the one after it: these loads are issued before that step's parts, so
+    // they are there when the parts are waited for and no wait grows by them.
+    // Past the last step they are loaded again: a branch here would divide the
+    // loop, and its products would be moved behind the meeting.
     struct Scales {
         uint32_t a[IM], b[IN];
     };
@@ -535,16 +553,27 @@ __device__ __forceinline__ void tile_product(unsigned char* lds, const Product& 
     RowScales<IM> scales_a;
     RowScales<IN> scales_b;
     auto load_scales = [&](int s, Scales& to) {
-        if (!kScaled || s >= steps) return;
-        const int blocks = s < whole ? 4 : min(max(left / 16 - 4 * (l >> 5), 0), 4);
-        const uint32_t mask = blocks == 4 ? ~0u : (1u << (8 * blocks)) - 1u;
-        scales_a.load(step0 + s, mask, to.a);
-        scales_b.load(step0 + s, mask, to.b);
+        scales_a.load(min(s, steps - 1), to.a);
+        scales_b.load(min(s, steps - 1), to.b);
+        asm volatile("" ::: "memory");
+    };
+    // Said to be read here: a copy that the loop carries would be made before
+    // they have come, and wait.
+    auto take_scales = [&](const Scales& from, Scales& to) {
+        auto take = [&](uint32_t v) {
+            uint32_t t;
+            asm volatile("v_mov_b32 %0, %1" : "=v"(t) : "v"(v) : "memory");
+            return t;
+        };
+#pragma unroll
+        for (int i = 0; i < IM; ++i) to.a[i] = take(from.a[i]);
+#pragma unroll
+        for (int j = 0; j < IN; ++j) to.b[j] = take(from.b[j]);
     };
     if constexpr (kScaled) {
-        scales_a.init(p.a_scales, p.a_scales_stride, m0 + wm * TM, p.m, l);
-        scales_b.init(p.b_scales, p.b_scales_stride, n0 + wn * TN, p.n, l);
-        load_scales(0, scales);
+        scales_a.init(p.a_scales, m0 + wm * TM, p.m, step0, l);
+        scales_b.init(p.b_scales, n0 + wn * TN, p.n, step0, l);
+        load_scales(0, next_scales);
         load_scales(1, far_scales);
     }
     auto multiply = [&](const Operands& o, auto quarter) {
@@ -600,13 +629,14 @@ __device__ __forceinline__ void tile_product(unsigned char* lds, const Product& 
         wait_and_meet<kUnderWay + kPair>();
     else
         wait_and_meet<0>();
+    if constexpr (kScaled) take_scales(next_scales, scales);
     read(0, 0, even);
     int s = 0;
     for (; s + kSlotsA < whole; ++s) {
         quarters(s);
         wait_and_meet<kUnderWay>();
         if constexpr (kScaled) {
-            next_scales = far_scales;
+            take_scales(far_scales, next_scales);
             load_scales(s + 2, far_scales);
         }
         side_b.fetch(s + kSlotsB, ring_b + s % kSlotsB * SideB::kBytes, true, left, l);
@@ -620,7 +650,7 @@ __device__ __forceinline__ void tile_product(unsigned char* lds, const Product& 
         quarters(s);
         wait_and_meet<0>();
         if constexpr (kScaled) {
-            next_scales = far_scales;
+            take_scales(far_scales, next_scales);
             load_scales(s + 2, far_scales);
         }
         fetch_b(s + kSlotsB);

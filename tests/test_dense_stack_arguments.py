@@ -94,20 +94,25 @@ for call in (write, read):
     rc(1, "overlaps", lambda: call(codes=M + 64))
     rc(1, "overlaps", lambda: call(scales=M + 64))
 rc(1, "codes overlaps scales", lambda: write(scales=2 * M + 16))
-s = op.LinearShape(100, 64, 32, 2, 0, 2, 1)
+short = op.LinearShape(100, 64, 129, 2, 0, 2, 1)
 need = C.c_size_t()
+rc(1, "128", L.chimera_mx4_linear_workspace, C.byref(short), C.byref(need))
+short.out_features = 128
+assert L.chimera_mx4_linear_workspace(C.byref(short), C.byref(need)) == 0 and need.value == 0  # quantised on its way
+s = op.LinearShape(3000, 64, 544, 2, 0, 2, 0)
 assert L.chimera_mx4_linear_workspace(C.byref(s), C.byref(need)) == 0 and need.value > 0
-f = op.Mx4LinearArgs(M, 2 * M, 3 * M, 4 * M, 5 * M, 6 * M, 64, 32, 32, 7 * M, need.value)
+M = 1 << 24
+f = op.Mx4LinearArgs(M, 2 * M, 3 * M, 4 * M, 5 * M, 6 * M, 64, 544, 544, 7 * M, need.value)
 layer = lambda: L.chimera_mx4_linear_device(ctx.handle, C.byref(s), C.byref(f))
 for field, value, word in (("rows", -1, "negative row"), ("in_features", 0, "features"), ("in_features", 65537, "features"),
-                           ("out_features", 129, "128"), ("type", 3, "type"), ("out_type", 1, "output"),
+                           ("normalize", 1, "128"), ("type", 3, "type"), ("out_type", 1, "output"),
                            ("activation", 5, "activation"), ("normalize", 2, "normalize"), ("rows", 1 << 32, "too many rows")):
     refuses(layer, s, field, value, word)
 for field in ("x", "codes", "scales", "y"):
     refuses(layer, f, field, None, "null argument: " + field)
 for field, v in (("x", M + 1), ("codes", M + 8), ("scales", M + 4), ("bias", M + 1), ("residual", M + 1), ("y", M + 2)):
     refuses(layer, f, field, v, field + " is not aligned")
-for field, v in (("x_stride", 63), ("y_stride", 31), ("residual_stride", 31), ("y_stride", 1 << 61)):
+for field, v in (("x_stride", 63), ("y_stride", 543), ("residual_stride", 543), ("y_stride", 1 << 61)):
     refuses(layer, f, field, v, "row stride of " + field[:-7])
 refuses(layer, f, "workspace", None, "workspace", 4)
 refuses(layer, f, "workspace_bytes", 10, "workspace", 4)
@@ -242,7 +247,7 @@ raises(ValueError, op.Mx4Linear, ctx, codes, scales, 64, activation="swish")
 raises(ValueError, op.Mx4Linear, ctx, codes, scales, 64, type="int4")
 raises(ValueError, op.Mx4Linear, ctx, codes, scales, 64, bias=e((100,), np.float32))
 raises(capi.ChimeraError, op.Mx4Linear, ctx, e((129, 32), np.uint8), e((129, 8), np.uint8), 64, normalize=True)
-layer = op.Mx4Linear(ctx, codes, scales, 64, max_rows=100)
+layer = op.Mx4Linear(ctx, codes, scales, 64, max_rows=8000)
 out = e((100, 100), np.float32)
 layer.forward(x, out)
 raises(ValueError, layer.forward, y, out)
@@ -250,8 +255,11 @@ raises(ValueError, layer.forward, x, y)
 raises(ValueError, layer.forward, x, out, residual=out)
 raises(capi.ChimeraError, layer.forward, x, e((100, 100), np.float16))
 assert "workspace" in raises(capi.ChimeraError, layer.forward, many[0], e((9000, 100), np.float32))
+eight = e((8000, 64), "bf16"), e((8000, 100), np.float32)
+layer.forward(*eight)
 layer.close()
-assert "workspace" in raises(capi.ChimeraError, layer.forward, x, out)
+assert "workspace" in raises(capi.ChimeraError, layer.forward, *eight)
+layer.forward(x, out)  # needs none
 # orthogonal update
 raises(ValueError, op.OrthogonalUpdate, ctx, 32, 64, type="int8")
 raises(ValueError, op.OrthogonalUpdate, ctx, (1 << 32) + 32, 64)
