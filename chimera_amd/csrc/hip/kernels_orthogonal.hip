@@ -47,13 +47,6 @@ __device__ __forceinline__ void store_pairs(const Pairs& m, int64_t row, int col
     *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(hi);
     *reinterpret_cast<u32x4_t*>(to + 32) = *reinterpret_cast<const u32x4_t*>(lo);
 }
-__device__ __forceinline__ void load_pairs(const Pairs& m, int64_t row, int col, float (&v)[8]) {
-    const unsigned char* from = m.p + row * m.stride + pair_chunk(col);
-    const f16x8_t hi = *reinterpret_cast<const f16x8_t*>(from), lo = *reinterpret_cast<const f16x8_t*>(from + 32);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = (to_float(hi[i]) + to_float(lo[i])) * kUnscale;
-}
-
 // ---- what goes before the products ---------------------------------------------
 
 struct Update {
@@ -105,50 +98,64 @@ __global__ __launch_bounds__(256) void orthogonal_update_kernel(Update a) {
     if (threadIdx.x == 0) a.parts[blockIdx.x] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
 }
 
-// A tile of 64 x 64 values as pairs: rows [row0, row0 + 64) of `along` from
-// column col0 on, and the transposed tile of `across`. Columns up to the end of
-// a step are written, from values that are zeros there.
-constexpr int kTilePitch = 65;
-template <int kThreads>
+// A tile of values as pairs: rows [row0, row0 + rows) of `along` from column
+// col0 on, and the transposed tile of `across`. Columns up to the end of a step
+// are written, from values that are zeros there.
+template <int BM, int BN, int kThreads>
 __device__ __forceinline__ void put_tile(const float* tile, int rows, int cols, const Pairs& along, int64_t row0,
                                          const Pairs& across, int64_t col0) {
-    for (int i = static_cast<int>(threadIdx.x); i < 64 * 8; i += kThreads) {
-        const int r = i / 8, c = i % 8 * 8;
-        float v[8];
-        if (along.p && r < rows && c < (cols + 31) / 32 * 32) {
+    constexpr int kPitch = BN + 1;
+    const int wide = (cols + 31) / 32 * 32, high = (rows + 31) / 32 * 32;
+    if (along.p) {
+        for (int i = static_cast<int>(threadIdx.x); i < BM * BN / 8; i += kThreads) {
+            const int r = i / (BN / 8), c = i % (BN / 8) * 8;
+            if (r >= rows || c >= wide) continue;
+            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tile[r * kTilePitch + c + j];
+            for (int j = 0; j < 8; ++j) v[j] = tile[r * kPitch + c + j];
             store_pairs(along, row0 + r, static_cast<int>(col0) + c, v);
         }
-        if (across.p && r < cols && c < (rows + 31) / 32 * 32) {
+    }
+    if (across.p) {
+        for (int i = static_cast<int>(threadIdx.x); i < BM * BN / 8; i += kThreads) {
+            const int c = i / (BM / 8), r = i % (BM / 8) * 8;
+            if (c >= cols || r >= high) continue;
+            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tile[(c + j) * kTilePitch + r];
-            store_pairs(across, col0 + r, static_cast<int>(row0) + c, v);
+            for (int j = 0; j < 8; ++j) v[j] = tile[(r + j) * kPitch + c];
+            store_pairs(across, col0 + c, static_cast<int>(row0) + r, v);
         }
     }
 }
 
+constexpr int kMostBlocks = 256;  // of the update, whose sums a block of the scaling adds up
+
 // X = U / |U| as pairs, along and across; a U of zeros stays zeros.
 __global__ __launch_bounds__(256) void orthogonal_scale_kernel(const float* u, const double* parts, int count, int rows,
                                                                int cols, Pairs along, Pairs across) {
-    __shared__ float tile[64 * kTilePitch];
+    constexpr int kPitch = 65;
+    __shared__ float tile[64 * kPitch];
     __shared__ double sums[4];
-    double sum = 0.0;
-    for (int i = static_cast<int>(threadIdx.x); i < count; i += 256) sum += parts[i];
+    const int row0 = static_cast<int>(blockIdx.y) * 64, col0 = static_cast<int>(blockIdx.x) * 64;
+    const int r0 = static_cast<int>(threadIdx.x) / 8, c0 = static_cast<int>(threadIdx.x) % 8 * 8;
+    float v[2][8] = {};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (row0 + r0 + 32 * i < rows && col0 + c0 < cols)
+            load8(u + static_cast<int64_t>(row0 + r0 + 32 * i) * cols + col0 + c0, cols - col0 - c0, v[i]);
+    double sum = static_cast<int>(threadIdx.x) < count ? parts[threadIdx.x] : 0.0;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
     if (lane_id() == 0) sums[wave_id()] = sum;
     __syncthreads();
     sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
     const double by = sum == 0.0 ? 0.0 : 1.0 / sqrt(sum);
-    const int row0 = static_cast<int>(blockIdx.y) * 64, col0 = static_cast<int>(blockIdx.x) * 64;
-    for (int i = static_cast<int>(threadIdx.x); i < 64 * 64; i += 256) {
-        const int r = i / 64, c = i % 64;
-        const bool in = row0 + r < rows && col0 + c < cols;
-        tile[r * kTilePitch + c] = in ? static_cast<float>(u[static_cast<int64_t>(row0 + r) * cols + col0 + c] * by) : 0.0f;
-    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) tile[(r0 + 32 * i) * kPitch + c0 + j] = static_cast<float>(v[i][j] * by);
     __syncthreads();
-    put_tile<256>(tile, min(64, rows - row0), min(64, cols - col0), along, row0, across, col0);
+    put_tile<64, 64, 256>(tile, min(64, rows - row0), min(64, cols - col0), along, row0, across, col0);
 }
 
 // ---- products ------------------------------------------------------------------
@@ -175,123 +182,341 @@ struct Schulz {
     Finish f;
 };
 
-template <typename T>
-__device__ __forceinline__ void put_as(void* p, int64_t at, float v) {
-    static_cast<T*>(p)[at] = from_float<T>(v);
-}
-__device__ __forceinline__ void put(void* p, int64_t at, float v, int type) {
-    if (type == CHIMERA_F32)
-        put_as<float>(p, at, v);
-    else if (type == CHIMERA_F16)
-        put_as<_Float16>(p, at, v);
-    else
-        put_as<__bf16>(p, at, v);
+// Which tile of a symmetric result the t-th on and below the diagonal is.
+__device__ __forceinline__ void below_diagonal(int t, int* tm, int* tn) {
+    int m = static_cast<int>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
+    while ((m + 1) * (m + 2) / 2 <= t) ++m;
+    while (m * (m + 1) / 2 > t) --m;
+    *tm = m;
+    *tn = t - m * (m + 1) / 2;
 }
 
-// C = P Q^T of pairs on a tile of 64 x 64, four waves, the operands straight
-// to a ring of LDS slots. C becomes from_by F + sum_by C, stored along and
-// across; of the symmetric results only tiles on and below the diagonal are
-// computed.
-constexpr int kSlots = 4;
+// Eight neighbours of a row of the result.
+template <typename T>
+__device__ __forceinline__ void put8(const Finish& f, int64_t row, int64_t col, int count, const float (&v)[8]) {
+    if (f.out) {
+        if (f.out_f32)
+            store8(static_cast<float*>(f.out) + row * f.out_stride + col, count, v);
+        else
+            store8(static_cast<T*>(f.out) + row * f.out_stride + col, count, v);
+    }
+    if (f.weight) {
+        float w[8];
+        load8(f.weight + row * f.weight_stride + col, count, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = fmaf(f.keep, w[j], -f.rate * v[j]);
+        store8(f.new_weight + row * f.new_weight_stride + col, count, w);
+        if (f.rounded) store8(static_cast<T*>(f.rounded) + row * f.rounded_stride + col, count, w);
+    }
+}
+__device__ __forceinline__ void finish8(const Finish& f, int64_t row, int64_t col, int count, const float (&v)[8]) {
+    switch (f.type) {
+        case CHIMERA_F32: put8<float>(f, row, col, count, v); break;
+        case CHIMERA_F16: put8<_Float16>(f, row, col, count, v); break;
+        default: put8<__bf16>(f, row, col, count, v);
+    }
+}
+
 template <Kind kKind>
-__global__ __launch_bounds__(256) void orthogonal_tile_kernel(Schulz a) {
-    using Part = Side<float, 64, 4, false>;
-    constexpr int kRing = kSlots * 2 * Part::kBytes;
-    static_assert(kRing >= 64 * kTilePitch * 4, "the tile goes through the ring's memory");
-    __shared__ __align__(1024) unsigned char lds[kRing];
-    const Product& p = a.p;
-    const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
+constexpr bool kSymmetric = kKind == kGram || kKind == kSquare;
+
+struct Place {
     int tm, tn;
-    if constexpr (kKind == kGram || kKind == kSquare) {
-        const int id = static_cast<int>(blockIdx.x);
-        tm = static_cast<int>((sqrtf(8.0f * static_cast<float>(id) + 1.0f) - 1.0f) * 0.5f);
-        while ((tm + 1) * (tm + 2) / 2 <= id) ++tm;
-        while (tm * (tm + 1) / 2 > id) --tm;
-        tn = id - tm * (tm + 1) / 2;
+};
+
+// Blocks go round the 8 XCDs; each takes a run of tiles, so that an L2 holds what
+// its blocks share.
+template <Kind kKind>
+__device__ __forceinline__ Place place(const Schulz& a) {
+    const int id = static_cast<int>(blockIdx.x), xcd = id % 8, tiles = static_cast<int>(gridDim.x);
+    const int tile = xcd * (tiles / 8) + min(xcd, tiles % 8) + id / 8;
+    Place o;
+    if constexpr (kSymmetric<kKind>) {
+        below_diagonal(tile, &o.tm, &o.tn);
     } else {
-        tm = static_cast<int>(blockIdx.x) % p.tiles_m;
-        tn = static_cast<int>(blockIdx.x) / p.tiles_m;
+        o.tm = tile % a.p.tiles_m;
+        o.tn = tile / a.p.tiles_m;
     }
-    const int64_t m0 = tm * 64ll, n0 = tn * 64ll;
-    Part side_a, side_b;
-    side_a.init(p.a, p.a_stride, m0, p.m, 0, w, l);
-    side_b.init(p.b, p.b_stride, n0, p.n, 0, w, l);
-    Reader<float, 1, false, kStepBytes> reader_a, reader_b;
-    reader_a.init(w / 2 * 32, l);
-    reader_b.init(w % 2 * 32, l);
-    auto fetch = [&](int s) {
-        unsigned char* to = lds + s % kSlots * 2 * Part::kBytes;
-        side_a.fetch(s, to, true, 0, l);
-        side_b.fetch(s, to + Part::kBytes, true, 0, l);
-    };
-    f32x16_t acc = {};
-    auto step = [&](int s) {
-        const unsigned char* from = lds + s % kSlots * 2 * Part::kBytes;
-        u32x4_t x[4][1], y[4][1];
+    return o;
+}
+
+// A tile's result from the sums in LDS, of kSums equal parts: C = from_by F +
+// sum_by C, stored along and across. A thread takes eights of a row; F's are
+// loaded before the sums are there.
+template <Kind kKind, int B, int kSums, int kThreads>
+struct Result {
+    static constexpr int kPitch = B + 4, kTurned = B + 1, kSumBytes = kSums * B * kPitch * 4;
+    static constexpr int kBytes = kSumBytes + B * kTurned * 4;
+    static constexpr int kEights = (B * B / 8 + kThreads - 1) / kThreads;
+    static constexpr bool kAdds = kKind != kGram;
+    int rows, cols;
+    int64_t m0, n0;
+    f16x8_t hi[kEights], lo[kEights];
+
+    __device__ __forceinline__ int row(int i) const { return (i * kThreads + static_cast<int>(threadIdx.x)) / (B / 8); }
+    __device__ __forceinline__ int col(int i) const { return (i * kThreads + static_cast<int>(threadIdx.x)) % (B / 8) * 8; }
+    __device__ __forceinline__ void init(const Schulz& a, const Place& at) {
+        m0 = static_cast<int64_t>(at.tm) * B;
+        n0 = static_cast<int64_t>(at.tn) * B;
+        rows = static_cast<int>(min(a.p.m - m0, int64_t{B}));
+        cols = static_cast<int>(min(a.p.n - n0, int64_t{B}));
+    }
+    __device__ __forceinline__ void load(const Schulz& a) {
+        if constexpr (kAdds) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            reader_a.read(from, q, x[q]);
-            reader_b.read(from + Part::kBytes, q, y[q]);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; q += 2) {
-            acc = mma32<_Float16>(y[q + 1][0], x[q][0], acc);
-            acc = mma32<_Float16>(y[q][0], x[q + 1][0], acc);
-            acc = mma32<_Float16>(y[q][0], x[q][0], acc);
-        }
-    };
-    const int steps = p.steps;
-    for (int s = 0; s < kSlots - 1 && s < steps; ++s) fetch(s);
-    int s = 0;
-    for (; s + kSlots - 1 < steps; ++s) {
-        wait_and_meet<(kSlots - 2) * 2 * Part::kLoads>();
-        fetch(s + kSlots - 1);
-        step(s);
-    }
-    for (; s < steps; ++s) {
-        wait_and_meet<0>();
-        step(s);
-    }
-    __syncthreads();
-    float* tile = reinterpret_cast<float*>(lds);
-    const int rows = static_cast<int>(min(p.m - m0, int64_t{64})), cols = static_cast<int>(min(p.n - n0, int64_t{64}));
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int i = w / 2 * 32 + (l & 31), j = w % 2 * 32 + 8 * (r >> 2) + 4 * (l >> 5) + (r & 3);
-        tile[i * kTilePitch + j] = i < rows && j < cols ? acc[r] * a.sum_by : 0.0f;
-    }
-    __syncthreads();
-    if constexpr (kKind != kGram) {
-        for (int i = static_cast<int>(threadIdx.x); i < 64 * 8; i += 256) {
-            const int r = i / 8, c = i % 8 * 8;
-            if (r >= rows || c >= cols) continue;
-            float v[8];
-            load_pairs(a.from, m0 + r, static_cast<int>(n0) + c, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) tile[r * kTilePitch + c + j] = fmaf(a.from_by, v[j], tile[r * kTilePitch + c + j]);
-        }
-        __syncthreads();
-    }
-    if constexpr (kKind != kLast) {
-        Pairs across = a.across;
-        if ((kKind == kGram || kKind == kSquare) && tm == tn) across.p = nullptr;
-        put_tile<256>(tile, rows, cols, a.along, m0, across, n0);
-    } else {
-        const Finish& f = a.f;
-        for (int i = static_cast<int>(threadIdx.x); i < 64 * 64; i += 256) {
-            // neighbouring threads write neighbouring columns of the results
-            const int r = f.turned ? i % 64 : i / 64, c = f.turned ? i / 64 : i % 64;
-            if (r >= rows || c >= cols) continue;
-            const float v = tile[r * kTilePitch + c];
-            const int64_t row = f.turned ? n0 + c : m0 + r, col = f.turned ? m0 + r : n0 + c;
-            if (f.out) put(f.out, row * f.out_stride + col, v, f.out_f32 ? CHIMERA_F32 : f.type);
-            if (f.weight) {
-                const float next = fmaf(f.keep, f.weight[row * f.weight_stride + col], -f.rate * v);
-                f.new_weight[row * f.new_weight_stride + col] = next;
-                if (f.rounded) put(f.rounded, row * f.rounded_stride + col, next, f.type);
+            for (int i = 0; i < kEights; ++i) {
+                hi[i] = lo[i] = f16x8_t{};
+                if (row(i) < rows && col(i) < cols) {
+                    const unsigned char* from = a.from.p + (m0 + row(i)) * a.from.stride + pair_chunk(static_cast<int>(n0) + col(i));
+                    hi[i] = *reinterpret_cast<const f16x8_t*>(from);
+                    lo[i] = *reinterpret_cast<const f16x8_t*>(from + 32);
+                }
             }
         }
     }
+    // 16 values of a lane: of row `row` of the tile and of part `sum`
+    static __device__ __forceinline__ void put(unsigned char* lds, int sum, int row, int col0, const f32x16_t& v) {
+        float* to = reinterpret_cast<float*>(lds) + (sum * B + row) * kPitch + col0 + 4 * (lane_id() >> 5);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<f32x4_t*>(to + 8 * q) = f32x4_t{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+    }
+    __device__ __forceinline__ void store(const Schulz& a, const Place& at, unsigned char* lds) const {
+        const float* sums = reinterpret_cast<const float*>(lds);
+        float* turned = reinterpret_cast<float*>(lds + kSumBytes);
+        const bool across = kKind == kLast ? a.f.turned : !(kSymmetric<kKind> && at.tm == at.tn);
+        const int wide = (cols + 31) / 32 * 32, high = (rows + 31) / 32 * 32;
+#pragma unroll
+        for (int i = 0; i < kEights; ++i) {
+            const int r = row(i), c = col(i);
+            if (r >= high) break;
+            float v[8] = {};
+#pragma unroll
+            for (int o = 0; o < kSums; ++o) {
+                const f32x4_t* from = reinterpret_cast<const f32x4_t*>(sums + (o * B + r) * kPitch + c);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] += from[j / 4][j % 4];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] *= a.sum_by;
+                if constexpr (kAdds) v[j] = fmaf(a.from_by * kUnscale, to_float(hi[i][j]) + to_float(lo[i][j]), v[j]);
+                v[j] = r < rows && c + j < cols ? v[j] : 0.0f;
+            }
+            if constexpr (kKind == kLast) {
+                if (!across && r < rows && c < cols) finish8(a.f, m0 + r, n0 + c, cols - c, v);
+            } else {
+                if (r < rows && c < wide) store_pairs(a.along, m0 + r, static_cast<int>(n0) + c, v);
+            }
+            if (across) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) turned[r * kTurned + c + j] = v[j];
+            }
+        }
+        if (!across) return;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kEights; ++i) {
+            const int c = row(i), r = col(i);
+            if (c >= cols || r >= high) continue;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = turned[(r + j) * kTurned + c];
+            if constexpr (kKind == kLast) {
+                if (r < rows) finish8(a.f, n0 + c, m0 + r, rows - r, v);
+            } else {
+                store_pairs(a.across, n0 + c, static_cast<int>(m0) + r, v);
+            }
+        }
+    }
+};
+
+// The parts of a half step that a wave multiplies: I x J tiles of 32 x 32.
+template <int I, int J>
+struct Halves {
+    u32x4_t ah[I], al[I], bh[J], bl[J];
+
+    __device__ __forceinline__ void multiply(f32x16_t (&acc)[I][J]) const {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    acc[i][j] = mma32<_Float16>(k == 1 ? bl[j] : bh[j], k == 0 ? al[i] : ah[i], acc[i][j]);
+        // with the reads of the half step after it in between
+        constexpr int kMfmas = 3 * I * J, kReads = 2 * (I + J), kPer = (kReads + kMfmas - 1) / kMfmas;
+#pragma unroll
+        for (int g = 0; g < kReads / kPer; ++g) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, kPer, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
+// Until at most kUnderWay of this wave's loads are under way and its LDS reads have come.
+template <int kUnderWay>
+__device__ __forceinline__ void arrived() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt((kUnderWay & 15) | (kUnderWay >> 4 << 14) | (7 << 4));
+    asm volatile("" ::: "memory");
+}
+
+// C = P Q^T of pairs on a tile of B x B, for results of few tiles. Each of four
+// waves takes the whole tile and every fourth step of the sum, with LDS slots of
+// its own that the operands go straight to, so that the loop has no meeting, and
+// half a step's parts, upper and lower, are read while the half before it is
+// multiplied. Of the symmetric results only tiles on and below the diagonal are
+// computed. A step of a tile of 64 is 256 cycles of loads into LDS (64 bytes a
+// cycle) and of LDS reads, and 96 of the matrix cores; a launch of these sizes
+// is bound by its first loads and its stores (2 us each).
+template <Kind kKind, int B, int kSlots>
+__global__ __launch_bounds__(256) void orthogonal_few_kernel(Schulz a) {
+    constexpr int kWaves = 4, I = B / 32;
+    using Part = Side<float, B, 1, false>;
+    using End = Result<kKind, B, kWaves, 256>;
+    constexpr int kSlot = 2 * Part::kBytes, kLoads = 2 * Part::kLoads, kRings = kWaves * kSlots * kSlot;
+    __shared__ __align__(1024) unsigned char lds[kRings > End::kBytes ? kRings : End::kBytes];
+    const Product& p = a.p;
+    const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
+    const Place at = place<kKind>(a);
+    End end;
+    end.init(a, at);
+    const int steps = (p.steps - w + kWaves - 1) / kWaves;  // of this wave
+    Part side_a, side_b;
+    side_a.init(p.a, p.a_stride, end.m0, p.m, w, 0, l);
+    side_b.init(p.b, p.b_stride, end.n0, p.n, w, 0, l);
+    Reader<float, I, false, kStepBytes> reader;
+    reader.init(0, l);
+    unsigned char* const ring = lds + w * kSlots * kSlot;
+    auto fetch = [&](int s) {
+        unsigned char* to = ring + s % kSlots * kSlot;
+        side_a.fetch(kWaves * s, to, true, 0, l);
+        side_b.fetch(kWaves * s, to + Part::kBytes, true, 0, l);
+    };
+    auto read = [&](int s, int h, Halves<I, I>& o) {
+        const unsigned char* from = ring + s % kSlots * kSlot;
+        reader.read(from, 2 * h + 1, o.al);
+        reader.read(from + Part::kBytes, 2 * h, o.bh);
+        reader.read(from, 2 * h, o.ah);
+        reader.read(from + Part::kBytes, 2 * h + 1, o.bl);
+    };
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+        if (s < steps) fetch(s);
+    end.load(a);
+    f32x16_t acc[I][I];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < I; ++j) acc[i][j] = f32x16_t{};
+    if (steps > 0) {
+        Halves<I, I> even, odd;
+        arrived<0>();
+        read(0, 0, even);
+        int s = 0;
+        for (; s + kSlots < steps; ++s) {
+            read(s, 1, odd);
+            even.multiply(acc);
+            arrived<63>();  // the reads: the slot takes new loads
+            fetch(s + kSlots);
+            arrived<(kSlots - 1) * kLoads>();  // the next step's loads
+            read(s + 1, 0, even);
+            odd.multiply(acc);
+        }
+        for (; s < steps; ++s) {
+            read(s, 1, odd);
+            even.multiply(acc);
+            arrived<0>();
+            if (s + 1 < steps) read(s + 1, 0, even);
+            odd.multiply(acc);
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < I; ++j) End::put(lds, w, 32 * i + (l & 31), 32 * j, acc[i][j]);
+    __syncthreads();
+    end.store(a, at, lds);
+}
+
+// The same for many tiles: the block's WM x WN waves divide the tile and share a
+// ring of kSlots slots, with one meeting a step. The loads of a step are issued
+// in two halves between the products.
+template <Kind kKind, int B, int WM, int WN, int kSlots>
+__global__ __launch_bounds__(WM* WN* kWave) void orthogonal_tile_kernel(Schulz a) {
+    constexpr int W = WM * WN, TM = B / WM, TN = B / WN, I = TM / 32, J = TN / 32;
+    using Part = Side<float, B, W, false>;
+    using End = Result<kKind, B, 1, W * kWave>;
+    constexpr int kSlot = 2 * Part::kBytes, kLoads = 2 * Part::kLoads, kRing = kSlots * kSlot;
+    __shared__ __align__(1024) unsigned char lds[kRing > End::kBytes ? kRing : End::kBytes];
+    const Product& p = a.p;
+    const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id()), wm = w / WN, wn = w % WN;
+    const Place at = place<kKind>(a);
+    End end;
+    end.init(a, at);
+    const int steps = p.steps;
+    Part side_a, side_b;
+    side_a.init(p.a, p.a_stride, end.m0, p.m, 0, w, l);
+    side_b.init(p.b, p.b_stride, end.n0, p.n, 0, w, l);
+    Reader<float, I, false, kStepBytes> reader_a;
+    Reader<float, J, false, kStepBytes> reader_b;
+    reader_a.init(wm * TM, l);
+    reader_b.init(wn * TN, l);
+    auto fetch_a = [&](int s) { side_a.fetch(s, lds + s % kSlots * kSlot, true, 0, l); };
+    auto fetch_b = [&](int s) { side_b.fetch(s, lds + s % kSlots * kSlot + Part::kBytes, true, 0, l); };
+    auto read = [&](int s, int h, Halves<I, J>& o) {
+        const unsigned char* from = lds + s % kSlots * kSlot;
+        reader_a.read(from, 2 * h, o.ah);
+        reader_b.read(from + Part::kBytes, 2 * h, o.bh);
+        reader_a.read(from, 2 * h + 1, o.al);
+        reader_b.read(from + Part::kBytes, 2 * h + 1, o.bl);
+    };
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s) {
+        if (s < steps) fetch_a(s);
+        if (s + 1 < kSlots && s < steps) fetch_b(s);
+    }
+    if (steps >= kSlots)
+        wait_and_meet<(kSlots - 2) * kLoads + Part::kLoads>();
+    else
+        wait_and_meet<0>();
+    f32x16_t acc[I][J];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[i][j] = f32x16_t{};
+    Halves<I, J> even, odd;
+    read(0, 0, even);
+    int s = 0;
+    for (; s + kSlots < steps; ++s) {
+        fetch_b(s + kSlots - 1);
+        read(s, 1, odd);
+        even.multiply(acc);
+        wait_and_meet<(kSlots - 2) * kLoads>();
+        fetch_a(s + kSlots);
+        read(s + 1, 0, even);
+        odd.multiply(acc);
+        __builtin_amdgcn_s_waitcnt(kWaitLds);
+    }
+    end.load(a);
+    for (; s < steps; ++s) {
+        if (s + kSlots - 1 < steps) fetch_b(s + kSlots - 1);
+        read(s, 1, odd);
+        even.multiply(acc);
+        wait_and_meet<0>();
+        if (s + 1 < steps) read(s + 1, 0, even);
+        odd.multiply(acc);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < J; ++j) End::put(lds, 0, wm * TM + 32 * i + (l & 31), wn * TN + 32 * j, acc[i][j]);
+    __syncthreads();
+    end.store(a, at, lds);
 }
 
 // ---- plan ----------------------------------------------------------------------
@@ -308,7 +533,7 @@ size_t carve(const chimera_orthogonal_shape& s, void* base, Plan* plan) {
     const int m = std::min(s.rows, s.cols), k = std::max(s.rows, s.cols);
     plan->m = m;
     plan->k = k;
-    plan->blocks = static_cast<int>(std::min<int64_t>(ceil_div(static_cast<int64_t>(s.rows) * ceil_div(s.cols, 8), 256), 1024));
+    plan->blocks = static_cast<int>(std::min<int64_t>(ceil_div(static_cast<int64_t>(s.rows) * ceil_div(s.cols, 8), 256), kMostBlocks));
     auto pairs = [&](int rows, int cols) {
         const int64_t stride = ceil_div(cols, 32) * 128;
         return Pairs{static_cast<unsigned char*>(c.take(static_cast<size_t>(rows) * stride)), stride};
@@ -333,11 +558,31 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
     a.p.m = m;
     a.p.n = n;
     a.p.steps = static_cast<int>(ceil_div(sum, 32));
-    a.p.tiles_m = static_cast<int>(ceil_div(m, 64));
-    a.p.tiles_n = static_cast<int>(ceil_div(n, 64));
     a.sum_by *= kUnscaleSum;
-    const int tiles = kKind == kGram || kKind == kSquare ? a.p.tiles_m * (a.p.tiles_m + 1) / 2 : a.p.tiles_m * a.p.tiles_n;
-    hipLaunchKernelGGL((orthogonal_tile_kernel<kKind>), dim3(static_cast<unsigned>(tiles)), dim3(256), 0, st, a);
+    auto tiles_of = [&](int tile) {
+        a.p.tiles_m = static_cast<int>(ceil_div(m, tile));
+        a.p.tiles_n = static_cast<int>(ceil_div(n, tile));
+        return kSymmetric<kKind> ? int64_t{a.p.tiles_m} * (a.p.tiles_m + 1) / 2 : int64_t{a.p.tiles_m} * a.p.tiles_n;
+    };
+    auto launch = [&](auto kernel, int tile, int threads) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_of(tile))), dim3(static_cast<unsigned>(threads)), 0, st, a);
+    };
+    // As long as each CU has at most one block of four waves that divide the sum
+    // (tiles of 32 take two for X), that kernel; then tiles of 64, and of 128 once
+    // they fill the CUs. us of A, B and X: 128 x 768 6.5, 4.3, 4.3; 512 x 2048 9.8,
+    // 5.9, 10.8 (64: 17.9, 9.4, 10.7); 1024 x 1024 11.6, 12.4, 13.8 (32: 19, 21, 23;
+    // shared tiles of 64: 11.9, 13.0, 14.8); 1024 x 4096 27.8, 12.0, 34.5 (X in
+    // tiles of 64 38 and, by four waves that divide the sum, 48; A in four parts
+    // of its sum and their join 25 and 5); 4096 x 4096 274, 290, 428.
+    if (tiles_of(32) <= (kSymmetric<kKind> ? 256 : 400)) {
+        launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 4 : 2>, 32, 256);
+    } else if (tiles_of(64) <= kCus) {
+        launch(orthogonal_few_kernel<kKind, 64, 2>, 64, 256);
+    } else if (tiles_of(128) < 224) {
+        launch(orthogonal_tile_kernel<kKind, 64, 2, 2, 4>, 64, 256);
+    } else {
+        launch(orthogonal_tile_kernel<kKind, 128, 2, 4, 4>, 128, 512);
+    }
 }
 
 }  // namespace
