@@ -106,25 +106,21 @@ __device__ __forceinline__ void put_tile(const float* tile, int rows, int cols, 
                                          const Pairs& across, int64_t col0) {
     constexpr int kPitch = BN + 1;
     const int wide = (cols + 31) / 32 * 32, high = (rows + 31) / 32 * 32;
-    if (along.p) {
-        for (int i = static_cast<int>(threadIdx.x); i < BM * BN / 8; i += kThreads) {
-            const int r = i / (BN / 8), c = i % (BN / 8) * 8;
-            if (r >= rows || c >= wide) continue;
-            float v[8];
+    for (int i = static_cast<int>(threadIdx.x); i < BM * BN / 8; i += kThreads) {
+        const int r = i / (BN / 8), c = i % (BN / 8) * 8;
+        if (r >= rows || c >= wide) continue;
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tile[r * kPitch + c + j];
-            store_pairs(along, row0 + r, static_cast<int>(col0) + c, v);
-        }
+        for (int j = 0; j < 8; ++j) v[j] = tile[r * kPitch + c + j];
+        store_pairs(along, row0 + r, static_cast<int>(col0) + c, v);
     }
-    if (across.p) {
-        for (int i = static_cast<int>(threadIdx.x); i < BM * BN / 8; i += kThreads) {
-            const int c = i / (BM / 8), r = i % (BM / 8) * 8;
-            if (c >= cols || r >= high) continue;
-            float v[8];
+    for (int i = static_cast<int>(threadIdx.x); i < BM * BN / 8; i += kThreads) {
+        const int c = i / (BM / 8), r = i % (BM / 8) * 8;
+        if (c >= cols || r >= high) continue;
+        float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = tile[(r + j) * kPitch + c];
-            store_pairs(across, col0 + c, static_cast<int>(row0) + r, v);
-        }
+        for (int j = 0; j < 8; ++j) v[j] = tile[(r + j) * kPitch + c];
+        store_pairs(across, col0 + c, static_cast<int>(row0) + r, v);
     }
 }
 
