@@ -359,19 +359,21 @@ __device__ __forceinline__ void arrived() {
     asm volatile("" ::: "memory");
 }
 
-// C = P Q^T of pairs on a tile of B x B, for results of few tiles. Each of four
-// waves takes the whole tile and every fourth step of the sum, with LDS slots of
-// its own that the operands go straight to, so that the loop has no meeting, and
-// half a step's parts, upper and lower, are read while the half before it is
-// multiplied. Of the symmetric results only tiles on and below the diagonal are
-// computed. A step of a tile of 64 is 256 cycles of loads into LDS (64 bytes a
-// cycle) and of LDS reads, and 96 of the matrix cores; a launch of these sizes
-// is bound by its first loads and its stores (2 us each).
-template <Kind kKind, int B, int kSlots>
-__global__ __launch_bounds__(256) void orthogonal_few_kernel(Schulz a) {
-    constexpr int kWaves = 4, I = B / 32;
+// C = P Q^T of pairs on a tile of B x B, for results of few tiles. Each of kWaves
+// waves takes the whole tile and every kWaves-th step of the sum, with LDS slots
+// of its own that the operands go straight to, so that the loop has no meeting.
+// With two slots half a step's parts, upper and lower, are read while the half
+// before it is multiplied; with one a step is read, and the next one's loads
+// pass under its products. Of the symmetric results only tiles on and below the
+// diagonal are computed. A step of a tile of 64 is 256 cycles of loads into LDS
+// (64 bytes a cycle) and 96 of the matrix cores. 1024 x 1024 x 1024 takes 9 us
+// in its blocks: 2 until the first loads are there, 4.3 of loop (50 bytes a
+// cycle), 0.6 for the sums and 1.5 for what is stored.
+template <Kind kKind, int B, int kWaves, int kSlots>
+__global__ __launch_bounds__(kWaves* kWave) void orthogonal_few_kernel(Schulz a) {
+    constexpr int I = B / 32;
     using Part = Side<float, B, 1, false>;
-    using End = Result<kKind, B, kWaves, 256>;
+    using End = Result<kKind, B, kWaves, kWaves * kWave>;
     constexpr int kSlot = 2 * Part::kBytes, kLoads = 2 * Part::kLoads, kRings = kWaves * kSlots * kSlot;
     __shared__ __align__(1024) unsigned char lds[kRings > End::kBytes ? kRings : End::kBytes];
     const Product& p = a.p;
@@ -398,10 +400,10 @@ __global__ __launch_bounds__(256) void orthogonal_few_kernel(Schulz a) {
         reader.read(from, 2 * h, o.ah);
         reader.read(from + Part::kBytes, 2 * h + 1, o.bl);
     };
+    end.load(a);
 #pragma unroll
     for (int s = 0; s < kSlots; ++s)
         if (s < steps) fetch(s);
-    end.load(a);
     f32x16_t acc[I][I];
 #pragma unroll
     for (int i = 0; i < I; ++i)
@@ -409,17 +411,24 @@ __global__ __launch_bounds__(256) void orthogonal_few_kernel(Schulz a) {
         for (int j = 0; j < I; ++j) acc[i][j] = f32x16_t{};
     if (steps > 0) {
         Halves<I, I> even, odd;
-        arrived<0>();
+        if (steps >= kSlots)
+            arrived<(kSlots - 1) * kLoads>();
+        else
+            arrived<0>();
         read(0, 0, even);
         int s = 0;
         for (; s + kSlots < steps; ++s) {
             read(s, 1, odd);
-            even.multiply(acc);
+            if constexpr (kSlots > 1) even.multiply(acc);
             arrived<63>();  // the reads: the slot takes new loads
             fetch(s + kSlots);
+            if constexpr (kSlots == 1) {
+                even.multiply(acc);
+                odd.multiply(acc);
+            }
             arrived<(kSlots - 1) * kLoads>();  // the next step's loads
             read(s + 1, 0, even);
-            odd.multiply(acc);
+            if constexpr (kSlots > 1) odd.multiply(acc);
         }
         for (; s < steps; ++s) {
             read(s, 1, odd);
@@ -563,17 +572,20 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
     auto launch = [&](auto kernel, int tile, int threads) {
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_of(tile))), dim3(static_cast<unsigned>(threads)), 0, st, a);
     };
-    // As long as each CU has at most one block of four waves that divide the sum
-    // (tiles of 32 take two for X), that kernel; then tiles of 64, and of 128 once
-    // they fill the CUs. us of A, B and X: 128 x 768 6.5, 4.3, 4.3; 512 x 2048 9.8,
-    // 5.9, 10.8 (64: 17.9, 9.4, 10.7); 1024 x 1024 11.6, 12.4, 13.8 (32: 19, 21, 23;
-    // shared tiles of 64: 11.9, 13.0, 14.8); 1024 x 4096 27.8, 12.0, 34.5 (X in
-    // tiles of 64 38 and, by four waves that divide the sum, 48; A in four parts
-    // of its sum and their join 25 and 5); 4096 x 4096 274, 290, 428.
+    // As long as each CU has at most one block whose waves divide the sum (of
+    // tiles of 32 for X, two), that kernel; then tiles of 64, and of 128 once they
+    // fill the CUs. us of A, B and X: 128 x 768 5.9, 3.8, 4.1; 512 x 2048 9.5, 5.7,
+    // 10.3 (in tiles of 64 17.9, 9.4, 10.7); 1024 x 1024 11.0, 12.3, 13.7 (tiles of
+    // 32 19, 21, 23; shared tiles of 64 11.9, 13.0, 14.8); 1024 x 4096 27.4, 11.4,
+    // 35.0 (X in tiles of 64 38, by waves that divide the sum 48; A in four parts
+    // of its sum 25 and 5 for their join); 4096 x 4096 274, 290, 428, which is
+    // 1,000 TF of products, with a plain fp16 product's 1,300 in reach.
+    // Eight waves a tile of 32 take 0.3 us less for A and B and 0.3 more for X.
     if (tiles_of(32) <= (kSymmetric<kKind> ? 256 : 400)) {
-        launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 4 : 2>, 32, 256);
+        launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 8 : 4, kSymmetric<kKind> ? 1 : 2>, 32,
+               kSymmetric<kKind> ? 512 : 256);
     } else if (tiles_of(64) <= kCus) {
-        launch(orthogonal_few_kernel<kKind, 64, 2>, 64, 256);
+        launch(orthogonal_few_kernel<kKind, 64, 4, 2>, 64, 256);
     } else if (tiles_of(128) < 224) {
         launch(orthogonal_tile_kernel<kKind, 64, 2, 2, 4>, 64, 256);
     } else {
