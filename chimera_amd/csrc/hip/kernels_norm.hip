@@ -210,7 +210,8 @@ __global__ __launch_bounds__(block_threads(kLanes)) void norm_forward_kernel(Nor
                 }
             row_sums<kLanes>(s, lds);
             rest = s[0] * inv;
-            var = fmaf(-rest, rest, s[1] * inv);
+            // of rows of one value: what rounding leaves of it is no deviation
+            var = fmaxf(fmaf(-rest, rest, s[1] * inv), rest * rest * 0x1p-18f);
             return s[1] - s[1] == 0.0f;  // neither infinite nor NaN
         };
         float scale = 1.0f;
@@ -226,10 +227,11 @@ __global__ __launch_bounds__(block_threads(kLanes)) void norm_forward_kernel(Nor
             }
             (void)moments();
         }
-        const float rstd = 1.0f / sqrtf(var + a.eps * scale * scale), by = -rest * rstd;
+        const float spread = var + a.eps * scale * scale;  // 0 for scaled rows of one value
+        const float rstd = spread == 0.0f ? 0.0f : 1.0f / sqrtf(spread), by = -rest * rstd;
         if (at.t == 0) {
             if (a.mean) a.mean[r] = (mean + rest) * (scale == 1.0f ? 1.0f : kLarge);
-            if (a.rstd) a.rstd[r] = rstd * scale;
+            if (a.rstd) a.rstd[r] = spread == 0.0f ? 1.0f / sqrtf(a.eps) : rstd * scale;
         }
         Out* to = static_cast<Out*>(a.y) + r * a.y_stride;
 #pragma unroll

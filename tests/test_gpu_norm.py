@@ -182,6 +182,30 @@ def test_rows_far_from_zero_and_near_the_ends_of_the_range(n):
     c.close()
 
 
+@pytest.mark.parametrize("eps", [1e-5, 1e-30])
+@pytest.mark.parametrize("n", [5, 96, 1000, 3000, 30_000])
+def test_rows_of_one_value(n, eps):
+    """x - mean is what the mean's rounding left out, the same in all columns,
+    and its mean is within D u of it, so z, over a deviation of at least 2^-9 of
+    that, is below D u 2^9 + 2^-15 < 2^-8. Gradients are finite."""
+    rng = np.random.default_rng(n)
+    values = [0.0, 1.0, 12345.678, -3e6, 1e8, 1.7e19, 3e30, 2.0**115, 1e36, 2.0**127, 3e38, -3.4e38, 1e-30, 1e-42]
+    x = to_type(np.repeat(np.array(values)[:, None], n, 1), "f32")
+    w, b = to_type(1 + 0.3 * rng.standard_normal(n), "f32"), to_type(rng.standard_normal(n), "f32")
+    dy = to_type(rng.standard_normal(x.shape), "f32")
+    c = Case(x, w, b, dy, "f32", "f32", eps=eps)
+    c.forward()
+    c.backward()
+    assert (np.abs(c.value("y") - b) <= 2.0**-8 * np.abs(w) + U * np.abs(b)).all()
+    assert np.isfinite(c.value("dx")).all() and np.isfinite(c.value("dw")).all()
+    rstd = 1 / np.sqrt(np.float64(np.float32(eps)))
+    near = np.abs(x[:, 0]) <= 1e-30  # the others' means may be a rounding off, and eps below its square
+    have = c.value("rstd").ravel()
+    assert (np.abs(have - rstd)[near] <= 2.0**-20 * rstd).all()
+    assert (have > 0).all() and (have <= rstd * (1 + 2.0**-20)).all()
+    c.close()
+
+
 @pytest.mark.parametrize("type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("n", [40, 300, 5000])
 def test_rows_that_are_not_finite_stay_apart(type, n):
