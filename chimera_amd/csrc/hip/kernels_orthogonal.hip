@@ -35,14 +35,16 @@ struct Pairs {
 __device__ __forceinline__ int64_t pair_chunk(int col) {  // the bytes of eight upper parts; the lower ones are 32 on
     return static_cast<int64_t>(col / 32) * 128 + (col & 16) * 4 + (col & 8) * 2;
 }
+typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
+    const float s = v * kPairScale;
+    hi = from_float<_Float16>(s);
+    lo = from_float<_Float16>(s - to_float(hi));
+}
 __device__ __forceinline__ void store_pairs(const Pairs& m, int64_t row, int col, const float (&v)[8]) {
     _Float16 hi[8], lo[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float s = v[i] * kPairScale;
-        hi[i] = from_float<_Float16>(s);
-        lo[i] = from_float<_Float16>(s - to_float(hi[i]));
-    }
+    for (int i = 0; i < 8; ++i) split(v[i], hi[i], lo[i]);
     unsigned char* to = m.p + row * m.stride + pair_chunk(col);
     *reinterpret_cast<u32x4_t*>(to) = *reinterpret_cast<const u32x4_t*>(hi);
     *reinterpret_cast<u32x4_t*>(to + 32) = *reinterpret_cast<const u32x4_t*>(lo);
@@ -175,6 +177,7 @@ struct Schulz {
     Pairs along;    // the result
     Pairs across;   // its transpose
     float from_by, sum_by;
+    float linear_by, square_by;  // B = linear_by A + square_by A^2, where a kernel makes it itself
     Finish f;
 };
 
@@ -447,6 +450,95 @@ __global__ __launch_bounds__(kWaves* kWave) void orthogonal_few_kernel(Schulz a)
     end.store(a, at, lds);
 }
 
+// X' = a X + B X for a shorter side of at most 128 with B = b A + c A^2 made on
+// the way, which saves a launch: 5 us where the two take 8. A block takes 32 x 32 of X'; a wave makes 32
+// columns of B's 32 rows, whose places in the lanes are, after one exchange of
+// the half waves, those of the next product's operand: its 32 values of the sum.
+template <Kind kKind>
+__global__ __launch_bounds__(256) void orthogonal_both_kernel(Schulz a) {
+    constexpr int B = 32, kSteps = 4;  // a wave each
+    using Part = Side<float, B, 1, false>;
+    using End = Result<kKind, B, kSteps, 256>;
+    constexpr int kShared = kSteps * Part::kBytes, kOwn = (kSteps + 1) * Part::kBytes, kAll = kShared + kSteps * kOwn;
+    __shared__ __align__(1024) unsigned char lds[kAll > End::kBytes ? kAll : End::kBytes];
+    const Product& p = a.p;
+    const int l = lane_id(), half = l >> 5, w = __builtin_amdgcn_readfirstlane(wave_id());
+    const Place at = place<kKind>(a);
+    End end;
+    end.init(a, at);
+    end.load(a);
+    unsigned char* const own = lds + kShared + w * kOwn;
+    const bool works = w < p.steps;
+    if (works) {
+        Part rows, columns, values;
+        rows.init(p.a, p.a_stride, end.m0, p.m, 0, 0, l);
+        rows.fetch(w, lds + w * Part::kBytes, true, 0, l);
+        columns.init(p.a, p.a_stride, 32 * w, p.m, 0, 0, l);
+        for (int s = 0; s < p.steps; ++s) columns.fetch(s, own + s * Part::kBytes, true, 0, l);
+        values.init(p.b, p.b_stride, end.n0, p.n, 0, 0, l);
+        values.fetch(w, own + kSteps * Part::kBytes, true, 0, l);
+    }
+    __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // all loads
+    __syncthreads();
+    Reader<float, 1, false, kStepBytes> reader;
+    reader.init(0, l);
+    f32x16_t acc[1][1] = {};
+    if (works) {
+        Halves<1, 1> even, odd, x[2];
+        auto read = [&](int s, int h, Halves<1, 1>& o) {
+            reader.read(lds + s * Part::kBytes, 2 * h + 1, o.al);
+            reader.read(own + s * Part::kBytes, 2 * h, o.bh);
+            reader.read(lds + s * Part::kBytes, 2 * h, o.ah);
+            reader.read(own + s * Part::kBytes, 2 * h + 1, o.bl);
+        };
+        read(0, 0, even);
+        for (int s = 0; s < p.steps; ++s) {
+            read(s, 1, odd);
+            even.multiply(acc);
+            if (s + 1 < p.steps) read(s + 1, 0, even);
+            odd.multiply(acc);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            reader.read(own + kSteps * Part::kBytes, 2 * h, x[h].bh);
+            reader.read(own + kSteps * Part::kBytes, 2 * h + 1, x[h].bl);
+        }
+        // this lane's values of B: row l % 32, columns 8 q + 4 half + i of the step
+        uint32_t hi[8], lo[8];
+        const unsigned char* from = lds + w * Part::kBytes + (l & 31) * kStepBytes;
+        const int turn = ((l & 31) >> 1) & 7;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            // eights 0 and 1 of the upper parts, of the lower ones, then 2 and 3
+            const int chunk = q / 2 * 4 + q % 2;
+            const f16x4_t ah = *reinterpret_cast<const f16x4_t*>(from + ((chunk ^ turn) << 4) + 8 * half);
+            const f16x4_t al = *reinterpret_cast<const f16x4_t*>(from + (((chunk + 2) ^ turn) << 4) + 8 * half);
+            _Float16 h[4], r[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                split(fmaf(a.square_by, acc[0][0][4 * q + i], a.linear_by * (to_float(ah[i]) + to_float(al[i]))), h[i], r[i]);
+            __builtin_memcpy(&hi[2 * q], h, 8);
+            __builtin_memcpy(&lo[2 * q], r, 8);
+        }
+        acc[0][0] = f32x16_t{};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            auto operand = [&](const uint32_t* u) {
+                const auto x = __builtin_amdgcn_permlane32_swap(u[4 * h], u[4 * h + 2], false, false);
+                const auto y = __builtin_amdgcn_permlane32_swap(u[4 * h + 1], u[4 * h + 3], false, false);
+                return u32x4_t{x[0], y[0], x[1], y[1]};
+            };
+            x[h].ah[0] = operand(hi);
+            x[h].al[0] = operand(lo);
+            x[h].multiply(acc);
+        }
+    }
+    __syncthreads();
+    End::put(lds, w, l & 31, 0, acc[0][0]);
+    __syncthreads();
+    end.store(a, at, lds);
+}
+
 // The same for many tiles: the block's WM x WN waves divide the tile and share a
 // ring of kSlots slots, with one meeting a step. The loads of a step are issued
 // in two halves between the products.
@@ -554,16 +646,36 @@ size_t carve(const chimera_orthogonal_shape& s, void* base, Plan* plan) {
     return c.off;
 }
 
+void operands(Schulz* a, const Pairs& p, int64_t m, const Pairs& q, int n, int sum) {
+    a->p.a = p.p;
+    a->p.a_stride = p.stride;
+    a->p.b = q.p;
+    a->p.b_stride = q.stride;
+    a->p.m = m;
+    a->p.n = n;
+    a->p.steps = static_cast<int>(ceil_div(sum, 32));
+    a->sum_by *= kUnscaleSum;
+}
+
+// Whether X' = a X + B X makes B itself: a block more for each 32 x 32 of X makes
+// all of its rows, which pays while each CU has one. All five steps of 64 x 64
+// take 64 us with two launches and 47 so, 128 x 768 78 and 62, 128 x 2048 93
+// and 78.
+bool both_at_once(int m, int k) { return m <= 128 && ceil_div(m, 32) * ceil_div(k, 32) <= kCus; }
+
+template <Kind kKind>
+void launch_both(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const Pairs& q, int n) {
+    operands(&a, p, m, q, n, static_cast<int>(m));
+    a.linear_by *= kUnscale;
+    a.square_by *= kUnscaleSum;
+    a.p.tiles_m = static_cast<int>(ceil_div(m, 32));
+    a.p.tiles_n = static_cast<int>(ceil_div(n, 32));
+    hipLaunchKernelGGL((orthogonal_both_kernel<kKind>), dim3(static_cast<unsigned>(a.p.tiles_m * a.p.tiles_n)), dim3(256), 0, st, a);
+}
+
 template <Kind kKind>
 void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const Pairs& q, int n, int sum) {
-    a.p.a = p.p;
-    a.p.a_stride = p.stride;
-    a.p.b = q.p;
-    a.p.b_stride = q.stride;
-    a.p.m = m;
-    a.p.n = n;
-    a.p.steps = static_cast<int>(ceil_div(sum, 32));
-    a.sum_by *= kUnscaleSum;
+    operands(&a, p, m, q, n, sum);
     auto tiles_of = [&](int tile) {
         a.p.tiles_m = static_cast<int>(ceil_div(m, tile));
         a.p.tiles_n = static_cast<int>(ceil_div(n, tile));
@@ -578,8 +690,8 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
     // 10.3 (in tiles of 64 17.9, 9.4, 10.7); 1024 x 1024 11.0, 12.3, 13.7 (tiles of
     // 32 19, 21, 23; shared tiles of 64 11.9, 13.0, 14.8); 1024 x 4096 27.4, 11.4,
     // 35.0 (X in tiles of 64 38, by waves that divide the sum 48; A in four parts
-    // of its sum 25 and 5 for their join); 4096 x 4096 274, 290, 428, which is
-    // 1,000 TF of products, with a plain fp16 product's 1,300 in reach.
+    // of its sum 25 and 5 for their join); 4096 x 4096 274, 290, 428 (960 TF of
+    // products, a plain fp16 product reaches 1,300).
     // Eight waves a tile of 32 take 0.3 us less for A and B and 0.3 more for X.
     if (tiles_of(32) <= (kSymmetric<kKind> ? 256 : 400)) {
         launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 8 : 4, kSymmetric<kKind> ? 1 : 2>, 32,
@@ -634,20 +746,28 @@ hipError_t launch_orthogonal(hipStream_t st, const chimera_orthogonal_shape& s, 
         gram.along = gram.across = plan.a;
         gram.sum_by = 1.0f;
         launch_product<kGram>(st, gram, x, plan.m, x, plan.m, plan.k);
-        Schulz square = {};
-        square.from = plan.a;
-        square.from_by = s.b;
-        square.sum_by = s.c;
-        square.along = square.across = plan.b;
-        launch_product<kSquare>(st, square, plan.a, plan.m, plan.a, plan.m, plan.m);
+        const bool both = both_at_once(plan.m, plan.k);
+        if (!both) {
+            Schulz square = {};
+            square.from = plan.a;
+            square.from_by = s.b;
+            square.sum_by = s.c;
+            square.along = square.across = plan.b;
+            launch_product<kSquare>(st, square, plan.a, plan.m, plan.a, plan.m, plan.m);
+        }
         Schulz apply = {};
         apply.from = x;
         apply.from_by = s.a;
         apply.sum_by = 1.0f;
         apply.along = plan.x[1 - i % 2];
         apply.across = plan.xt[1 - i % 2];
+        apply.linear_by = s.b;
+        apply.square_by = s.c;
         if (i + 1 < s.steps) {
-            launch_product<kApply>(st, apply, plan.b, plan.m, xt, plan.k, plan.m);
+            if (both)
+                launch_both<kApply>(st, apply, plan.a, plan.m, xt, plan.k);
+            else
+                launch_product<kApply>(st, apply, plan.b, plan.m, xt, plan.k, plan.m);
             continue;
         }
         Finish& f = apply.f;
@@ -664,7 +784,10 @@ hipError_t launch_orthogonal(hipStream_t st, const chimera_orthogonal_shape& s, 
         f.type = s.type;
         f.out_f32 = s.out_type == CHIMERA_F32;
         f.turned = turned;
-        launch_product<kLast>(st, apply, plan.b, plan.m, xt, plan.k, plan.m);
+        if (both)
+            launch_both<kLast>(st, apply, plan.a, plan.m, xt, plan.k);
+        else
+            launch_product<kLast>(st, apply, plan.b, plan.m, xt, plan.k, plan.m);
     }
     return hipGetLastError();
 }

@@ -67,9 +67,13 @@ for rows, cols, symmetric, x in {UPDATES}:
     bytes = need(L.chimera_orthogonal_workspace, C.byref(s))
     a = op.OrthogonalArgs(gradient=A, out=2 * A, gradient_stride=cols, out_stride=cols, workspace=3 * A, workspace_bytes=bytes)
     capi.check(L.chimera_orthogonal_update_device(ctx.handle, C.byref(s), C.byref(a)))
-    for kind, kernel, count in ((0, symmetric, 2), (1, symmetric, 2), (2, x, 1), (3, x, 1)):
+    both = x == "both"
+    for kind in (2, 3):
+        assert launches(f"orthogonal_both_kernelILNS0_4KindE{{kind}}E") == int(both), (rows, cols)
+    for kind, kernel, count in ((0, symmetric, 2), (1, symmetric, 2), (2, x, 1), (3, x, 1))[:1 if both else 4]:
         name = f"orthogonal_{{kernel[0]}}_kernelILNS0_4KindE{{kind}}E" + numbers(kernel[1:])
         assert launches(name) == count, (rows, cols, name)
+    assert launches("orthogonal_") == 2 + (4 if both else 6), (rows, cols)
 """)
 
 
@@ -83,4 +87,4 @@ def test_every_kernel_has_a_shape(host_hip):  # noqa: F811
                       ("walk", 8, 8, 1)} | {("walk", s, 4, 1) for s in (1, 2, 3, 4, 8)} | {("walk", s, 8, 2) for s in (1, 2, 3, 4)}
     few, tiles = {("few", 64, 4, 2)}, {("tile", 64, 2, 2, 4), ("tile", 128, 2, 4, 4)}
     assert {s for *_, s, _ in UPDATES} == few | tiles | {("few", 32, 8, 1)}
-    assert {x for *_, x in UPDATES} == few | tiles | {("few", 32, 4, 2)}
+    assert {x for *_, x in UPDATES} == few | tiles | {("few", 32, 4, 2), "both"}
