@@ -100,24 +100,7 @@ __device__ __forceinline__ float gelu_16(float z) {
     return z * (z > 0.0f ? 1.0f - tail : tail);
 }
 
-// The same with P of degree 7, within 2^-17 of the size down to -6: for sums of
-// 4-bit values, whose rounding to 16 bits is seldom another for it (about one
-// fp16 result in a hundred). Three instructions less: 65,536 x 4096 outputs of
-// such a layer 316 -> 302 us.
-__device__ __forceinline__ float gelu_short(float z) {
-    const float a = fabsf(z);
-    float p = fmaf(-1.8348062e-6f, a, 6.1598182e-5f);
-    p = fmaf(p, a, -9.3052391e-4f);
-    p = fmaf(p, a, 8.5078869e-3f);
-    p = fmaf(p, a, -5.3960058e-2f);
-    p = fmaf(p, a, -4.5846441e-1f);
-    p = fmaf(p, a, -1.1512511f);
-    p = fmaf(p, a, -0.99999529f);
-    const float tail = __builtin_amdgcn_exp2f(p);
-    return z * (z > 0.0f ? 1.0f - tail : tail);
-}
-
-constexpr int kRoundedGelu = -1, kShortGelu = -2;  // gelu_16 and gelu_short for CHIMERA_ACT_GELU
+constexpr int kRoundedGelu = -1;  // gelu_16 for CHIMERA_ACT_GELU
 
 __device__ __forceinline__ float activation(float z, int act) {
     switch (act) {
@@ -127,7 +110,6 @@ __device__ __forceinline__ float activation(float z, int act) {
             return z * normal_cdf(z, &gauss);
         }
         case kRoundedGelu: return gelu_16(z);
-        case kShortGelu: return gelu_short(z);
         case CHIMERA_ACT_GELU_TANH:  // (1 + tanh u) / 2 is the sigmoid of 2 u
             return z * sigmoid(2.0f * kGeluTanhC * fmaf(kGeluTanhA * z * z, z, z));
         case CHIMERA_ACT_SILU: return z * sigmoid(z);

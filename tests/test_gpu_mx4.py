@@ -4,6 +4,8 @@ them against its definition in 64 bits.
 Tolerances of the layer: products of codes are exact, so a sum of n of them in
 32 bits is within n 2^-23 of the sum of their magnitudes; activations and the
 rounding as for the dense layer."""
+import math
+
 import numpy as np
 import pytest
 
@@ -207,6 +209,44 @@ def test_values_that_are_not_finite_stay_apart(rows, normalize):
     else:
         lost[:, 7] = True
     assert np.array_equal(np.isnan(y), lost)
+    layer.close()
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("n", [20_000, 45_000])
+def test_gelu_of_all_biases(n, type):
+    """GELU of 16-bit results, over values from -6 on: rows of zeros leave the
+    bias. Within 2^-17 of its size and half a step of f16, 2^-14 and half a step
+    of bf16, on few columns and on many; past -6 below 1e-8."""
+    b = np.arange(1 << 16, dtype=np.uint16)
+    b = (b.view(np.float16) if type == "f16" else (b.astype(np.uint32) << 16).view(np.float32)).astype(np.float64)
+    b = np.sort(b[np.isfinite(b) & (b >= -3e4) & (np.abs(b) >= 2.0**-14)])
+    b = b[:: max(1, -(-b.size // n))]
+    b = np.concatenate([b, np.ones(n - b.size)])
+    want = np.array([z * 0.5 * math.erfc(-z / math.sqrt(2)) for z in b])
+    x, w = np.zeros((1, 32)), np.ones((n, 32))
+    layer = Layer(x, w, b, None, type, type, "gelu", False)
+    layer.forward()
+    off = np.abs(layer.d["y"].values()[0] - want)
+    bound = (2.0**-17 + 2.0**-11 if type == "f16" else 2.0**-14 + 2.0**-8) * np.abs(want) + (2.0**-25 if type == "f16" else 0)
+    assert (off <= np.where(b >= -6, bound, 1e-8 + bound)).all()
+    layer.close()
+
+
+@pytest.mark.parametrize("type", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [2, 900])
+@pytest.mark.parametrize("act", ["relu", "gelu", "gelu_tanh", "silu"])
+def test_activations_of_sums_that_are_not_finite(rows, type, act):
+    """Biases of NaN and both infinities: NaN stays, infinity too, and minus
+    infinity gives zero or NaN (0 times it)."""
+    b = np.array([np.nan, np.inf, -np.inf, 1.0] * 200)
+    layer = Layer(np.zeros((rows, 40)), np.ones((800, 40)), b, None, type, type, act, False)
+    layer.forward()
+    y = layer.d["y"].values().reshape(rows, 200, 4)
+    assert np.isnan(y[..., 0]).all() and np.isfinite(y[..., 3]).all()
+    if act != "gelu_tanh":  # inf / inf in its argument's cube stays NaN or infinite
+        assert (y[..., 1] == np.inf).all()
+    assert (np.isnan(y[..., 2]) | (y[..., 2] == 0)).all()
     layer.close()
 
 
