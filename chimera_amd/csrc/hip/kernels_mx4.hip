@@ -252,23 +252,34 @@ __device__ __forceinline__ void activate_few(Values& v, int act) {
     }
 }
 
-// Activation, residual, length and the stores of a tile's 32 x 32 values:
-// lane l holds row l % 32 and the columns 8 g + 4 (l / 32) + i, i < 4.
+// What is added to a tile's 32 x 32 values, where its columns are whole: loaded
+// before the products, as they take less time than a trip to memory.
 template <typename T>
-__device__ __forceinline__ void finish_tile(f32x16_t& v, const Epilogue& e, int64_t m, int n0, bool full, int half) {
+struct Residual {
+    typedef T four_t __attribute__((ext_vector_type(4)));
+    four_t r[4];
+
+    __device__ __forceinline__ void load(const Epilogue& e, int64_t m, int n0, int half) {
+        typedef four_t any_t __attribute__((aligned(sizeof(T))));
+        const T* from = static_cast<const T*>(e.residual) + min(m, e.m - 1) * e.residual_stride + n0 + 4 * half;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) r[g] = *reinterpret_cast<const any_t*>(from + 8 * g);
+    }
+};
+
+// Activation, residual and the stores of a tile's 32 x 32 values: lane l holds
+// row l % 32 and the columns 8 g + 4 (l / 32) + i, i < 4.
+template <typename T>
+__device__ __forceinline__ void finish_tile(f32x16_t& v, const Epilogue& e, const Residual<T>& added, int64_t m, int n0,
+                                            bool full, int half) {
     activate_few<T>(v, e.act);
     if (m >= e.m) return;
     if (e.residual) {
-        const T* from = static_cast<const T*>(e.residual) + m * e.residual_stride + n0 + 4 * half;
-        typedef T four_t __attribute__((ext_vector_type(4)));
-        typedef four_t any_t __attribute__((aligned(sizeof(T))));
         if (full) {
-            four_t r[4];
 #pragma unroll
-            for (int g = 0; g < 4; ++g) r[g] = *reinterpret_cast<const any_t*>(from + 8 * g);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] += to_float(static_cast<T>(r[j / 4][j % 4]));
+            for (int j = 0; j < 16; ++j) v[j] += to_float(static_cast<T>(added.r[j / 4][j % 4]));
         } else {
+            const T* from = static_cast<const T*>(e.residual) + m * e.residual_stride + n0 + 4 * half;
 #pragma unroll
             for (int j = 0; j < 16; ++j)
                 if (n0 + 8 * (j / 4) + 4 * half + j % 4 < e.n) v[j] += to_float(from[8 * (j / 4) + j % 4]);
@@ -433,12 +444,6 @@ __global__ __launch_bounds__(kWaves* kWave) void mx4_walk_kernel(Mx4Args a, Epil
             quarter(std::integral_constant<int, 3>{});
         }
     };
-    auto finish = [&](int tile) {
-#pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            finish_tile<T>(acc[u], e, (tile * int64_t{kUnits} + u) * 32 + (l & 31), n0, full, half);
-        }
-    };
     const bool narrow = sizeof(T) == 2 && !e.out_f32;
     for (int tile = first; tile < last; ++tile) {
         // the stores of a whole tile come after the loads that are waited for
@@ -453,8 +458,15 @@ __global__ __launch_bounds__(kWaves* kWave) void mx4_walk_kernel(Mx4Args a, Epil
         asm volatile("" ::: "memory");
         if (tile + 1 < last) fetch(tile + 1);
         if (!works) continue;
+        Residual<T> added[kUnits];
+        const int64_t row = tile * int64_t{kUnits} * 32 + (l & 31);
+        if (e.residual && full) {
+#pragma unroll
+            for (int u = 0; u < kUnits; ++u) added[u].load(e, row + 32 * u, n0, half);
+        }
         multiply(lds + (tile - first) % 2 * kTileBytes);
-        finish(tile);
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) finish_tile<T>(acc[u], e, added[u], row + 32 * u, n0, full, half);
     }
 }
 
