@@ -248,7 +248,8 @@ struct Result {
     static constexpr int kBytes = kSumBytes + B * kTurned * 4;
     static constexpr int kEights = (B * B / 8 + kThreads - 1) / kThreads;
     static constexpr bool kAdds = kKind != kGram;
-    int rows, cols;
+    int rows, cols;  // of the tile, and with those up to the end of a step
+    int high, wide;
     int64_t m0, n0;
     f16x8_t hi[kEights], lo[kEights];
 
@@ -259,6 +260,8 @@ struct Result {
         n0 = static_cast<int64_t>(at.tn) * B;
         rows = static_cast<int>(min(a.p.m - m0, int64_t{B}));
         cols = static_cast<int>(min(a.p.n - n0, int64_t{B}));
+        high = static_cast<int>(min((a.p.m + 31) / 32 * 32 - m0, int64_t{B}));
+        wide = static_cast<int>(min((a.p.n + 31) / 32 * 32 - n0, int64_t{B}));
     }
     __device__ __forceinline__ void load(const Schulz& a) {
         if constexpr (kAdds) {
@@ -273,6 +276,10 @@ struct Result {
             }
         }
     }
+    // four neighbours of a row
+    static __device__ __forceinline__ void put(unsigned char* lds, int sum, int row, int col, const f32x4_t& v) {
+        *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(lds) + (sum * B + row) * kPitch + col) = v;
+    }
     // 16 values of a lane: of row `row` of the tile and of part `sum`
     static __device__ __forceinline__ void put(unsigned char* lds, int sum, int row, int col0, const f32x16_t& v) {
         float* to = reinterpret_cast<float*>(lds) + (sum * B + row) * kPitch + col0 + 4 * (lane_id() >> 5);
@@ -284,7 +291,6 @@ struct Result {
         const float* sums = reinterpret_cast<const float*>(lds);
         float* turned = reinterpret_cast<float*>(lds + kSumBytes);
         const bool across = kKind == kLast ? a.f.turned : !(kSymmetric<kKind> && at.tm == at.tn);
-        const int wide = (cols + 31) / 32 * 32, high = (rows + 31) / 32 * 32;
 #pragma unroll
         for (int i = 0; i < kEights; ++i) {
             const int r = row(i), c = col(i);
@@ -446,6 +452,111 @@ __global__ __launch_bounds__(kWaves* kWave) void orthogonal_few_kernel(Schulz a)
     for (int i = 0; i < I; ++i)
 #pragma unroll
         for (int j = 0; j < I; ++j) End::put(lds, w, 32 * i + (l & 31), 32 * j, acc[i][j]);
+    __syncthreads();
+    end.store(a, at, lds);
+}
+
+// The same for tiles of 48, in products of 16 x 16: of symmetric results up to 22
+// such tiles a side each CU then has one, where tiles of 64 leave half of the CUs
+// idle and load a third more for each. A step is read while the one before it is
+// multiplied.
+template <Kind kKind>
+__global__ __launch_bounds__(256) void orthogonal_few48_kernel(Schulz a) {
+    constexpr int B = 48, I = B / 16, kWaves = 4, kSlots = 3;
+    using Part = Side<float, B, 1, false>;
+    using End = Result<kKind, B, kWaves, 256>;
+    constexpr int kSlot = 2 * Part::kBytes, kLoads = 2 * Part::kLoads, kRings = kWaves * kSlots * kSlot;
+    __shared__ __align__(1024) unsigned char lds[kRings > End::kBytes ? kRings : End::kBytes];
+    const Product& p = a.p;
+    const int l = lane_id(), w = __builtin_amdgcn_readfirstlane(wave_id());
+    const Place at = place<kKind>(a);
+    End end;
+    end.init(a, at);
+    const int steps = (p.steps - w + kWaves - 1) / kWaves;  // of this wave
+    Part side_a, side_b;
+    side_a.init(p.a, p.a_stride, end.m0, p.m, w, 0, l);
+    side_b.init(p.b, p.b_stride, end.n0, p.n, w, 0, l);
+    unsigned char* const ring = lds + w * kSlots * kSlot;
+    auto fetch = [&](int s) {
+        unsigned char* to = ring + s % kSlots * kSlot;
+        side_a.fetch(kWaves * s, to, true, 0, l);
+        side_b.fetch(kWaves * s, to + Part::kBytes, true, 0, l);
+    };
+    // lane l's eight of row l % 16 is the l / 16-th of the step, upper parts
+    // here, lower ones two chunks on
+    const int group = l >> 4, place16 = ((group >> 1) * 4 + (group & 1)) ^ ((l >> 1) & 7);
+    const int off = (l & 15) * kStepBytes + (place16 << 4);
+    struct Operands {
+        u32x4_t ah[I], al[I], bh[I], bl[I];
+    };
+    auto read = [&](int s, Operands& o) {
+        const unsigned char* from = ring + s % kSlots * kSlot;
+#pragma unroll
+        for (int i = 0; i < I; ++i) {
+            const unsigned char *x = from + 16 * i * kStepBytes, *y = x + Part::kBytes;
+            o.al[i] = *reinterpret_cast<const u32x4_t*>(x + (off ^ 32));
+            o.bh[i] = *reinterpret_cast<const u32x4_t*>(y + off);
+            o.ah[i] = *reinterpret_cast<const u32x4_t*>(x + off);
+            o.bl[i] = *reinterpret_cast<const u32x4_t*>(y + (off ^ 32));
+        }
+    };
+    f32x4_t acc[I][I];
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < I; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](const Operands& o) {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+#pragma unroll
+                for (int j = 0; j < I; ++j)
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                        __builtin_bit_cast(f16x8_t, k == 1 ? o.bl[j] : o.bh[j]),
+                        __builtin_bit_cast(f16x8_t, k == 0 ? o.al[i] : o.ah[i]), acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int g = 0; g < 4 * I; ++g) {
+            __builtin_amdgcn_sched_group_barrier(kSchedMfma, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    end.load(a);
+#pragma unroll
+    for (int s = 0; s < kSlots; ++s)
+        if (s < steps) fetch(s);
+    if (steps > 0) {
+        Operands even, odd;
+        if (steps >= kSlots)
+            arrived<(kSlots - 1) * kLoads>();
+        else
+            arrived<0>();
+        read(0, even);
+        // `now` has come from LDS for step s; the next step's into `then`
+        auto turn = [&](int s, Operands& now, Operands& then) {
+            arrived<63>();  // the reads: the slot takes new loads
+            if (s + kSlots < steps) {
+                fetch(s + kSlots);
+                arrived<(kSlots - 1) * kLoads>();
+            } else {
+                arrived<0>();
+            }
+            if (s + 1 < steps) read(s + 1, then);
+            multiply(now);
+        };
+        int s = 0;
+        for (; s + 1 < steps; s += 2) {
+            turn(s, even, odd);
+            turn(s + 1, odd, even);
+        }
+        if (s < steps) turn(s, even, odd);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < I; ++i)
+#pragma unroll
+        for (int j = 0; j < I; ++j) End::put(lds, w, 16 * i + (l & 15), 16 * j + 4 * group, acc[i][j]);
     __syncthreads();
     end.store(a, at, lds);
 }
@@ -676,6 +787,8 @@ void launch_both(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const Pair
 template <Kind kKind>
 void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const Pairs& q, int n, int sum) {
     operands(&a, p, m, q, n, sum);
+    // whether tiles of 48 cover the rows' padding too
+    auto ends_with_steps = [](int64_t v) { return ceil_div(v, 48) * 48 >= ceil_div(v, 32) * 32; };
     auto tiles_of = [&](int tile) {
         a.p.tiles_m = static_cast<int>(ceil_div(m, tile));
         a.p.tiles_n = static_cast<int>(ceil_div(n, tile));
@@ -685,17 +798,21 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
         hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(tiles_of(tile))), dim3(static_cast<unsigned>(threads)), 0, st, a);
     };
     // As long as each CU has at most one block whose waves divide the sum (of
-    // tiles of 32 for X, two), that kernel; then tiles of 64, and of 128 once they
-    // fill the CUs. us of A, B and X: 128 x 768 5.9, 3.8, 4.1; 512 x 2048 9.5, 5.7,
-    // 10.3 (in tiles of 64 17.9, 9.4, 10.7); 1024 x 1024 11.0, 12.3, 13.7 (tiles of
-    // 32 19, 21, 23; shared tiles of 64 11.9, 13.0, 14.8); 1024 x 4096 27.4, 11.4,
-    // 35.0 (X in tiles of 64 38, by waves that divide the sum 48; A in four parts
-    // of its sum 25 and 5 for their join); 4096 x 4096 274, 290, 428 (960 TF of
-    // products, a plain fp16 product reaches 1,300).
-    // Eight waves a tile of 32 take 0.3 us less for A and B and 0.3 more for X.
+    // tiles of 32 for X, two), that kernel, on tiles as small as that allows; then
+    // tiles of 64 that waves share, and of 128 once they fill the CUs. us of A, B
+    // and X: 128 x 768 5.9, 3.8, 4.1; 512 x 2048 9.5, 5.7, 10.3 (in tiles of 64
+    // 17.9, 9.4, 10.7); 768 x 768 8.7, 10.8, 9.7 (64: 10.8, 12.4, 11.2); 1024 x
+    // 1024 11.1, 11.3, 13.7 (64: 11.3, 12.7; shared tiles of 64 11.9, 13.0, 14.8; 32
+    // 19, 21, 23); 1024 x 4096 23.8, 10.3, 35.0 (64: 29.0, 11.6; X in tiles of 64
+    // 38, by waves that divide the sum 48; A in four parts of its sum 25 and 5 for
+    // their join); 4096 x 4096 274, 290, 428 (960 TF of products, a plain fp16
+    // product reaches 1,300). Eight waves a tile of 32 take 0.3 us less for A and
+    // B and 0.3 more for X.
     if (tiles_of(32) <= (kSymmetric<kKind> ? 256 : 400)) {
         launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 8 : 4, kSymmetric<kKind> ? 1 : 2>, 32,
                kSymmetric<kKind> ? 512 : 256);
+    } else if (tiles_of(48) <= kCus && ends_with_steps(m) && ends_with_steps(n)) {
+        launch(orthogonal_few48_kernel<kKind>, 48, 256);
     } else if (tiles_of(64) <= kCus) {
         launch(orthogonal_few_kernel<kKind, 64, 4, 2>, 64, 256);
     } else if (tiles_of(128) < 224) {
