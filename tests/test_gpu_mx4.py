@@ -219,7 +219,8 @@ def test_gelu_of_all_biases(n, type):
     bias. Within 2^-17 of its size and half a step of f16, 2^-14 and half a step
     of bf16, on few columns and on many; past -6 below 1e-8."""
     b = np.arange(1 << 16, dtype=np.uint16)
-    b = (b.view(np.float16) if type == "f16" else (b.astype(np.uint32) << 16).view(np.float32)).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        b = (b.view(np.float16) if type == "f16" else (b.astype(np.uint32) << 16).view(np.float32)).astype(np.float64)
     b = np.sort(b[np.isfinite(b) & (b >= -3e4) & (np.abs(b) >= 2.0**-14)])
     b = b[:: max(1, -(-b.size // n))]
     b = np.concatenate([b, np.ones(n - b.size)])
