@@ -472,18 +472,18 @@ __global__ __launch_bounds__(kWaves* kWave) void mx4_walk_kernel(Mx4Args a, Epil
 
 // ---- few rows, and rows of length one ------------------------------------------
 
-// A block takes 32 rows of X and 32 kCols columns. 1,024 values of the sum at a
+// A block takes kRows rows of X and 32 kCols columns. 1,024 values of the sum at a
 // time it quantises its rows to LDS, while W's codes are on their way to the
 // registers of kSplit waves for each 32 columns, which divide the sum; the
 // parts are joined in LDS, and each wave finishes a share of the columns.
 // Bound by the latency of a trip to memory and of the meetings (one row, 1024
 // -> 4096) or, with many rows of length one, by reading X.
-template <typename T, int kCols, int kSplit, bool kNormalize>
+template <typename T, int kCols, int kSplit, bool kNormalize, int kRows = 32>
 __global__ __launch_bounds__(kCols* kSplit* kWave) void mx4_few_kernel(Mx4Args a, Epilogue e) {
     using Unit = Mx4Unit<4>;
     constexpr int kWaves = kCols * kSplit, kThreads = kWaves * kWave;
     constexpr int kChunk = 1024, kEights = kChunk / 8;  // of the sum
-    constexpr int kRound = 32 * kEights / kThreads;     // eights of a thread
+    constexpr int kRound = kRows * kEights / kThreads;  // eights of a thread
     constexpr int kShare = 16 / kSplit;                 // values of a lane that it finishes
     constexpr int kQuarters = 16 / kSplit;              // of a chunk, of a wave
     constexpr int kParts = kSplit > 1 ? kWaves * 16 * kWave * 4 : 0;
@@ -502,9 +502,9 @@ __global__ __launch_bounds__(kCols* kSplit* kWave) void mx4_few_kernel(Mx4Args a
     const int x0 = ((half ^ Unit::swizzle(l & 31)) << 4), row_at = (l & 31) * Unit::kRowBytes;
     const int row0 = t / kEights, col0 = t % kEights * 8;
     constexpr int kRowsARound = kThreads / kEights;
-    const int64_t m0 = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * 32, m = m0 + (l & 31);
+    const int64_t m0 = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kRows, m = m0 + (l & 31);
     if (m0 >= e.m) return;
-    const int rows = static_cast<int>(min(e.m - m0, int64_t{32}));
+    const int rows = static_cast<int>(min(e.m - m0, int64_t{kRows}));
     f32x16_t acc = {};
     for (int chunk = 0; chunk < a.cols; chunk += kChunk) {
         eight_t x[kRound];
@@ -565,7 +565,7 @@ __global__ __launch_bounds__(kCols* kSplit* kWave) void mx4_few_kernel(Mx4Args a
     float v[kShare];
     const int j0 = part * kShare;
     auto column = [&](int i) { return n0 + 8 * ((j0 + i) / 4) + 4 * half + (j0 + i) % 4; };
-    const bool in = m < e.m;
+    const bool in = (l & 31) < rows;
     if constexpr (kSplit > 1) {
         __syncthreads();  // the parts take the codes' place
 #pragma unroll
@@ -751,15 +751,28 @@ hipError_t walk(hipStream_t st, const chimera_linear_shape& s, const chimera_mx4
 
 template <typename T>
 hipError_t few(hipStream_t st, const chimera_linear_shape& s, const Mx4Args& g, const Epilogue& e) {
-    auto launch = [&](auto kernel, int cols, int split) {
+    auto launch = [&](auto kernel, int cols, int split, int rows = 32) {
         // the rows' tiles in two dimensions of at most 2^16 blocks
-        const int64_t tiles = ceil_div(s.rows, 32), high = ceil_div(tiles, 65535);
+        const int64_t tiles = ceil_div(s.rows, rows), high = ceil_div(tiles, 65535);
         const dim3 grid(static_cast<unsigned>(ceil_div(s.out_features, 32 * cols)), static_cast<unsigned>(ceil_div(tiles, high)),
                         static_cast<unsigned>(high));
         hipLaunchKernelGGL(kernel, grid, dim3(static_cast<unsigned>(cols * split * kWave)), 0, st, g, e);
     };
-    if (!s.normalize)
+    // Blocks of eight rows, a quarter of the products' 32, while each CU has at most
+    // one (of 512 threads, two): a block's time is that of quantising its rows. us
+    // with 8 and with 32: 32 x 768 -> 128 of length one 6.8 and 8.2, 2,048 of them
+    // 7.2 and 8.5, 4,000 11.5 and 8.4; 32 x 1024 -> 4096 6.2 and 7.4, 128 x 1024 ->
+    // 1024 6.0 and 7.4, 512 x 1024 -> 512 8.3 and 7.6.
+    const int64_t columns = s.normalize ? 1 : ceil_div(s.out_features, 32);
+    const bool eight = ceil_div(s.rows, 8) * columns <= (s.normalize ? 1 : 2) * kCus;
+    if (!s.normalize && eight)
+        launch(mx4_few_kernel<T, 1, 8, false, 8>, 1, 8, 8);
+    else if (!s.normalize)
         launch(mx4_few_kernel<T, 1, 8, false>, 1, 8);
+    else if (s.out_features > 64 && eight)
+        launch(mx4_few_kernel<T, 4, 4, true, 8>, 4, 4, 8);
+    else if (eight)
+        launch(mx4_few_kernel<T, 2, 8, true, 8>, 2, 8, 8);
     else if (s.out_features > 64 && s.rows > 32 * kCus)
         launch(mx4_few_kernel<T, 4, 1, true>, 4, 1);
     else if (s.out_features > 64)

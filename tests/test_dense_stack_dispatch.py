@@ -55,7 +55,7 @@ for rows, k, n, type, normalize, kernel in {MX4_LAYERS}:
     name = f"mx4_{{kernel[0]}}_kernelI" + NAME[type] + numbers(found)
     assert launches(name) == 1, (rows, k, n, type)
     if kernel[0] == "few":
-        assert launches(name + f"Lb{{kernel[3]}}E") == 1
+        assert launches(name + f"Lb{{kernel[3]}}ELi{{kernel[4]}}E") == 1
     assert launches("mx4_quantise_kernel") == int(kernel[0] != "few")
 """)
 
@@ -83,8 +83,8 @@ def test_every_kernel_has_a_shape(host_hip):  # noqa: F811
     assert forward == {(16, 1, 2), (16, 1, 1)} | {(64, c, f) for c in (1, 2) for f in (0, 1)} | \
         {(256, c, f) for c in (1, 2, 4) for f in (0, 1)} | {(1024, c, f) for c in (2, 4, 8) for f in (0, 1)}
     layers = {k for *_, k in MX4_LAYERS}
-    assert layers == {("few", 1, 8, 0), ("few", 4, 1, 1), ("few", 4, 4, 1), ("few", 2, 8, 1), ("tile", 64, 64), ("tile", 128, 128),
-                      ("walk", 8, 8, 1)} | {("walk", s, 4, 1) for s in (1, 2, 3, 4, 8)} | {("walk", s, 8, 2) for s in (1, 2, 3, 4)}
+    assert layers == {("few", *v, r) for v in ((1, 8, 0), (4, 4, 1), (2, 8, 1)) for r in (8, 32)} | {
+        ("few", 4, 1, 1, 32), ("tile", 64, 64), ("tile", 128, 128), ("walk", 8, 8, 1)} | {("walk", s, 4, 1) for s in (1, 2, 3, 4, 8)} | {("walk", s, 8, 2) for s in (1, 2, 3, 4)}
     few, tiles = {("few", 64, 4, 2), ("few48",)}, {("tile", 64, 2, 2, 4), ("tile", 128, 2, 4, 4)}
     assert {s for *_, s, _ in UPDATES} == few | tiles | {("few", 32, 8, 1)}
     assert {x for *_, x in UPDATES} == few | tiles | {("few", 32, 4, 2), "both"}
