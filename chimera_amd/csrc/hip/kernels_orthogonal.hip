@@ -377,12 +377,13 @@ __device__ __forceinline__ void arrived() {
 // diagonal are computed. A step of a tile of 64 is 256 cycles of loads into LDS
 // (64 bytes a cycle) and 96 of the matrix cores. 1024 x 1024 x 1024 takes 9 us
 // in its blocks: 2 until the first loads are there, 4.3 of loop (50 bytes a
-// cycle), 0.6 for the sums and 1.5 for what is stored.
-template <Kind kKind, int B, int kWaves, int kSlots>
-__global__ __launch_bounds__(kWaves* kWave) void orthogonal_few_kernel(Schulz a) {
+// cycle), and 2 for the sums and what is stored, which waves without a share of
+// the sum (kAll in all) halve.
+template <Kind kKind, int B, int kWaves, int kSlots, int kAll = kWaves>
+__global__ __launch_bounds__(kAll* kWave) void orthogonal_few_kernel(Schulz a) {
     constexpr int I = B / 32;
     using Part = Side<float, B, 1, false>;
-    using End = Result<kKind, B, kWaves, kWaves * kWave>;
+    using End = Result<kKind, B, kWaves, kAll * kWave>;
     constexpr int kSlot = 2 * Part::kBytes, kLoads = 2 * Part::kLoads, kRings = kWaves * kSlots * kSlot;
     __shared__ __align__(1024) unsigned char lds[kRings > End::kBytes ? kRings : End::kBytes];
     const Product& p = a.p;
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(kWaves* kWave) void orthogonal_few_kernel(Schulz a)
     const Place at = place<kKind>(a);
     End end;
     end.init(a, at);
-    const int steps = (p.steps - w + kWaves - 1) / kWaves;  // of this wave
+    const int steps = w < kWaves ? (p.steps - w + kWaves - 1) / kWaves : 0;  // of this wave
     Part side_a, side_b;
     side_a.init(p.a, p.a_stride, end.m0, p.m, w, 0, l);
     side_b.init(p.b, p.b_stride, end.n0, p.n, w, 0, l);
@@ -448,10 +449,12 @@ __global__ __launch_bounds__(kWaves* kWave) void orthogonal_few_kernel(Schulz a)
         }
     }
     __syncthreads();
+    if (w < kWaves) {
 #pragma unroll
-    for (int i = 0; i < I; ++i)
+        for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int j = 0; j < I; ++j) End::put(lds, w, 32 * i + (l & 31), 32 * j, acc[i][j]);
+            for (int j = 0; j < I; ++j) End::put(lds, w, 32 * i + (l & 31), 32 * j, acc[i][j]);
+    }
     __syncthreads();
     end.store(a, at, lds);
 }
@@ -461,10 +464,10 @@ __global__ __launch_bounds__(kWaves* kWave) void orthogonal_few_kernel(Schulz a)
 // idle and load a third more for each. A step is read while the one before it is
 // multiplied.
 template <Kind kKind>
-__global__ __launch_bounds__(256) void orthogonal_few48_kernel(Schulz a) {
+__global__ __launch_bounds__(512) void orthogonal_few48_kernel(Schulz a) {
     constexpr int B = 48, I = B / 16, kWaves = 4, kSlots = 3;
     using Part = Side<float, B, 1, false>;
-    using End = Result<kKind, B, kWaves, 256>;
+    using End = Result<kKind, B, kWaves, 512>;
     constexpr int kSlot = 2 * Part::kBytes, kLoads = 2 * Part::kLoads, kRings = kWaves * kSlots * kSlot;
     __shared__ __align__(1024) unsigned char lds[kRings > End::kBytes ? kRings : End::kBytes];
     const Product& p = a.p;
@@ -472,7 +475,7 @@ __global__ __launch_bounds__(256) void orthogonal_few48_kernel(Schulz a) {
     const Place at = place<kKind>(a);
     End end;
     end.init(a, at);
-    const int steps = (p.steps - w + kWaves - 1) / kWaves;  // of this wave
+    const int steps = w < kWaves ? (p.steps - w + kWaves - 1) / kWaves : 0;  // of this wave
     Part side_a, side_b;
     side_a.init(p.a, p.a_stride, end.m0, p.m, w, 0, l);
     side_b.init(p.b, p.b_stride, end.n0, p.n, w, 0, l);
@@ -553,10 +556,12 @@ __global__ __launch_bounds__(256) void orthogonal_few48_kernel(Schulz a) {
         if (s < steps) turn(s, even, odd);
     }
     __syncthreads();
+    if (w < kWaves) {
 #pragma unroll
-    for (int i = 0; i < I; ++i)
+        for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int j = 0; j < I; ++j) End::put(lds, w, 16 * i + (l & 15), 16 * j + 4 * group, acc[i][j]);
+            for (int j = 0; j < I; ++j) End::put(lds, w, 16 * i + (l & 15), 16 * j + 4 * group, acc[i][j]);
+    }
     __syncthreads();
     end.store(a, at, lds);
 }
@@ -812,9 +817,9 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
         launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 8 : 4, kSymmetric<kKind> ? 1 : 2>, 32,
                kSymmetric<kKind> ? 512 : 256);
     } else if (tiles_of(48) <= kCus && ends_with_steps(m) && ends_with_steps(n)) {
-        launch(orthogonal_few48_kernel<kKind>, 48, 256);
+        launch(orthogonal_few48_kernel<kKind>, 48, 512);
     } else if (tiles_of(64) <= kCus) {
-        launch(orthogonal_few_kernel<kKind, 64, 4, 2>, 64, 256);
+        launch(orthogonal_few_kernel<kKind, 64, 4, 2, 8>, 64, 512);
     } else if (tiles_of(128) < 224) {
         launch(orthogonal_tile_kernel<kKind, 64, 2, 2, 4>, 64, 256);
     } else {
