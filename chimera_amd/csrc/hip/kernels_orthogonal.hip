@@ -810,8 +810,9 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
     // 1024 11.1, 11.3, 13.7 (64: 11.3, 12.7; shared tiles of 64 11.9, 13.0, 14.8; 32
     // 19, 21, 23); 1024 x 4096 23.8, 10.3, 35.0 (64: 29.0, 11.6; X in tiles of 64
     // 38, by waves that divide the sum 48; A in four parts of its sum 25 and 5 for
-    // their join); 4096 x 4096 274, 290, 428 (960 TF of products, a plain fp16
-    // product reaches 1,300). Eight waves a tile of 32 take 0.3 us less for A and
+    // their join); 4096 x 4096 271, 268, 429 (960 TF of products, a plain fp16
+    // product reaches 1,300; by eight waves of 64 x 32, which read a third more
+    // from LDS, 285, 291, 439). Eight waves a tile of 32 take 0.3 us less for A and
     // B and 0.3 more for X.
     if (tiles_of(32) <= (kSymmetric<kKind> ? 256 : 400)) {
         launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 8 : 4, kSymmetric<kKind> ? 1 : 2>, 32,
@@ -823,7 +824,7 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
     } else if (tiles_of(128) < 224) {
         launch(orthogonal_tile_kernel<kKind, 64, 2, 2, 4>, 64, 256);
     } else {
-        launch(orthogonal_tile_kernel<kKind, 128, 2, 4, 4>, 128, 512);
+        launch(orthogonal_tile_kernel<kKind, 128, 2, 2, 4>, 128, 256);
     }
 }
 

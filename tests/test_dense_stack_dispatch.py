@@ -85,6 +85,6 @@ def test_every_kernel_has_a_shape(host_hip):  # noqa: F811
     layers = {k for *_, k in MX4_LAYERS}
     assert layers == {("few", *v, r) for v in ((1, 8, 0), (4, 4, 1), (2, 8, 1)) for r in (8, 32)} | {
         ("few", 4, 1, 1, 32), ("tile", 64, 64), ("tile", 128, 128), ("walk", 8, 8, 1)} | {("walk", s, 4, 1) for s in (1, 2, 3, 4, 8)} | {("walk", s, 8, 2) for s in (1, 2, 3, 4)}
-    few, tiles = {("few", 64, 4, 2, 8), ("few48",)}, {("tile", 64, 2, 2, 4), ("tile", 128, 2, 4, 4)}
+    few, tiles = {("few", 64, 4, 2, 8), ("few48",)}, {("tile", 64, 2, 2, 4), ("tile", 128, 2, 2, 4)}
     assert {s for *_, s, _ in UPDATES} == few | tiles | {("few", 32, 8, 1, 8)}
     assert {x for *_, x in UPDATES} == few | tiles | {("few", 32, 4, 2, 4), "both"}
