@@ -823,6 +823,8 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
         launch(orthogonal_few_kernel<kKind, 64, 4, 2, 8>, 64, 512);
     } else if (tiles_of(128) < 224) {
         launch(orthogonal_tile_kernel<kKind, 64, 2, 2, 4>, 64, 256);
+    } else if (kKind == kLast) {  // whose end, with the weight, is more of its time: 36 us with 1024 x 4096, 42 by four waves
+        launch(orthogonal_tile_kernel<kKind, 128, 2, 4, 4>, 128, 512);
     } else {
         launch(orthogonal_tile_kernel<kKind, 128, 2, 2, 4>, 128, 256);
     }
