@@ -209,26 +209,23 @@ __device__ __forceinline__ void wait_before_stores() {
     asm volatile("" ::: "memory");
 }
 
-// GELU as max(z, 0) - |z| 2^P(|z|) with the polynomial P fitted to log2 of the
-// normal distribution's tail down to -6, where the result is rounded to 16 bits:
-// degree 7 for fp16, within 2^-17 of the size, and 6 for bf16, within 2^-14.3;
-// one or two results in a hundred are another neighbour for it. The tail is 0
-// past 16. 65,536 x 1024 -> 4096 takes 287 us in all, with a comparison and a
-// selection instead of the two limits 295, without an activation 241.
+// GELU as max(z, 0) - |z| 2^P(|z|) with the polynomial P of degree 7 fitted to
+// log2 of the normal distribution's tail down to -6, where the result is rounded
+// to 16 bits: within 2^-17 of the size, which makes about one fp16 result in a
+// hundred another neighbour. The tail is 0 past 16. 65,536 x 1024 -> 4096 takes
+// 287 us in all, with a comparison and a selection instead of the two limits
+// 295, without an activation 241; of degree 6 (2^-14) as long.
 constexpr int kShortGelu = -2;
-template <typename T, int kCount, typename Values>
+template <int kCount, typename Values>
 __device__ __forceinline__ void gelu_short(Values& v) {
-    constexpr bool kLong = std::is_same<T, _Float16>::value;
-    constexpr float kHalf[8] = {-1.8348062e-6f, 6.1598182e-5f, -9.3052391e-4f, 8.5078869e-3f,
-                                -5.3960058e-2f, -4.5846441e-1f, -1.1512511f,   -0.99999529f};
-    constexpr float kBrain[7] = {2.298957e-5f,   -6.1109092e-4f, 7.1955039e-3f, -5.1185161e-2f,
-                                 -4.6127209e-1f, -1.1501743f,    -1.0000647f};
+    constexpr float kP[8] = {-1.8348062e-6f, 6.1598182e-5f, -9.3052391e-4f, 8.5078869e-3f,
+                             -5.3960058e-2f, -4.5846441e-1f, -1.1512511f,   -0.99999529f};
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
         const float a = __builtin_elementwise_minimum(fabsf(v[j]), 16.0f);  // NaN stays
-        float p = kLong ? kHalf[0] : kBrain[0];
+        float p = kP[0];
 #pragma unroll
-        for (int i = 1; i < (kLong ? 8 : 7); ++i) p = fmaf(p, a, kLong ? kHalf[i] : kBrain[i]);
+        for (int i = 1; i < 8; ++i) p = fmaf(p, a, kP[i]);
         v[j] = fmaf(-a, __builtin_amdgcn_exp2f(p), __builtin_elementwise_maximum(v[j], 0.0f));
     }
 }
@@ -244,7 +241,7 @@ __device__ __forceinline__ void activate_few(Values& v, int act) {
         case CHIMERA_ACT_RELU: all(std::integral_constant<int, CHIMERA_ACT_RELU>{}); break;
         case CHIMERA_ACT_GELU: all(std::integral_constant<int, CHIMERA_ACT_GELU>{}); break;
         case kShortGelu:
-            if constexpr (sizeof(T) == 2) gelu_short<T, static_cast<int>(sizeof(Values) / sizeof(float))>(v);
+            if constexpr (sizeof(T) == 2) gelu_short<static_cast<int>(sizeof(Values) / sizeof(float))>(v);
             break;
         case CHIMERA_ACT_GELU_TANH: all(std::integral_constant<int, CHIMERA_ACT_GELU_TANH>{}); break;
         case CHIMERA_ACT_SILU: all(std::integral_constant<int, CHIMERA_ACT_SILU>{}); break;

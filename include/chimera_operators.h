@@ -204,8 +204,8 @@ int chimera_mx4_read_device(chimera_ctx* ctx, const uint8_t* d_codes, const uint
  *   Y = act(Q(X) W^T + b) + R, divided row by row by its length with normalize,
  * with Q(X) the values of X's rows quantised as above. Shape, types, epilogue
  * and limits are those of the dense layer (CHIMERA_ACT_GELU is within 2^-17 of its
- * size for fp16 Y and 2^-14 for bf16 Y down to z = -6); products are exact and
- * sums held in 32 bits. */
+ * size down to z = -6 where Y has 16 bits); products are exact and sums held in
+ * 32 bits. */
 typedef struct {
     const void* x;           /* [rows, in_features], type */
     const uint8_t* codes;    /* [out_features, row_bytes of in_features], 16-byte aligned */
