@@ -7,12 +7,16 @@
 // that the rows of all products lie along their sums.
 //
 // Small singular values grow up to a^steps times, and with them every error,
-// so X, A and B = b A + c A^2 are held to 22 bits: a value is two fp16 parts
-// (times 2^8, which keeps the lower part of values down to 2^-11 a normal
-// number and leaves room up to 255), and a product is hi hi + hi lo + lo hi
-// on the matrix cores, summed in 32 bits. That is as near to 64 bits as 32-bit
-// products are (2e-6 to 1e-5 of the result's size at 256 to 2,048 columns; one
-// fp16 part gives 2e-3), at five times their rate.
+// so X, A and B = b A + c A^2 are held to 22 bits: a value is two fp16 parts,
+// times 2^8, which leaves room up to 255, the lower one times another 2^11. So
+// both are normal numbers down to 2^-22, below which values are 2^-43 apart.
+// (With one factor for both, values are 2^-32 apart from 2^-11 down; 1024 x 1024
+// with rows that are 1e-5 of one row was off by 4.9e-5 of the result instead of
+// 5e-7, and took 164 us instead of 167.) A product is hi hi + (hi lo + lo hi)
+// 2^-11 on the matrix cores, two sums in 32 bits. That is as near to 64 bits as
+// 32-bit products are (1e-7 to 2e-6 of the result's size at 300 to 1,024
+// columns, those 3e-8 to 1e-5; one fp16 part gives 2e-3), at twice their rate:
+// 4096 x 4096 takes 894 us a step, 310 TF of results where 32 bits reach 154.
 #include "dense_tile.hpp"
 
 namespace chimera {
@@ -21,6 +25,7 @@ namespace {
 
 constexpr float kPairScale = 256.0f;
 constexpr float kUnscale = 1.0f / kPairScale, kUnscaleSum = kUnscale * kUnscale;
+constexpr float kLowScale = 2048.0f, kUnscaleLow = 1.0f / kLowScale;
 
 // ---- pairs ---------------------------------------------------------------------
 
@@ -39,8 +44,9 @@ typedef _Float16 f16x4_t __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
     const float s = v * kPairScale;
     hi = from_float<_Float16>(s);
-    lo = from_float<_Float16>(s - to_float(hi));
+    lo = from_float<_Float16>((s - to_float(hi)) * kLowScale);
 }
+__device__ __forceinline__ float join(_Float16 hi, _Float16 lo) { return fmaf(to_float(lo), kUnscaleLow, to_float(hi)); }
 __device__ __forceinline__ void store_pairs(const Pairs& m, int64_t row, int col, const float (&v)[8]) {
     _Float16 hi[8], lo[8];
 #pragma unroll
@@ -305,7 +311,7 @@ struct Result {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[j] *= a.sum_by;
-                if constexpr (kAdds) v[j] = fmaf(a.from_by * kUnscale, to_float(hi[i][j]) + to_float(lo[i][j]), v[j]);
+                if constexpr (kAdds) v[j] = fmaf(a.from_by * kUnscale, join(hi[i][j], lo[i][j]), v[j]);
                 v[j] = r < rows && c + j < cols ? v[j] : 0.0f;
             }
             if constexpr (kKind == kLast) {
@@ -336,19 +342,37 @@ struct Result {
     }
 };
 
+// The sums of I x J tiles: of the upper parts' products and of an upper and a
+// lower part's, 2^11 times as large.
+template <typename Tile, int I, int J = I>
+struct Sums {
+    Tile high[I][J] = {}, low[I][J] = {};
+
+    __device__ __forceinline__ Tile value(int i, int j) const {
+        Tile v;
+#pragma unroll
+        for (int q = 0; q < static_cast<int>(sizeof(Tile) / sizeof(float)); ++q) v[q] = fmaf(low[i][j][q], kUnscaleLow, high[i][j][q]);
+        return v;
+    }
+};
+
 // The parts of a half step that a wave multiplies: I x J tiles of 32 x 32.
 template <int I, int J>
 struct Halves {
     u32x4_t ah[I], al[I], bh[J], bl[J];
 
-    __device__ __forceinline__ void multiply(f32x16_t (&acc)[I][J]) const {
+    __device__ __forceinline__ void multiply(Sums<f32x16_t, I, J>& sums) const {
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int i = 0; i < I; ++i)
 #pragma unroll
                 for (int j = 0; j < J; ++j)
-                    acc[i][j] = mma32<_Float16>(k == 1 ? bl[j] : bh[j], k == 0 ? al[i] : ah[i], acc[i][j]);
+                    sums.low[i][j] = mma32<_Float16>(k == 1 ? bl[j] : bh[j], k == 0 ? al[i] : ah[i], sums.low[i][j]);
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) sums.high[i][j] = mma32<_Float16>(bh[j], ah[i], sums.high[i][j]);
         // with the reads of the half step after it in between
         constexpr int kMfmas = 3 * I * J, kReads = 2 * (I + J), kPer = (kReads + kMfmas - 1) / kMfmas;
 #pragma unroll
@@ -359,6 +383,16 @@ struct Halves {
         __builtin_amdgcn_sched_barrier(0);
     }
 };
+
+// A step's loads with the address in scalar registers and a lane's offset beside
+// it: where the compiler can see the address it keeps each load's sum of the two
+// in vector registers over the loop, and spills (768 x 768 159 us, so 143).
+template <typename Part>
+__device__ __forceinline__ void fetch_step(const Part& part, int s, unsigned char* to, int l) {
+    Part from = part;
+    asm volatile("" : "+s"(from.base));
+    from.fetch(s, to, true, 0, l);
+}
 
 // Until at most kUnderWay of this wave's loads are under way and its LDS reads have come.
 template <int kUnderWay>
@@ -414,11 +448,7 @@ __global__ __launch_bounds__(kAll* kWave) void orthogonal_few_kernel(Schulz a) {
 #pragma unroll
     for (int s = 0; s < kSlots; ++s)
         if (s < steps) fetch(s);
-    f32x16_t acc[I][I];
-#pragma unroll
-    for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int j = 0; j < I; ++j) acc[i][j] = f32x16_t{};
+    Sums<f32x16_t, I> acc;
     if (steps > 0) {
         Halves<I, I> even, odd;
         if (steps >= kSlots)
@@ -453,7 +483,7 @@ __global__ __launch_bounds__(kAll* kWave) void orthogonal_few_kernel(Schulz a) {
 #pragma unroll
         for (int i = 0; i < I; ++i)
 #pragma unroll
-            for (int j = 0; j < I; ++j) End::put(lds, w, 32 * i + (l & 31), 32 * j, acc[i][j]);
+            for (int j = 0; j < I; ++j) End::put(lds, w, 32 * i + (l & 31), 32 * j, acc.value(i, j));
     }
     __syncthreads();
     end.store(a, at, lds);
@@ -482,8 +512,8 @@ __global__ __launch_bounds__(512) void orthogonal_few48_kernel(Schulz a) {
     unsigned char* const ring = lds + w * kSlots * kSlot;
     auto fetch = [&](int s) {
         unsigned char* to = ring + s % kSlots * kSlot;
-        side_a.fetch(kWaves * s, to, true, 0, l);
-        side_b.fetch(kWaves * s, to + Part::kBytes, true, 0, l);
+        fetch_step(side_a, kWaves * s, to, l);
+        fetch_step(side_b, kWaves * s, to + Part::kBytes, l);
     };
     // lane l's eight of row l % 16 is the l / 16-th of the step, upper parts
     // here, lower ones two chunks on
@@ -503,21 +533,22 @@ __global__ __launch_bounds__(512) void orthogonal_few48_kernel(Schulz a) {
             o.bl[i] = *reinterpret_cast<const u32x4_t*>(y + (off ^ 32));
         }
     };
-    f32x4_t acc[I][I];
-#pragma unroll
-    for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int j = 0; j < I; ++j) acc[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    Sums<f32x4_t, I> acc;
     auto multiply = [&](const Operands& o) {
+        auto product = [](u32x4_t x, u32x4_t y, f32x4_t sum) {
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, x), __builtin_bit_cast(f16x8_t, y), sum, 0, 0, 0);
+        };
 #pragma unroll
-        for (int k = 0; k < 3; ++k)
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
             for (int i = 0; i < I; ++i)
 #pragma unroll
                 for (int j = 0; j < I; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                        __builtin_bit_cast(f16x8_t, k == 1 ? o.bl[j] : o.bh[j]),
-                        __builtin_bit_cast(f16x8_t, k == 0 ? o.al[i] : o.ah[i]), acc[i][j], 0, 0, 0);
+                    acc.low[i][j] = product(k == 1 ? o.bl[j] : o.bh[j], k == 0 ? o.al[i] : o.ah[i], acc.low[i][j]);
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < I; ++j) acc.high[i][j] = product(o.bh[j], o.ah[i], acc.high[i][j]);
 #pragma unroll
         for (int g = 0; g < 4 * I; ++g) {
             __builtin_amdgcn_sched_group_barrier(kSchedMfma, 2, 0);
@@ -560,7 +591,7 @@ __global__ __launch_bounds__(512) void orthogonal_few48_kernel(Schulz a) {
 #pragma unroll
         for (int i = 0; i < I; ++i)
 #pragma unroll
-            for (int j = 0; j < I; ++j) End::put(lds, w, 16 * i + (l & 15), 16 * j + 4 * group, acc[i][j]);
+            for (int j = 0; j < I; ++j) End::put(lds, w, 16 * i + (l & 15), 16 * j + 4 * group, acc.value(i, j));
     }
     __syncthreads();
     end.store(a, at, lds);
@@ -598,7 +629,7 @@ __global__ __launch_bounds__(256) void orthogonal_both_kernel(Schulz a) {
     __syncthreads();
     Reader<float, 1, false, kStepBytes> reader;
     reader.init(0, l);
-    f32x16_t acc[1][1] = {};
+    Sums<f32x16_t, 1> acc;
     if (works) {
         Halves<1, 1> even, odd, x[2];
         auto read = [&](int s, int h, Halves<1, 1>& o) {
@@ -620,6 +651,7 @@ __global__ __launch_bounds__(256) void orthogonal_both_kernel(Schulz a) {
             reader.read(own + kSteps * Part::kBytes, 2 * h + 1, x[h].bl);
         }
         // this lane's values of B: row l % 32, columns 8 q + 4 half + i of the step
+        const f32x16_t square = acc.value(0, 0);
         uint32_t hi[8], lo[8];
         const unsigned char* from = lds + w * Part::kBytes + (l & 31) * kStepBytes;
         const int turn = ((l & 31) >> 1) & 7;
@@ -632,11 +664,11 @@ __global__ __launch_bounds__(256) void orthogonal_both_kernel(Schulz a) {
             _Float16 h[4], r[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                split(fmaf(a.square_by, acc[0][0][4 * q + i], a.linear_by * (to_float(ah[i]) + to_float(al[i]))), h[i], r[i]);
+                split(fmaf(a.linear_by, join(ah[i], al[i]), a.square_by * square[4 * q + i]), h[i], r[i]);  // as Result's
             __builtin_memcpy(&hi[2 * q], h, 8);
             __builtin_memcpy(&lo[2 * q], r, 8);
         }
-        acc[0][0] = f32x16_t{};
+        acc = {};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             auto operand = [&](const uint32_t* u) {
@@ -650,7 +682,7 @@ __global__ __launch_bounds__(256) void orthogonal_both_kernel(Schulz a) {
         }
     }
     __syncthreads();
-    End::put(lds, w, l & 31, 0, acc[0][0]);
+    End::put(lds, w, l & 31, 0, acc.value(0, 0));
     __syncthreads();
     end.store(a, at, lds);
 }
@@ -696,11 +728,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void orthogonal_tile_kernel(Schulz a
         wait_and_meet<(kSlots - 2) * kLoads + Part::kLoads>();
     else
         wait_and_meet<0>();
-    f32x16_t acc[I][J];
-#pragma unroll
-    for (int i = 0; i < I; ++i)
-#pragma unroll
-        for (int j = 0; j < J; ++j) acc[i][j] = f32x16_t{};
+    Sums<f32x16_t, I, J> acc;
     Halves<I, J> even, odd;
     read(0, 0, even);
     int s = 0;
@@ -727,7 +755,7 @@ __global__ __launch_bounds__(WM* WN* kWave) void orthogonal_tile_kernel(Schulz a
 #pragma unroll
     for (int i = 0; i < I; ++i)
 #pragma unroll
-        for (int j = 0; j < J; ++j) End::put(lds, 0, wm * TM + 32 * i + (l & 31), wn * TN + 32 * j, acc[i][j]);
+        for (int j = 0; j < J; ++j) End::put(lds, 0, wm * TM + 32 * i + (l & 31), wn * TN + 32 * j, acc.value(i, j));
     __syncthreads();
     end.store(a, at, lds);
 }

@@ -1,0 +1,42 @@
+"""The orthogonal update of gradients whose rows or columns differ in size, as
+those of seldom used embeddings do: the small ones' values are far below the
+largest one's, and the steps multiply them by up to 485.
+
+Tolerance: close_to's, four times the distance that the same steps have in 32
+bits, as values are held to 22 bits instead of 24, and 2^-22 of the size. It
+needs the 22 bits at every size that counts: with a spacing of d for small
+values the result is off by about 485 d / 3.5 sqrt(rows cols), which at 1,024 x
+1,024 is 1.6e-8 for d = 2^-43 and 1.6e-5 for 2^-33."""
+import numpy as np
+import pytest
+
+from operator_checks import context, to_type
+from test_gpu_orthogonal import close_to, run
+
+pytestmark = pytest.mark.gpu
+
+# each kernel of the products; see UPDATES in dense_stack_shapes
+SHAPES = [(100, 300), (200, 330), (768, 760), (900, 880), (1300, 1000), (1500, 1450), (1400, 2600)]
+
+
+def graded(rng, rows, cols, kind, small):
+    """One large row, one large column, or rows of all sizes down to `small`."""
+    g = rng.standard_normal((rows, cols))
+    if kind == "row":
+        g[1:] *= small
+    elif kind == "column":
+        g[:, 1:] *= small
+    else:
+        g *= small ** rng.random((rows, 1))
+    return to_type(1e-3 * g, "f32")
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("kind", ["row", "column", "all sizes"])
+def test_rows_and_columns_of_different_sizes(rows, cols, kind):
+    ctx = context()
+    for small in (1e-3, 1e-5) if rows < 1000 else (1e-4,):
+        g = graded(np.random.default_rng(rows + cols), rows, cols, kind, small)
+        print(f"{rows} x {cols} {kind} {small}", flush=True)
+        close_to(run(ctx, g, "f32", "f32"), g, "f32")
+    ctx.close()
