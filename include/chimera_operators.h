@@ -235,10 +235,11 @@ int chimera_mx4_linear_device(chimera_ctx* ctx, const chimera_linear_shape* shap
  * products do to a singular value s is a s + b s^3 + c s^5, step by step. G has
  * the layer's type, M and W are 32-bit; a 16-bit layer reads the rounded copy.
  * Products are sums in 32 bits of values that are held to 22 bits (those of
- * less than 2^-22 to 2^-44); sums of squares are held in 64. The coefficients
- * should keep singular values below 100 from step to step (the values 3.4445,
- * -4.7750, 2.0315 keep them below 1.3): X and b A + c A^2 become infinite from
- * 255 on. A U that is not finite gives X that is not. */
+ * less than 2^-22 to 2^-44); sums of squares are held in 64. X, A and b A + c A^2
+ * become infinite from 255 on, so the coefficients should keep singular values
+ * s below 15 from step to step, and b s^2 + c s^4 within 255 of zero (the values
+ * 3.4445, -4.7750, 2.0315 keep s below 1.3 and that above -2.9). A U that is not
+ * finite gives X that is not. */
 typedef struct {
     int32_t rows, cols; /* 1..65536; rows * cols at most 2^28, the smaller at most 8192 */
     int32_t type;       /* of the gradient and the rounded copy */

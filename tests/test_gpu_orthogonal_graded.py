@@ -11,7 +11,7 @@ import numpy as np
 import pytest
 
 from operator_checks import context, to_type
-from test_gpu_orthogonal import close_to, run
+from test_gpu_orthogonal import close_to, run, steps_of
 
 pytestmark = pytest.mark.gpu
 
@@ -39,4 +39,23 @@ def test_rows_and_columns_of_different_sizes(rows, cols, kind):
         g = graded(np.random.default_rng(rows + cols), rows, cols, kind, small)
         print(f"{rows} x {cols} {kind} {small}", flush=True)
         close_to(run(ctx, g, "f32", "f32"), g, "f32")
+    ctx.close()
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 5), (100, 300), (200, 330), (600, 640)])
+def test_singular_values_up_to_the_documented_size(rows, cols):
+    """A gradient of rank one, whose singular value of 1 becomes 15 after a step,
+    so that A is 225 in the next, and B up to 250 in size. Each of X, A and B has
+    the errors of a few roundings of 2^-22 of its size, 4 taken here, and the
+    result a X + B X those of the three: 4 2^-22 of |a s| + 3 |B s|."""
+    rng = np.random.default_rng(rows)
+    left, right = rng.standard_normal(rows), rng.standard_normal(cols)
+    g = to_type(np.outer(left / np.linalg.norm(left), right / np.linalg.norm(right)), "f32")
+    ctx = context()
+    for steps, abc in ((2, (15.0, 0.0, 0.0)), (2, (15.5, -0.5, 0.0)), (1, (10.0, -250.0, 0.0))):
+        a, b, _ = abc
+        s = 1.0 if steps == 1 else a + b  # before the last step
+        have = run(ctx, g, "f32", "f32", steps=steps, coefficients=abc)
+        off = 4 * 2.0**-22 * (abs(a * s) + 3 * abs(b * s**3)) + (steps - 1) * 4 * 2.0**-22 * abs(a + 3 * b * s**2) * s
+        assert np.linalg.norm(have - steps_of(g, np.float64, steps, abc)) <= off
     ctx.close()
