@@ -16,6 +16,11 @@ int64_t ceil_div(int64_t v, int64_t by) { return (v + by - 1) / by; }
 // Rows whose squares pass the 32-bit range are taken times kSmall, and so are
 // those in the backward pass whose rstd is below kLowRstd.
 constexpr float kSmall = 0x1p-80f, kLarge = 0x1p80f, kLowRstd = 0x1p-60f;
+// What the rounding of a row's mean left out, over the row's deviation, from
+// which on it is taken away, and how often at the most: each turn leaves 2^-17
+// of it.
+constexpr float kSmallRest = 0x1p-4f;
+constexpr int kMostTurns = 16;
 
 struct NormArgs {
     const void* x;
@@ -160,7 +165,12 @@ struct Columns {
 // wave for each row, without what it keeps: 50, and 60 with loads that wait for
 // the row before them). A row of 64 lanes needs no LDS; longer ones meet twice.
 // The variance is taken about a mean that is corrected by what is left of the
-// row's sum after it, so that rows far from zero keep their digits.
+// row's sum after it, so that rows far from zero keep their digits. Where that
+// rest is not small beside the row's deviation (rows of one value, or of a few
+// neighbouring ones, far from zero) it is taken away and the sums are made
+// again, in turns, from the caches. (In registers all rows would need more of
+// them: 65,536 x 1024 53.4 us, not 51.8, and 500 x 65,536 of 32 bits 87, not 81;
+// without the turns these take 51.8 and 70.)
 template <typename T, typename Out, int kLanes, int kChunks, Fit kFit>
 __global__ __launch_bounds__(block_threads(kLanes)) void norm_forward_kernel(NormArgs a) {
     constexpr int kRows = block_threads(kLanes) / kLanes;
@@ -190,6 +200,13 @@ __global__ __launch_bounds__(block_threads(kLanes)) void norm_forward_kernel(Nor
         const int64_t after = r + static_cast<int64_t>(gridDim.x) * kRows;
         if constexpr (kAhead) at.load(x0 + (after < a.rows ? after : r) * a.x_stride, next);
         float mean, rest, var;
+        auto spread = [&](float (&s)[2]) {  // from the sums of x - mean and of its squares
+            row_sums<kLanes>(s, lds);
+            rest = s[0] * inv;
+            // what rounding leaves of one value is no deviation
+            var = fmaxf(fmaf(-rest, rest, s[1] * inv), rest * rest * 0x1p-18f);
+            return s[1] - s[1] == 0.0f;  // neither infinite nor NaN
+        };
         auto moments = [&] {  // x becomes x - mean
             float sum[1] = {0.0f};
 #pragma unroll
@@ -208,11 +225,7 @@ __global__ __launch_bounds__(block_threads(kLanes)) void norm_forward_kernel(Nor
                     s[0] += d;
                     s[1] = fmaf(d, d, s[1]);
                 }
-            row_sums<kLanes>(s, lds);
-            rest = s[0] * inv;
-            // of rows of one value: what rounding leaves of it is no deviation
-            var = fmaxf(fmaf(-rest, rest, s[1] * inv), rest * rest * 0x1p-18f);
-            return s[1] - s[1] == 0.0f;  // neither infinite nor NaN
+            return spread(s);
         };
         float scale = 1.0f;
         if (!moments()) {
@@ -227,11 +240,39 @@ __global__ __launch_bounds__(block_threads(kLanes)) void norm_forward_kernel(Nor
             }
             (void)moments();
         }
-        const float spread = var + a.eps * scale * scale;  // 0 for scaled rows of one value
-        const float rstd = spread == 0.0f ? 0.0f : 1.0f / sqrtf(spread), by = -rest * rstd;
+        const float eps = a.eps * scale * scale;
+        float more = 0.0f;  // of the mean
+        auto is_large = [&] { return rest * rest > kSmallRest * kSmallRest * (var + eps); };
+        if (is_large()) {
+            auto less = [&](int j, float (&v)[8]) {
+                at.load(x0 + r * a.x_stride, 0.0f, j, v);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = fmaf(v[i], scale, -mean) - more;
+            };
+            for (int turn = 0; turn < kMostTurns && is_large(); ++turn) {
+                more += rest;
+                float s[2] = {0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < kChunks; ++j) {
+                    float v[8];
+                    less(j, v);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float d = at.counts(j, i) ? v[i] : 0.0f;
+                        s[0] += d;
+                        s[1] = fmaf(d, d, s[1]);
+                    }
+                }
+                (void)spread(s);
+            }
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) less(j, x[j]);
+        }
+        const float square = var + eps;  // 0 for scaled rows of one value
+        const float rstd = square == 0.0f ? 0.0f : 1.0f / sqrtf(square), by = -rest * rstd;
         if (at.t == 0) {
-            if (a.mean) a.mean[r] = (mean + rest) * (scale == 1.0f ? 1.0f : kLarge);
-            if (a.rstd) a.rstd[r] = spread == 0.0f ? 1.0f / sqrtf(a.eps) : rstd * scale;
+            if (a.mean) a.mean[r] = (mean + (more + rest)) * (scale == 1.0f ? 1.0f : kLarge);
+            if (a.rstd) a.rstd[r] = square == 0.0f ? 1.0f / sqrtf(a.eps) : rstd * scale;
         }
         Out* to = static_cast<Out*>(a.y) + r * a.y_stride;
 #pragma unroll
@@ -256,7 +297,9 @@ __global__ __launch_bounds__(block_threads(kLanes)) void norm_forward_kernel(Nor
 // for the row before). So do the thread's columns of the sums over rows; these
 // are joined over the block's rows in order and written for the join, 4 us. What
 // the rounding of the mean left out is the sum of x - mean, and is taken away
-// again.
+// again, in turns where it is not small (see the forward pass; here from the
+// registers, as loads in the branch make all rows wait for the next one's:
+// 16,384 x 1024 29.4 us with the join, not 23.7; without the turns 23.4).
 template <typename T, typename Out, int kLanes, int kChunks, Fit kFit>
 __global__ __launch_bounds__(kBackThreads) void norm_backward_kernel(NormArgs a) {
     constexpr int kRows = kBackThreads / kLanes;
@@ -293,28 +336,40 @@ __global__ __launch_bounds__(kBackThreads) void norm_backward_kernel(NormArgs a)
         const float scale = low ? kSmall : 1.0f, mean = next_mean * scale, by = low ? rstd * kLarge : rstd;
         const int64_t after = r + static_cast<int64_t>(gridDim.x) * kRows;
         load(after < a.rows ? after : r);
-        float s[3] = {0.0f, 0.0f, 0.0f};
+        float s[3], rest;
+        auto sum_up = [&](float more) {  // of x - mean - more
+            s[0] = s[1] = s[2] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float d = at.counts(j, i) ? x[j][i] - more : 0.0f;
+                    const float g = at.counts(j, i) ? dy[j][i] * w[j][i] : 0.0f;
+                    s[0] += d;
+                    s[1] += g;
+                    s[2] = fmaf(g, d, s[2]);
+                }
+            row_sums<kLanes>(s, lds);
+            rest = s[0] * inv;
+        };
 #pragma unroll
         for (int j = 0; j < kChunks; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[j][i] = fmaf(x[j][i], scale, -mean);
-                const float d = at.counts(j, i) ? x[j][i] : 0.0f;
-                const float g = at.counts(j, i) ? dy[j][i] * w[j][i] : 0.0f;
-                s[0] += d;
-                s[1] += g;
-                s[2] = fmaf(g, d, s[2]);
-            }
-        row_sums<kLanes>(s, lds);
-        const float rest = s[0] * inv, mean_g = s[1] * inv;
-        const float mean_gz = by * fmaf(-rest, s[1], s[2]) * inv, off = -rest * by;
+            for (int i = 0; i < 8; ++i) x[j][i] = fmaf(x[j][i], scale, -mean);
+        sum_up(0.0f);
+        float more = 0.0f;
+        for (int turn = 0; turn < kMostTurns && fabsf(rest) * by > kSmallRest; ++turn) {
+            more += rest;
+            sum_up(more);
+        }
+        const float mean_g = s[1] * inv, mean_gz = by * fmaf(-rest, s[1], s[2]) * inv, off = -rest * by;
         T* to = static_cast<T*>(a.y) + r * a.y_stride;
 #pragma unroll
         for (int j = 0; j < kChunks; ++j) {
             float v[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float z = fmaf(x[j][i], by, off);
+                const float z = fmaf(x[j][i] - more, by, off);
                 v[i] = rstd * fmaf(-z, mean_gz, fmaf(dy[j][i], w[j][i], -mean_g));
                 dw[j][i] = fmaf(dy[j][i], z, dw[j][i]);
                 db[j][i] += dy[j][i];
@@ -352,12 +407,14 @@ __global__ __launch_bounds__(kBackThreads) void norm_backward_kernel(NormArgs a)
 }
 
 // Rows too long for registers: two passes over a row, the second from the
-// caches. `rests` [rows] gets what the saved mean left out.
+// caches. `rests` [rows][2] gets what the saved mean left out, in two parts: what
+// was taken away in turns, and what is left.
 template <typename T, typename Out>
 __global__ __launch_bounds__(1024) void norm_wide_kernel(NormArgs a, float* rests) {
     __shared__ float lds[16 * 3];
     const float inv = 1.0f / static_cast<float>(a.cols);
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        float more = 0.0f;
         const T* from = static_cast<const T*>(a.x) + r * a.x_stride;
         const Out* grad = static_cast<const Out*>(a.dy) + r * a.dy_stride;
         const float rstd = a.rstd[r];
@@ -372,25 +429,36 @@ __global__ __launch_bounds__(1024) void norm_wide_kernel(NormArgs a, float* rest
                 if (a.weight) load8(static_cast<const T*>(a.weight) + c, count, w);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    x[i] = i < count ? fmaf(x[i], scale, -mean) : 0.0f;
+                    x[i] = i < count ? fmaf(x[i], scale, -mean) - more : 0.0f;
                     dy[i] = i < count ? a.weight ? dy[i] * w[i] : dy[i] : 0.0f;
                 }
                 visit(c, count, x, dy);
             }
         };
-        float s[3] = {0.0f, 0.0f, 0.0f};
-        each([&](int, int, float(&d)[8], float(&g)[8]) {
+        float s[3], rest;
+        auto sum_up = [&] {
+            s[0] = s[1] = s[2] = 0.0f;
+            each([&](int, int, float(&d)[8], float(&g)[8]) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                s[0] += d[i];
-                s[1] += g[i];
-                s[2] = fmaf(g[i], d[i], s[2]);
-            }
-        });
-        row_sums<1024>(s, lds);
-        const float rest = s[0] * inv, mean_g = s[1] * inv;
-        const float mean_gz = by * fmaf(-rest, s[1], s[2]) * inv;
-        if (rests && threadIdx.x == 0) rests[r] = rest;
+                for (int i = 0; i < 8; ++i) {
+                    s[0] += d[i];
+                    s[1] += g[i];
+                    s[2] = fmaf(g[i], d[i], s[2]);
+                }
+            });
+            row_sums<1024>(s, lds);
+            rest = s[0] * inv;
+        };
+        sum_up();
+        for (int turn = 0; turn < kMostTurns && fabsf(rest) * by > kSmallRest; ++turn) {
+            more += rest;
+            sum_up();
+        }
+        const float mean_g = s[1] * inv, mean_gz = by * fmaf(-rest, s[1], s[2]) * inv;
+        if (rests && threadIdx.x == 0) {
+            rests[2 * r] = more;
+            rests[2 * r + 1] = rest;
+        }
         if (!a.wants_dx) continue;
         T* to = static_cast<T*>(a.y) + r * a.y_stride;
         each([&](int c, int count, float(&d)[8], float(&g)[8]) {
@@ -414,12 +482,13 @@ __global__ __launch_bounds__(256) void norm_wide_sums_kernel(NormArgs a, const f
         const float rstd = a.rstd[r];
         const bool low = rstd < kLowRstd;
         const float scale = low ? kSmall : 1.0f, mean = a.mean[r] * scale, by = low ? rstd * kLarge : rstd;
+        const float more = rests[2 * r], rest = rests[2 * r + 1];
         float x[8], dy[8];
         load8(static_cast<const T*>(a.x) + r * a.x_stride + c, count, x);
         load8(static_cast<const Out*>(a.dy) + r * a.dy_stride + c, count, dy);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            dw[i] = fmaf(dy[i], (fmaf(x[i], scale, -mean) - rests[r]) * by, dw[i]);
+            dw[i] = fmaf(dy[i], (fmaf(x[i], scale, -mean) - more - rest) * by, dw[i]);
             db[i] += dy[i];
         }
     }
@@ -562,7 +631,7 @@ auto by_types(int type, int out_type, Call&& call) {
 }  // namespace
 
 size_t norm_workspace(const chimera_norm_shape& s) {
-    const int64_t rests = s.features > kMostRegisters ? s.rows : 0;
+    const int64_t rests = s.features > kMostRegisters ? 2 * s.rows : 0;
     return static_cast<size_t>(parts_of(s.rows, s.features) * 2 * s.features + rests) * sizeof(float);
 }
 

@@ -125,11 +125,12 @@ int chimera_linear_backward_device(chimera_ctx* ctx, const chimera_linear_shape*
  *
  * x, w and b have one type, y has it too or is 32-bit; statistics and sums are
  * held in 32 bits, results rounded once. The mean is corrected by what is left
- * of a row's sum after it, and rows whose squares pass the 32-bit range are
- * scaled, so rows of any finite values are normalized; a row with a value that
- * is not finite becomes NaN. Rows may lie apart and have any alignment of whole
- * elements, as for dense layers. Outputs and workspace overlap neither inputs
- * nor each other. */
+ * of a row's sum after it, in turns where that is not small beside the row's
+ * deviation, and rows whose squares pass the 32-bit range are scaled, so rows of
+ * any finite values are normalized, those of one value too (z is zero and rstd
+ * 1 / sqrt(eps)); a row with a value that is not finite becomes NaN. Rows may
+ * lie apart and have any alignment of whole elements, as for dense layers.
+ * Outputs and workspace overlap neither inputs nor each other. */
 typedef struct {
     int64_t rows;     /* 0..2^31 */
     int32_t features; /* 1..65536 */
