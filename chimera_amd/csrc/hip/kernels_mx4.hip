@@ -658,6 +658,25 @@ void quantise(hipStream_t st, RowsArgs a) {
     hipLaunchKernelGGL((mx4_quantise_kernel<T>), dim3(a.row_blocks + static_cast<unsigned>(weight_blocks)), dim3(256), 0, st, a);
 }
 
+// What rows_args describes, in launches of at most 2^20 blocks, which take most of
+// a millisecond each: the most rows that a call may have are up to 2^31 blocks of
+// 256 threads, and a launch has less than 2^32 threads. (A layer's rows, at most
+// 2^23 blocks, are one launch.)
+template <typename Call>
+void by_parts(const RowsArgs& all, const void* x, void* out, int type, Call&& call) {
+    constexpr int64_t kMostBlocks = 1 << 20;
+    const int64_t most = std::max<int64_t>(1, kMostBlocks / all.steps) * 32, row = all.stride * static_cast<int64_t>(type_bytes(type));
+    for (int64_t at = 0; at < all.rows; at += most) {
+        RowsArgs a = all;
+        a.rows = std::min(most, all.rows - at);
+        a.x = x ? static_cast<const char*>(x) + at * row : nullptr;
+        a.out = out ? static_cast<char*>(out) + at * row : nullptr;
+        a.codes += at * all.units * 4;
+        a.scales += at * all.steps * kStepBlocks;
+        call(a);
+    }
+}
+
 RowsArgs rows_args(int64_t rows, int cols, int64_t stride, uint8_t* codes, uint8_t* scales) {
     RowsArgs a = {};
     a.codes = codes;
@@ -865,18 +884,19 @@ size_t mx4_linear_workspace(const chimera_linear_shape& s) {
 
 hipError_t launch_mx4_quantise(hipStream_t st, const void* x, int type, int64_t stride, int64_t rows, int cols,
                                uint8_t* codes, uint8_t* scales) {
-    RowsArgs a = rows_args(rows, cols, stride, codes, scales);
-    a.x = x;
-    by_type(type, [&](auto t) { quantise<decltype(t)>(st, a); });
+    by_parts(rows_args(rows, cols, stride, codes, scales), x, nullptr, type,
+             [&](const RowsArgs& a) { by_type(type, [&](auto t) { quantise<decltype(t)>(st, a); }); });
     return hipGetLastError();
 }
 
 hipError_t launch_mx4_read(hipStream_t st, const uint8_t* codes, const uint8_t* scales, int64_t rows, int cols, void* out,
                            int type, int64_t stride) {
-    RowsArgs a = rows_args(rows, cols, stride, const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales));
-    a.out = out;
-    const dim3 grid(row_blocks(a));
-    by_type(type, [&](auto t) { hipLaunchKernelGGL((mx4_read_kernel<decltype(t)>), grid, dim3(256), 0, st, a); });
+    by_parts(rows_args(rows, cols, stride, const_cast<uint8_t*>(codes), const_cast<uint8_t*>(scales)), nullptr, out, type,
+             [&](const RowsArgs& a) {
+                 by_type(type, [&](auto t) {
+                     hipLaunchKernelGGL((mx4_read_kernel<decltype(t)>), dim3(row_blocks(a)), dim3(256), 0, st, a);
+                 });
+             });
     return hipGetLastError();
 }
 

@@ -177,6 +177,9 @@ hipError_t hipLaunchKernel(const void* function, dim3 grid, dim3 block, void** a
     if (grid.x == 0 || grid.y == 0 || grid.z == 0 || block.x * block.y * block.z == 0 ||
         block.x * block.y * block.z > 1024)
         return done(hipErrorInvalidConfiguration);
+    // a dimension has less than 2^32 threads
+    if (uint64_t{grid.x} * block.x >> 32 || uint64_t{grid.y} * block.y >> 32 || uint64_t{grid.z} * block.z >> 32)
+        return done(hipErrorInvalidConfiguration);
     const std::string& name = g_names[function];
     ++g_launches[name];
     g_threads[name] = static_cast<int>(block.x * block.y * block.z);
