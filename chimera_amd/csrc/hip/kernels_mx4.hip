@@ -328,12 +328,11 @@ __global__ __launch_bounds__(kWaves* kWave) void mx4_walk_kernel(Mx4Args a, Epil
     __shared__ __align__(1024) unsigned char lds[2 * kTileBytes];
     const int l = lane_id(), half = l >> 5;
     const int w = __builtin_amdgcn_readfirstlane(wave_id());
-    // blocks go round the 8 XCDs; the groups of columns that walk the same rows
-    // share one's L2
-    const int id = static_cast<int>(blockIdx.x), ranges_per_xcd = (a.ranges + 7) / 8;
-    const int in_xcd = id / 8;
-    const int group = in_xcd % a.groups, range = id % 8 * ranges_per_xcd + in_xcd / a.groups;
-    if (range >= a.ranges) return;
+    // blocks go round the 8 XCDs; each takes a run of a range's groups of columns
+    // after the other, so that those that walk the same rows share an L2
+    const int id = static_cast<int>(blockIdx.x), xcd = id % 8, blocks = static_cast<int>(gridDim.x);
+    const int at = xcd * (blocks / 8) + min(xcd, blocks % 8) + id / 8;
+    const int group = at % a.groups, range = at / a.groups;
     const int first = static_cast<int>(static_cast<int64_t>(a.m_tiles) * range / a.ranges);
     const int last = static_cast<int>(static_cast<int64_t>(a.m_tiles) * (range + 1) / a.ranges);
     const int n0 = (group * kWaves + w) * 32;
@@ -746,7 +745,7 @@ hipError_t walk(hipStream_t st, const chimera_linear_shape& s, const chimera_mx4
         g.m_tiles = static_cast<int>(ceil_div(s.rows, 32 * kUnits));
         g.groups = static_cast<int>(ceil_div(s.out_features, 32 * kWaves));
         g.ranges = static_cast<int>(std::min<int64_t>(g.m_tiles, std::max(1, blocks_a_cu * kCus / g.groups)));
-        const unsigned blocks = static_cast<unsigned>(ceil_div(g.ranges, 8) * 8 * g.groups);
+        const unsigned blocks = static_cast<unsigned>(g.ranges * g.groups);
         hipLaunchKernelGGL((mx4_walk_kernel<T, kSteps, kWaves, kUnits>), dim3(blocks), dim3(kWaves * kWave), 0, st, g, e);
     };
     constexpr std::integral_constant<int, 1> k1;

@@ -37,3 +37,22 @@ for _ in range(300):
         a = op.Mx4LinearArgs(A, 1 << 50, 1 << 51, None, None, 1 << 52, k, n, n, 1 << 54 if bytes else None, bytes)
         capi.check(L.chimera_mx4_linear_device(ctx.handle, C.byref(s), C.byref(a)))
 """)
+
+
+def test_every_block_of_a_walk_has_work(host_hip):  # noqa: F811
+    """A block for each group of columns and range of rows and none besides, as
+    they go round the XCDs: idle ones would leave some of these without work.
+    As many ranges as the CUs hold blocks, or as there are tiles of rows."""
+    host_hip(SETUP + """
+for rows, k, n, waves, units, a_cu in ((65_536, 1024, 4096, 8, 2, 1), (65_536, 1024, 2560, 8, 2, 1), (65_536, 1024, 3584, 8, 2, 1),
+                                       (128, 2048, 4096, 4, 1, 2), (288, 1024, 4096, 4, 1, 2), (2048, 1024, 16384, 8, 2, 1),
+                                       (1, 1024, 32768, 4, 1, 2), (32, 256, 65536, 4, 1, 2), (10_007, 777, 520, 4, 1, 2),
+                                       (8200, 1500, 4096, 8, 1, 1)):
+    s = op.LinearShape(rows, k, n, 2, 2, 0, 0)
+    bytes = need(L.chimera_mx4_linear_workspace, C.byref(s))
+    a = op.Mx4LinearArgs(A, 1 << 50, 1 << 51, None, None, 1 << 52, k, n, n, 1 << 54, bytes)
+    capi.check(L.chimera_mx4_linear_device(ctx.handle, C.byref(s), C.byref(a)))
+    assert launches(f"Li{waves}ELi{units}E") == launches("mx4_walk_kernel") == 1, (rows, k, n)
+    groups, tiles = -(-n // (32 * waves)), -(-rows // (32 * units))
+    assert hip.host_hip_blocks(b"mx4_walk_kernel") == groups * min(tiles, max(1, 256 * a_cu // groups)), (rows, k, n)
+""")
