@@ -209,23 +209,30 @@ __device__ __forceinline__ void wait_before_stores() {
     asm volatile("" ::: "memory");
 }
 
-// GELU as max(z, 0) - |z| 2^P(|z|) with the polynomial P of degree 7 fitted to
-// log2 of the normal distribution's tail down to -6, where the result is rounded
-// to 16 bits: within 2^-17 of the size, which makes about one fp16 result in a
-// hundred another neighbour. The tail is 0 past 16. 65,536 x 1024 -> 4096 takes
-// 287 us in all, with a comparison and a selection instead of the two limits
-// 295, without an activation 241; of degree 6 (2^-14) as long.
+// GELU as max(z, 0) - |z| 2^P(|z|) with a polynomial P fitted to log2 of the
+// normal distribution's tail, where the result is rounded to 16 bits. fp16 ends
+// near -6: degree 7 is within 2^-17 of the size down to there, which makes about
+// one result in a hundred another neighbour. bf16 goes on: degree 9 is within
+// 2^-16.8 down to -6 and 2^-12 from there to -12.9, where the tail is no normal
+// number any more (degree 7 is 16 % off at -10). The tail is 0 past 16. 65,536 x
+// 1024 -> 4096 of bf16 takes 297 us in all, with degree 7 286, with 10 302, and
+// without an activation 241; a comparison and a selection instead of the two
+// limits take 8 more.
 constexpr int kShortGelu = -2;
-template <int kCount, typename Values>
+template <typename T, int kCount, typename Values>
 __device__ __forceinline__ void gelu_short(Values& v) {
-    constexpr float kP[8] = {-1.8348062e-6f, 6.1598182e-5f, -9.3052391e-4f, 8.5078869e-3f,
-                             -5.3960058e-2f, -4.5846441e-1f, -1.1512511f,   -0.99999529f};
+    constexpr bool kLong = __is_same(T, __bf16);
+    constexpr int kTerms = kLong ? 10 : 8;
+    constexpr float kP[2][10] = {
+        {-1.8348062e-6f, 6.1598182e-5f, -9.3052391e-4f, 8.5078869e-3f, -5.3960058e-2f, -4.5846441e-1f, -1.1512511f, -0.99999529f},
+        {-2.1041304e-9f, 1.5312204e-7f, -4.8620313e-6f, 8.9347304e-5f, -1.067303e-3f, 8.883602e-3f, -5.4517057e-2f, -4.5806479e-1f,
+         -1.1513578f, -0.99999088f}};
 #pragma unroll
     for (int j = 0; j < kCount; ++j) {
         const float a = __builtin_elementwise_minimum(fabsf(v[j]), 16.0f);  // NaN stays
-        float p = kP[0];
+        float p = kP[kLong][0];
 #pragma unroll
-        for (int i = 1; i < 8; ++i) p = fmaf(p, a, kP[i]);
+        for (int i = 1; i < kTerms; ++i) p = fmaf(p, a, kP[kLong][i]);
         v[j] = fmaf(-a, __builtin_amdgcn_exp2f(p), __builtin_elementwise_maximum(v[j], 0.0f));
     }
 }
@@ -241,7 +248,7 @@ __device__ __forceinline__ void activate_few(Values& v, int act) {
         case CHIMERA_ACT_RELU: all(std::integral_constant<int, CHIMERA_ACT_RELU>{}); break;
         case CHIMERA_ACT_GELU: all(std::integral_constant<int, CHIMERA_ACT_GELU>{}); break;
         case kShortGelu:
-            if constexpr (sizeof(T) == 2) gelu_short<static_cast<int>(sizeof(Values) / sizeof(float))>(v);
+            if constexpr (sizeof(T) == 2) gelu_short<T, static_cast<int>(sizeof(Values) / sizeof(float))>(v);
             break;
         case CHIMERA_ACT_GELU_TANH: all(std::integral_constant<int, CHIMERA_ACT_GELU_TANH>{}); break;
         case CHIMERA_ACT_SILU: all(std::integral_constant<int, CHIMERA_ACT_SILU>{}); break;
@@ -831,7 +838,8 @@ hipError_t layer(hipStream_t st, const chimera_linear_shape& s, const chimera_mx
         case 8: return walk<T, 8>(st, s, a, g, e);
         default: break;
     }
-    if (e.act == kShortGelu) e.act = kRoundedGelu;  // what the dense layers' tiles have
+    // what the dense layers' tiles have; that for 16 bits ends at -6, too
+    if (e.act == kShortGelu) e.act = s.type == CHIMERA_BF16 ? CHIMERA_ACT_GELU : kRoundedGelu;
     Mx4Plan plan;
     (void)carve(s, a.workspace, &plan);
     RowsArgs rows = rows_args(s.rows, s.in_features, a.x_stride, plan.codes, plan.scales);

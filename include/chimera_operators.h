@@ -204,9 +204,10 @@ int chimera_mx4_read_device(chimera_ctx* ctx, const uint8_t* d_codes, const uint
 /* A dense layer on a weight that is held so,
  *   Y = act(Q(X) W^T + b) + R, divided row by row by its length with normalize,
  * with Q(X) the values of X's rows quantised as above. Shape, types, epilogue
- * and limits are those of the dense layer (CHIMERA_ACT_GELU is within 2^-17 of its
- * size down to z = -6 where Y has 16 bits); products are exact and sums held in
- * 32 bits. */
+ * and limits are those of the dense layer, but for CHIMERA_ACT_GELU where Y has 16
+ * bits: down to z = -6 it is within 2^-17 of its size in fp16, which ends there,
+ * and 2^-16 in bf16; in bf16 from there to -12.9 within 2^-12. Products are exact
+ * and sums held in 32 bits. */
 typedef struct {
     const void* x;           /* [rows, in_features], type */
     const uint8_t* codes;    /* [out_features, row_bytes of in_features], 16-byte aligned */

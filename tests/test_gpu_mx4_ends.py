@@ -5,6 +5,8 @@ tile's) and with one, in blocks that walk several tiles.
 A row of Y is its row of X's alone, so X is the same 331 rows over and over, which
 no tile's are a multiple of, and every row has its known result. Tolerances as in
 test_gpu_mx4."""
+import math
+
 import numpy as np
 import pytest
 
@@ -47,4 +49,23 @@ def test_layers_in_their_own_type(rows, k, n, type, pad, residual):
     for v in (d_x, d_y, d_r):
         if v is not None:
             v.free()
+    few.close()
+
+
+@pytest.mark.parametrize("rows,k,n", [(1, 32, 400), (1000, 200, 800), (8200, 256, 4090), (500, 2100, 600), (2100, 2500, 2000)])
+def test_gelu_far_below_zero(rows, k, n):
+    """bf16 holds GELU down to -12.9, where the normal distribution's tail is no
+    normal 32-bit number any more: of all biases from there to -6, in the kernels
+    of few rows, of walks and of tiles. Rows of zeros leave the bias."""
+    b = np.arange(0xC0C0, 0xC14F, dtype=np.uint32)  # -6 to -12.875
+    b = np.resize((b << 16).view(np.float32).astype(np.float64), n)
+    want = b * np.array([0.5 * math.erfc(-z / math.sqrt(2)) for z in b])
+    few = Layer(np.zeros((1, k)), np.ones((n, k)), b, None, "bf16", "bf16", "gelu", False)
+    d_x, d_y = Matrix(few.ctx, np.zeros((rows, k)), "bf16"), Matrix(few.ctx, None, "bf16", shape=(rows, n))
+    layer = operators.Mx4Linear(few.ctx, few.d["codes"], few.d["scales"], k, few.d["b"], type="bf16", activation="gelu", max_rows=rows)
+    layer.forward(d_x, d_y)
+    assert (np.abs(d_y.values() - want) <= (2.0**-12 + 2.0**-8) * np.abs(want)).all()
+    layer.close()
+    d_x.free()
+    d_y.free()
     few.close()
