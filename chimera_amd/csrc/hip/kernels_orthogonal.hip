@@ -833,15 +833,17 @@ void launch_product(hipStream_t st, Schulz a, const Pairs& p, int64_t m, const P
     // As long as each CU has at most one block whose waves divide the sum (of
     // tiles of 32 for X, two), that kernel, on tiles as small as that allows; then
     // tiles of 64 that waves share, and of 128 once they fill the CUs. us of A, B
-    // and X: 128 x 768 5.9, 3.8, 4.1; 512 x 2048 9.5, 5.7, 10.3 (in tiles of 64
-    // 17.9, 9.4, 10.7); 768 x 768 8.7, 10.8, 9.7 (64: 10.8, 12.4, 11.2); 1024 x
-    // 1024 11.1, 11.3, 13.7 (64: 11.3, 12.7; shared tiles of 64 11.9, 13.0, 14.8; 32
-    // 19, 21, 23); 1024 x 4096 23.8, 10.3, 35.0 (64: 29.0, 11.6; X in tiles of 64
-    // 38, by waves that divide the sum 48; A in four parts of its sum 25 and 5 for
-    // their join); 4096 x 4096 271, 268, 429 (960 TF of products, a plain fp16
-    // product reaches 1,300; by eight waves of 64 x 32, which read a third more
-    // from LDS, 285, 291, 439). Eight waves a tile of 32 take 0.3 us less for A and
-    // B and 0.3 more for X.
+    // and X: 512 x 2048 9.8, 5.7, 11.1; 768 x 768 8.8, 10.1, 9.5; 1024 x 1024 10.3,
+    // 10.2, 14.1; 1024 x 4096 23.5, 9.7, 35.6; 4096 x 4096 283, 289, 446 (920 TF of
+    // products, a plain fp16 product reaches 1,300). What was compared, when the
+    // lower parts' products went into the same sum as the upper ones': 512 x 2048
+    // 9.5, 5.7, 10.3 and in tiles of 64 17.9, 9.4, 10.7; 768 x 768 8.7, 10.8, 9.7
+    // (64: 10.8, 12.4, 11.2); 1024 x 1024 11.1, 11.3, 13.7 (64: 11.3, 12.7; shared
+    // tiles of 64 11.9, 13.0, 14.8; 32 19, 21, 23); 1024 x 4096 23.8, 10.3, 35.0
+    // (64: 29.0, 11.6; X in tiles of 64 38, by waves that divide the sum 48; A in
+    // four parts of its sum 25 and 5 for their join); 4096 x 4096 271, 268, 429 (by
+    // eight waves of 64 x 32, which read a third more from LDS, 285, 291, 439).
+    // Eight waves a tile of 32 take 0.3 us less for A and B and 0.3 more for X.
     if (tiles_of(32) <= (kSymmetric<kKind> ? 256 : 400)) {
         launch(orthogonal_few_kernel<kKind, 32, kSymmetric<kKind> ? 8 : 4, kSymmetric<kKind> ? 1 : 2>, 32,
                kSymmetric<kKind> ? 512 : 256);
