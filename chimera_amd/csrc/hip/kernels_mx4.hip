@@ -700,11 +700,12 @@ RowsArgs rows_args(int64_t rows, int cols, int64_t stride, uint8_t* codes, uint8
 constexpr int kMostSteps = 8;  // of a sum in registers
 
 // Whether each 32 rows and columns quantise their rows for themselves: with
-// normalize, where a block has all columns, and where there are few. That takes
-// 5.5 us and 0.01 for each block and 1,024 values of the sum, quantising first
-// 13.5 to 15: 1024 -> 512 with 512 rows 7.7 and 13.4, with 1,024 10.8 and 13.5,
-// with 2,048 18.4 and 13.7; 64 rows of 1024 -> 4096 8.0 and 14.4, 256 16.0 and
-// 14.5.
+// normalize, where a block has all columns, and where there are few. us of that
+// and of quantising first: 1024 -> 512 with 512 rows 7.3 and 10.3, with 1,024 10.6
+// and 10.4, with 2,048 18.4 and 10.8; 1024 -> 4096 with 64 rows 7.0 and 10.2, with
+// 128 8.9 and 10.3, with 192 12.9 and 10.5. So with sums of 1024 the line could
+// lie at 550; longer ones, which take tiles that walk the whole sum, have not been
+// compared.
 bool few_rows(const chimera_linear_shape& s) {
     return s.normalize || ceil_div(s.rows, 32) * ceil_div(s.out_features, 32) * ceil_div(s.in_features, 1024) <= 768;
 }
