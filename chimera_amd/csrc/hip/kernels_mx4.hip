@@ -761,9 +761,9 @@ hipError_t walk(hipStream_t st, const chimera_linear_shape& s, const chimera_mx4
     constexpr std::integral_constant<int, 8> k8;
     constexpr std::integral_constant<int, (kSteps > 4 ? 1 : 2)> k2;  // the weight takes half of the registers
     // Blocks of 256 columns that walk many tiles of 64 rows, or of 128 and 32:
-    // 65,536 x 1024 -> 4096 with GELU 313 and 333 us, 10,007 x 777 -> 520 31 and
-    // 25, 65,536 rows of it 104 and 81 (768 columns and 640), 2,048 x 1024 -> 512
-    // 13.5 and 10.8.
+    // 65,536 x 1024 -> 4096 with GELU 288 and 312 us, -> 2560 195 and 205, -> 1088
+    // 97 and 94 (1,280 columns and 1,152), 16,384 x 1024 -> 1024 31.8 and 30.2,
+    // 32,768 of these 51 and 51, 2,048 x 1024 -> 512 13.9 and 10.7.
     const int64_t n = s.out_features;
     if (ceil_div(s.rows, 64) * ceil_div(n, 256) >= 8 * kCus && round_up(n, 256) * 16 <= round_up(n, 128) * 17)
         launch(k8, k2, 1);
